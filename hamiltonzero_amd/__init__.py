@@ -13,6 +13,8 @@ Public surface, named after the reference modules it replaces:
   ``src/hamiltonzero/evaluation/sequence_parallel.py``), the large-N evaluation forward, and
   the large-N caller's head collapse fused into it (``gated_rectangular_edge_attention``,
   ``sequence_attention_output``: ``src/hamiltonzero/evaluation/sequence_trunk.py``).
+* :mod:`hamiltonzero_amd.tokens` — operators of token sequences (no reference counterpart):
+  ``qk_norm_rotary``, ``token_attention`` and ``bucket_bias`` with ``relative_buckets``.
 * :mod:`hamiltonzero_amd.kernels` — tensor-level calls of the C ABI
   (``include/hz_mhsea.h``): forward, tangent, fused forward+tangent, backward,
   gated forward+tangent, rectangular forward.
@@ -35,9 +37,11 @@ from .rect_attention import (
     pallas_rectangular_edge_attention,
     sequence_attention_output,
 )
+from .tokens import bucket_bias, qk_norm_rotary, relative_buckets, token_attention
 
 __all__ = [
     "BlockSizes",
+    "bucket_bias",
     "gated_edge_attention",
     "gated_rectangular_edge_attention",
     "mhsea_ad",
@@ -49,6 +53,9 @@ __all__ = [
     "mhsea_with_tuned_ad",
     "noncausal_bias_mha",
     "pallas_rectangular_edge_attention",
+    "qk_norm_rotary",
     "reference_edge_attention",
+    "relative_buckets",
     "sequence_attention_output",
+    "token_attention",
 ]

@@ -1,5 +1,5 @@
 """ctypes binding of ``libhz_mhsea.so`` (the C ABI declared in ``include/hz_mhsea.h``,
-``include/hz_executor.h`` and ``include/hz_pair_bias.h``).
+``include/hz_executor.h``, ``include/hz_pair_bias.h`` and ``include/hz_token.h``).
 
 The library is the only compute path of this package: there is no CPU fallback. A
 missing library raises :class:`NativeLibraryMissing` on first use.
@@ -8,6 +8,7 @@ missing library raises :class:`NativeLibraryMissing` on first use.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -49,6 +50,16 @@ EXPORTED_SYMBOLS = (
     "hz_compiled_wavefunction",
     "hz_pair_bias",
     "hz_pair_mlp_bias",
+    "hz_qk_norm_rotary_fwd",
+    "hz_qk_norm_rotary_workspace",
+    "hz_qk_norm_rotary_bwd",
+    "hz_token_attention_fwd_workspace",
+    "hz_token_attention_fwd",
+    "hz_token_attention_bwd_workspace",
+    "hz_token_attention_bwd",
+    "hz_bucket_bias_fwd",
+    "hz_bucket_bias_workspace",
+    "hz_bucket_bias_bwd",
 )
 
 
@@ -64,6 +75,13 @@ class HzError(RuntimeError):
         self.code = code
 
 
+# The structures of hz_token.h as the bytes that the calls take (native alignment).
+TOKEN_TENSOR = struct.Struct("@Pqqq")  # data, strides of batch, token, head
+# q, k, q_out, k_out, w_q, w_k, freqs, positions, B, N, H, Hk, D, n_freqs, eps, interleaved, dtype
+QK_NORM_ROTARY = struct.Struct("@" + 4 * "Pqqq" + "4P6qf2i4x")
+# q, k, v, out, lse, slopes, prefix, documents, kv_len, B, Nq, Nk, H, Hk, D, scale, softcap, causal, dtype
+TOKEN_ATTENTION = struct.Struct("@" + 3 * "Pqqq" + "6P6q2f2i")
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -71,6 +89,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _F = ctypes.c_float
+_S = ctypes.c_char_p  # a structure of hz_token.h as bytes
 
 _SIGNATURES = {
     "hz_version": ([], _INT),
@@ -125,6 +144,26 @@ _SIGNATURES = {
     # out_norm_w, w_out, b_out, alibi_slopes, e, e_t, B, Nq, Nk, C, hidden, H, n_blocks, T,
     # row_offset, inner_gain, eps, bias_div, flags
     "hz_pair_mlp_bias": ([_P] * 19 + [_I64] * 9 + [_F, _F, _F, _INT], _INT),
+    # stream, p
+    "hz_qk_norm_rotary_fwd": ([_P, _S], _INT),
+    # B, N, D
+    "hz_qk_norm_rotary_workspace": ([_I64] * 3, _I64),
+    # stream, p, dq, dk, dw_q, dw_k, workspace, workspace_bytes
+    "hz_qk_norm_rotary_bwd": ([_P, _S] + [_P] * 5 + [_I64], _INT),
+    # p
+    "hz_token_attention_fwd_workspace": ([_S], _I64),
+    # stream, p, workspace, workspace_bytes
+    "hz_token_attention_fwd": ([_P, _S, _P, _I64], _INT),
+    "hz_token_attention_bwd_workspace": ([_S], _I64),
+    # stream, p, dout, dq, dk, dv, workspace, workspace_bytes
+    "hz_token_attention_bwd": ([_P, _S, _S] + [_P] * 4 + [_I64], _INT),
+    # stream, table, buckets, q_positions, k_positions, e, B, Nq, Nk, H, n_buckets, R, dtype, flags
+    "hz_bucket_bias_fwd": ([_P] * 6 + [_I64] * 6 + [_INT, _INT], _INT),
+    # B, Nq, Nk, H, n_buckets, flags
+    "hz_bucket_bias_workspace": ([_I64] * 5 + [_INT], _I64),
+    # stream, de, buckets, q_positions, k_positions, dtable, workspace, workspace_bytes, B, Nq, Nk, H,
+    # n_buckets, R, dtype, flags
+    "hz_bucket_bias_bwd": ([_P] * 7 + [_I64] * 7 + [_INT, _INT], _INT),
 }
 
 

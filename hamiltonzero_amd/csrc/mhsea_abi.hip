@@ -4,11 +4,13 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <utility>
 
 #include "../../include/hz_executor.h"
 #include "../../include/hz_pair_bias.h"
 #include "../../include/hz_mhsea.h"
 #include "mhsea_launch.h"
+#include "token_launch.h"
 
 namespace {
 
@@ -213,6 +215,128 @@ int rect_attention(hipStream_t stream, const float* q, const float* k, const flo
   p.scale = scale;
   p.gated = gated ? 1 : 0;
   return launched(hz::launch_rect_fwd(p, static_cast<int>(D), stream));
+}
+
+// The token operators (hz_token.h).
+int check_strided(const char* name, const hz_token_tensor& t) {
+  if (t.data == nullptr) return fail(HZ_ENULL, "%s must not be NULL", name);
+  if (!aligned16(t.data)) return fail(HZ_EALIGN, "%s must be 16-byte aligned", name);
+  for (int64_t s : {t.batch, t.token, t.head})
+    if (s < 0 || s % 8 != 0)
+      return fail(HZ_EINVAL, "%s: strides must be multiples of 8 elements and not negative, got %lld", name, (long long)s);
+  return HZ_OK;
+}
+
+int check_elements(const char* name, const void* ptr, size_t size) {
+  if ((reinterpret_cast<uintptr_t>(ptr) & (size - 1)) != 0) return fail(HZ_EALIGN, "%s must be aligned to its elements", name);
+  return HZ_OK;
+}
+
+int check_dtype(int dtype) {
+  if (dtype != HZ_DTYPE_F32 && dtype != HZ_DTYPE_BF16)
+    return fail(HZ_EINVAL, "dtype must be HZ_DTYPE_F32 (0) or HZ_DTYPE_BF16 (1), got %d", dtype);
+  return HZ_OK;
+}
+
+int check_workspace(const void* workspace, int64_t bytes, int64_t need) {
+  if (need == 0) return HZ_OK;
+  if (workspace == nullptr) return fail(HZ_ENULL, "workspace must not be NULL");
+  if (!aligned16(workspace)) return fail(HZ_EALIGN, "workspace must be 16-byte aligned");
+  if (bytes < need) return fail(HZ_EINVAL, "workspace holds %lld bytes, needs %lld", (long long)bytes, (long long)need);
+  return HZ_OK;
+}
+
+constexpr int64_t kTokenAxis = int64_t(1) << 30;
+
+int check_norm_rotary(const hz_qk_norm_rotary* p) {
+  if (p == nullptr) return fail(HZ_ENULL, "p must not be NULL");
+  if (int rc = check_dtype(p->dtype)) return rc;
+  if (p->B < 1 || p->N < 1 || p->H < 1 || p->Hk < 1)
+    return fail(HZ_EINVAL, "B, N, H and Hk must be >= 1, got %lld, %lld, %lld and %lld", (long long)p->B, (long long)p->N,
+                (long long)p->H, (long long)p->Hk);
+  if (p->B > kTokenAxis || p->N > kTokenAxis || p->H > 65536 || p->Hk > 65536 || p->B * p->N > (int64_t(1) << 40))
+    return fail(HZ_EINVAL, "B, N, H or Hk exceeds the supported size");
+  if (p->D < 8 || p->D > HZ_ROTARY_MAX_HEAD || p->D % 8 != 0)
+    return fail(HZ_EINVAL, "head dimension must be a multiple of 8 in [8, %d], got %lld", HZ_ROTARY_MAX_HEAD, (long long)p->D);
+  if (p->n_freqs < 0 || p->n_freqs % 4 != 0 || 2 * p->n_freqs > p->D)
+    return fail(HZ_EINVAL, "n_freqs must be a multiple of 4 in [0, D / 2], got %lld", (long long)p->n_freqs);
+  if (!(p->eps >= 0.f) || !std::isfinite(p->eps)) return fail(HZ_EINVAL, "eps must be finite and >= 0");
+  if (p->n_freqs > 0 && p->freqs == nullptr) return fail(HZ_ENULL, "freqs must not be NULL");
+  if (int rc = check_elements("w_q", p->w_q, 4)) return rc;
+  if (int rc = check_elements("w_k", p->w_k, 4)) return rc;
+  if (int rc = check_elements("freqs", p->freqs, 8)) return rc;
+  if (int rc = check_elements("positions", p->positions, 4)) return rc;
+  if (int rc = check_strided("q", p->q)) return rc;
+  if (int rc = check_strided("k", p->k)) return rc;
+  if (int rc = check_strided("q_out", p->q_out)) return rc;
+  return check_strided("k_out", p->k_out);
+}
+
+int check_token_dims(const hz_token_attention* p) {
+  if (p == nullptr) return fail(HZ_ENULL, "p must not be NULL");
+  if (int rc = check_dtype(p->dtype)) return rc;
+  if (p->B < 1 || p->Nq < 1 || p->Nk < 1 || p->H < 1 || p->Hk < 1)
+    return fail(HZ_EINVAL, "B, Nq, Nk, H and Hk must be >= 1, got %lld, %lld, %lld, %lld and %lld", (long long)p->B,
+                (long long)p->Nq, (long long)p->Nk, (long long)p->H, (long long)p->Hk);
+  if (p->Nq >= kTokenAxis || p->Nk >= kTokenAxis) return fail(HZ_EINVAL, "Nq and Nk must be below 2^30");
+  if (p->H % p->Hk != 0)
+    return fail(HZ_EINVAL, "H must be a multiple of Hk, got %lld and %lld", (long long)p->H, (long long)p->Hk);
+  if (p->D < 8 || p->D > HZ_TOKEN_MAX_HEAD || p->D % 8 != 0)
+    return fail(HZ_EINVAL, "head dimension must be a multiple of 8 in [8, %d], got %lld", HZ_TOKEN_MAX_HEAD, (long long)p->D);
+  // grids of one-dimensional launches, with room for their thread counts
+  const int64_t most = int64_t(1) << 20;
+  if (p->B > most || p->H > most || p->B * p->H > most || p->B * p->H * ((p->Nq + 127) / 128) > most ||
+      p->B * p->Hk * ((p->Nk + 127) / 128) > most)
+    return fail(HZ_EINVAL, "B * heads * ceil(N / 128) exceeds the grid limit of %lld", (long long)most);
+  return HZ_OK;
+}
+
+int check_token_attention(const hz_token_attention* p) {
+  if (int rc = check_token_dims(p)) return rc;
+  if (!std::isfinite(p->scale)) return fail(HZ_EINVAL, "scale must be finite");
+  if (!(p->softcap >= 0.f) || !std::isfinite(p->softcap)) return fail(HZ_EINVAL, "softcap must be finite and >= 0");
+  if (p->causal != 0 && p->causal != 1) return fail(HZ_EINVAL, "causal must be 0 or 1, got %d", p->causal);
+  if (p->prefix != nullptr && !p->causal) return fail(HZ_EINVAL, "prefix needs causal");
+  if (int rc = check_strided("q", p->q)) return rc;
+  if (int rc = check_strided("k", p->k)) return rc;
+  if (int rc = check_strided("v", p->v)) return rc;
+  if (int rc = check_elements("lse", p->lse, 4)) return rc;
+  if (int rc = check_elements("slopes", p->slopes, 4)) return rc;
+  if (int rc = check_elements("prefix", p->prefix, 4)) return rc;
+  if (int rc = check_elements("documents", p->documents, 4)) return rc;
+  if (int rc = check_elements("kv_len", p->kv_len, 4)) return rc;
+  if (p->out == nullptr) return fail(HZ_ENULL, "out must not be NULL");
+  if (!aligned16(p->out)) return fail(HZ_EALIGN, "out must be 16-byte aligned");
+  return HZ_OK;
+}
+
+int check_bucket_bias(int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t nb, int64_t R, int dtype, int flags) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (flags & ~HZ_FLAG_E_QKH) return fail(HZ_EINVAL, "unknown flag bits 0x%x", flags);
+  if (B < 1 || Nq < 1 || Nk < 1) return fail(HZ_EINVAL, "B, Nq and Nk must be >= 1");
+  if (H < 1 || H > 256) return fail(HZ_EINVAL, "H must be in [1, 256], got %lld", (long long)H);
+  if (nb < 1 || nb > HZ_BUCKET_MAX) return fail(HZ_EINVAL, "n_buckets must be in [1, %d], got %lld", HZ_BUCKET_MAX, (long long)nb);
+  if (R < 0 || R > HZ_BUCKET_MAX_RANGE)
+    return fail(HZ_EINVAL, "R must be in [0, %d], got %lld", HZ_BUCKET_MAX_RANGE, (long long)R);
+  if ((nb + 1) * ((H + 63) / 64 * 64) > HZ_BUCKET_MAX_TABLE)
+    return fail(HZ_EINVAL, "a table of %lld buckets for %lld heads exceeds the supported size", (long long)nb, (long long)H);
+  if (Nq >= kTokenAxis || Nk >= kTokenAxis || B >= kTokenAxis || B * Nq > (int64_t(1) << 46) / Nk)
+    return fail(HZ_EINVAL, "B * Nq * Nk exceeds the supported tensor size");
+  return HZ_OK;
+}
+
+hz::BucketParams bucket_params(const int32_t* buckets, const int32_t* qpos, const int32_t* kpos, int64_t B, int64_t Nq,
+                               int64_t Nk, int64_t H, int64_t nb, int64_t R, int dtype, int flags) {
+  return {buckets, qpos, kpos, B, Nq, Nk, static_cast<int>(H), static_cast<int>(nb), static_cast<int>(R),
+          (flags & HZ_FLAG_E_QKH) != 0, dtype};
+}
+
+int check_bucket_arrays(const int32_t* buckets, const int32_t* qpos, const int32_t* kpos) {
+  for (auto [name, ptr] : {std::pair<const char*, const int32_t*>{"buckets", buckets}, {"q_positions", qpos}, {"k_positions", kpos}}) {
+    if (ptr == nullptr) return fail(HZ_ENULL, "%s must not be NULL", name);
+    if (int rc = check_elements(name, ptr, 4)) return rc;
+  }
+  return HZ_OK;
 }
 
 }  // namespace
@@ -753,6 +877,86 @@ int hz_mhsea_bwd_gated(hipStream_t stream, const void* q, const void* k, const v
     return rc;
   return hz_mhsea_bwd(stream, q, k, e, v, mask, lse, out, dout_work, dq, dk, de, dv, B, N, H, D, HZ_DTYPE_F32, scale,
                       flags);
+}
+
+int hz_qk_norm_rotary_fwd(hipStream_t stream, const hz_qk_norm_rotary* p) {
+  if (int rc = check_norm_rotary(p)) return rc;
+  return launched(hz::launch_qk_norm_rotary_fwd(*p, stream));
+}
+
+int64_t hz_qk_norm_rotary_workspace(int64_t B, int64_t N, int64_t D) {
+  if (B < 1 || N < 1 || D < 1 || B > kTokenAxis || N > kTokenAxis || D > HZ_ROTARY_MAX_HEAD) return -1;
+  return hz::qk_norm_rotary_workspace(B * N, D);
+}
+
+int hz_qk_norm_rotary_bwd(hipStream_t stream, const hz_qk_norm_rotary* p, void* dq, void* dk, float* dw_q, float* dw_k,
+                          void* workspace, int64_t workspace_bytes) {
+  if (int rc = check_norm_rotary(p)) return rc;
+  HZ_REQUIRE(dq);
+  HZ_REQUIRE(dk);
+  if (int rc = check_elements("dw_q", dw_q, 4)) return rc;
+  if (int rc = check_elements("dw_k", dw_k, 4)) return rc;
+  if (int rc = check_workspace(workspace, workspace_bytes, hz::qk_norm_rotary_workspace(p->B * p->N, p->D))) return rc;
+  return launched(hz::launch_qk_norm_rotary_bwd(*p, dq, dk, dw_q, dw_k, workspace, stream));
+}
+
+int64_t hz_token_attention_fwd_workspace(const hz_token_attention* p) {
+  if (check_token_dims(p)) return -1;
+  return hz::token_attention_fwd_workspace(*p);
+}
+
+int hz_token_attention_fwd(hipStream_t stream, const hz_token_attention* p, void* workspace, int64_t workspace_bytes) {
+  if (int rc = check_token_attention(p)) return rc;
+  if (int rc = check_workspace(workspace, workspace_bytes, hz::token_attention_fwd_workspace(*p))) return rc;
+  return launched(hz::launch_token_attention_fwd(*p, workspace, stream));
+}
+
+int64_t hz_token_attention_bwd_workspace(const hz_token_attention* p) {
+  if (check_token_dims(p)) return -1;
+  return hz::token_attention_bwd_workspace(*p);
+}
+
+int hz_token_attention_bwd(hipStream_t stream, const hz_token_attention* p, const hz_token_tensor* dout, void* dq,
+                           void* dk, void* dv, void* workspace, int64_t workspace_bytes) {
+  if (int rc = check_token_attention(p)) return rc;
+  if (p->lse == nullptr) return fail(HZ_ENULL, "lse must not be NULL");
+  if (dout == nullptr) return fail(HZ_ENULL, "dout must not be NULL");
+  if (int rc = check_strided("dout", *dout)) return rc;
+  HZ_REQUIRE(dq);
+  HZ_REQUIRE(dk);
+  HZ_REQUIRE(dv);
+  if (int rc = check_workspace(workspace, workspace_bytes, hz::token_attention_bwd_workspace(*p))) return rc;
+  return launched(hz::launch_token_attention_bwd(*p, *dout, dq, dk, dv, workspace, stream));
+}
+
+int hz_bucket_bias_fwd(hipStream_t stream, const float* table, const int32_t* buckets, const int32_t* q_positions,
+                       const int32_t* k_positions, void* e, int64_t B, int64_t Nq, int64_t Nk, int64_t H,
+                       int64_t n_buckets, int64_t R, int dtype, int flags) {
+  if (int rc = check_bucket_bias(B, Nq, Nk, H, n_buckets, R, dtype, flags)) return rc;
+  if (table == nullptr) return fail(HZ_ENULL, "table must not be NULL");
+  if (int rc = check_elements("table", table, 4)) return rc;
+  if (int rc = check_bucket_arrays(buckets, q_positions, k_positions)) return rc;
+  HZ_REQUIRE(e);
+  return launched(hz::launch_bucket_bias_fwd(
+      bucket_params(buckets, q_positions, k_positions, B, Nq, Nk, H, n_buckets, R, dtype, flags), table, e, stream));
+}
+
+int64_t hz_bucket_bias_workspace(int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t n_buckets, int flags) {
+  if (check_bucket_bias(B, Nq, Nk, H, n_buckets, 0, HZ_DTYPE_F32, flags)) return -1;
+  return hz::bucket_bias_workspace(
+      bucket_params(nullptr, nullptr, nullptr, B, Nq, Nk, H, n_buckets, 0, HZ_DTYPE_F32, flags));
+}
+
+int hz_bucket_bias_bwd(hipStream_t stream, const void* de, const int32_t* buckets, const int32_t* q_positions,
+                       const int32_t* k_positions, float* dtable, void* workspace, int64_t workspace_bytes, int64_t B,
+                       int64_t Nq, int64_t Nk, int64_t H, int64_t n_buckets, int64_t R, int dtype, int flags) {
+  if (int rc = check_bucket_bias(B, Nq, Nk, H, n_buckets, R, dtype, flags)) return rc;
+  HZ_REQUIRE(de);
+  if (int rc = check_bucket_arrays(buckets, q_positions, k_positions)) return rc;
+  HZ_REQUIRE(dtable);
+  const hz::BucketParams p = bucket_params(buckets, q_positions, k_positions, B, Nq, Nk, H, n_buckets, R, dtype, flags);
+  if (int rc = check_workspace(workspace, workspace_bytes, hz::bucket_bias_workspace(p))) return rc;
+  return launched(hz::launch_bucket_bias_bwd(p, de, dtable, workspace, stream));
 }
 
 }  // extern "C"

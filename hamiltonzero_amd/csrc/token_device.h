@@ -1,0 +1,224 @@
+// Device helpers shared by the token attention kernels (include/hz_token.h).
+//
+// One kernel text serves both storage types: an operand of a product is PARTS registers quadruples of
+// eight bfloat16, one for bfloat16 tensors, three for float32 ones (the split of split_f32.h, whose six
+// products give float32's precision). Products are v_mfma_f32_32x32x16_bf16 with the layouts of
+// split_f32.h: lane l = 32 hh + c.
+//
+// Scores are formed transposed, S^T = K Q^T (keys in a lane's sixteen registers, one query a lane), so
+// a row's softmax is a sum over registers and one exchange with the other half wave, and a lane's
+// weights of keys kappa(s, hh, j) = 16 s + 8 (j / 4) + 4 hh + j % 4, j = 0..7, are its B operand of the
+// product with V's rows in that order, without moving a value between lanes.
+//
+// LDS tiles hold rows of DP bfloat16 in chunks of eight; chunk i of row r lies at chunk
+// i ^ swizzle(r). Rows of one 256-byte line then differ where sixteen rows are read at one chunk (the
+// A operand of K Q^T) and where four rows are read at four chunks (the transposing reads of the A
+// operand V^T), so both go through without bank conflicts and without padding.
+#pragma once
+
+#include "mhsea_device.h"
+#include "split_f32.h"
+#include "token_launch.h"
+
+namespace hz {
+namespace token {
+
+constexpr float kNegInf = -__builtin_inff();
+
+struct Params {
+  hz_token_tensor q, k, v;
+  void* out;
+  float* lse;
+  const float* slopes;
+  const int32_t *prefix, *documents, *kv_len;
+  int B, Nq, Nk, H, Hk, G, D, causal;
+  float scale;      // of the dot products
+  float cap;        // 0: not capped
+  float to_tanh;    // scale / cap
+  float to_score2;  // base-2 score of a dot product (scale log2 e) or of a tanh (cap log2 e)
+};
+
+inline Params make_params(const hz_token_attention& a) {
+  Params p{};
+  p.q = a.q, p.k = a.k, p.v = a.v, p.out = a.out, p.lse = a.lse;
+  p.slopes = a.slopes, p.prefix = a.prefix, p.documents = a.documents, p.kv_len = a.kv_len;
+  p.B = static_cast<int>(a.B), p.Nq = static_cast<int>(a.Nq), p.Nk = static_cast<int>(a.Nk);
+  p.H = static_cast<int>(a.H), p.Hk = static_cast<int>(a.Hk), p.G = p.H / p.Hk, p.D = static_cast<int>(a.D);
+  p.causal = a.causal, p.scale = a.scale, p.cap = a.softcap;
+  p.to_tanh = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+  p.to_score2 = (a.softcap > 0.f ? a.softcap : a.scale) * kLog2e;
+  return p;
+}
+
+// Eight consecutive elements in storage format, as loaded early and used late.
+template <int PARTS>
+struct Raw8;
+template <>
+struct Raw8<1> {
+  v4u u;
+  __device__ __forceinline__ void load(const void* base, int64_t off, bool on) {
+    u = on ? *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(base) + off) : v4u{0u, 0u, 0u, 0u};
+  }
+};
+template <>
+struct Raw8<3> {
+  v4f a, b;
+  __device__ __forceinline__ void load(const void* base, int64_t off, bool on) {
+    const v4f* const p = reinterpret_cast<const v4f*>(static_cast<const float*>(base) + off);
+    a = on ? p[0] : zero4();
+    b = on ? p[1] : zero4();
+  }
+};
+
+__device__ __forceinline__ void floats(const Raw8<1>& r, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(r.u[i] << 16);
+    x[2 * i + 1] = __uint_as_float(r.u[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void floats(const Raw8<3>& r, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = r.a[i], x[4 + i] = r.b[i];
+}
+
+// An operand of eight bfloat16 a part.
+template <int PARTS>
+struct Frag {
+  v4u p[PARTS];
+};
+__device__ __forceinline__ Frag<1> frag(const Raw8<1>& r) { return Frag<1>{{r.u}}; }
+__device__ __forceinline__ Frag<3> frag(const Raw8<3>& r) {
+  const float x[8] = {r.a[0], r.a[1], r.a[2], r.a[3], r.b[0], r.b[1], r.b[2], r.b[3]};
+  const Split8 s = split8(x);
+  return Frag<3>{{s.h, s.m, s.l}};
+}
+// Elements 8 s .. 8 s + 7 of a score tile.
+template <int PARTS>
+__device__ __forceinline__ Frag<PARTS> frag_of(const v16f& x, int s) {
+  if constexpr (PARTS == 1) {
+    Frag<1> f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.p[0][i] = pack2_bf16(x[8 * s + 2 * i], x[8 * s + 2 * i + 1]);
+    return f;
+  } else {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[8 * s + i];
+    const Split8 f = split8(y);
+    return Frag<3>{{f.h, f.m, f.l}};
+  }
+}
+
+__device__ __forceinline__ v16f mma(const Frag<1>& a, const Frag<1>& b, v16f c) {
+  return mfma32_bf16(as_bf16x8(a.p[0]), as_bf16x8(b.p[0]), c);
+}
+__device__ __forceinline__ v16f mma(const Frag<3>& a, const Frag<3>& b, v16f c) {
+#pragma unroll
+  for (int t = 0; t < kSplitTerms; ++t) c = mfma32_bf16(as_bf16x8(a.p[kSplitA[t]]), as_bf16x8(b.p[kSplitB[t]]), c);
+  return c;
+}
+
+// A tile of ROWS rows of DP elements in LDS, PARTS planes.
+template <int ROWS, int DP, int PARTS>
+struct Tile {
+  static constexpr int kPlane = ROWS * DP;
+  static constexpr int kBytes = kPlane * PARTS * 2;
+  uint16_t* base;
+
+  __device__ __forceinline__ static int swizzle(int row) {
+    const int low = (row >> 2) & 3;
+    return DP == 128 ? ((row & 3) << 2) | low : DP == 64 ? (((row >> 1) & 1) << 2) | low : low;
+  }
+  __device__ __forceinline__ static int at(int row, int chunk) { return row * DP + ((chunk ^ swizzle(row)) << 3); }
+
+  __device__ __forceinline__ void put(int row, int chunk, const Frag<PARTS>& f) const {
+    const int o = at(row, chunk);
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) *reinterpret_cast<v4u*>(base + i * kPlane + o) = f.p[i];
+  }
+  // A operand of a product over the columns: lane (hh, c) gets row row0 + c, elements 16 s + 8 hh .. + 7.
+  __device__ __forceinline__ Frag<PARTS> rows(int row0, int s, int lane) const {
+    const int o = at(row0 + (lane & 31), 2 * s + (lane >> 5));
+    Frag<PARTS> f;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) f.p[i] = *reinterpret_cast<const v4u*>(base + i * kPlane + o);
+    return f;
+  }
+  // A operand of a product over the rows: lane (hh, c) gets column 32 dt + c of the rows row0 + 8 (j / 4)
+  // + 4 hh + j % 4, j = 0..7. Lane 16 g + 4 j + q addresses row 4 (g / 2) + j (then eight rows on),
+  // columns 32 dt + 16 (g % 2) + 4 q .. + 3; the hardware transposes the 16-lane groups. row0 is a
+  // multiple of 16.
+  __device__ __forceinline__ Frag<PARTS> columns(int row0, int dt, int lane) const {
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    const int g = lane >> 4, m = lane & 15, row = row0 + 4 * (g >> 1) + (m >> 2);
+    const int chunk = 4 * dt + 2 * (g & 1) + ((m & 3) >> 1), half = 4 * (m & 1);
+    const int o0 = at(row, chunk) + half, o1 = at(row + 8, chunk) + half;
+    Frag<PARTS> f;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(base + i * kPlane + o0));
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(base + i * kPlane + o1));
+      const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
+      f.p[i] = v4u{l.x, l.y, h.x, h.y};
+    }
+    return f;
+  }
+};
+
+// tanh by 1 - 2 / (1 + e^2y). Its error, an absolute 1e-7, is a relative one of small scores, which
+// float32 tensors get from the series instead (the first term left out is 4e-11 of the result at 1/4).
+template <int PARTS>
+__device__ __forceinline__ float tanh_of(float y) {
+  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + fast_exp2(2.f * kLog2e * y));
+  if constexpr (PARTS == 1) return big;
+  const float z = y * y;
+  const float odd = z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835 - z * (1382.f / 155925)))));
+  return fabsf(y) < 0.25f ? y + y * odd : big;
+}
+
+// Element i of a lane's sixteen scores of a 32-row block belongs to row 8 (i / 4) + 4 hh + i % 4.
+__device__ __forceinline__ int row_of(int i, int hh) { return 8 * (i >> 2) + 4 * hh + (i & 3); }
+
+__device__ __forceinline__ int kv_length(const Params& p, int b) {
+  if (p.kv_len == nullptr) return p.Nk;
+  const int n = p.kv_len[b];
+  return n < 0 ? 0 : n > p.Nk ? p.Nk : n;
+}
+
+// What one query may see: keys up to `last`, and where there are documents those of `doc`.
+constexpr int kNoDocument = -2147483647 - 1;
+struct Sight {
+  int pos, last, doc;
+  __device__ __forceinline__ Sight(const Params& p, int b, int i, int n) {
+    pos = n - p.Nq + i;
+    last = n - 1;
+    if (p.causal) {
+      const int pre = p.prefix != nullptr ? max(p.prefix[b], 0) : 0;
+      const int near = max(pos, pre - 1);
+      last = near < last ? near : last;
+    }
+    doc = kNoDocument;
+    if (p.documents != nullptr && pos >= 0) {
+      const int d = p.documents[static_cast<int64_t>(b) * p.Nk + pos];
+      doc = d >= 0 ? d : kNoDocument;
+    }
+  }
+};
+// A key's document, with every padding number the same.
+__device__ __forceinline__ int key_document(const Params& p, int b, int j) {
+  const int d = p.documents[static_cast<int64_t>(b) * p.Nk + j];
+  return d >= 0 ? d : -1;
+}
+
+// Four consecutive elements in the tensor's type.
+template <int PARTS>
+__device__ __forceinline__ void store_four(void* out, int64_t off, float a, float b, float c, float d) {
+  if constexpr (PARTS == 1)
+    store4<BF16>(out, off, a, b, c, d);
+  else
+    store4<F32>(out, off, a, b, c, d);
+}
+
+}  // namespace token
+}  // namespace hz
