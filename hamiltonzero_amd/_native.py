@@ -79,8 +79,8 @@ class HzError(RuntimeError):
 TOKEN_TENSOR = struct.Struct("@Pqqq")  # data, strides of batch, token, head
 # q, k, q_out, k_out, w_q, w_k, freqs, positions, B, N, H, Hk, D, n_freqs, eps, interleaved, dtype
 QK_NORM_ROTARY = struct.Struct("@" + 4 * "Pqqq" + "4P6qf2i4x")
-# q, k, v, out, lse, slopes, prefix, documents, kv_len, B, Nq, Nk, H, Hk, D, scale, softcap, causal, dtype
-TOKEN_ATTENTION = struct.Struct("@" + 3 * "Pqqq" + "6P6q2f2i")
+# q, k, v, out, out_low, lse, slopes, prefix, documents, kv_len, B, Nq, Nk, H, Hk, D, scale, softcap, causal, dtype
+TOKEN_ATTENTION = struct.Struct("@" + 3 * "Pqqq" + "7P6q2f2i")
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

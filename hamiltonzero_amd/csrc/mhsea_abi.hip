@@ -307,6 +307,7 @@ int check_token_attention(const hz_token_attention* p) {
   if (int rc = check_elements("kv_len", p->kv_len, 4)) return rc;
   if (p->out == nullptr) return fail(HZ_ENULL, "out must not be NULL");
   if (!aligned16(p->out)) return fail(HZ_EALIGN, "out must be 16-byte aligned");
+  if (!aligned16(p->out_low)) return fail(HZ_EALIGN, "out_low must be 16-byte aligned");
   return HZ_OK;
 }
 

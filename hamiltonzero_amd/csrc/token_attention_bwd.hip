@@ -4,7 +4,8 @@
 // Two kernels, each with its sums in registers, so that nothing is added atomically: one owns queries and
 // streams keys (dq, and rowsum(dout out) for the other), one owns keys and streams the queries of
 // every head that shares them (dk, dv). Both rebuild P = exp(s - lse) from the forward's lse: seven products
-// a tile pair where one kernel with atomic dq sums would need five.
+// a tile pair where one kernel with atomic dq sums would need five. Tiles are copied, skipped and
+// masked as in the forward.
 #include "token_device.h"
 
 namespace hz {
@@ -12,52 +13,71 @@ namespace {
 
 using namespace token;
 
-constexpr int kThreads = 256;
 constexpr int kBlock = 128;  // queries (dq) or keys (dk, dv) a workgroup, 32 a wave
 
 // Rows of a streamed tile: two tensors, float32 ones in three parts.
 template <int DP, int PARTS>
 constexpr int kRows = (DP == 128 && PARTS == 3) ? 32 : 64;
 
-// Weight and score gradient (without the scale) of one visible pair, from its dot product x, its dP and the
+// Weight and score gradient (without the scale) of one pair, from its dot product x, its dP and the
 // distance between query and key.
 template <int PARTS, bool CAP>
-__device__ __forceinline__ void pair(const Params& p, float x, float dp, float slope2, int distance, float lse2,
-                                     float delta, bool seen, float& w, float& ds) {
-  float t = 0.f;
+__device__ __forceinline__ void pair(const Params& p, float x, float dp, float slope2, float distance, float lse2,
+                                     float delta, float& w, float& ds) {
+  float g = 0.f;
   if constexpr (CAP) {
-    t = tanh_of<PARTS>(x * p.to_tanh);
+    const float t = tanh_of<PARTS>(x * p.to_tanh);
     x = t;
+    g = 1.f - t * t;
   }
-  const float s = x * p.to_score2 - slope2 * static_cast<float>(distance);
-  w = seen ? fast_exp2(s - lse2) : 0.f;
-  float g = w * (dp - delta);
-  if constexpr (CAP) g *= 1.f - t * t;
-  ds = seen ? g : 0.f;
+  float s = x * p.to_score2 - lse2;
+  if (slope2 != 0.f) s -= slope2 * fabsf(distance);
+  w = fast_exp2(s);
+  ds = w * (dp - delta);
+  if constexpr (CAP) ds *= g;
 }
 
 template <int DP, int PARTS, bool CAP>
-__global__ void __launch_bounds__(kThreads) token_dq_kernel(Params p, hz_token_tensor dout, void* dq, float* deltas) {
+__global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Params p, hz_token_tensor dout, void* dq,
+                                                                           float* deltas, const DocTile* doc_tiles) {
   constexpr int KB = kRows<DP, PARTS>, NB = KB / 32, DT = DP / 32, CH = DP / 8;
-  constexpr int LOADS = KB * CH / kThreads, STEP = kThreads / CH;
+  constexpr int LOADS = KB * CH / 256, STEP = 256 / CH;
+  constexpr int BUFS = PARTS == 1 ? 2 : 1;
   typedef Tile<KB, DP, PARTS> KV;
-  __shared__ __align__(16) uint16_t k_lds[KV::kPlane * PARTS], v_lds[KV::kPlane * PARTS];
-  __shared__ int doc_lds[KB];
-  const KV kt{k_lds}, vt{v_lds};
+  __shared__ __align__(16) uint16_t k_lds0[KV::kPlane * PARTS], v_lds0[KV::kPlane * PARTS];
+  __shared__ __align__(16) uint16_t k_lds1[PARTS == 1 ? KV::kPlane : 8], v_lds1[PARTS == 1 ? KV::kPlane : 8];
+  __shared__ __align__(16) int doc_lds[BUFS][KB];
+  __shared__ int range_lds[4][2];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, hh = lane >> 5, c = lane & 31;
   const int tiles = (p.Nq + kBlock - 1) / kBlock;
-  int64_t id = xcd_logical_block(blockIdx.x, gridDim.x);
-  const int h = static_cast<int>(id % p.H);
-  id /= p.H;
+  int64_t id = xcd_run(blockIdx.x, gridDim.x);
+  const int head = static_cast<int>(id % p.G);
+  id /= p.G;
   const int q0 = static_cast<int>(tiles - 1 - id % tiles) * kBlock;
-  const int b = static_cast<int>(id / tiles);
-  const int hk = h / p.G, n = kv_length(p, b);
+  id /= tiles;
+  const int hk = static_cast<int>(id % p.Hk), b = static_cast<int>(id / p.Hk), h = hk * p.G + head;
+  const int n = kv_length(p, b);
   const int i = q0 + 32 * wave + c, row = i < p.Nq ? i : p.Nq - 1;
   const Sight me(p, b, row, n);
   const float slope2 = p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
-  const int end = Sight(p, b, min(q0 + kBlock, p.Nq) - 1, n).last + 1;
   const int wave_first = __builtin_amdgcn_readfirstlane(me.last);
-  const int wave_last = Sight(p, b, min(q0 + 32 * wave + 31, p.Nq - 1), n).last;
+  const int wave_last = __builtin_amdgcn_readlane(me.last, 31);
+  const int keys = Sight(p, b, min(q0 + kBlock, p.Nq) - 1, n).last + 1;
+  const int end = keys > 0 ? (keys + KB - 1) / KB : 0;
+  const bool by_document = p.documents != nullptr;
+  int wave_lo = 0, wave_hi = 0, lo = 0, hi = 0;
+  bool one_document = false;
+  if (by_document) {
+    document_range(me.doc, wave_lo, wave_hi);
+    one_document = wave_lo == wave_hi && !__any(me.doc < 0);
+    if (lane == 0) range_lds[wave][0] = wave_lo, range_lds[wave][1] = wave_hi;
+    __syncthreads();
+    lo = min(min(range_lds[0][0], range_lds[1][0]), min(range_lds[2][0], range_lds[3][0]));
+    hi = max(max(range_lds[0][1], range_lds[1][1]), max(range_lds[2][1], range_lds[3][1]));
+  }
+  const DocTile* const row_tiles = doc_tiles + static_cast<int64_t>(b) * ((p.Nk + kDocTile - 1) / kDocTile);
+  auto range = [row_tiles](int t) { return row_tiles[t * KB / kDocTile]; };
+  Walk<decltype(range)> walk(0, end, by_document, lo, hi, range);
   const int64_t at = (static_cast<int64_t>(b) * p.Nq + row) * p.H + h;
 
   Frag<PARTS> q[DP / 16], go[DP / 16];
@@ -74,6 +94,12 @@ __global__ void __launch_bounds__(kThreads) token_dq_kernel(Params p, hz_token_t
     floats(ro, y);
 #pragma unroll
     for (int j = 0; j < 8; ++j) delta += x[j] * y[j];
+    if (PARTS == 1 && p.out_low != nullptr) {
+      ro.load(p.out_low, at * p.D + d, d < p.D);
+      floats(ro, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta += x[j] * y[j];
+    }
     q[s] = frag(rq);
     go[s] = frag(rg);
   }
@@ -85,93 +111,158 @@ __global__ void __launch_bounds__(kThreads) token_dq_kernel(Params p, hz_token_t
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = v16f{};
 
+  const Copy<KB, DP> copy_k(p.k, b, hk, p.D, tid), copy_v(p.v, b, hk, p.D, tid);
   const int lr = tid / CH, lc = tid % CH;
-  Raw8<PARTS> rk[LOADS], rv[LOADS];
-  int rdoc = -1;
-  auto load = [&](int k0) {
+  Raw8<PARTS> rk[PARTS == 3 ? LOADS : 1], rv[PARTS == 3 ? LOADS : 1];
+  int rdoc = -1;  // as loaded: waited for where it is used
+  auto load = [&](int t, auto to) __attribute__((always_inline)) {
+    const int k0 = t * KB;
+    if (by_document && tid < KB) rdoc = k0 + tid < n ? p.documents[static_cast<int64_t>(b) * p.Nk + k0 + tid] : -1;
+    if constexpr (PARTS == 1) {
+      copy_k(to.value == 0 ? k_lds0 : k_lds1, k0, n);
+      copy_v(to.value == 0 ? v_lds0 : v_lds1, k0, n);
+    } else {
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int key = k0 + lr + STEP * j;
-      bool on = key < n && 8 * lc < p.D;
-      if (p.documents != nullptr && on) on = key_document(p, b, key) >= 0;  // padding may hold anything
-      rk[j].load(p.k.data, b * p.k.batch + key * p.k.token + hk * p.k.head + 8 * lc, on);
-      rv[j].load(p.v.data, b * p.v.batch + key * p.v.token + hk * p.v.head + 8 * lc, on);
+      for (int j = 0; j < LOADS; ++j) {
+        const int key = k0 + lr + STEP * j;
+        bool on = key < n && 8 * lc < p.D;
+        if (by_document && on) on = key_document(p, b, key) >= 0;  // padding may hold anything
+        rk[j].load(p.k.data, b * p.k.batch + key * p.k.token + hk * p.k.head + 8 * lc, on);
+        rv[j].load(p.v.data, b * p.v.batch + key * p.v.token + hk * p.v.head + 8 * lc, on);
+      }
     }
-    if (p.documents != nullptr && tid < KB) rdoc = k0 + tid < n ? key_document(p, b, k0 + tid) : -1;
   };
-  if (end > 0) load(0);
-  for (int k0 = 0; k0 < end; k0 += KB) {
+  DocTile here{}, there{};
+  int t = walk.next(0, lane, here);
+  if (t < end) load(t, std::integral_constant<int, 0>{});
+  // one tile, in buffer B
+  auto step = [&](auto which) __attribute__((always_inline)) {
+    constexpr int B = which.value;
+    const KV kt{B == 0 ? k_lds0 : k_lds1}, vt{B == 0 ? v_lds0 : v_lds1};
+    if (by_document && PARTS == 1 && tid < KB) doc_lds[B][tid] = max(rdoc, -1);
+    if constexpr (PARTS == 1) copies_done();
     __syncthreads();
+    if constexpr (PARTS == 3) {
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      kt.put(lr + STEP * j, lc, frag(rk[j]));
-      vt.put(lr + STEP * j, lc, frag(rv[j]));
+      for (int j = 0; j < LOADS; ++j) {
+        kt.put(lr + STEP * j, lc, frag(rk[j]));
+        vt.put(lr + STEP * j, lc, frag(rv[j]));
+      }
+      if (by_document && tid < KB) doc_lds[0][tid] = max(rdoc, -1);
+      __syncthreads();
+    } else if (by_document && here.pad) {  // padding may hold anything: its rows become zeros
+      constexpr int each = 256 / KB;
+      const int r = tid / each;
+      if (doc_lds[B][r] < 0)
+        for (int ch = tid % each; ch < CH; ch += each) kt.put(r, ch, Frag<PARTS>{}), vt.put(r, ch, Frag<PARTS>{});
+      __syncthreads();
     }
-    if (p.documents != nullptr && tid < KB) doc_lds[tid] = rdoc;
-    __syncthreads();
-    if (k0 + KB < end) load(k0 + KB);
-    if (k0 > wave_last) continue;
-    const bool masked = p.documents != nullptr || k0 + KB - 1 > wave_first;
+    const int after = walk.next(t + 1, lane, there);
+    if (after < end) load(after, std::integral_constant<int, BUFS == 2 ? 1 - B : 0>{});
+    const int k0 = t * KB;
+    const bool unseen = k0 > wave_last || (by_document && (here.lo > wave_hi || here.hi < wave_lo));
+    if (!unseen) {
+      const bool mixed = by_document && !(one_document && here.lo == here.hi && here.lo == wave_lo && !here.pad);
+      const bool masked = mixed || k0 + KB - 1 > wave_first;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      v16f s = v16f{}, dp = v16f{};
+      for (int nb = 0; nb < NB; ++nb) {
+        v16f s = v16f{}, dp = v16f{};
 #pragma unroll
-      for (int ds = 0; ds < DP / 16; ++ds) {
-        s = mma(kt.rows(32 * nb, ds, lane), q[ds], s);
-        dp = mma(vt.rows(32 * nb, ds, lane), go[ds], dp);
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int r = 32 * nb + row_of(e, hh), key = k0 + r;
-        bool seen = true;
-        if (masked) {
-          seen = key <= me.last;
-          if (p.documents != nullptr) seen = seen && doc_lds[r] == me.doc;
+        for (int ds = 0; ds < DP / 16; ++ds) {
+          s = mma(kt.rows(32 * nb, ds, lane), q[ds], s);
+          dp = mma(vt.rows(32 * nb, ds, lane), go[ds], dp);
         }
-        float w, g;
-        pair<PARTS, CAP>(p, s[e], dp[e], slope2, abs(me.pos - key), lse2, delta, seen, w, g);
-        s[e] = g;
-      }
+        const int k1 = k0 + 32 * nb + 4 * hh;
+        const float away = static_cast<float>(me.pos - k1);
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const Frag<PARTS> g = frag_of<PARTS>(s, st);
+        for (int e = 0; e < 16; ++e) {
+          float w, g;
+          pair<PARTS, CAP>(p, s[e], dp[e], slope2, away - static_cast<float>(row_of(e, 0)), lse2, delta, w, g);
+          s[e] = g;
+        }
+        if (masked) {
+          const int last = me.last - k1;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[dt] = mma(kt.columns(32 * nb + 16 * st, dt, lane), g, acc[dt]);
+          for (int e = 0; e < 16; ++e) s[e] = row_of(e, 0) <= last ? s[e] : 0.f;
+          if (mixed) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int4 d = *reinterpret_cast<const int4*>(&doc_lds[B][32 * nb + 8 * e + 4 * hh]);
+              s[4 * e] = d.x == me.doc ? s[4 * e] : 0.f;
+              s[4 * e + 1] = d.y == me.doc ? s[4 * e + 1] : 0.f;
+              s[4 * e + 2] = d.z == me.doc ? s[4 * e + 2] : 0.f;
+              s[4 * e + 3] = d.w == me.doc ? s[4 * e + 3] : 0.f;
+            }
+          }
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const Frag<PARTS> g = frag_of<PARTS>(s, st);
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) acc[dt] = mma(kt.columns(32 * nb + 16 * st, dt, lane), g, acc[dt]);
+        }
       }
+    }
+    t = after;
+    here = there;
+  };
+  while (t < end) {
+    step(std::integral_constant<int, 0>{});
+    if constexpr (BUFS == 2) {
+      if (t < end) step(std::integral_constant<int, 1>{});
     }
   }
+  settle(acc);
   if (i >= p.Nq) return;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * dt + 8 * g + 4 * hh;
+    for (int x = 0; x < 4; ++x) {
+      const int d = 32 * dt + 8 * x + 4 * hh;
       if (d < p.D)
-        store_four<PARTS>(dq, at * p.D + d, acc[dt][4 * g] * p.scale, acc[dt][4 * g + 1] * p.scale,
-                          acc[dt][4 * g + 2] * p.scale, acc[dt][4 * g + 3] * p.scale);
+        store_four<PARTS>(dq, at * p.D + d, acc[dt][4 * x] * p.scale, acc[dt][4 * x + 1] * p.scale,
+                          acc[dt][4 * x + 2] * p.scale, acc[dt][4 * x + 3] * p.scale);
     }
 }
 
-template <int DP, int PARTS, bool CAP>
-__global__ void __launch_bounds__(kThreads) token_dkv_kernel(Params p, hz_token_tensor dout, const float* deltas, void* dk,
-                                                             void* dv) {
-  constexpr int QB = kRows<DP, PARTS>, NB = QB / 32, DT = DP / 32, CH = DP / 8;
-  constexpr int LOADS = QB * CH / kThreads, STEP = kThreads / CH;
+// WAVES = 8 (bfloat16): waves w and w + 4 own the same 32 keys and take the tile's first and second 32 queries;
+// their sums meet in LDS at the end. So two waves share a SIMD although a workgroup owns 128 keys only.
+template <int DP, int PARTS, bool CAP, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params p, hz_token_tensor dout, const float* deltas,
+                                                                          void* dk, void* dv, const DocTile* doc_tiles) {
+  constexpr int THREADS = 64 * WAVES, SETS = WAVES / 4;
+  constexpr int QB = kRows<DP, PARTS>, NB = QB / 32 / SETS, DT = DP / 32, CH = DP / 8;
+  constexpr int LOADS = QB * CH / THREADS, STEP = THREADS / CH;
+  constexpr int BUFS = PARTS == 1 ? 2 : 1;
   typedef Tile<QB, DP, PARTS> QT;
-  __shared__ __align__(16) uint16_t q_lds[QT::kPlane * PARTS], g_lds[QT::kPlane * PARTS];
-  __shared__ __align__(16) float lse_lds[QB], delta_lds[QB];
-  __shared__ __align__(16) int last_lds[QB], doc_lds[QB];
-  const QT qt{q_lds}, gt{g_lds};
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, hh = lane >> 5, c = lane & 31;
+  __shared__ __align__(16) uint16_t q_lds0[QT::kPlane * PARTS], g_lds0[QT::kPlane * PARTS];
+  __shared__ __align__(16) uint16_t q_lds1[PARTS == 1 ? QT::kPlane : 8], g_lds1[PARTS == 1 ? QT::kPlane : 8];
+  __shared__ __align__(16) float lse_lds[BUFS][QB], delta_lds[BUFS][QB];
+  __shared__ __align__(16) int doc_lds[BUFS][QB];
+  __shared__ uint64_t bad_lds[BUFS];
+  __shared__ int range_lds[4][2];
+  const int tid = threadIdx.x, wave = (tid >> 6) & 3, set = tid >> 8, lane = tid & 63, hh = lane >> 5, c = lane & 31;
   const int tiles = (p.Nk + kBlock - 1) / kBlock;
-  int64_t id = xcd_logical_block(blockIdx.x, gridDim.x);
-  const int hk = static_cast<int>(id % p.Hk);
-  id /= p.Hk;
+  int64_t id = xcd_run(blockIdx.x, gridDim.x);
   const int key0 = static_cast<int>(id % tiles) * kBlock;  // the first keys are seen by the most queries
-  const int b = static_cast<int>(id / tiles);
-  const int n = kv_length(p, b);
+  id /= tiles;
+  const int hk = static_cast<int>(id % p.Hk), b = static_cast<int>(id / p.Hk);
+  const int n = kv_length(p, b), shift = n - p.Nq;  // position of query 0
   const int wave0 = key0 + 32 * wave, key = wave0 + c, row = key < n ? key : max(n - 1, 0);
-  const int my_doc = p.documents != nullptr && key < n ? key_document(p, b, key) : -1;
+  const int prefix = p.causal && p.prefix != nullptr ? p.prefix[b] : 0;
+  const bool always = !p.causal || key < prefix;  // seen from every position, else from `key` on
+  const bool by_document = p.documents != nullptr;
+  const int my_doc = by_document && key < n ? key_document(p, b, key) : -1;
+  int wave_lo = 0, wave_hi = 0, lo = 0, hi = 0;
+  bool one_document = false;
+  if (by_document) {
+    document_range(my_doc, wave_lo, wave_hi);
+    one_document = wave_lo == wave_hi && !__any(my_doc < 0);
+    if (lane == 0) range_lds[wave][0] = wave_lo, range_lds[wave][1] = wave_hi;
+    __syncthreads();
+    lo = min(min(range_lds[0][0], range_lds[1][0]), min(range_lds[2][0], range_lds[3][0]));
+    hi = max(max(range_lds[0][1], range_lds[1][1]), max(range_lds[2][1], range_lds[3][1]));
+  }
 
   Frag<PARTS> k[DP / 16], v[DP / 16];
 #pragma unroll
@@ -187,117 +278,238 @@ __global__ void __launch_bounds__(kThreads) token_dkv_kernel(Params p, hz_token_
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) ak[dt] = v16f{}, av[dt] = v16f{};
 
-  // the first query that may see a key of this block
-  int begin = 0;
-  if (p.causal && key0 >= (p.prefix != nullptr ? p.prefix[b] : 0)) begin = max(0, key0 - (n - p.Nq));
-  begin = key0 < n ? begin / QB * QB : p.Nq;
+  // the tiles of queries that may see a key of this block
+  const int begin = p.causal && key0 >= prefix ? max(0, key0 - shift) / QB : 0;
+  const int end = key0 < n ? (p.Nq + QB - 1) / QB : 0;
+  const int doc_row = (p.Nk + kDocTile - 1) / kDocTile;
+  const DocTile* const row_tiles = doc_tiles + static_cast<int64_t>(b) * doc_row;
+  auto range = [row_tiles, shift, n](int t) {
+    // the tile's queries stand at 64 or fewer consecutive positions, which meet at most two tiles of keys
+    const int first = shift + t * QB, last = min(first + QB, n) - 1;
+    if (last < 0) return DocTile{2147483647, -1, 1, 0};
+    DocTile a = row_tiles[max(first, 0) / kDocTile];
+    const DocTile z = row_tiles[last / kDocTile];
+    return DocTile{min(a.lo, z.lo), max(a.hi, z.hi), a.pad | z.pad | (first < 0), 0};
+  };
+  Walk<decltype(range)> walk(begin, end, by_document, lo, hi, range);
   const int lr = tid / CH, lc = tid % CH;
-  Raw8<PARTS> rq[LOADS], rg[LOADS];
-  float rlse = 0.f, rdelta = 0.f;
-  int rlast = -1, rdoc = kNoDocument;
-  auto load = [&](int h, int q0) {
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int i = q0 + lr + STEP * j;
-      bool on = i < p.Nq && 8 * lc < p.D;
-      if (on) on = p.lse[(static_cast<int64_t>(b) * p.Nq + i) * p.H + h] != kNegInf;  // padding may hold anything
-      rq[j].load(p.q.data, b * p.q.batch + i * p.q.token + h * p.q.head + 8 * lc, on);
-      rg[j].load(dout.data, b * dout.batch + i * dout.token + h * dout.head + 8 * lc, on);
-    }
+  Raw8<PARTS> rq[PARTS == 3 ? LOADS : 1], rg[PARTS == 3 ? LOADS : 1];
+  float rlse = 0.f, rdelta = 0.f;  // as loaded: waited for where they are used
+  int rdoc = 0;
+  auto load = [&](int head, int t, auto to) __attribute__((always_inline)) {
+    const int h = hk * p.G + head, q0 = t * QB;
     if (tid < QB) {
-      const int i = q0 + tid;
-      rlse = 0.f, rdelta = 0.f, rlast = -1, rdoc = kNoDocument;
-      if (i < p.Nq) {
-        const int64_t at = (static_cast<int64_t>(b) * p.Nq + i) * p.H + h;
-        rlse = p.lse[at] * kLog2e;
-        if (rlse == kNegInf) rlse = 0.f;
-        rdelta = deltas[at];
-        const Sight s(p, b, i, n);
-        rlast = s.last;
-        rdoc = s.doc;
+      const int i = min(q0 + tid, p.Nq - 1);
+      const int64_t at = (static_cast<int64_t>(b) * p.Nq + i) * p.H + h;
+      rlse = q0 + tid < p.Nq ? p.lse[at] : kNegInf;
+      rdelta = deltas[at];
+      if (by_document) rdoc = shift + i >= 0 ? p.documents[static_cast<int64_t>(b) * p.Nk + shift + i] : -1;
+    }
+    if constexpr (PARTS == 1) {
+      if (set == 0) {
+        const Copy<QB, DP> copy(p.q, b, h, p.D, tid & 255);
+        copy(to.value == 0 ? q_lds0 : q_lds1, q0, p.Nq);
+      }
+      if (set == SETS - 1) {
+        const Copy<QB, DP> copy(dout, b, h, p.D, tid & 255);
+        copy(to.value == 0 ? g_lds0 : g_lds1, q0, p.Nq);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int i = q0 + lr + STEP * j;
+        bool on = i < p.Nq && 8 * lc < p.D;
+        if (on) on = p.lse[(static_cast<int64_t>(b) * p.Nq + i) * p.H + h] != kNegInf;  // padding may hold anything
+        rq[j].load(p.q.data, b * p.q.batch + i * p.q.token + h * p.q.head + 8 * lc, on);
+        rg[j].load(dout.data, b * dout.batch + i * dout.token + h * dout.head + 8 * lc, on);
       }
     }
   };
-  for (int g = 0; g < p.G; ++g) {
-    const int h = hk * p.G + g;
-    const float slope2 = p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
-    if (begin < p.Nq) load(h, begin);
-    for (int q0 = begin; q0 < p.Nq; q0 += QB) {
-      __syncthreads();
+  DocTile here{}, there{};
+  int head = 0, t = walk.next(begin, lane, here);
+  if (t < end) load(0, t, std::integral_constant<int, 0>{});
+  // one tile of one head, in buffer B
+  auto step = [&](auto which) __attribute__((always_inline)) {
+    constexpr int B = which.value;
+    const QT qt{B == 0 ? q_lds0 : q_lds1}, gt{B == 0 ? g_lds0 : g_lds1};
+    auto put_rows = [&] {
+      if (tid < QB) {
+        // a query that sees nothing, or is none: weights of 2^-inf
+        const bool bad = rlse == kNegInf;
+        const uint64_t votes = __ballot(bad);
+        lse_lds[B][tid] = bad ? -kNegInf : rlse * kLog2e;
+        delta_lds[B][tid] = bad ? 0.f : rdelta;
+        if (by_document) doc_lds[B][tid] = rdoc >= 0 ? rdoc : kNoDocument;
+        if (tid == 0) bad_lds[B] = votes;
+      }
+    };
+    if constexpr (PARTS == 1) {
+      put_rows();
+      copies_done();
+    }
+    __syncthreads();
+    if constexpr (PARTS == 3) {
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
         qt.put(lr + STEP * j, lc, frag(rq[j]));
         gt.put(lr + STEP * j, lc, frag(rg[j]));
       }
-      if (tid < QB) lse_lds[tid] = rlse, delta_lds[tid] = rdelta, last_lds[tid] = rlast, doc_lds[tid] = rdoc;
+      put_rows();
       __syncthreads();
-      if (q0 + QB < p.Nq) load(h, q0 + QB);
-      const int top = min(q0 + QB, p.Nq) - 1 - q0;
-      if (last_lds[top] < wave0) continue;  // no query of the tile sees a key of this wave
-      const bool masked = p.documents != nullptr || q0 + QB > p.Nq || last_lds[0] < wave0 + 31;
+    } else if (const uint64_t bad = bad_lds[B]; bad != 0) {  // such rows may hold anything: they become zeros
+      constexpr int each = THREADS / QB;
+      const int r = tid / each;
+      if ((bad >> r) & 1)
+        for (int ch = tid % each; ch < CH; ch += each) qt.put(r, ch, Frag<PARTS>{}), gt.put(r, ch, Frag<PARTS>{});
+      __syncthreads();
+    }
+    int after = walk.next(t + 1, lane, there), next_head = head;
+    if (after >= end && head + 1 < p.G) {
+      next_head = head + 1;
+      after = walk.next(begin, lane, there);
+    }
+    if (after < end) load(next_head, after, std::integral_constant<int, BUFS == 2 ? 1 - B : 0>{});
+    const int p0 = shift + t * QB;  // position of the tile's first query
+    const float slope2 = p.slopes != nullptr ? p.slopes[hk * p.G + head] * kLog2e : 0.f;
+    const bool unseen = (p.causal && wave0 >= prefix && p0 + QB - 1 < wave0) ||
+                        (by_document && (here.lo > wave_hi || here.hi < wave_lo));
+    if (!unseen) {
+      const bool mixed = by_document && !(one_document && here.lo == here.hi && here.lo == wave_lo && !here.pad);
+      const bool masked = mixed || wave0 + 31 >= n || (p.causal && wave0 + 31 >= prefix && p0 < wave0 + 31);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
+        const int r0 = 32 * (nb + (SETS == 2 ? set : 0));
         v16f s = v16f{}, dp = v16f{};
 #pragma unroll
         for (int ds = 0; ds < DP / 16; ++ds) {
-          s = mma(qt.rows(32 * nb, ds, lane), k[ds], s);
-          dp = mma(gt.rows(32 * nb, ds, lane), v[ds], dp);
+          s = mma(qt.rows(r0, ds, lane), k[ds], s);
+          dp = mma(gt.rows(r0, ds, lane), v[ds], dp);
         }
+        const int r1 = r0 + 4 * hh;
+        const float away = static_cast<float>(p0 + r1 - key);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int r = 32 * nb + row_of(e, hh);
-          bool seen = true;
-          if (masked) {
-            seen = key <= last_lds[r];
-            if (p.documents != nullptr) seen = seen && doc_lds[r] == my_doc;
+        for (int e = 0; e < 4; ++e) {
+          const v4f l = *reinterpret_cast<const v4f*>(&lse_lds[B][r1 + 8 * e]);
+          const v4f d = *reinterpret_cast<const v4f*>(&delta_lds[B][r1 + 8 * e]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float w, gs;
+            pair<PARTS, CAP>(p, s[4 * e + x], dp[4 * e + x], slope2, away + static_cast<float>(8 * e + x), l[x], d[x], w, gs);
+            s[4 * e + x] = w;
+            dp[4 * e + x] = gs;
           }
-          float w, gs;
-          pair<PARTS, CAP>(p, s[e], dp[e], slope2, abs(n - p.Nq + q0 + r - key), lse_lds[r], delta_lds[r], seen, w, gs);
-          s[e] = w;
-          dp[e] = gs;
+        }
+        if (masked) {
+          const int first = key >= n ? 32 : always ? 0 : key - p0 - r1;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const bool seen = row_of(e, 0) >= first;
+            s[e] = seen ? s[e] : 0.f;
+            dp[e] = seen ? dp[e] : 0.f;
+          }
+          if (mixed) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int4 d = *reinterpret_cast<const int4*>(&doc_lds[B][r1 + 8 * e]);
+              const bool seen[4] = {d.x == my_doc, d.y == my_doc, d.z == my_doc, d.w == my_doc};
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                s[4 * e + x] = seen[x] ? s[4 * e + x] : 0.f;
+                dp[4 * e + x] = seen[x] ? dp[4 * e + x] : 0.f;
+              }
+            }
+          }
         }
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
           const Frag<PARTS> w = frag_of<PARTS>(s, st), gs = frag_of<PARTS>(dp, st);
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            av[dt] = mma(gt.columns(32 * nb + 16 * st, dt, lane), w, av[dt]);
-            ak[dt] = mma(qt.columns(32 * nb + 16 * st, dt, lane), gs, ak[dt]);
+            av[dt] = mma(gt.columns(r0 + 16 * st, dt, lane), w, av[dt]);
+            ak[dt] = mma(qt.columns(r0 + 16 * st, dt, lane), gs, ak[dt]);
           }
         }
       }
     }
+    t = after;
+    head = next_head;
+    here = there;
+  };
+  while (t < end) {
+    step(std::integral_constant<int, 0>{});
+    if constexpr (BUFS == 2) {
+      if (t < end) step(std::integral_constant<int, 1>{});
+    }
+  }
+  settle(ak);
+  settle(av);
+  if constexpr (SETS == 2) {
+    // 16 accumulators a lane and round: 4 waves of 64 lanes fill the 16 DP KiB of one tile buffer's two halves
+    float* const to[2] = {reinterpret_cast<float*>(q_lds0), reinterpret_cast<float*>(g_lds0)};
+    constexpr int each = QT::kBytes / (4 * 64 * 16);  // quadruples a lane that one buffer holds
+    auto join = [&](v16f(&a)[DT]) {
+#pragma unroll
+      for (int r = 0; r < 4 * DT; r += 2 * each) {
+        __syncthreads();
+        if (set == 1) {
+#pragma unroll
+          for (int x = r; x < r + 2 * each && x < 4 * DT; ++x)
+            *reinterpret_cast<v4f*>(to[(x - r) / each] + (((x - r) % each * 4 + wave) * 64 + lane) * 4) =
+                v4f{a[x / 4][4 * (x % 4)], a[x / 4][4 * (x % 4) + 1], a[x / 4][4 * (x % 4) + 2], a[x / 4][4 * (x % 4) + 3]};
+        }
+        __syncthreads();
+        if (set == 0) {
+#pragma unroll
+          for (int x = r; x < r + 2 * each && x < 4 * DT; ++x) {
+            const v4f y = *reinterpret_cast<const v4f*>(to[(x - r) / each] + (((x - r) % each * 4 + wave) * 64 + lane) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[x / 4][4 * (x % 4) + e] += y[e];
+          }
+        }
+      }
+    };
+    join(ak);
+    join(av);
+    if (set == 1) return;
   }
   if (key >= p.Nk) return;
   const int64_t at = ((static_cast<int64_t>(b) * p.Nk + key) * p.Hk + hk) * p.D;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * dt + 8 * g + 4 * hh;
+    for (int x = 0; x < 4; ++x) {
+      const int d = 32 * dt + 8 * x + 4 * hh;
       if (d < p.D) {
-        store_four<PARTS>(dk, at + d, ak[dt][4 * g] * p.scale, ak[dt][4 * g + 1] * p.scale, ak[dt][4 * g + 2] * p.scale,
-                          ak[dt][4 * g + 3] * p.scale);
-        store_four<PARTS>(dv, at + d, av[dt][4 * g], av[dt][4 * g + 1], av[dt][4 * g + 2], av[dt][4 * g + 3]);
+        store_four<PARTS>(dk, at + d, ak[dt][4 * x] * p.scale, ak[dt][4 * x + 1] * p.scale, ak[dt][4 * x + 2] * p.scale,
+                          ak[dt][4 * x + 3] * p.scale);
+        store_four<PARTS>(dv, at + d, av[dt][4 * x], av[dt][4 * x + 1], av[dt][4 * x + 2], av[dt][4 * x + 3]);
       }
     }
+}
+
+int64_t delta_bytes(const hz_token_attention& a) {
+  return (a.B * a.Nq * a.H * static_cast<int64_t>(sizeof(float)) + 15) / 16 * 16;
 }
 
 template <int DP, int PARTS, bool CAP>
 hipError_t run(const hz_token_attention& a, const hz_token_tensor& dout, void* dq, void* dk, void* dv, void* workspace,
                hipStream_t stream) {
+  constexpr int WAVES = PARTS == 1 ? 8 : 4;
   const Params p = make_params(a);
   float* const deltas = static_cast<float*>(workspace);
+  DocTile* const tiles = reinterpret_cast<DocTile*>(static_cast<char*>(workspace) + delta_bytes(a));
+  if (p.documents != nullptr)
+    if (hipError_t err = launch_doc_tiles(p, tiles, stream); err != hipSuccess) return err;
   const int64_t nq = a.B * a.H * ((a.Nq + kBlock - 1) / kBlock), nk = a.B * a.Hk * ((a.Nk + kBlock - 1) / kBlock);
-  token_dq_kernel<DP, PARTS, CAP><<<static_cast<unsigned>(nq), kThreads, 0, stream>>>(p, dout, dq, deltas);
-  token_dkv_kernel<DP, PARTS, CAP><<<static_cast<unsigned>(nk), kThreads, 0, stream>>>(p, dout, deltas, dk, dv);
+  token_dq_kernel<DP, PARTS, CAP><<<static_cast<unsigned>(nq), 256, 0, stream>>>(p, dout, dq, deltas, tiles);
+  token_dkv_kernel<DP, PARTS, CAP, WAVES><<<static_cast<unsigned>(nk), 64 * WAVES, 0, stream>>>(p, dout, deltas, dk, dv, tiles);
   return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t token_attention_bwd_workspace(const hz_token_attention& a) {
-  return a.B * a.Nq * a.H * static_cast<int64_t>(sizeof(float));
+  return delta_bytes(a) + static_cast<int64_t>(doc_tiles_bytes(a));
 }
 
 hipError_t launch_token_attention_bwd(const hz_token_attention& a, const hz_token_tensor& dout, void* dq, void* dk,

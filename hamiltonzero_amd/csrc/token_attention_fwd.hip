@@ -1,14 +1,47 @@
 // Forward of the token attention (formulas and masks: include/hz_token.h; operand layouts:
 // token_device.h).
 //
-// Two kernels. Many queries: a workgroup of four waves owns 128 queries of a head, 32 a wave, and
-// streams the keys they can see through LDS in tiles of KB with the running maximum and sum of the
-// softmax; the next tile's loads are in flight during a tile's products. Few queries (at most 32 rows of
-// query and head share a key head): a wave owns a run of keys and all of those rows, so the
-// cache is read once, and a second kernel joins the runs.
+// Many queries: a workgroup of four waves owns 128 queries of a head, 32 a wave, and streams the keys they
+// can see through LDS in tiles of KB with the running maximum and sum of the softmax. bfloat16 tiles
+// are copied straight into one of two LDS buffers while the other is used; float32 ones pass through
+// registers, where they are split. Tiles that no query of the workgroup can see (behind the last visible key,
+// or of other documents) are not visited; a wave forms masks only in tiles where some pair is hidden. Where
+// there are few workgroups and many keys, the keys are divided and the parts joined by a second kernel.
+//
+// Few queries (at most 32 rows of query and head share a key head): a wave owns a run of keys and
+// all of those rows, so the cache is read once, and the same second kernel joins the runs.
 #include "token_device.h"
 
 namespace hz {
+namespace token {
+
+// One wave a tile of 64 keys.
+__global__ void __launch_bounds__(256) doc_tiles_kernel(Params p, DocTile* tiles, int per_row) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int b = static_cast<int>(id / per_row);
+  if (b >= p.B) return;
+  const int t = static_cast<int>(id - static_cast<int64_t>(b) * per_row), key = t * kDocTile + lane;
+  const int doc = key < kv_length(p, b) ? key_document(p, b, key) : -1;
+  int lo, hi;
+  document_range(doc, lo, hi);
+  const bool pad = __any(doc < 0);
+  if (lane == 0) tiles[id] = DocTile{lo, hi, pad, 0};
+}
+
+static int64_t doc_tiles_per_row(int64_t Nk) { return (Nk + kDocTile - 1) / kDocTile; }
+
+size_t doc_tiles_bytes(const hz_token_attention& a) {
+  return a.documents == nullptr ? 0 : static_cast<size_t>(a.B * doc_tiles_per_row(a.Nk)) * sizeof(DocTile);
+}
+
+hipError_t launch_doc_tiles(const Params& p, DocTile* tiles, hipStream_t stream) {
+  const int64_t per_row = doc_tiles_per_row(p.Nk), n = p.B * per_row;
+  doc_tiles_kernel<<<static_cast<unsigned>((n + 3) / 4), 256, 0, stream>>>(p, tiles, static_cast<int>(per_row));
+  return hipGetLastError();
+}
+
+}  // namespace token
 namespace {
 
 using namespace token;
@@ -25,82 +58,171 @@ struct Running {
   float m = kNegInf, l = 0.f;
 };
 
-// Scores of a 32-key block (first key k0) from their dot products, base 2, hidden ones -inf.
-// docs: the block's documents in LDS, or null.
-template <int PARTS, bool CAP>
-__device__ __forceinline__ void scores(v16f& s, const Params& p, const Sight& me, float slope2, int k0, int hh,
+// A score is a base-2 number s, or, where there is a cap and no distance bias, u = 1 / (1 + e^2y) with
+// s = cap2 - 2 cap2 u (tanh y = 1 - 2 u), so that the map to the exponent of 2 is one fused operation.
+// Hidden pairs are -inf, or u = +inf.
+template <int PARTS, bool CAP, bool U, int N>
+__device__ __forceinline__ void scores(v16f (&s)[N], const Params& p, const Sight& me, float slope2, int k0, int hh,
                                        bool masked, const int* docs) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float x = s[i];
-    if constexpr (CAP) x = tanh_of<PARTS>(x * p.to_tanh);
-    s[i] = x * p.to_score2;
-  }
-  if (slope2 != 0.f) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] -= slope2 * static_cast<float>(abs(me.pos - (k0 + row_of(i, hh))));
-  }
-  if (masked) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = k0 + row_of(i, hh) <= me.last ? s[i] : kNegInf;
-    if (docs != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = docs[row_of(i, hh)] == me.doc ? s[i] : kNegInf;
-    }
-  }
-}
-
-// Softmax weights of NB score blocks against the running maximum; returns the factor of what was
-// summed before.
-template <int NB>
-__device__ __forceinline__ float weigh(v16f (&s)[NB], Running& r) {
-  float top = kNegInf;
-#pragma unroll
-  for (int n = 0; n < NB; ++n)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
-  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-  top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-  const float m = fmaxf(r.m, top), base = m == kNegInf ? 0.f : m;  // nothing seen yet: weights of 2^-inf
-  const float alpha = fast_exp2(r.m - base);
-  float sum = 0.f;
-#pragma unroll
-  for (int n = 0; n < NB; ++n)
+  for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      s[n][i] = fast_exp2(s[n][i] - base);
-      sum += s[n][i];
+      if constexpr (U)
+        s[n][i] = __builtin_amdgcn_rcpf(1.f + fast_exp2(s[n][i] * p.to_exp2));
+      else if constexpr (CAP)
+        s[n][i] = tanh_of<PARTS>(s[n][i] * p.to_tanh) * p.to_score2;
+      else
+        s[n][i] *= p.to_score2;
     }
-  r.m = m;
-  r.l = r.l * alpha + sum;  // this half wave's keys; both halves' at the end
-  return alpha;
+  if (!U && slope2 != 0.f) {
+    const float at = static_cast<float>(me.pos - k0 - 4 * hh);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[n][i] -= slope2 * fabsf(at - static_cast<float>(32 * n + row_of(i, 0)));
+  }
+  constexpr float kHidden = U ? -kNegInf : kNegInf;
+  if (masked) {
+    const int last = me.last - k0 - 4 * hh;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[n][i] = 32 * n + row_of(i, 0) <= last ? s[n][i] : kHidden;
+    if (docs != nullptr) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int4 d = *reinterpret_cast<const int4*>(docs + 32 * n + 8 * g + 4 * hh);
+          s[n][4 * g] = d.x == me.doc ? s[n][4 * g] : kHidden;
+          s[n][4 * g + 1] = d.y == me.doc ? s[n][4 * g + 1] : kHidden;
+          s[n][4 * g + 2] = d.z == me.doc ? s[n][4 * g + 2] : kHidden;
+          s[n][4 * g + 3] = d.w == me.doc ? s[n][4 * g + 3] : kHidden;
+        }
+    }
+  }
 }
 
-template <int DP, int PARTS, bool CAP>
-__global__ void __launch_bounds__(kThreads) token_fwd_kernel(Params p) {
+// The base of a row's weights moves only when a tile's largest score passes it by more than 2^kLazy: weights
+// stay below 2^kLazy and most tiles need no rescaling of what was summed before. Where a reverse pass
+// follows, or the products are not what bounds the kernel, the base is the maximum itself: a row's largest weight
+// is then 1, which bfloat16 rounds exactly.
+constexpr float kLazy = 8.f;
+
+// Softmax weights of N score blocks; true (in every lane of the wave) if sums made before have to
+// be multiplied by alpha.
+template <bool U, int N>
+__device__ __forceinline__ bool weigh(v16f (&s)[N], const Params& p, Running& r, float lazy, float& alpha) {
+  float top = s[0][0];
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = U ? fminf(top, s[n][i]) : fmaxf(top, s[n][i]);
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+  top = U ? fminf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) : fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+  const float cap2 = p.to_score2;
+  if (U) top = cap2 - 2.f * cap2 * top;
+  const bool move = top > r.m + lazy || (r.m == kNegInf && top > r.m);
+  const bool any = __any(move);
+  if (any) {
+    const float m = move ? top : r.m;
+    alpha = r.m == kNegInf ? 0.f : fast_exp2(r.m - m);
+    r.m = m;
+    r.l *= alpha;
+  }
+  const float base = r.m == kNegInf ? 0.f : r.m;  // nothing seen yet: every weight is 2^-inf
+  const float a = U ? cap2 - base : -base;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[n][i] = fast_exp2(U ? a - 2.f * cap2 * s[n][i] : s[n][i] + a);
+  return any;
+}
+
+// The weights' sum, of the rounded ones where the products take rounded ones: numerator and denominator
+// of the mean then err together.
+__device__ __forceinline__ void add_weights(const Frag<1>& w, const v16f&, int, float& l) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 one = __builtin_bit_cast(bf16x2, 0x3f803f80u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t two = w.p[0][i];  // a copy: a bit cast of the vector's element reads its first one
+    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), one, l, false);
+  }
+}
+__device__ __forceinline__ void add_weights(const Frag<3>&, const v16f& s, int half, float& l) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) l += s[8 * half + i];
+}
+
+// Four consecutive outputs, and what their rounding left out where that is wanted.
+template <int PARTS>
+__device__ __forceinline__ void store_out(const Params& p, int64_t off, float a, float b, float c, float d) {
+  store_four<PARTS>(p.out, off, a, b, c, d);
+  if constexpr (PARTS == 1) {
+    if (p.out_low != nullptr) {
+      auto low = [](float x) { return x - bf16_to_f32(f32_to_bf16(x)); };
+      store_four<PARTS>(p.out_low, off, low(a), low(b), low(c), low(d));
+    }
+  }
+}
+
+// Divided keys: partial [rows of (b, i, h)][parts][D] sums and stats [..][parts][2] (base, sum).
+struct Parts {
+  float *partial, *stats;
+  int n;  // 1: not divided, the results go to out and lse
+};
+
+template <int DP, int PARTS, bool CAP, bool U>
+__global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel(Params p, const DocTile* doc_tiles, Parts parts) {
   constexpr int KB = kKeys<DP, PARTS>, NB = KB / 32, DT = DP / 32, CH = DP / 8;
-  constexpr int LOADS = KB * CH / kThreads;  // chunks a thread and tensor
-  constexpr int STEP = kThreads / CH;        // rows between a thread's chunks
+  constexpr int LOADS = KB * CH / kThreads, STEP = kThreads / CH;  // of the copies through registers
+  constexpr int BUFS = PARTS == 1 ? 2 : 1;
   typedef Tile<KB, DP, PARTS> KV;
-  __shared__ __align__(16) uint16_t k_lds[KV::kPlane * PARTS], v_lds[KV::kPlane * PARTS];
-  __shared__ int doc_lds[KB];
-  const KV kt{k_lds}, vt{v_lds};
+  // two buffers by name: the compiler has to see that a copy into one does not change what is read from the other
+  __shared__ __align__(16) uint16_t k_lds0[KV::kPlane * PARTS], v_lds0[KV::kPlane * PARTS];
+  __shared__ __align__(16) uint16_t k_lds1[PARTS == 1 ? KV::kPlane : 8], v_lds1[PARTS == 1 ? KV::kPlane : 8];
+  __shared__ __align__(16) int doc_lds[BUFS][KB];
+  __shared__ int range_lds[4][2];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, hh = lane >> 5, c = lane & 31;
   const int tiles = (p.Nq + kQB - 1) / kQB;
-  int64_t id = xcd_logical_block(blockIdx.x, gridDim.x);
-  const int h = static_cast<int>(id % p.H);
-  id /= p.H;
+  int64_t id = xcd_run(blockIdx.x, gridDim.x);
+  const int part = static_cast<int>(id % parts.n);
+  id /= parts.n;
+  const int g = static_cast<int>(id % p.G);
+  id /= p.G;
   const int q0 = static_cast<int>(tiles - 1 - id % tiles) * kQB;  // the longest rows of a causal mask first
-  const int b = static_cast<int>(id / tiles);
-  const int hk = h / p.G, n = kv_length(p, b);
+  id /= tiles;
+  const int hk = static_cast<int>(id % p.Hk), b = static_cast<int>(id / p.Hk), h = hk * p.G + g;
+  const int n = kv_length(p, b);
 
   const int i = q0 + 32 * wave + c, row = i < p.Nq ? i : p.Nq - 1;
   const Sight me(p, b, row, n);
   const float slope2 = p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
-  const int last_row = min(q0 + kQB, p.Nq) - 1;
-  const int end = Sight(p, b, last_row, n).last + 1;  // the last query sees the most keys
   const int wave_first = __builtin_amdgcn_readfirstlane(me.last);
-  const int wave_last = Sight(p, b, min(q0 + 32 * wave + 31, p.Nq - 1), n).last;
+  const int wave_last = __builtin_amdgcn_readlane(me.last, 31);
+  // keys that any query of the workgroup may see: the last query's
+  const int keys = Sight(p, b, min(q0 + kQB, p.Nq) - 1, n).last + 1;
+  int begin = 0, end = keys > 0 ? (keys + KB - 1) / KB : 0;
+  if (parts.n > 1) {
+    begin = static_cast<int>(static_cast<int64_t>(end) * part / parts.n);
+    end = static_cast<int>(static_cast<int64_t>(end) * (part + 1) / parts.n);
+  }
+  const bool by_document = p.documents != nullptr;
+  int wave_lo = 0, wave_hi = 0, lo = 0, hi = 0;
+  bool one_document = false;
+  if (by_document) {
+    document_range(me.doc, wave_lo, wave_hi);
+    one_document = wave_lo == wave_hi && !__any(me.doc < 0);
+    if (lane == 0) range_lds[wave][0] = wave_lo, range_lds[wave][1] = wave_hi;
+    __syncthreads();
+    lo = min(min(range_lds[0][0], range_lds[1][0]), min(range_lds[2][0], range_lds[3][0]));
+    hi = max(max(range_lds[0][1], range_lds[1][1]), max(range_lds[2][1], range_lds[3][1]));
+  }
+  const DocTile* const row_tiles = doc_tiles + static_cast<int64_t>(b) * ((p.Nk + kDocTile - 1) / kDocTile);
+  auto range = [row_tiles](int t) { return row_tiles[t * KB / kDocTile]; };
+  Walk<decltype(range)> walk(begin, end, by_document, lo, hi, range);
 
   Frag<PARTS> q[DP / 16];
 #pragma unroll
@@ -115,75 +237,130 @@ __global__ void __launch_bounds__(kThreads) token_fwd_kernel(Params p) {
   for (int dt = 0; dt < DT; ++dt) o[dt] = v16f{};
   Running run;
 
+  const Copy<KB, DP> copy_k(p.k, b, hk, p.D, tid), copy_v(p.v, b, hk, p.D, tid);
   const int lr = tid / CH, lc = tid % CH;
-  Raw8<PARTS> rk[LOADS], rv[LOADS];
-  int rdoc = -1;
-  auto load = [&](int k0) {
+  Raw8<PARTS> rk[PARTS == 3 ? LOADS : 1], rv[PARTS == 3 ? LOADS : 1];
+  int rdoc = -1;  // as loaded: waited for where it is used
+  auto load = [&](int t, auto to) __attribute__((always_inline)) {
+    const int k0 = t * KB;
+    if (by_document && tid < KB) rdoc = k0 + tid < n ? p.documents[static_cast<int64_t>(b) * p.Nk + k0 + tid] : -1;
+    if constexpr (PARTS == 1) {
+      copy_k(to.value == 0 ? k_lds0 : k_lds1, k0, n);
+      copy_v(to.value == 0 ? v_lds0 : v_lds1, k0, n);
+    } else {
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int key = k0 + lr + STEP * j;
-      bool on = key < n && 8 * lc < p.D;
-      rk[j].load(p.k.data, b * p.k.batch + key * p.k.token + hk * p.k.head + 8 * lc, on);
-      if (p.documents != nullptr && on) on = key_document(p, b, key) >= 0;  // padding may hold anything
-      rv[j].load(p.v.data, b * p.v.batch + key * p.v.token + hk * p.v.head + 8 * lc, on);
+      for (int j = 0; j < LOADS; ++j) {
+        const int key = k0 + lr + STEP * j;
+        bool on = key < n && 8 * lc < p.D;
+        rk[j].load(p.k.data, b * p.k.batch + key * p.k.token + hk * p.k.head + 8 * lc, on);
+        if (by_document && on) on = key_document(p, b, key) >= 0;  // padding may hold anything
+        rv[j].load(p.v.data, b * p.v.batch + key * p.v.token + hk * p.v.head + 8 * lc, on);
+      }
     }
-    if (p.documents != nullptr && tid < KB) rdoc = k0 + tid < n ? key_document(p, b, k0 + tid) : -1;
   };
-  if (end > 0) load(0);
-  for (int k0 = 0; k0 < end; k0 += KB) {
+  DocTile here{}, there{};
+  int t = walk.next(begin, lane, here);
+  if (t < end) load(t, std::integral_constant<int, 0>{});
+  // one tile, in buffer B
+  auto step = [&](auto which) __attribute__((always_inline)) {
+    constexpr int B = which.value;
+    const KV kt{B == 0 ? k_lds0 : k_lds1}, vt{B == 0 ? v_lds0 : v_lds1};
+    if (by_document && PARTS == 1 && tid < KB) doc_lds[B][tid] = max(rdoc, -1);
+    if constexpr (PARTS == 1) copies_done();
     __syncthreads();
+    if constexpr (PARTS == 3) {
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      kt.put(lr + STEP * j, lc, frag(rk[j]));
-      vt.put(lr + STEP * j, lc, frag(rv[j]));
+      for (int j = 0; j < LOADS; ++j) {
+        kt.put(lr + STEP * j, lc, frag(rk[j]));
+        vt.put(lr + STEP * j, lc, frag(rv[j]));
+      }
+      if (by_document && tid < KB) doc_lds[0][tid] = max(rdoc, -1);
+      __syncthreads();
+    } else if (by_document && here.pad) {  // padding may hold anything: its value rows become zeros
+      constexpr int each = kThreads / KB;
+      const int r = tid / each;
+      if (doc_lds[B][r] < 0)
+        for (int ch = tid % each; ch < CH; ch += each) vt.put(r, ch, Frag<PARTS>{});
+      __syncthreads();
     }
-    if (p.documents != nullptr && tid < KB) doc_lds[tid] = rdoc;
-    __syncthreads();
-    if (k0 + KB < end) load(k0 + KB);
-    if (k0 > wave_last) continue;  // no query of this wave sees the tile
-    v16f s[NB];
-    const bool masked = p.documents != nullptr || k0 + KB - 1 > wave_first;
+    const int after = walk.next(t + 1, lane, there);
+    if (after < end) load(after, std::integral_constant<int, BUFS == 2 ? 1 - B : 0>{});
+    const int k0 = t * KB;
+    const bool unseen = k0 > wave_last || (by_document && (here.lo > wave_hi || here.hi < wave_lo));
+    if (!unseen) {
+      // decided ahead of the products: see token_device.h on branches between a product and its first use
+      const bool mixed = by_document && !(one_document && here.lo == here.hi && here.lo == wave_lo && !here.pad);
+      const bool masked = mixed || k0 + KB - 1 > wave_first;
+      v16f s[NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      s[nb] = v16f{};
+      for (int nb = 0; nb < NB; ++nb) {
+        s[nb] = v16f{};
 #pragma unroll
-      for (int ds = 0; ds < DP / 16; ++ds) s[nb] = mma(kt.rows(32 * nb, ds, lane), q[ds], s[nb]);
-      scores<PARTS, CAP>(s[nb], p, me, slope2, k0 + 32 * nb, hh, masked, p.documents != nullptr ? doc_lds + 32 * nb : nullptr);
+        for (int ds = 0; ds < DP / 16; ++ds) s[nb] = mma(kt.rows(32 * nb, ds, lane), q[ds], s[nb]);
+      }
+      settle(s);
+      scores<PARTS, CAP, U>(s, p, me, slope2, k0, hh, masked, mixed ? doc_lds[B] : nullptr);
+      float alpha = 1.f;
+      if (weigh<U>(s, p, run, p.lse != nullptr ? 0.f : kLazy, alpha)) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+      }
+#pragma unroll
+      for (int st = 0; st < 2 * NB; ++st) {
+        const Frag<PARTS> w = frag_of<PARTS>(s[st / 2], st % 2);
+        add_weights(w, s[st / 2], st % 2, run.l);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = mma(vt.columns(16 * st, dt, lane), w, o[dt]);
+      }
     }
-    const float alpha = weigh<NB>(s, run);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-#pragma unroll
-    for (int st = 0; st < 2 * NB; ++st) {
-      const Frag<PARTS> w = frag_of<PARTS>(s[st / 2], st % 2);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] = mma(vt.columns(16 * st, dt, lane), w, o[dt]);
+    t = after;
+    here = there;
+  };
+  while (t < end) {
+    step(std::integral_constant<int, 0>{});
+    if constexpr (BUFS == 2) {
+      if (t < end) step(std::integral_constant<int, 1>{});
     }
   }
+  settle(o);
   const float l = xor32_pair_sum(run.l);
   if (i >= p.Nq) return;
   const int64_t at = (static_cast<int64_t>(b) * p.Nq + i) * p.H + h;
+  if (parts.n > 1) {
+    const int64_t to = at * parts.n + part;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int d = 32 * dt + 8 * x + 4 * hh;
+        if (d < p.D)
+          *reinterpret_cast<v4f*>(parts.partial + to * p.D + d) =
+              v4f{o[dt][4 * x], o[dt][4 * x + 1], o[dt][4 * x + 2], o[dt][4 * x + 3]};
+      }
+    if (hh == 0) parts.stats[to * 2] = run.m, parts.stats[to * 2 + 1] = l;
+    return;
+  }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * dt + 8 * g + 4 * hh;
+    for (int x = 0; x < 4; ++x) {
+      const int d = 32 * dt + 8 * x + 4 * hh;
       if (d < p.D)
-        store_four<PARTS>(p.out, at * p.D + d, o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv,
-                          o[dt][4 * g + 3] * inv);
+        store_out<PARTS>(p, at * p.D + d, o[dt][4 * x] * inv, o[dt][4 * x + 1] * inv, o[dt][4 * x + 2] * inv,
+                         o[dt][4 * x + 3] * inv);
     }
   if (p.lse != nullptr && hh == 0) p.lse[at] = l == 0.f ? kNegInf : (run.m + log2f(l)) * kLn2;
 }
 
 // Few queries: column pr of the products is query pr / G, head hk G + pr % G. Runs of `chunk` keys, one a
-// wave; partial [rows of (b, i, h)][runs][D] sums and stats [..][runs][2] (maximum, sum).
+// wave.
 template <int DP, int PARTS, bool CAP>
-__global__ void __launch_bounds__(kThreads) token_few_kernel(Params p, int chunk, int runs, float* partial, float* stats) {
+__global__ void __launch_bounds__(kThreads) token_few_kernel(Params p, int chunk, int runs, Parts parts) {
   constexpr int DT = DP / 32, CH = DP / 8, LOADS = 32 * CH / 64, STEP = 64 / CH;
   typedef Tile<32, DP, PARTS> V;
   __shared__ __align__(16) uint16_t v_lds[4][V::kPlane * PARTS];
-  __shared__ int doc_lds[4][32];
+  __shared__ __align__(16) int doc_lds[4][32];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, hh = lane >> 5, c = lane & 31;
   const V vt{v_lds[wave]};
   const int per = (runs + 3) / 4;
@@ -234,13 +411,17 @@ __global__ void __launch_bounds__(kThreads) token_few_kernel(Params p, int chunk
     v16f s[1] = {v16f{}};
 #pragma unroll
     for (int ds = 0; ds < DP / 16; ++ds) s[0] = mma(frag(rk[ds]), q[ds], s[0]);
-    scores<PARTS, CAP>(s[0], p, me, slope2, k0, hh, true, p.documents != nullptr ? doc_lds[wave] : nullptr);
-    const float alpha = weigh<1>(s, run);
+    settle(s);
+    scores<PARTS, CAP, false>(s, p, me, slope2, k0, hh, true, p.documents != nullptr ? doc_lds[wave] : nullptr);
+    float alpha = 1.f;
+    if (weigh<false>(s, p, run, 0.f, alpha)) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+    }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const Frag<PARTS> w = frag_of<PARTS>(s[0], st);
+      add_weights(w, s[0], st, run.l);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] = mma(vt.columns(16 * st, dt, lane), w, o[dt]);
     }
@@ -248,6 +429,7 @@ __global__ void __launch_bounds__(kThreads) token_few_kernel(Params p, int chunk
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
+  settle(o);
   const float l = xor32_pair_sum(run.l);
   if (c >= rows) return;
   const int64_t at = ((static_cast<int64_t>(b) * p.Nq + i) * p.H + h) * runs + run_id;
@@ -257,45 +439,44 @@ __global__ void __launch_bounds__(kThreads) token_few_kernel(Params p, int chunk
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * dt + 8 * g + 4 * hh;
       if (d < p.D)
-        *reinterpret_cast<v4f*>(partial + at * p.D + d) =
+        *reinterpret_cast<v4f*>(parts.partial + at * p.D + d) =
             v4f{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
     }
   if (hh == 0) {
-    stats[at * 2] = run.m;
-    stats[at * 2 + 1] = l;
+    parts.stats[at * 2] = run.m;
+    parts.stats[at * 2 + 1] = l;
   }
 }
 
-// Joins the runs of one row of (b, i, h): a workgroup of 64 threads a row.
+// Joins the parts of one row of (b, i, h), a wave a row. chunk: keys a part, of which those that begin behind the
+// row's end were not written; 0: all parts were.
 template <int PARTS>
-__global__ void __launch_bounds__(64) token_join_kernel(Params p, int chunk, int runs, const float* partial,
-                                                        const float* stats) {
-  const int64_t at = blockIdx.x;
-  const int b = static_cast<int>(at / (static_cast<int64_t>(p.Nq) * p.H)), lane = threadIdx.x;
-  const int used = (kv_length(p, b) + chunk - 1) / chunk;
-  const float* const st = stats + at * runs * 2;
+__global__ void __launch_bounds__(kThreads) token_join_kernel(Params p, int chunk, Parts parts) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (at >= static_cast<int64_t>(p.B) * p.Nq * p.H) return;
+  const int b = static_cast<int>(at / (static_cast<int64_t>(p.Nq) * p.H)), lane = threadIdx.x & 63;
+  const int used = chunk > 0 ? (kv_length(p, b) + chunk - 1) / chunk : parts.n;
+  const float* const st = parts.stats + at * parts.n * 2;
   float m = kNegInf;
   for (int r = lane; r < used; r += 64) m = fmaxf(m, st[2 * r]);
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
   const float base = m == kNegInf ? 0.f : m;
-  float l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int r = 0; r < used; ++r) {
+  // four elements a lane, two half waves on parts of their own
+  const int d = 4 * (lane & 31), half = lane >> 5;
+  float l = 0.f;
+  v4f o = zero4();
+#pragma unroll 4
+  for (int r = half; r < used; r += 2) {
     const float a = fast_exp2(st[2 * r] - base);
     l += a * st[2 * r + 1];
-    const float* const o = partial + (at * runs + r) * p.D;
-    if (2 * lane < p.D) {
-      o0 += a * o[2 * lane];
-      o1 += a * o[2 * lane + 1];
-    }
+    if (d < p.D) o += a * *reinterpret_cast<const v4f*>(parts.partial + (at * parts.n + r) * p.D + d);
   }
+  l = xor32_pair_sum(l);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) o[x] = xor32_pair_sum(o[x]);
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  if (2 * lane < p.D) {
-    if constexpr (PARTS == 1)
-      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + at * p.D + 2 * lane) = pack2_bf16(o0 * inv, o1 * inv);
-    else
-      *reinterpret_cast<float2*>(static_cast<float*>(p.out) + at * p.D + 2 * lane) = make_float2(o0 * inv, o1 * inv);
-  }
+  if (half == 0 && d < p.D) store_out<PARTS>(p, at * p.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
   if (p.lse != nullptr && lane == 0) p.lse[at] = l == 0.f ? kNegInf : (m + log2f(l)) * kLn2;
 }
 
@@ -307,33 +488,55 @@ int run_keys(const hz_token_attention& a) {
   const int64_t keys = (a.B * a.Hk * a.Nk + 8191) / 8192;
   return static_cast<int>((keys + 31) / 32 * 32);
 }
-int runs_of(const hz_token_attention& a) {
-  const int c = run_keys(a);
-  return static_cast<int>((a.Nk + c - 1) / c);
+
+int64_t blocks_of(const hz_token_attention& a) { return a.B * a.H * ((a.Nq + kQB - 1) / kQB); }
+
+// Parts of a row's keys. Many queries: as many as 512 workgroups (two a CU) want, each of at least 512 keys.
+int parts_of(const hz_token_attention& a) {
+  if (few(a)) {
+    const int c = run_keys(a);
+    return static_cast<int>((a.Nk + c - 1) / c);
+  }
+  const int64_t want = 512 / blocks_of(a), most = a.Nk / 512, n = want < most ? want : most;
+  return static_cast<int>(n > 1 ? n : 1);
+}
+
+int64_t parts_bytes(const hz_token_attention& a) {
+  const int n = parts_of(a);
+  return few(a) || n > 1 ? a.B * a.Nq * a.H * n * (a.D + 2) * static_cast<int64_t>(sizeof(float)) : 0;
 }
 
 template <int DP, int PARTS, bool CAP>
 hipError_t run(const hz_token_attention& a, void* workspace, hipStream_t stream) {
   const Params p = make_params(a);
-  if (!few(a)) {
-    const int64_t grid = a.B * a.H * ((a.Nq + kQB - 1) / kQB);
-    token_fwd_kernel<DP, PARTS, CAP><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
-    return hipGetLastError();
+  const int64_t rows = a.B * a.Nq * a.H;
+  Parts parts{static_cast<float*>(workspace), nullptr, parts_of(a)};
+  parts.stats = parts.partial + rows * parts.n * a.D;
+  int chunk = 0;
+  if (few(a)) {
+    chunk = run_keys(a);
+    token_few_kernel<DP, PARTS, CAP><<<static_cast<unsigned>(a.B * a.Hk * ((parts.n + 3) / 4)), kThreads, 0, stream>>>(
+        p, chunk, parts.n, parts);
+  } else {
+    DocTile* const tiles = reinterpret_cast<DocTile*>(static_cast<char*>(workspace) + (parts_bytes(a) + 15) / 16 * 16);
+    if (p.documents != nullptr)
+      if (hipError_t err = launch_doc_tiles(p, tiles, stream); err != hipSuccess) return err;
+    const unsigned grid = static_cast<unsigned>(blocks_of(a) * parts.n);
+    if (CAP && PARTS == 1 && p.slopes == nullptr)
+      token_fwd_kernel<DP, PARTS, CAP, CAP && PARTS == 1><<<grid, kThreads, 0, stream>>>(p, tiles, parts);
+    else
+      token_fwd_kernel<DP, PARTS, CAP, false><<<grid, kThreads, 0, stream>>>(p, tiles, parts);
+    if (parts.n == 1) return hipGetLastError();
   }
-  const int chunk = run_keys(a), runs = runs_of(a);
-  float* const partial = static_cast<float*>(workspace);
-  float* const stats = partial + a.B * a.Nq * a.H * runs * a.D;
-  token_few_kernel<DP, PARTS, CAP><<<static_cast<unsigned>(a.B * a.Hk * ((runs + 3) / 4)), kThreads, 0, stream>>>(
-      p, chunk, runs, partial, stats);
-  token_join_kernel<PARTS><<<static_cast<unsigned>(a.B * a.Nq * a.H), 64, 0, stream>>>(p, chunk, runs, partial, stats);
+  token_join_kernel<PARTS><<<static_cast<unsigned>((rows + 3) / 4), kThreads, 0, stream>>>(p, chunk, parts);
   return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t token_attention_fwd_workspace(const hz_token_attention& a) {
-  if (!few(a)) return 0;
-  return a.B * a.Nq * a.H * runs_of(a) * (a.D + 2) * static_cast<int64_t>(sizeof(float));
+  const int64_t parts = (parts_bytes(a) + 15) / 16 * 16;
+  return few(a) ? parts : parts + static_cast<int64_t>(doc_tiles_bytes(a));
 }
 
 hipError_t launch_token_attention_fwd(const hz_token_attention& a, void* workspace, hipStream_t stream) {

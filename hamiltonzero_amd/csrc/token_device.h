@@ -27,7 +27,7 @@ constexpr float kNegInf = -__builtin_inff();
 
 struct Params {
   hz_token_tensor q, k, v;
-  void* out;
+  void *out, *out_low;
   float* lse;
   const float* slopes;
   const int32_t *prefix, *documents, *kv_len;
@@ -35,17 +35,19 @@ struct Params {
   float scale;      // of the dot products
   float cap;        // 0: not capped
   float to_tanh;    // scale / cap
+  float to_exp2;    // 2 log2 e scale / cap: e^2y = 2^(this x)
   float to_score2;  // base-2 score of a dot product (scale log2 e) or of a tanh (cap log2 e)
 };
 
 inline Params make_params(const hz_token_attention& a) {
   Params p{};
-  p.q = a.q, p.k = a.k, p.v = a.v, p.out = a.out, p.lse = a.lse;
+  p.q = a.q, p.k = a.k, p.v = a.v, p.out = a.out, p.out_low = a.out_low, p.lse = a.lse;
   p.slopes = a.slopes, p.prefix = a.prefix, p.documents = a.documents, p.kv_len = a.kv_len;
   p.B = static_cast<int>(a.B), p.Nq = static_cast<int>(a.Nq), p.Nk = static_cast<int>(a.Nk);
   p.H = static_cast<int>(a.H), p.Hk = static_cast<int>(a.Hk), p.G = p.H / p.Hk, p.D = static_cast<int>(a.D);
   p.causal = a.causal, p.scale = a.scale, p.cap = a.softcap;
   p.to_tanh = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+  p.to_exp2 = 2.f * kLog2e * p.to_tanh;
   p.to_score2 = (a.softcap > 0.f ? a.softcap : a.scale) * kLog2e;
   return p;
 }
@@ -119,6 +121,19 @@ __device__ __forceinline__ v16f mma(const Frag<3>& a, const Frag<3>& b, v16f c) 
   return c;
 }
 
+// Products are waited for here, before any branch: a vector instruction may read a product's result only some
+// wait states after it, and where paths of different lengths lead from one to the other the compiler
+// (ROCm 7.2's) counts them on one path only. Twenty wait states are more than the twelve that the 32 x 32 x 16
+// product needs.
+template <int N>
+__device__ __forceinline__ void settle(v16f (&x)[N]) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 3");
+#pragma unroll
+  for (int n = 0; n < N; ++n) asm volatile("" : "+v"(x[n]));
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // A tile of ROWS rows of DP elements in LDS, PARTS planes.
 template <int ROWS, int DP, int PARTS>
 struct Tile {
@@ -139,7 +154,7 @@ struct Tile {
   }
   // A operand of a product over the columns: lane (hh, c) gets row row0 + c, elements 16 s + 8 hh .. + 7.
   __device__ __forceinline__ Frag<PARTS> rows(int row0, int s, int lane) const {
-    const int o = at(row0 + (lane & 31), 2 * s + (lane >> 5));
+    const int o = at(row0 + (lane & 31), lane >> 5) ^ (s << 4);  // chunk 2 s + hh: s flips bits above hh's
     Frag<PARTS> f;
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) f.p[i] = *reinterpret_cast<const v4u*>(base + i * kPlane + o);
@@ -152,8 +167,8 @@ struct Tile {
   __device__ __forceinline__ Frag<PARTS> columns(int row0, int dt, int lane) const {
     typedef short v4s __attribute__((ext_vector_type(4)));
     const int g = lane >> 4, m = lane & 15, row = row0 + 4 * (g >> 1) + (m >> 2);
-    const int chunk = 4 * dt + 2 * (g & 1) + ((m & 3) >> 1), half = 4 * (m & 1);
-    const int o0 = at(row, chunk) + half, o1 = at(row + 8, chunk) + half;
+    const int o0 = (at(row, 2 * (g & 1) + ((m & 3) >> 1)) ^ (dt << 5)) + 4 * (m & 1);  // chunk 4 dt + ..
+    const int o1 = (o0 ^ 16) + 8 * DP;  // eight rows on, the swizzle differs in one bit
     Frag<PARTS> f;
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
@@ -211,6 +226,97 @@ __device__ __forceinline__ int key_document(const Params& p, int b, int j) {
   return d >= 0 ? d : -1;
 }
 
+// Documents of 64 consecutive keys: the smallest and largest number among them (lo > hi: none), and
+// whether any of the 64 is padding or behind the row's end.
+struct DocTile {
+  int lo, hi, pad, unused;
+};
+constexpr int kDocTile = 64;
+
+// The blocks of one kernel in an order that gives each of the 8 XCDs (their L2 caches) a consecutive run.
+__device__ __forceinline__ int64_t xcd_run(int64_t hw, int64_t n) {
+  const int64_t x = hw % 8, each = n / 8, more = n % 8;
+  return x * each + (x < more ? x : more) + hw / 8;
+}
+
+// Copies rows of a strided tensor straight into a Tile of bfloat16 (16 bytes a lane, no registers): what a lane
+// reads is chosen so that lane i's 16 bytes land where the tile wants them. Rows behind the last one
+// repeat it and chunks behind D repeat the first: finite, and multiplied by zeros.
+template <int ROWS, int DP>
+struct Copy {
+  static constexpr int CH = DP / 8, LOADS = ROWS * CH / 256;
+  const uint16_t* base;
+  int64_t token;
+  int row, wave;  // this lane's row in the first of LOADS parts; STEP rows between parts
+  static constexpr int STEP = 256 / CH;
+  __device__ __forceinline__ Copy(const hz_token_tensor& t, int64_t b, int64_t h, int D, int tid) {
+    row = tid / CH;
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int chunk = (tid % CH) ^ Tile<ROWS, DP, 1>::swizzle(row);
+    base = static_cast<const uint16_t*>(t.data) + b * t.batch + h * t.head + (8 * chunk < D ? 8 * chunk : 0);
+    token = t.token;
+  }
+  __device__ __forceinline__ void operator()(uint16_t* lds, int r0, int rows) const {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const uint16_t* const src = base + static_cast<int64_t>(min(r0 + row + STEP * j, rows - 1)) * token;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                       (__attribute__((address_space(3))) void*)(lds + (4 * j + wave) * 512), 16, 0, 0);
+    }
+  }
+};
+// The copies issued so far have landed in LDS for every wave that passes the barrier behind this.
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// The tiles of KB rows that a block has to visit, in order: all of [begin, end), or with documents those
+// whose range of numbers meets the block's. One load and one vote decide 64 tiles.
+template <class Range>
+struct Walk {
+  int begin, end, group;
+  uint64_t votes;
+  DocTile mine;
+  bool by_document;
+  Range range;  // tile index -> DocTile
+  int lo, hi;
+  __device__ __forceinline__ Walk(int begin_, int end_, bool by_document_, int lo_, int hi_, Range range_)
+      : begin(begin_), end(end_), group(-1), votes(0), mine{}, by_document(by_document_), range(range_), lo(lo_), hi(hi_) {}
+  // The first tile >= t to visit (end: none), and its documents.
+  __device__ __forceinline__ int next(int t, int lane, DocTile& doc) {
+    if (!by_document) return t;
+    while (t < end) {
+      const int g = t & ~63;
+      if (g != group) {
+        group = g;
+        mine = DocTile{2147483647, -1, 1, 0};
+        if (g + lane < end) mine = range(g + lane);
+        votes = __ballot(mine.lo <= hi && mine.hi >= lo);
+      }
+      const uint64_t rest = votes >> (t - g);
+      if (rest != 0) {
+        t += __ffsll(static_cast<unsigned long long>(rest)) - 1;
+        if (t >= end) return end;
+        doc.lo = __builtin_amdgcn_readlane(mine.lo, t - g);
+        doc.hi = __builtin_amdgcn_readlane(mine.hi, t - g);
+        doc.pad = __builtin_amdgcn_readlane(mine.pad, t - g);
+        return t;
+      }
+      t = g + 64;
+    }
+    return end;
+  }
+};
+
+// Smallest and largest document of a wave's queries; lo > hi if it has none.
+__device__ __forceinline__ void document_range(int doc, int& lo, int& hi) {
+  lo = doc >= 0 ? doc : 2147483647;
+  hi = doc >= 0 ? doc : -1;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    lo = min(lo, __shfl_xor(lo, x, 64));
+    hi = max(hi, __shfl_xor(hi, x, 64));
+  }
+}
+
 // Four consecutive elements in the tensor's type.
 template <int PARTS>
 __device__ __forceinline__ void store_four(void* out, int64_t off, float a, float b, float c, float d) {
@@ -219,6 +325,10 @@ __device__ __forceinline__ void store_four(void* out, int64_t off, float a, floa
   else
     store4<F32>(out, off, a, b, c, d);
 }
+
+// Launch of the pass over the documents (token_attention_fwd.hip), where a call has some.
+size_t doc_tiles_bytes(const hz_token_attention& a);
+hipError_t launch_doc_tiles(const Params& p, DocTile* tiles, hipStream_t stream);
 
 }  // namespace token
 }  // namespace hz

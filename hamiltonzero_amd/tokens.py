@@ -196,47 +196,50 @@ def qk_norm_rotary(
 # --- attention ------------------------------------------------------------------------------------
 
 
-def _attention_args(q, k, v, out, lse, opts) -> bytes:
+def _attention_args(q, k, v, out, out_low, lse, opts) -> bytes:
     slopes, prefix, documents, kv_len, scale, softcap, causal = opts
     B, Nq, H, D = q.shape
     return _native.TOKEN_ATTENTION.pack(
-        *_fields(q), *_fields(k), *_fields(v), out.data_ptr(), _ptr(lse), _ptr(slopes), _ptr(prefix), _ptr(documents),
-        _ptr(kv_len), B, Nq, k.shape[1], H, k.shape[2], D, scale, softcap, causal, _DTYPES[q.dtype])
+        *_fields(q), *_fields(k), *_fields(v), out.data_ptr(), _ptr(out_low), _ptr(lse), _ptr(slopes), _ptr(prefix),
+        _ptr(documents), _ptr(kv_len), B, Nq, k.shape[1], H, k.shape[2], D, scale, softcap, causal, _DTYPES[q.dtype])
 
 
-def token_attention_fwd(q: Tensor, k: Tensor, v: Tensor, opts: tuple, with_lse: bool) -> Tuple[Tensor, Optional[Tensor]]:
-    """The forward call with checked operands: ``(out, lse)``."""
+def token_attention_fwd(q: Tensor, k: Tensor, v: Tensor, opts: tuple,
+                        for_backward: bool) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
+    """The forward call with checked operands: ``(out, out_low, lse)``, the last two what the reverse pass
+    needs besides (``out_low``, what the rounding of ``out`` left out, for bfloat16 only)."""
     q, k, v = _strided(q), _strided(k), _strided(v)
     dev = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if with_lse else None
-    args = _attention_args(q, k, v, out, lse, opts)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if for_backward else None
+    out_low = torch.empty_like(out) if for_backward and q.dtype == torch.bfloat16 else None
+    args = _attention_args(q, k, v, out, out_low, lse, opts)
     lib = _native.lib()
     with _on(dev):
         size = lib.hz_token_attention_fwd_workspace(args)
         work = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
         _native.check(lib.hz_token_attention_fwd(_stream(dev), args, _ptr(work), size))
-    return out, lse
+    return out, out_low, lse
 
 
 class _TokenAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, opts):
-        out, lse = token_attention_fwd(q, k, v, opts, True)
-        ctx.save_for_backward(q, k, v, out, lse, *opts[:4])
+        out, out_low, lse = token_attention_fwd(q, k, v, opts, True)
+        ctx.save_for_backward(q, k, v, out, out_low, lse, *opts[:4])
         ctx.options = opts[4:]
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, *tables = ctx.saved_tensors
+        q, k, v, out, out_low, lse, *tables = ctx.saved_tensors
         q, k, v, dout = _strided(q), _strided(k), _strided(v), _strided(dout)
         dev = q.device
         dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
         dk = torch.empty(k.shape, dtype=q.dtype, device=dev)
         dv = torch.empty(v.shape, dtype=q.dtype, device=dev)
-        args = _attention_args(q, k, v, out, lse, (*tables, *ctx.options))
+        args = _attention_args(q, k, v, out, out_low, lse, (*tables, *ctx.options))
         lib = _native.lib()
         with _on(dev):
             size = lib.hz_token_attention_bwd_workspace(args)

@@ -90,13 +90,16 @@ int hz_qk_norm_rotary_bwd(hipStream_t stream, const hz_qk_norm_rotary* p, void* 
  * forward without a reverse pass). slopes [H] float32, prefix [B], documents [B, Nk] and kv_len [B]
  * int32. D a multiple of 8 up to HZ_TOKEN_MAX_HEAD, H a multiple of Hk, Nq, Nk < 2^30; prefix only
  * with causal.
+ * out_low [B, Nq, H, D] or NULL, for bfloat16: what out's rounding left out, rounded to bfloat16. The
+ * reverse pass takes rowsum(dout out) from both where it is given: from out alone the row sum's error is as large
+ * as that of all other roundings of dq and dk together.
  * The weights of the products with v and the score gradients are rounded to bfloat16 for bfloat16
- * tensors; for float32 ones every product keeps float32's precision (three bfloat16 parts an operand,
+ * tensors (and the rounded weights are summed); for float32 ones every product keeps float32's precision (three bfloat16 parts an operand,
  * split_f32.h, whose remarks on values that are not finite or above 3.39e38 hold).
  */
 typedef struct {
   hz_token_tensor q, k, v;
-  void* out;
+  void *out, *out_low;
   float* lse;
   const float* slopes;
   const int32_t *prefix, *documents, *kv_len;

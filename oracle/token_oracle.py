@@ -3,7 +3,9 @@ rounds as documented may be off by.
 
 Rounding model of :func:`attention`: a rounding to a type of significand eps is off by at most eps / 2
 relative, ``u = 2^-24`` (float32) or ``2^-8`` (bfloat16); weights and score gradients go into their products
-rounded to bfloat16 (``2^-8``) for bfloat16 tensors and in three parts (``2^-23``) for float32 ones; a sum of n
+rounded to bfloat16 (``2^-8``) for bfloat16 tensors and in three parts (``2^-23``) for float32 ones; the rounded
+weights are also what is summed, so with w' = w (1 + d), |d| <= up, the mean's error is at most up (sum of P |v| +
+|out|), log of the sum's is at most up (1 + up), and so is the relative error of a P rebuilt from it; a sum of n
 float32 terms in steps of sixteen, six products each, is off by at most ``(6 n / 16 + 16) 2^-24`` of the sum of
 their magnitudes.
 """
@@ -101,10 +103,10 @@ def attention(q, k, v, *, scale, softcap=0.0, slopes=None, causal=False, prefix=
             lse = (m + np.log(np.where(z == 0, 1, z)))[:, 0]
             rho = (2 * np.where(seen, es, 0).max(1, initial=0) + _sum_error(Nk) + 8 * F)[:, None]
             out = w @ vh
-            t_out = (rho + up) * (w @ np.abs(vh)) + u * np.abs(out)
+            t_out = (rho + up) * (w @ np.abs(vh)) + (up + u) * np.abs(out)
             r["out"][b, :, h], r["t_out"][b, :, h] = out, t_out
             r["lse"][b, :, h] = np.where(some, lse, -np.inf)
-            r["t_lse"][b, :, h] = rho[:, 0] + 4 * F * (np.abs(lse) + 1)
+            r["t_lse"][b, :, h] = up * (1 + up) + rho[:, 0] + 4 * F * (np.abs(lse) + 1)
             if dout is None:
                 continue
             go = np.where(some[:, None], dout[b, :, h], 0)
@@ -112,7 +114,7 @@ def attention(q, k, v, *, scale, softcap=0.0, slopes=None, causal=False, prefix=
             delta = (go * out).sum(1, keepdims=True)
             e_dp = _sum_error(D) * np.abs(go) @ np.abs(vh).T
             e_delta = (np.abs(go) * (t_out + D * F * np.abs(out))).sum(1, keepdims=True)
-            rho2 = 2 * rho + 8 * F * (np.abs(lse)[:, None] + 2)
+            rho2 = up * (1 + up) + 2 * rho + 8 * F * (np.abs(lse)[:, None] + 2)
             cap = 1 - t * t if softcap else np.ones_like(t)
             ds = w * (dp - delta) * cap
             e_ds = rho2 * np.abs(ds) + w * (e_dp + e_delta) * cap + w * np.abs(dp - delta) * 32 * F

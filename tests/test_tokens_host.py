@@ -116,7 +116,7 @@ def _norm(**over):
 
 
 def _attn(**over):
-    f = dict(q=(A, 8192, 512, 64), k=(A, 8192, 512, 64), v=(A, 8192, 512, 64), out=A, lse=A, slopes=0, prefix=0, documents=0,
+    f = dict(q=(A, 8192, 512, 64), k=(A, 8192, 512, 64), v=(A, 8192, 512, 64), out=A, out_low=0, lse=A, slopes=0, prefix=0, documents=0,
              kv_len=0, B=2, Nq=16, Nk=16, H=8, Hk=8, D=64, scale=0.125, softcap=0.0, causal=1, dtype=0)
     f.update(over)
     flat = [x for v in f.values() for x in (v if isinstance(v, tuple) else (v,))]
@@ -162,7 +162,7 @@ def test_norm_backward_refuses(lib):
     (dict(causal=0, prefix=A), E.HZ_EINVAL, "prefix needs causal"), (dict(prefix=A + 2), E.HZ_EALIGN, "prefix"),
     (dict(documents=A + 1), E.HZ_EALIGN, "documents"), (dict(kv_len=A + 1), E.HZ_EALIGN, "kv_len"),
     (dict(slopes=A + 2), E.HZ_EALIGN, "slopes"), (dict(lse=A + 2), E.HZ_EALIGN, "lse"), (dict(out=0), E.HZ_ENULL, "out"),
-    (dict(out=A + 4), E.HZ_EALIGN, "out"), (dict(v=(0, 0, 0, 0)), E.HZ_ENULL, "v must"),
+    (dict(out=A + 4), E.HZ_EALIGN, "out"), (dict(out_low=A + 8), E.HZ_EALIGN, "out_low"), (dict(v=(0, 0, 0, 0)), E.HZ_ENULL, "v must"),
     (dict(k=(A, 0, 12, 0)), E.HZ_EINVAL, "k: strides"), (dict(q=(A + 4, 0, 0, 0)), E.HZ_EALIGN, "q must"),
 ])
 def test_attention_refuses(lib, over, code, needle):
