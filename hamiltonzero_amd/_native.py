@@ -159,8 +159,8 @@ _SIGNATURES = {
     "hz_token_attention_bwd": ([_P, _S, _S] + [_P] * 4 + [_I64], _INT),
     # stream, table, buckets, q_positions, k_positions, e, B, Nq, Nk, H, n_buckets, R, dtype, flags
     "hz_bucket_bias_fwd": ([_P] * 6 + [_I64] * 6 + [_INT, _INT], _INT),
-    # B, Nq, Nk, H, n_buckets, flags
-    "hz_bucket_bias_workspace": ([_I64] * 5 + [_INT], _I64),
+    # B, Nq, Nk, H, n_buckets, dtype, flags
+    "hz_bucket_bias_workspace": ([_I64] * 5 + [_INT, _INT], _I64),
     # stream, de, buckets, q_positions, k_positions, dtable, workspace, workspace_bytes, B, Nq, Nk, H,
     # n_buckets, R, dtype, flags
     "hz_bucket_bias_bwd": ([_P] * 7 + [_I64] * 7 + [_INT, _INT], _INT),

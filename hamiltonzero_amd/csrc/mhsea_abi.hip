@@ -321,8 +321,9 @@ int check_bucket_bias(int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t nb, 
     return fail(HZ_EINVAL, "R must be in [0, %d], got %lld", HZ_BUCKET_MAX_RANGE, (long long)R);
   if ((nb + 1) * ((H + 63) / 64 * 64) > HZ_BUCKET_MAX_TABLE)
     return fail(HZ_EINVAL, "a table of %lld buckets for %lld heads exceeds the supported size", (long long)nb, (long long)H);
-  if (Nq >= kTokenAxis || Nk >= kTokenAxis || B >= kTokenAxis || B * Nq > (int64_t(1) << 46) / Nk)
-    return fail(HZ_EINVAL, "B * Nq * Nk exceeds the supported tensor size");
+  if (Nq >= kTokenAxis || Nk >= kTokenAxis || B >= kTokenAxis || B * Nq > 0x7fffffffLL ||
+      B * Nq > (int64_t(1) << 46) / Nk)
+    return fail(HZ_EINVAL, "B * Nq (31 bits) or B * Nq * Nk (46 bits) exceeds the supported tensor size");
   return HZ_OK;
 }
 
@@ -942,10 +943,9 @@ int hz_bucket_bias_fwd(hipStream_t stream, const float* table, const int32_t* bu
       bucket_params(buckets, q_positions, k_positions, B, Nq, Nk, H, n_buckets, R, dtype, flags), table, e, stream));
 }
 
-int64_t hz_bucket_bias_workspace(int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t n_buckets, int flags) {
-  if (check_bucket_bias(B, Nq, Nk, H, n_buckets, 0, HZ_DTYPE_F32, flags)) return -1;
-  return hz::bucket_bias_workspace(
-      bucket_params(nullptr, nullptr, nullptr, B, Nq, Nk, H, n_buckets, 0, HZ_DTYPE_F32, flags));
+int64_t hz_bucket_bias_workspace(int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t n_buckets, int dtype, int flags) {
+  if (check_bucket_bias(B, Nq, Nk, H, n_buckets, 0, dtype, flags)) return -1;
+  return hz::bucket_bias_workspace(bucket_params(nullptr, nullptr, nullptr, B, Nq, Nk, H, n_buckets, 0, dtype, flags));
 }
 
 int hz_bucket_bias_bwd(hipStream_t stream, const void* de, const int32_t* buckets, const int32_t* q_positions,

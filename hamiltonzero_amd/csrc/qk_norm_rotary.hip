@@ -5,9 +5,10 @@
 // chosen so that both elements of each rotated pair are in one lane and no lane exchanges data but
 // for the sum of squares: with half-split pairs lane t holds elements 4 t .. 4 t + 3 and
 // n_freqs + 4 t .. + 3, with interleaved ones (and behind the rotated part) 8 t .. 8 t + 7. Either
-// way it turns pairs 4 t .. 4 t + 3, so a lane's four angles serve every head of a token: they are
-// formed once a token, in float64 turns (an angle at position 10^5 has no bits to lose in float32's
-// 24), and the workgroup's lanes then loop over the token's query and key heads.
+// way it turns pairs 4 t .. 4 t + 3. A workgroup takes up to four tokens at a time: it forms their angles
+// once, in float64 turns (an angle at position 10^5 has no bits to lose in float32's 24), puts the sines
+// and cosines into LDS, and then runs over the tokens' query and key heads, the next one's data in flight
+// while one is normalised.
 // Bound by the bytes: x is read and y written once; the backward reads x and dy and writes dx.
 #include "mhsea_device.h"
 #include "token_launch.h"
@@ -16,7 +17,8 @@ namespace hz {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxBlocks = 2048;  // of the backward: rows of partial weight gradients
+constexpr int kMaxTokens = 4;     // a workgroup at a time
+constexpr int kMaxBlocks = 1024;  // of the backward: rows of partial weight gradients
 
 struct NormParams {
   hz_token_tensor q, k, qo, ko;
@@ -24,11 +26,11 @@ struct NormParams {
   const double* freqs;
   const int32_t* positions;
   int64_t tokens;
-  int N, H, HT, D, nf, interleaved;
+  int N, H, HT, D, nf, interleaved, each;  // each: tokens a workgroup at a time
   float eps;
 };
 
-// Where a lane's two chunks of four elements lie in its head, and its four angles.
+// Where a lane's two chunks of four elements lie in its head, and whether they turn.
 struct Lane {
   int o0, o1;
   bool on, turns;
@@ -41,30 +43,36 @@ struct Lane {
   }
 };
 
-__device__ __forceinline__ void angles(const NormParams& p, int64_t token, int t, float (&cs)[4], float (&sn)[4]) {
-  const double pos = p.positions != nullptr ? p.positions[token] : static_cast<int>(token % p.N);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    double turn = pos * p.freqs[4 * t + i] * 0.15915494309189533577;  // radians to turns
+typedef float2 Angles[kMaxTokens][HZ_ROTARY_MAX_HEAD / 2];
+
+__device__ __forceinline__ void put_angles(const NormParams& p, int64_t token0, int count, Angles& angles) {
+  for (int a = threadIdx.x; a < count * p.nf; a += kThreads) {
+    const int x = a / p.nf, f = a - x * p.nf;
+    const int64_t token = token0 + x;
+    const double pos = p.positions != nullptr ? p.positions[token] : static_cast<int>(token % p.N);
+    double turn = pos * p.freqs[f] * 0.15915494309189533577;  // radians to turns
     turn -= rint(turn);
-    sincospif(2.f * static_cast<float>(turn), &sn[i], &cs[i]);
+    float s, c;
+    sincospif(2.f * static_cast<float>(turn), &s, &c);
+    angles[x][f] = make_float2(c, s);
   }
 }
 
-// The eight elements turned by their four angles (dir 1) or back (dir -1).
-__device__ __forceinline__ void turn8(float (&x)[8], const float (&cs)[4], const float (&sn)[4], int interleaved,
-                                      float dir) {
+// The eight elements turned by their four angles (dir 1) or back (dir -1). (A template: chosen at run time, the
+// pairs' places become indices into an array in scratch memory.)
+template <bool INTERLEAVED>
+__device__ __forceinline__ void turn8(float (&x)[8], const float2* angle, float dir) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float s = dir * sn[i];
-    if (interleaved) {
+    const float c = angle[i].x, s = dir * angle[i].y;
+    if constexpr (INTERLEAVED) {
       const float a = x[2 * i], b = x[2 * i + 1];
-      x[2 * i] = a * cs[i] - b * s;
-      x[2 * i + 1] = b * cs[i] + a * s;
+      x[2 * i] = a * c - b * s;
+      x[2 * i + 1] = b * c + a * s;
     } else {
       const float a = x[i], b = x[i + 4];
-      x[i] = a * cs[i] - b * s;
-      x[i + 4] = b * cs[i] + a * s;
+      x[i] = a * c - b * s;
+      x[i + 4] = b * c + a * s;
     }
   }
 }
@@ -77,11 +85,21 @@ __device__ __forceinline__ float head_sum(float x) {
 }
 
 template <class S>
-__device__ __forceinline__ void load8(const void* base, int64_t off, const Lane& l, float (&x)[8]) {
-  const float4 a = load4<S>(base, off + l.o0), b = load4<S>(base, off + l.o1);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-  x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
+struct Raw {
+  Raw4<S> a, b;
+  __device__ __forceinline__ void load(const void* base, int64_t off, const Lane& l) {
+    a = Raw4<S>::load(base, off + l.o0);
+    b = Raw4<S>::load(base, off + l.o1);
+  }
+  __device__ __forceinline__ void get(float (&x)[8], bool on) const {
+    const float4 u = a.f(), v = b.f();
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+    x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = on ? x[i] : 0.f;
+  }
+};
+
 template <class S>
 __device__ __forceinline__ void store8(void* base, int64_t off, const Lane& l, const float (&x)[8]) {
   store4<S>(base, off + l.o0, x[0], x[1], x[2], x[3]);
@@ -96,141 +114,168 @@ __device__ __forceinline__ void weights(const float* w, const Lane& l, float (&x
   }
 }
 
-// A workgroup's slots of GS lanes: all on one token's heads, or on several tokens where their heads
-// are few.
-struct Slots {
-  int per, token, head, step;  // tokens a workgroup; this slot's token and first head; heads a step
-  bool on;
-  __device__ __forceinline__ Slots(int HT, int gs) {
-    const int n = kThreads / gs, s = threadIdx.x / gs;
-    per = n / HT > 1 ? n / HT : 1;
-    token = per > 1 ? s / HT : 0;
-    head = per > 1 ? s % HT : s;
-    step = per > 1 ? HT : n;
-    on = token < per;
+// One (token, head) of the tokens at hand: which tensor, and where its head lies in the strided ones and in
+// a contiguous one.
+struct Item {
+  bool is_q;
+  int token, head;
+  int64_t b, n;
+  __device__ __forceinline__ Item(const NormParams& p, int64_t token0, int i) {
+    token = i / p.HT;
+    const int h = i - token * p.HT;
+    is_q = h < p.H;
+    head = is_q ? h : h - p.H;
+    const int64_t at = token0 + token;
+    b = at / p.N;
+    n = at - b * p.N;
+  }
+  // (by value: a reference to one of two kernel arguments would put both into scratch memory)
+  __device__ __forceinline__ const void* data(const hz_token_tensor& q, const hz_token_tensor& k) const {
+    return is_q ? q.data : k.data;
+  }
+  __device__ __forceinline__ int64_t offset(const hz_token_tensor& q, const hz_token_tensor& k) const {
+    return b * (is_q ? q.batch : k.batch) + n * (is_q ? q.token : k.token) + head * (is_q ? q.head : k.head);
   }
 };
 
-__device__ __forceinline__ int64_t head_offset(const hz_token_tensor& x, int64_t b, int64_t n, int h) {
-  return b * x.batch + n * x.token + h * x.head;
-}
-
-template <class S, int GS>
+template <class S, int GS, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p) {
-  const int t = threadIdx.x % GS;
+  __shared__ Angles angles;
+  constexpr int SLOTS = kThreads / GS;
+  const int t = threadIdx.x % GS, slot = threadIdx.x / GS;
   const Lane lane(p, t);
-  const Slots slot(p.HT, GS);
   float wq[8], wk[8];
   weights(p.wq, lane, wq);
   weights(p.wk, lane, wk);
-  if (!slot.on) return;
-  for (int64_t tok = static_cast<int64_t>(blockIdx.x) * slot.per + slot.token; tok < p.tokens;
-       tok += static_cast<int64_t>(gridDim.x) * slot.per) {
-    const int64_t b = tok / p.N, n = tok - b * p.N;
-    float cs[4], sn[4];
-    if (lane.turns) angles(p, tok, t, cs, sn);
-    for (int h = slot.head; h < p.HT; h += slot.step) {
-      const bool is_q = h < p.H;
-      const hz_token_tensor& in = is_q ? p.q : p.k;
-      const hz_token_tensor& out = is_q ? p.qo : p.ko;
-      const int hd = is_q ? h : h - p.H;
-      float x[8] = {};
-      if (lane.on) load8<S>(in.data, head_offset(in, b, n, hd), lane, x);
+  for (int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.each; token0 < p.tokens;
+       token0 += static_cast<int64_t>(gridDim.x) * p.each) {
+    const int count = static_cast<int>(p.tokens - token0 < p.each ? p.tokens - token0 : p.each), items = count * p.HT;
+    Raw<S> next;
+    auto load = [&](int i) {
+      if (i < items && lane.on) {
+        const Item it(p, token0, i);
+        next.load(it.data(p.q, p.k), it.offset(p.q, p.k), lane);
+      }
+    };
+    load(slot);
+    put_angles(p, token0, count, angles);
+    __syncthreads();
+    for (int i = slot; i < items; i += SLOTS) {
+      const Item it(p, token0, i);
+      float x[8];
+      next.get(x, lane.on);
+      load(i + SLOTS);
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
       const float r = 1.f / sqrtf(head_sum<GS>(ss) / static_cast<float>(p.D) + p.eps);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= r * (is_q ? wq[i] : wk[i]);
-      if (lane.turns) turn8(x, cs, sn, p.interleaved, 1.f);
-      if (lane.on) store8<S>(out.data, head_offset(out, b, n, hd), lane, x);
+      for (int e = 0; e < 8; ++e) x[e] *= r * (it.is_q ? wq[e] : wk[e]);
+      if (lane.turns) turn8<INTERLEAVED>(x, &angles[it.token][4 * t], 1.f);
+      if (lane.on) store8<S>(const_cast<void*>(it.data(p.qo, p.ko)), it.offset(p.qo, p.ko), lane, x);
     }
+    __syncthreads();
   }
 }
 
 // q and k: the forward's inputs; qo and ko: the cotangents. partial: [gridDim.x][2][D].
-template <class S, int GS>
+template <class S, int GS, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) norm_rotary_bwd_kernel(NormParams p, void* dq, void* dk, float* partial) {
+  __shared__ Angles angles;
   __shared__ float red[kThreads * 8];
-  const int t = threadIdx.x % GS;
+  constexpr int SLOTS = kThreads / GS;
+  const int t = threadIdx.x % GS, slot = threadIdx.x / GS;
   const Lane lane(p, t);
-  const Slots slot(p.HT, GS);
   float wq[8], wk[8], aq[8] = {}, ak[8] = {};
   weights(p.wq, lane, wq);
   weights(p.wk, lane, wk);
   const int Hk = p.HT - p.H;
-  for (int64_t tok = static_cast<int64_t>(blockIdx.x) * slot.per + slot.token; slot.on && tok < p.tokens;
-       tok += static_cast<int64_t>(gridDim.x) * slot.per) {
-    const int64_t b = tok / p.N, n = tok - b * p.N;
-    float cs[4], sn[4];
-    if (lane.turns) angles(p, tok, t, cs, sn);
-    for (int h = slot.head; h < p.HT; h += slot.step) {
-      const bool is_q = h < p.H;
-      const hz_token_tensor& in = is_q ? p.q : p.k;
-      const hz_token_tensor& cot = is_q ? p.qo : p.ko;
-      const int hd = is_q ? h : h - p.H;
-      float x[8] = {}, g[8] = {};
-      if (lane.on) {
-        load8<S>(in.data, head_offset(in, b, n, hd), lane, x);
-        load8<S>(cot.data, head_offset(cot, b, n, hd), lane, g);
+  for (int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.each; token0 < p.tokens;
+       token0 += static_cast<int64_t>(gridDim.x) * p.each) {
+    const int count = static_cast<int>(p.tokens - token0 < p.each ? p.tokens - token0 : p.each), items = count * p.HT;
+    Raw<S> next_x, next_g;
+    auto load = [&](int i) {
+      if (i < items && lane.on) {
+        const Item it(p, token0, i);
+        next_x.load(it.data(p.q, p.k), it.offset(p.q, p.k), lane);
+        next_g.load(it.data(p.qo, p.ko), it.offset(p.qo, p.ko), lane);
       }
+    };
+    load(slot);
+    put_angles(p, token0, count, angles);
+    __syncthreads();
+    for (int i = slot; i < items; i += SLOTS) {
+      const Item it(p, token0, i);
+      float x[8], g[8];
+      next_x.get(x, lane.on);
+      next_g.get(g, lane.on);
+      load(i + SLOTS);
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
       const float r = 1.f / sqrtf(head_sum<GS>(ss) / static_cast<float>(p.D) + p.eps);
-      if (lane.turns) turn8(g, cs, sn, p.interleaved, -1.f);
+      if (lane.turns) turn8<INTERLEAVED>(g, &angles[it.token][4 * t], -1.f);
       float dot = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] *= r;
-        const float gx = g[i] * x[i];
-        aq[i] += is_q ? gx : 0.f;
-        ak[i] += is_q ? 0.f : gx;
-        g[i] *= is_q ? wq[i] : wk[i];
-        dot += g[i] * x[i];
+      for (int e = 0; e < 8; ++e) {
+        x[e] *= r;
+        const float gx = g[e] * x[e];
+        aq[e] += it.is_q ? gx : 0.f;
+        ak[e] += it.is_q ? 0.f : gx;
+        g[e] *= it.is_q ? wq[e] : wk[e];
+        dot += g[e] * x[e];
       }
       dot = head_sum<GS>(dot) / static_cast<float>(p.D);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = r * (g[i] - x[i] * dot);
+      for (int e = 0; e < 8; ++e) x[e] = r * (g[e] - x[e] * dot);
       if (lane.on)
-        store8<S>(is_q ? dq : dk, (tok * (is_q ? p.H : Hk) + hd) * p.D, lane, x);
+        store8<S>(it.is_q ? dq : dk, ((token0 + it.token) * (it.is_q ? p.H : Hk) + it.head) * p.D, lane, x);
     }
+    __syncthreads();
   }
-  // the workgroup's weight gradients: one row of slots after the other, so their order is fixed
+  // the workgroup's weight gradients: one slot after the other, so their order is fixed
   for (int which = 0; which < 2; ++which) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) red[i * kThreads + threadIdx.x] = which == 0 ? aq[i] : ak[i];
+    for (int e = 0; e < 8; ++e) red[e * kThreads + threadIdx.x] = which == 0 ? aq[e] : ak[e];
     __syncthreads();
     for (int d = threadIdx.x; d < GS * 8; d += kThreads) {
-      const int tt = d / 8, i = d % 8;
+      const int tt = d / 8, e = d % 8;
       const Lane l(p, tt);
       if (!l.on) continue;
       float sum = 0.f;
-      for (int s = 0; s < kThreads / GS; ++s) sum += red[i * kThreads + s * GS + tt];
-      partial[(static_cast<int64_t>(blockIdx.x) * 2 + which) * p.D + (i < 4 ? l.o0 + i : l.o1 + i - 4)] = sum;
+#pragma unroll 8
+      for (int s = 0; s < SLOTS; ++s) sum += red[e * kThreads + s * GS + tt];
+      partial[(static_cast<int64_t>(blockIdx.x) * 2 + which) * p.D + (e < 4 ? l.o0 + e : l.o1 + e - 4)] = sum;
     }
   }
 }
 
-// Column sums of partial [rows][2 D]: 16 columns a workgroup, 64 threads a column.
-__global__ void __launch_bounds__(1024) weight_sum_kernel(const float* partial, int rows, int D, float* dw_q,
-                                                          float* dw_k) {
-  __shared__ float red[64][16];
-  const int c = threadIdx.x % 16, r0 = threadIdx.x / 16, col = blockIdx.x * 16 + c;
+// Column sums of partial [rows][2 D]: 4 columns a workgroup, 64 threads a column.
+__global__ void __launch_bounds__(kThreads) weight_sum_kernel(const float* partial, int rows, int D, float* dw_q,
+                                                              float* dw_k) {
+  __shared__ float red[64][4];
+  const int c = threadIdx.x % 4, r0 = threadIdx.x / 4, col = blockIdx.x * 4 + c;
   float sum = 0.f;
-  if (col < 2 * D)
-    for (int r = r0; r < rows; r += 64) sum += partial[static_cast<int64_t>(r) * 2 * D + col];
+#pragma unroll 8
+  for (int r = r0; r < rows; r += 64) sum += partial[static_cast<int64_t>(r) * 2 * D + col];
   red[r0][c] = sum;
   __syncthreads();
   for (int m = 32; m > 0; m >>= 1) {
     if (r0 < m) red[r0][c] += red[r0 + m][c];
     __syncthreads();
   }
-  if (r0 == 0 && col < 2 * D) {
+  if (r0 == 0) {
     float* const dw = col < D ? dw_q : dw_k;
     if (dw != nullptr) dw[col < D ? col : col - D] = red[0][c];
   }
+}
+
+// Tokens a workgroup at a time: several where that leaves at least `blocks` workgroups, so that the angles are
+// formed by all lanes and the loads of several heads overlap (qk_train_bf16's forward: 4 tokens 95 us, 1 token 132).
+int tokens_each(int64_t tokens, int64_t blocks) {
+  const int64_t n = tokens / blocks;
+  return static_cast<int>(n < 1 ? 1 : n > kMaxTokens ? kMaxTokens : n);
 }
 
 NormParams params(const hz_qk_norm_rotary& a) {
@@ -240,32 +285,34 @@ NormParams params(const hz_qk_norm_rotary& a) {
   p.tokens = a.B * a.N;
   p.N = static_cast<int>(a.N), p.H = static_cast<int>(a.H), p.HT = static_cast<int>(a.H + a.Hk);
   p.D = static_cast<int>(a.D), p.nf = static_cast<int>(a.n_freqs), p.interleaved = a.interleaved;
+  p.each = tokens_each(p.tokens, kMaxBlocks);
   p.eps = a.eps;
   return p;
 }
 
-int group_size(int64_t D) {
-  int gs = 1;
-  while (gs * 8 < D) gs *= 2;
-  return gs;
-}
-
 int64_t blocks(const NormParams& p, int64_t most) {
-  const int slots = kThreads / group_size(p.D), per = slots / p.HT > 1 ? slots / p.HT : 1;
-  const int64_t n = (p.tokens + per - 1) / per;
+  const int64_t n = (p.tokens + p.each - 1) / p.each;
   return n < most ? n : most;
 }
 
 template <class F>
-void by_group(int gs, F f) {
-  switch (gs) {
-    case 1: f(std::integral_constant<int, 1>{}); break;
-    case 2: f(std::integral_constant<int, 2>{}); break;
-    case 4: f(std::integral_constant<int, 4>{}); break;
-    case 8: f(std::integral_constant<int, 8>{}); break;
-    case 16: f(std::integral_constant<int, 16>{}); break;
-    default: f(std::integral_constant<int, 32>{}); break;
-  }
+void by_group(int64_t D, F f) {
+  if (D <= 8) return f(std::integral_constant<int, 1>{});
+  if (D <= 16) return f(std::integral_constant<int, 2>{});
+  if (D <= 32) return f(std::integral_constant<int, 4>{});
+  if (D <= 64) return f(std::integral_constant<int, 8>{});
+  if (D <= 128) return f(std::integral_constant<int, 16>{});
+  f(std::integral_constant<int, 32>{});
+}
+
+template <class F>
+void by_variant(const hz_qk_norm_rotary& a, F f) {
+  by_group(a.D, [&](auto gs) {
+    if (a.dtype == HZ_DTYPE_BF16)
+      a.interleaved ? f(BF16{}, gs, std::true_type{}) : f(BF16{}, gs, std::false_type{});
+    else
+      a.interleaved ? f(F32{}, gs, std::true_type{}) : f(F32{}, gs, std::false_type{});
+  });
 }
 
 }  // namespace
@@ -277,11 +324,8 @@ int64_t qk_norm_rotary_workspace(int64_t tokens, int64_t D) {
 hipError_t launch_qk_norm_rotary_fwd(const hz_qk_norm_rotary& a, hipStream_t stream) {
   const NormParams p = params(a);
   const dim3 grid(static_cast<unsigned>(blocks(p, 1 << 20)));
-  by_group(group_size(p.D), [&](auto gs) {
-    if (a.dtype == HZ_DTYPE_BF16)
-      norm_rotary_fwd_kernel<BF16, gs.value><<<grid, kThreads, 0, stream>>>(p);
-    else
-      norm_rotary_fwd_kernel<F32, gs.value><<<grid, kThreads, 0, stream>>>(p);
+  by_variant(a, [&](auto type, auto gs, auto inter) {
+    norm_rotary_fwd_kernel<decltype(type), gs.value, inter.value><<<grid, kThreads, 0, stream>>>(p);
   });
   return hipGetLastError();
 }
@@ -291,14 +335,11 @@ hipError_t launch_qk_norm_rotary_bwd(const hz_qk_norm_rotary& a, void* dq, void*
   const NormParams p = params(a);
   const int rows = static_cast<int>(blocks(p, kMaxBlocks));
   float* const partial = static_cast<float*>(workspace);
-  by_group(group_size(p.D), [&](auto gs) {
-    if (a.dtype == HZ_DTYPE_BF16)
-      norm_rotary_bwd_kernel<BF16, gs.value><<<rows, kThreads, 0, stream>>>(p, dq, dk, partial);
-    else
-      norm_rotary_bwd_kernel<F32, gs.value><<<rows, kThreads, 0, stream>>>(p, dq, dk, partial);
+  by_variant(a, [&](auto type, auto gs, auto inter) {
+    norm_rotary_bwd_kernel<decltype(type), gs.value, inter.value><<<rows, kThreads, 0, stream>>>(p, dq, dk, partial);
   });
   if (dw_q != nullptr || dw_k != nullptr)
-    weight_sum_kernel<<<(2 * p.D + 15) / 16, 1024, 0, stream>>>(partial, rows, p.D, dw_q, dw_k);
+    weight_sum_kernel<<<2 * p.D / 4, kThreads, 0, stream>>>(partial, rows, p.D, dw_q, dw_k);
   return hipGetLastError();
 }
 

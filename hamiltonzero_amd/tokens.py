@@ -356,7 +356,7 @@ def _bias_call(table, e, buckets, q_positions, k_positions, qkh, R, nb, H, backw
             _native.check(lib.hz_bucket_bias_fwd(_stream(dev), _ptr(table), _ptr(buckets), _ptr(q_positions),
                                                  _ptr(k_positions), _ptr(e), *sizes))
             return
-        size = lib.hz_bucket_bias_workspace(*sizes[:5], sizes[7])
+        size = lib.hz_bucket_bias_workspace(*sizes[:5], *sizes[6:])
         work = torch.empty(size, dtype=torch.uint8, device=dev)
         _native.check(lib.hz_bucket_bias_bwd(_stream(dev), _ptr(e), _ptr(buckets), _ptr(q_positions), _ptr(k_positions),
                                              _ptr(table), _ptr(work), size, *sizes))

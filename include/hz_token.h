@@ -133,8 +133,9 @@ int hz_bucket_bias_fwd(hipStream_t stream, const float* table, const int32_t* bu
                        const int32_t* k_positions, void* e, int64_t B, int64_t Nq, int64_t Nk, int64_t H,
                        int64_t n_buckets, int64_t R, int dtype, int flags);
 
-/* dtable[m, h] = sum of de[b, i, j, h] over the (b, i, j) of bucket m; float32 sums. */
-int64_t hz_bucket_bias_workspace(int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t n_buckets, int flags);
+/* dtable[m, h] = sum of de[b, i, j, h] over the (b, i, j) of bucket m; float32 sums. de must be finite (with
+ * HZ_FLAG_E_QKH a value that is not makes every bucket of its head NaN). */
+int64_t hz_bucket_bias_workspace(int64_t B, int64_t Nq, int64_t Nk, int64_t H, int64_t n_buckets, int dtype, int flags);
 int hz_bucket_bias_bwd(hipStream_t stream, const void* de, const int32_t* buckets, const int32_t* q_positions,
                        const int32_t* k_positions, float* dtable, void* workspace, int64_t workspace_bytes, int64_t B,
                        int64_t Nq, int64_t Nk, int64_t H, int64_t n_buckets, int64_t R, int dtype, int flags);

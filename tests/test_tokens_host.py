@@ -203,7 +203,7 @@ def test_bias_refuses(lib, over, code, needle):
     assert needle in lib.hz_last_error().decode()
     sizes = [f[n] for n in ("B", "Nq", "Nk", "H", "nb", "R", "dtype", "flags")]
     assert lib.hz_bucket_bias_bwd(None, f["x"], f["buckets"], f["qpos"], f["kpos"], A, A, 1 << 40, *sizes) == code
-    need = lib.hz_bucket_bias_workspace(2, 8, 8, 4, 32, 0)
+    need = lib.hz_bucket_bias_workspace(2, 8, 8, 4, 32, 0, 0)
     assert lib.hz_bucket_bias_bwd(None, A, A, A, A, A, A, need - 1, 2, 8, 8, 4, 32, 16, 0, 0) == E.HZ_EINVAL
 
 
