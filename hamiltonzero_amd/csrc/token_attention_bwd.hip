@@ -19,25 +19,50 @@ constexpr int kBlock = 128;  // queries (dq) or keys (dk, dv) a workgroup, 32 a 
 template <int DP, int PARTS>
 constexpr int kRows = (DP == 128 && PARTS == 3) ? 32 : 64;
 
-// Weight and score gradient (without the scale) of one pair, from its dot product x, its dP and the
-// distance between query and key.
-template <int PARTS, bool CAP>
-__device__ __forceinline__ void pair(const Params& p, float x, float dp, float slope2, float distance, float lse2,
+// Weight and score gradient of one pair from its dot product x, its dP and the distance between query and key;
+// `base` is the exponent's part of the query, as row_base gives it. bfloat16, capped: with u = 1 / (1 + e^2y), tanh y =
+// 1 - 2 u and its derivative is 4 u (1 - u), whose 4 is left to the end (grad_scale).
+template <int PARTS, bool CAP, bool SLOPE>
+__device__ __forceinline__ void pair(const Params& p, float x, float dp, float slope2, float distance, float base,
                                      float delta, float& w, float& ds) {
-  float g = 0.f;
-  if constexpr (CAP) {
+  constexpr bool U = CAP && PARTS == 1;
+  float g = 1.f, s;
+  if constexpr (U) {
+    const float u = __builtin_amdgcn_rcpf(1.f + fast_exp2(x * p.to_exp2));
+    s = base - 2.f * p.to_score2 * u;
+    g = u - u * u;
+  } else if constexpr (CAP) {
     const float t = tanh_of<PARTS>(x * p.to_tanh);
-    x = t;
+    s = t * p.to_score2 + base;
     g = 1.f - t * t;
+  } else {
+    s = x * p.to_score2 + base;
   }
-  float s = x * p.to_score2 - lse2;
-  if (slope2 != 0.f) s -= slope2 * fabsf(distance);
+  if constexpr (SLOPE) s -= slope2 * fabsf(distance);
   w = fast_exp2(s);
   ds = w * (dp - delta);
   if constexpr (CAP) ds *= g;
 }
+// Operands that are read together.
+template <int PARTS>
+struct Two {
+  Frag<PARTS> a, b;
+};
+template <int PARTS>
+struct Three {
+  Frag<PARTS> a, b, c;
+};
 
-template <int DP, int PARTS, bool CAP>
+template <int PARTS, bool CAP>
+__device__ __forceinline__ float row_base(const Params& p, float lse) {
+  return (CAP && PARTS == 1 ? p.to_score2 : 0.f) - lse * kLog2e;
+}
+template <int PARTS, bool CAP>
+__device__ __forceinline__ float grad_scale(const Params& p) {
+  return CAP && PARTS == 1 ? 4.f * p.scale : p.scale;
+}
+
+template <int DP, int PARTS, bool CAP, bool SLOPE>
 __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Params p, hz_token_tensor dout, void* dq,
                                                                            float* deltas, const DocTile* doc_tiles) {
   constexpr int KB = kRows<DP, PARTS>, NB = KB / 32, DT = DP / 32, CH = DP / 8;
@@ -50,16 +75,13 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
   __shared__ int range_lds[4][2];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, hh = lane >> 5, c = lane & 31;
   const int tiles = (p.Nq + kBlock - 1) / kBlock;
-  int64_t id = xcd_run(blockIdx.x, gridDim.x);
-  const int head = static_cast<int>(id % p.G);
-  id /= p.G;
-  const int q0 = static_cast<int>(tiles - 1 - id % tiles) * kBlock;
-  id /= tiles;
-  const int hk = static_cast<int>(id % p.Hk), b = static_cast<int>(id / p.Hk), h = hk * p.G + head;
+  const Unit unit(blockIdx.x, p.G, static_cast<int64_t>(p.B) * p.Hk);
+  const int q0 = (tiles - 1 - unit.tile) * kBlock;  // the longest rows of a causal mask first
+  const int hk = static_cast<int>(unit.pair % p.Hk), b = static_cast<int>(unit.pair / p.Hk), h = hk * p.G + unit.inner;
   const int n = kv_length(p, b);
   const int i = q0 + 32 * wave + c, row = i < p.Nq ? i : p.Nq - 1;
   const Sight me(p, b, row, n);
-  const float slope2 = p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
+  const float slope2 = SLOPE ? p.slopes[h] * kLog2e : 0.f;
   const int wave_first = __builtin_amdgcn_readfirstlane(me.last);
   const int wave_last = __builtin_amdgcn_readlane(me.last, 31);
   const int keys = Sight(p, b, min(q0 + kBlock, p.Nq) - 1, n).last + 1;
@@ -105,8 +127,8 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
   }
   delta = xor32_pair_sum(delta);
   if (i < p.Nq && hh == 0) deltas[at] = delta;
-  float lse2 = p.lse[at] * kLog2e;
-  if (lse2 == kNegInf) lse2 = 0.f;  // a row that sees nothing
+  const float lse = p.lse[at], base = row_base<PARTS, CAP>(p, lse == kNegInf ? 0.f : lse);  // -inf: a row that sees nothing
+  const float to_grad = grad_scale<PARTS, CAP>(p);
   v16f acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = v16f{};
@@ -167,17 +189,17 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         v16f s = v16f{}, dp = v16f{};
-#pragma unroll
-        for (int ds = 0; ds < DP / 16; ++ds) {
-          s = mma(kt.rows(32 * nb, ds, lane), q[ds], s);
-          dp = mma(vt.rows(32 * nb, ds, lane), go[ds], dp);
-        }
+        ahead<DP / 16>([&](int ds) { return Two<PARTS>{kt.rows(32 * nb, ds, lane), vt.rows(32 * nb, ds, lane)}; },
+                       [&](int ds, const Two<PARTS>& x) {
+                         s = mma(x.a, q[ds], s);
+                         dp = mma(x.b, go[ds], dp);
+                       });
         const int k1 = k0 + 32 * nb + 4 * hh;
         const float away = static_cast<float>(me.pos - k1);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float w, g;
-          pair<PARTS, CAP>(p, s[e], dp[e], slope2, away - static_cast<float>(row_of(e, 0)), lse2, delta, w, g);
+          pair<PARTS, CAP, SLOPE>(p, s[e], dp[e], slope2, away - static_cast<float>(row_of(e, 0)), base, delta, w, g);
           s[e] = g;
         }
         if (masked) {
@@ -195,12 +217,9 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
             }
           }
         }
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const Frag<PARTS> g = frag_of<PARTS>(s, st);
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) acc[dt] = mma(kt.columns(32 * nb + 16 * st, dt, lane), g, acc[dt]);
-        }
+        const Frag<PARTS> g[2] = {frag_of<PARTS>(s, 0), frag_of<PARTS>(s, 1)};
+        ahead<2 * DT>([&](int i) { return kt.columns(32 * nb + 16 * (i / DT), i % DT, lane); },
+                      [&](int i, const Frag<PARTS>& x) { acc[i % DT] = mma(x, g[i / DT], acc[i % DT]); });
       }
     }
     t = after;
@@ -220,16 +239,23 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
     for (int x = 0; x < 4; ++x) {
       const int d = 32 * dt + 8 * x + 4 * hh;
       if (d < p.D)
-        store_four<PARTS>(dq, at * p.D + d, acc[dt][4 * x] * p.scale, acc[dt][4 * x + 1] * p.scale,
-                          acc[dt][4 * x + 2] * p.scale, acc[dt][4 * x + 3] * p.scale);
+        store_four<PARTS>(dq, at * p.D + d, acc[dt][4 * x] * to_grad, acc[dt][4 * x + 1] * to_grad,
+                          acc[dt][4 * x + 2] * to_grad, acc[dt][4 * x + 3] * to_grad);
     }
 }
 
+// The query heads of a key head in `n` shares, a workgroup each: partial [n][dk, dv][elements] in float32.
+struct Splits {
+  float* partial;
+  int64_t elements;
+  int n;
+};
+
 // WAVES = 8 (bfloat16): waves w and w + 4 own the same 32 keys and take the tile's first and second 32 queries;
 // their sums meet in LDS at the end. So two waves share a SIMD although a workgroup owns 128 keys only.
-template <int DP, int PARTS, bool CAP, int WAVES>
+template <int DP, int PARTS, bool CAP, bool SLOPE, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params p, hz_token_tensor dout, const float* deltas,
-                                                                          void* dk, void* dv, const DocTile* doc_tiles) {
+                                                                          void* dk, void* dv, const DocTile* doc_tiles, Splits splits) {
   constexpr int THREADS = 64 * WAVES, SETS = WAVES / 4;
   constexpr int QB = kRows<DP, PARTS>, NB = QB / 32 / SETS, DT = DP / 32, CH = DP / 8;
   constexpr int LOADS = QB * CH / THREADS, STEP = THREADS / CH;
@@ -237,16 +263,16 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
   typedef Tile<QB, DP, PARTS> QT;
   __shared__ __align__(16) uint16_t q_lds0[QT::kPlane * PARTS], g_lds0[QT::kPlane * PARTS];
   __shared__ __align__(16) uint16_t q_lds1[PARTS == 1 ? QT::kPlane : 8], g_lds1[PARTS == 1 ? QT::kPlane : 8];
-  __shared__ __align__(16) float lse_lds[BUFS][QB], delta_lds[BUFS][QB];
+  __shared__ __align__(16) float base_lds[BUFS][QB], delta_lds[BUFS][QB];
   __shared__ __align__(16) int doc_lds[BUFS][QB];
+  __shared__ __align__(16) uint16_t v_lds[kBlock * DP * PARTS];
   __shared__ uint64_t bad_lds[BUFS];
   __shared__ int range_lds[4][2];
   const int tid = threadIdx.x, wave = (tid >> 6) & 3, set = tid >> 8, lane = tid & 63, hh = lane >> 5, c = lane & 31;
-  const int tiles = (p.Nk + kBlock - 1) / kBlock;
-  int64_t id = xcd_run(blockIdx.x, gridDim.x);
-  const int key0 = static_cast<int>(id % tiles) * kBlock;  // the first keys are seen by the most queries
-  id /= tiles;
-  const int hk = static_cast<int>(id % p.Hk), b = static_cast<int>(id / p.Hk);
+  const Unit unit(blockIdx.x, splits.n, static_cast<int64_t>(p.B) * p.Hk);
+  const int key0 = unit.tile * kBlock;  // the first keys are seen by the most queries
+  const int hk = static_cast<int>(unit.pair % p.Hk), b = static_cast<int>(unit.pair / p.Hk);
+  const int first_head = unit.inner * p.G / splits.n, last_head = (unit.inner + 1) * p.G / splits.n - 1;
   const int n = kv_length(p, b), shift = n - p.Nq;  // position of query 0
   const int wave0 = key0 + 32 * wave, key = wave0 + c, row = key < n ? key : max(n - 1, 0);
   const int prefix = p.causal && p.prefix != nullptr ? p.prefix[b] : 0;
@@ -264,15 +290,21 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
     hi = max(max(range_lds[0][1], range_lds[1][1]), max(range_lds[2][1], range_lds[3][1]));
   }
 
-  Frag<PARTS> k[DP / 16], v[DP / 16];
+  // the keys' rows stay in registers, the values' in LDS: with both in registers the sums would not fit
+  Frag<PARTS> k[DP / 16];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
-    Raw8<PARTS> rk, rv;
+    Raw8<PARTS> rk;
     const int d = 16 * s + 8 * hh;
     rk.load(p.k.data, b * p.k.batch + row * p.k.token + hk * p.k.head + d, key < n && d < p.D);
-    rv.load(p.v.data, b * p.v.batch + row * p.v.token + hk * p.v.head + d, key < n && d < p.D);
     k[s] = frag(rk);
-    v[s] = frag(rv);
+  }
+  const Tile<kBlock, DP, PARTS> vt{v_lds};
+  for (int i = tid; i < kBlock * CH; i += THREADS) {
+    const int r = i / CH, ch = i % CH;
+    Raw8<PARTS> rv;
+    rv.load(p.v.data, b * p.v.batch + (key0 + r) * p.v.token + hk * p.v.head + 8 * ch, key0 + r < n && 8 * ch < p.D);
+    vt.put(r, ch, frag(rv));
   }
   v16f ak[DT], av[DT];
 #pragma unroll
@@ -326,8 +358,8 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
     }
   };
   DocTile here{}, there{};
-  int head = 0, t = walk.next(begin, lane, here);
-  if (t < end) load(0, t, std::integral_constant<int, 0>{});
+  int head = first_head, t = walk.next(begin, lane, here);
+  if (t < end) load(head, t, std::integral_constant<int, 0>{});
   // one tile of one head, in buffer B
   auto step = [&](auto which) __attribute__((always_inline)) {
     constexpr int B = which.value;
@@ -337,7 +369,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
         // a query that sees nothing, or is none: weights of 2^-inf
         const bool bad = rlse == kNegInf;
         const uint64_t votes = __ballot(bad);
-        lse_lds[B][tid] = bad ? -kNegInf : rlse * kLog2e;
+        base_lds[B][tid] = bad ? kNegInf : row_base<PARTS, CAP>(p, rlse);
         delta_lds[B][tid] = bad ? 0.f : rdelta;
         if (by_document) doc_lds[B][tid] = rdoc >= 0 ? rdoc : kNoDocument;
         if (tid == 0) bad_lds[B] = votes;
@@ -364,13 +396,13 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
       __syncthreads();
     }
     int after = walk.next(t + 1, lane, there), next_head = head;
-    if (after >= end && head + 1 < p.G) {
+    if (after >= end && head < last_head) {
       next_head = head + 1;
       after = walk.next(begin, lane, there);
     }
     if (after < end) load(next_head, after, std::integral_constant<int, BUFS == 2 ? 1 - B : 0>{});
     const int p0 = shift + t * QB;  // position of the tile's first query
-    const float slope2 = p.slopes != nullptr ? p.slopes[hk * p.G + head] * kLog2e : 0.f;
+    const float slope2 = SLOPE ? p.slopes[hk * p.G + head] * kLog2e : 0.f;
     const bool unseen = (p.causal && wave0 >= prefix && p0 + QB - 1 < wave0) ||
                         (by_document && (here.lo > wave_hi || here.hi < wave_lo));
     if (!unseen) {
@@ -380,21 +412,23 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
       for (int nb = 0; nb < NB; ++nb) {
         const int r0 = 32 * (nb + (SETS == 2 ? set : 0));
         v16f s = v16f{}, dp = v16f{};
-#pragma unroll
-        for (int ds = 0; ds < DP / 16; ++ds) {
-          s = mma(qt.rows(r0, ds, lane), k[ds], s);
-          dp = mma(gt.rows(r0, ds, lane), v[ds], dp);
-        }
+        const int l = anew(lane);
+        ahead<DP / 16>(
+            [&](int ds) { return Three<PARTS>{qt.rows(r0, ds, l), gt.rows(r0, ds, l), vt.rows(32 * wave, ds, l)}; },
+            [&](int ds, const Three<PARTS>& x) {
+              s = mma(x.a, k[ds], s);
+              dp = mma(x.b, x.c, dp);
+            });
         const int r1 = r0 + 4 * hh;
         const float away = static_cast<float>(p0 + r1 - key);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const v4f l = *reinterpret_cast<const v4f*>(&lse_lds[B][r1 + 8 * e]);
+          const v4f b0 = *reinterpret_cast<const v4f*>(&base_lds[B][r1 + 8 * e]);
           const v4f d = *reinterpret_cast<const v4f*>(&delta_lds[B][r1 + 8 * e]);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             float w, gs;
-            pair<PARTS, CAP>(p, s[4 * e + x], dp[4 * e + x], slope2, away + static_cast<float>(8 * e + x), l[x], d[x], w, gs);
+            pair<PARTS, CAP, SLOPE>(p, s[4 * e + x], dp[4 * e + x], slope2, away + static_cast<float>(8 * e + x), b0[x], d[x], w, gs);
             s[4 * e + x] = w;
             dp[4 * e + x] = gs;
           }
@@ -420,15 +454,14 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
             }
           }
         }
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const Frag<PARTS> w = frag_of<PARTS>(s, st), gs = frag_of<PARTS>(dp, st);
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            av[dt] = mma(gt.columns(r0 + 16 * st, dt, lane), w, av[dt]);
-            ak[dt] = mma(qt.columns(r0 + 16 * st, dt, lane), gs, ak[dt]);
-          }
-        }
+        const Frag<PARTS> w[2] = {frag_of<PARTS>(s, 0), frag_of<PARTS>(s, 1)};
+        const Frag<PARTS> gs[2] = {frag_of<PARTS>(dp, 0), frag_of<PARTS>(dp, 1)};
+        ahead<2 * DT>(
+            [&](int i) { return Two<PARTS>{gt.columns(r0 + 16 * (i / DT), i % DT, l), qt.columns(r0 + 16 * (i / DT), i % DT, l)}; },
+            [&](int i, const Two<PARTS>& x) {
+              av[i % DT] = mma(x.a, w[i / DT], av[i % DT]);
+              ak[i % DT] = mma(x.b, gs[i / DT], ak[i % DT]);
+            });
       }
     }
     t = after;
@@ -474,53 +507,108 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
   }
   if (key >= p.Nk) return;
   const int64_t at = ((static_cast<int64_t>(b) * p.Nk + key) * p.Hk + hk) * p.D;
+  const float to_grad = grad_scale<PARTS, CAP>(p);
+  if (splits.n > 1) {
+    float* const to = splits.partial + unit.inner * 2 * splits.elements + at;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int d = 32 * dt + 8 * x + 4 * hh;
+        if (d < p.D) {
+          store_four<3>(to, d, ak[dt][4 * x] * to_grad, ak[dt][4 * x + 1] * to_grad, ak[dt][4 * x + 2] * to_grad,
+                        ak[dt][4 * x + 3] * to_grad);
+          store_four<3>(to + splits.elements, d, av[dt][4 * x], av[dt][4 * x + 1], av[dt][4 * x + 2], av[dt][4 * x + 3]);
+        }
+      }
+    return;
+  }
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int d = 32 * dt + 8 * x + 4 * hh;
       if (d < p.D) {
-        store_four<PARTS>(dk, at + d, ak[dt][4 * x] * p.scale, ak[dt][4 * x + 1] * p.scale, ak[dt][4 * x + 2] * p.scale,
-                          ak[dt][4 * x + 3] * p.scale);
+        store_four<PARTS>(dk, at + d, ak[dt][4 * x] * to_grad, ak[dt][4 * x + 1] * to_grad, ak[dt][4 * x + 2] * to_grad,
+                          ak[dt][4 * x + 3] * to_grad);
         store_four<PARTS>(dv, at + d, av[dt][4 * x], av[dt][4 * x + 1], av[dt][4 * x + 2], av[dt][4 * x + 3]);
       }
     }
+}
+
+// Sums of the shares, four elements a thread.
+template <int PARTS>
+__global__ void __launch_bounds__(256) token_dkv_sum_kernel(Splits splits, void* dk, void* dv) {
+  const int64_t quads = splits.elements / 4;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < 2 * quads; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t at = 4 * i;  // [dk, dv][elements]
+    v4f sum = *reinterpret_cast<const v4f*>(splits.partial + at);
+    for (int s = 1; s < splits.n; ++s) sum += *reinterpret_cast<const v4f*>(splits.partial + s * 2 * splits.elements + at);
+    if (i < quads)
+      store_four<PARTS>(dk, at, sum[0], sum[1], sum[2], sum[3]);
+    else
+      store_four<PARTS>(dv, at - splits.elements, sum[0], sum[1], sum[2], sum[3]);
+  }
+}
+
+int64_t dkv_blocks(const hz_token_attention& a) { return a.B * a.Hk * ((a.Nk + kBlock - 1) / kBlock); }
+
+// Shares of a key head's query heads: until there are two workgroups a CU, as far as the heads divide. (Documents and
+// causal masks make workgroups of very different lengths, which a single round of them cannot even out.)
+int dkv_splits(const hz_token_attention& a) {
+  const int64_t G = a.H / a.Hk, blocks = dkv_blocks(a);
+  int64_t n = 1;
+  while (n < G && (blocks * n < 512 || G % n != 0)) ++n;
+  return static_cast<int>(n);
+}
+
+int64_t split_bytes(const hz_token_attention& a) {
+  const int n = dkv_splits(a);
+  return n > 1 ? n * 2 * a.B * a.Nk * a.Hk * a.D * static_cast<int64_t>(sizeof(float)) : 0;
 }
 
 int64_t delta_bytes(const hz_token_attention& a) {
   return (a.B * a.Nq * a.H * static_cast<int64_t>(sizeof(float)) + 15) / 16 * 16;
 }
 
-template <int DP, int PARTS, bool CAP>
+template <int DP, int PARTS, bool CAP, bool SLOPE>
 hipError_t run(const hz_token_attention& a, const hz_token_tensor& dout, void* dq, void* dk, void* dv, void* workspace,
                hipStream_t stream) {
   constexpr int WAVES = PARTS == 1 ? 8 : 4;
   const Params p = make_params(a);
   float* const deltas = static_cast<float*>(workspace);
-  DocTile* const tiles = reinterpret_cast<DocTile*>(static_cast<char*>(workspace) + delta_bytes(a));
+  const Splits splits{reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a)), a.B * a.Nk * a.Hk * a.D, dkv_splits(a)};
+  DocTile* const tiles = reinterpret_cast<DocTile*>(static_cast<char*>(workspace) + delta_bytes(a) + split_bytes(a));
   if (p.documents != nullptr)
     if (hipError_t err = launch_doc_tiles(p, tiles, stream); err != hipSuccess) return err;
-  const int64_t nq = a.B * a.H * ((a.Nq + kBlock - 1) / kBlock), nk = a.B * a.Hk * ((a.Nk + kBlock - 1) / kBlock);
-  token_dq_kernel<DP, PARTS, CAP><<<static_cast<unsigned>(nq), 256, 0, stream>>>(p, dout, dq, deltas, tiles);
-  token_dkv_kernel<DP, PARTS, CAP, WAVES><<<static_cast<unsigned>(nk), 64 * WAVES, 0, stream>>>(p, dout, deltas, dk, dv, tiles);
+  const int64_t nq = a.B * a.H * ((a.Nq + kBlock - 1) / kBlock), nk = dkv_blocks(a) * splits.n;
+  token_dq_kernel<DP, PARTS, CAP, SLOPE><<<static_cast<unsigned>(nq), 256, 0, stream>>>(p, dout, dq, deltas, tiles);
+  token_dkv_kernel<DP, PARTS, CAP, SLOPE, WAVES><<<static_cast<unsigned>(nk), 64 * WAVES, 0, stream>>>(p, dout, deltas, dk, dv, tiles, splits);
+  if (splits.n > 1) {
+    const int64_t n = (splits.elements / 2 + 255) / 256;
+    token_dkv_sum_kernel<PARTS><<<static_cast<unsigned>(n < 8192 ? n : 8192), 256, 0, stream>>>(splits, dk, dv);
+  }
   return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t token_attention_bwd_workspace(const hz_token_attention& a) {
-  return delta_bytes(a) + static_cast<int64_t>(doc_tiles_bytes(a));
+  return delta_bytes(a) + split_bytes(a) + static_cast<int64_t>(doc_tiles_bytes(a));
 }
 
 hipError_t launch_token_attention_bwd(const hz_token_attention& a, const hz_token_tensor& dout, void* dq, void* dk,
                                       void* dv, void* workspace, hipStream_t stream) {
+  auto by_score = [&](auto dp, auto parts, auto cap) {
+    return a.slopes != nullptr ? run<dp.value, parts.value, cap.value, true>(a, dout, dq, dk, dv, workspace, stream)
+                               : run<dp.value, parts.value, cap.value, false>(a, dout, dq, dk, dv, workspace, stream);
+  };
   auto by_type = [&](auto dp) {
-    constexpr int DP = dp.value;
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 3> Split;
     if (a.dtype == HZ_DTYPE_BF16)
-      return a.softcap > 0.f ? run<DP, 1, true>(a, dout, dq, dk, dv, workspace, stream)
-                             : run<DP, 1, false>(a, dout, dq, dk, dv, workspace, stream);
-    return a.softcap > 0.f ? run<DP, 3, true>(a, dout, dq, dk, dv, workspace, stream)
-                           : run<DP, 3, false>(a, dout, dq, dk, dv, workspace, stream);
+      return a.softcap > 0.f ? by_score(dp, One{}, std::true_type{}) : by_score(dp, One{}, std::false_type{});
+    return a.softcap > 0.f ? by_score(dp, Split{}, std::true_type{}) : by_score(dp, Split{}, std::false_type{});
   };
   if (a.D <= 32) return by_type(std::integral_constant<int, 32>{});
   if (a.D <= 64) return by_type(std::integral_constant<int, 64>{});

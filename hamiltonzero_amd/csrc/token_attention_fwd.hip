@@ -61,7 +61,7 @@ struct Running {
 // A score is a base-2 number s, or, where there is a cap and no distance bias, u = 1 / (1 + e^2y) with
 // s = cap2 - 2 cap2 u (tanh y = 1 - 2 u), so that the map to the exponent of 2 is one fused operation.
 // Hidden pairs are -inf, or u = +inf.
-template <int PARTS, bool CAP, bool U, int N>
+template <int PARTS, bool CAP, bool SLOPE, bool U, int N>
 __device__ __forceinline__ void scores(v16f (&s)[N], const Params& p, const Sight& me, float slope2, int k0, int hh,
                                        bool masked, const int* docs) {
 #pragma unroll
@@ -75,7 +75,7 @@ __device__ __forceinline__ void scores(v16f (&s)[N], const Params& p, const Sigh
       else
         s[n][i] *= p.to_score2;
     }
-  if (!U && slope2 != 0.f) {
+  if constexpr (SLOPE) {
     const float at = static_cast<float>(me.pos - k0 - 4 * hh);
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -171,11 +171,12 @@ struct Parts {
   int n;  // 1: not divided, the results go to out and lse
 };
 
-template <int DP, int PARTS, bool CAP, bool U>
+template <int DP, int PARTS, bool CAP, bool SLOPE>
 __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel(Params p, const DocTile* doc_tiles, Parts parts) {
   constexpr int KB = kKeys<DP, PARTS>, NB = KB / 32, DT = DP / 32, CH = DP / 8;
   constexpr int LOADS = KB * CH / kThreads, STEP = kThreads / CH;  // of the copies through registers
   constexpr int BUFS = PARTS == 1 ? 2 : 1;
+  constexpr bool U = CAP && !SLOPE && PARTS == 1;
   typedef Tile<KB, DP, PARTS> KV;
   // two buffers by name: the compiler has to see that a copy into one does not change what is read from the other
   __shared__ __align__(16) uint16_t k_lds0[KV::kPlane * PARTS], v_lds0[KV::kPlane * PARTS];
@@ -184,19 +185,15 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel
   __shared__ int range_lds[4][2];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, hh = lane >> 5, c = lane & 31;
   const int tiles = (p.Nq + kQB - 1) / kQB;
-  int64_t id = xcd_run(blockIdx.x, gridDim.x);
-  const int part = static_cast<int>(id % parts.n);
-  id /= parts.n;
-  const int g = static_cast<int>(id % p.G);
-  id /= p.G;
-  const int q0 = static_cast<int>(tiles - 1 - id % tiles) * kQB;  // the longest rows of a causal mask first
-  id /= tiles;
-  const int hk = static_cast<int>(id % p.Hk), b = static_cast<int>(id / p.Hk), h = hk * p.G + g;
+  const Unit unit(blockIdx.x, p.G * parts.n, static_cast<int64_t>(p.B) * p.Hk);
+  const int part = unit.inner % parts.n, g = unit.inner / parts.n;
+  const int q0 = (tiles - 1 - unit.tile) * kQB;  // the longest rows of a causal mask first
+  const int hk = static_cast<int>(unit.pair % p.Hk), b = static_cast<int>(unit.pair / p.Hk), h = hk * p.G + g;
   const int n = kv_length(p, b);
 
   const int i = q0 + 32 * wave + c, row = i < p.Nq ? i : p.Nq - 1;
   const Sight me(p, b, row, n);
-  const float slope2 = p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
+  const float slope2 = SLOPE ? p.slopes[h] * kLog2e : 0.f;
   const int wave_first = __builtin_amdgcn_readfirstlane(me.last);
   const int wave_last = __builtin_amdgcn_readlane(me.last, 31);
   // keys that any query of the workgroup may see: the last query's
@@ -290,25 +287,24 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel
       const bool masked = mixed || k0 + KB - 1 > wave_first;
       v16f s[NB];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        s[nb] = v16f{};
-#pragma unroll
-        for (int ds = 0; ds < DP / 16; ++ds) s[nb] = mma(kt.rows(32 * nb, ds, lane), q[ds], s[nb]);
-      }
+      for (int nb = 0; nb < NB; ++nb) s[nb] = v16f{};
+      ahead<DP / 16 * NB>([&](int i) { return kt.rows(32 * (i % NB), i / NB, lane); },
+                          [&](int i, const Frag<PARTS>& x) { s[i % NB] = mma(x, q[i / NB], s[i % NB]); });
       settle(s);
-      scores<PARTS, CAP, U>(s, p, me, slope2, k0, hh, masked, mixed ? doc_lds[B] : nullptr);
+      scores<PARTS, CAP, SLOPE, U>(s, p, me, slope2, k0, hh, masked, mixed ? doc_lds[B] : nullptr);
       float alpha = 1.f;
       if (weigh<U>(s, p, run, alpha)) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
       }
+      Frag<PARTS> w[2 * NB];
 #pragma unroll
       for (int st = 0; st < 2 * NB; ++st) {
-        const Frag<PARTS> w = frag_of<PARTS>(s[st / 2], st % 2);
-        add_weights(w, s[st / 2], st % 2, run.l);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] = mma(vt.columns(16 * st, dt, lane), w, o[dt]);
+        w[st] = frag_of<PARTS>(s[st / 2], st % 2);
+        add_weights(w[st], s[st / 2], st % 2, run.l);
       }
+      ahead<2 * NB * DT>([&](int i) { return vt.columns(16 * (i / DT), i % DT, lane); },
+                         [&](int i, const Frag<PARTS>& x) { o[i % DT] = mma(x, w[i / DT], o[i % DT]); });
     }
     t = after;
     here = there;
@@ -350,139 +346,218 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel
   if (p.lse != nullptr && hh == 0) p.lse[at] = l == 0.f ? kNegInf : (run.m + log2f(l)) * kLn2;
 }
 
-// Few queries: column pr of the products is query pr / G, head hk G + pr % G. Runs of `chunk` keys, one a
-// wave.
-template <int DP, int PARTS, bool CAP>
-__global__ void __launch_bounds__(kThreads) token_few_kernel(Params p, int chunk, int runs, Parts parts) {
-  constexpr int DT = DP / 32, CH = DP / 8, LOADS = 32 * CH / 64, STEP = 64 / CH;
+// Few queries: column pr of the products is query pr / G, head hk G + pr % G; CB blocks of 16 columns. Runs of `chunk`
+// keys, one a wave, 32 keys at a time on v_mfma_f32_16x16x32_bf16 (token_device.h's layouts with 16-lane groups g: a
+// lane's weights belong to keys 16 (j / 4) + 4 g + j % 4). Keys go from memory into the products' registers, values
+// through LDS of the wave's own; each is loaded again as soon as its registers are free, so about 32 rows of
+// each are in flight a wave all the time.
+template <int DP, int PARTS, bool CAP, int CB>
+__global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_few_kernel(Params p, int chunk, Parts parts) {
+  constexpr int DS = DP / 32, DT = DP / 16, CH = DP / 8, LOADS = 32 * CH / 64, STEP = 64 / CH;
   typedef Tile<32, DP, PARTS> V;
   __shared__ __align__(16) uint16_t v_lds[4][V::kPlane * PARTS];
   __shared__ __align__(16) int doc_lds[4][32];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, hh = lane >> 5, c = lane & 31;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const V vt{v_lds[wave]};
-  const int per = (runs + 3) / 4;
+  const int per = (parts.n + 3) / 4;
   int64_t id = blockIdx.x;
   const int run_id = 4 * static_cast<int>(id % per) + wave;
   id /= per;
   const int hk = static_cast<int>(id % p.Hk), b = static_cast<int>(id / p.Hk);
-  const int n = kv_length(p, b), first = run_id * chunk;
-  if (run_id >= runs || first >= n) return;  // waves share nothing: no barriers
-  const int stop = min(n, first + chunk);
-  const int rows = p.Nq * p.G, pr = c < rows ? c : rows - 1, i = pr / p.G, h = hk * p.G + pr % p.G;
-  const Sight me(p, b, i, n);
-  const float slope2 = p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
-  Frag<PARTS> q[DP / 16];
+  const int n = kv_length(p, b);
+  const int64_t first64 = static_cast<int64_t>(run_id) * chunk;
+  if (run_id >= parts.n || first64 >= n) return;  // waves share nothing: no barriers
+  const int first = static_cast<int>(first64), stop = min(n, first + chunk);
+  const bool by_document = p.documents != nullptr;
+  const int rows = p.Nq * p.G;
+  Frag<PARTS> q[CB][DS];
+  Sight me[CB] = {};
+  float slope2[CB];
+  int64_t at[CB];
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    Raw8<PARTS> r;
-    const int d = 16 * s + 8 * hh;
-    r.load(p.q.data, b * p.q.batch + i * p.q.token + h * p.q.head + d, d < p.D);
-    q[s] = frag(r);
-  }
-  v16f o[DT];
+  for (int cb = 0; cb < CB; ++cb) {
+    const int pr = min(16 * cb + c, rows - 1), i = pr / p.G, h = hk * p.G + pr % p.G;
+    me[cb] = Sight(p, b, i, n);
+    slope2[cb] = p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
+    at[cb] = ((static_cast<int64_t>(b) * p.Nq + i) * p.H + h) * parts.n + run_id;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) o[dt] = v16f{};
-  Running run;
-  const int lr = lane / CH, lc = lane % CH;
-  for (int k0 = first; k0 < stop; k0 += 32) {
-    Raw8<PARTS> rk[DP / 16], rv[LOADS];
-    const int key = k0 + c;
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      const int d = 16 * s + 8 * hh;
-      rk[s].load(p.k.data, b * p.k.batch + key * p.k.token + hk * p.k.head + d, key < n && d < p.D);
+    for (int s = 0; s < DS; ++s) {
+      Raw8<PARTS> r;
+      const int d = 32 * s + 8 * g;
+      r.load(p.q.data, b * p.q.batch + i * p.q.token + h * p.q.head + d, d < p.D);
+      q[cb][s] = frag(r);
     }
+  }
+  v4f o[CB][DT];
+  Running run[CB];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[cb][dt] = zero4();
+
+  const int lr = lane / CH, lc = lane % CH;
+  Raw8<PARTS> rk[2][DS], rv[LOADS];
+  int rdoc = -1;
+  auto load_k = [&](int k0) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int64_t key = min(k0 + 16 * kb + c, n - 1);  // behind the end: a real row, hidden by the mask
+#pragma unroll
+      for (int s = 0; s < DS; ++s) {
+        const int d = 32 * s + 8 * g;
+        rk[kb][s].load(p.k.data, b * p.k.batch + key * p.k.token + hk * p.k.head + d, d < p.D);
+      }
+    }
+  };
+  auto load_v = [&](int k0) {
+    if (by_document && lane < 32) rdoc = k0 + lane < n ? p.documents[static_cast<int64_t>(b) * p.Nk + k0 + lane] : -1;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-      const int kv = k0 + lr + STEP * j;
-      bool on = kv < n && 8 * lc < p.D;
-      if (p.documents != nullptr && on) on = key_document(p, b, kv) >= 0;
-      rv[j].load(p.v.data, b * p.v.batch + kv * p.v.token + hk * p.v.head + 8 * lc, on);
+      const int64_t key = min(k0 + lr + STEP * j, n - 1);
+      bool on = 8 * lc < p.D;
+      if (by_document && on) on = p.documents[static_cast<int64_t>(b) * p.Nk + key] >= 0;  // padding may hold anything
+      rv[j].load(p.v.data, b * p.v.batch + key * p.v.token + hk * p.v.head + 8 * lc, on);
     }
-    if (p.documents != nullptr && lane < 32) doc_lds[wave][lane] = key < n ? key_document(p, b, key) : -1;
+  };
+  load_v(first);
+  load_k(first);
+  for (int k0 = first; k0 < stop; k0 += 32) {
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) vt.put(lr + STEP * j, lc, frag(rv[j]));
+    if (by_document && lane < 32) doc_lds[wave][lane] = max(rdoc, -1);
+    if (k0 + 32 < stop) load_v(k0 + 32);
+    v4f s[CB][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      Frag<PARTS> k[DS];
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) k[ds] = frag(rk[kb][ds]);
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        s[cb][kb] = zero4();
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) s[cb][kb] = mma16(k[ds], q[cb][ds], s[cb][kb]);
+      }
+    }
+    if (k0 + 32 < stop) load_k(k0 + 32);
+    settle(s);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    v16f s[1] = {v16f{}};
+    Frag<PARTS> w[CB];
 #pragma unroll
-    for (int ds = 0; ds < DP / 16; ++ds) s[0] = mma(frag(rk[ds]), q[ds], s[0]);
-    settle(s);
-    scores<PARTS, CAP, false>(s, p, me, slope2, k0, hh, true, p.documents != nullptr ? doc_lds[wave] : nullptr);
-    float alpha = 1.f;
-    if (weigh<false>(s, p, run, alpha)) {
+    for (int cb = 0; cb < CB; ++cb) {
+      const int k1 = k0 + 4 * g;
+      float x[8], top = kNegInf;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+      for (int i = 0; i < 8; ++i) {
+        const int key = k1 + 16 * (i / 4) + i % 4;
+        x[i] = s[cb][i / 4][i % 4];
+        x[i] = CAP ? tanh_of<PARTS>(x[i] * p.to_tanh) * p.to_score2 : x[i] * p.to_score2;
+        if (slope2[cb] != 0.f) x[i] -= slope2[cb] * static_cast<float>(abs(me[cb].pos - key));
+        x[i] = key <= me[cb].last ? x[i] : kNegInf;
+      }
+      if (by_document) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = doc_lds[wave][4 * g + 16 * (i / 4) + i % 4] == me[cb].doc ? x[i] : kNegInf;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
+      top = group_max(top);
+      Running& r = run[cb];
+      if (__any(top > r.m)) {
+        const float m = fmaxf(r.m, top), alpha = r.m == kNegInf ? 0.f : fast_exp2(r.m - m);
+        r.m = m;
+        r.l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[cb][dt] *= alpha;
+      }
+      const float base = r.m == kNegInf ? 0.f : r.m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = fast_exp2(x[i] - base);
+      v16f y = v16f{};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[i];
+      w[cb] = frag_of<PARTS>(y, 0);
+      add_weights(w[cb], y, 0, r.l);
     }
 #pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      const Frag<PARTS> w = frag_of<PARTS>(s[0], st);
-      add_weights(w, s[0], st, run.l);
+    for (int dt = 0; dt < DT; ++dt) {
+      const Frag<PARTS> v = vt.columns16(dt, lane);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] = mma(vt.columns(16 * st, dt, lane), w, o[dt]);
+      for (int cb = 0; cb < CB; ++cb) o[cb][dt] = mma16(v, w[cb], o[cb][dt]);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
   settle(o);
-  const float l = xor32_pair_sum(run.l);
-  if (c >= rows) return;
-  const int64_t at = ((static_cast<int64_t>(b) * p.Nq + i) * p.H + h) * runs + run_id;
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+  for (int cb = 0; cb < CB; ++cb) {
+    const float l = group_sum(run[cb].l);
+    if (16 * cb + c < rows) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * dt + 8 * g + 4 * hh;
-      if (d < p.D)
-        *reinterpret_cast<v4f*>(parts.partial + at * p.D + d) =
-            v4f{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+      for (int dt = 0; dt < DT; ++dt) {
+        const int d = 16 * dt + 4 * g;
+        if (d < p.D) *reinterpret_cast<v4f*>(parts.partial + at[cb] * p.D + d) = o[cb][dt];
+      }
+      if (g == 0) {
+        parts.stats[at[cb] * 2] = run[cb].m;
+        parts.stats[at[cb] * 2 + 1] = l;
+      }
     }
-  if (hh == 0) {
-    parts.stats[at * 2] = run.m;
-    parts.stats[at * 2 + 1] = l;
   }
 }
 
-// Joins the parts of one row of (b, i, h), a wave a row. chunk: keys a part, of which those that begin behind the
-// row's end were not written; 0: all parts were.
+// Joins the parts of one row of (b, i, h), a workgroup a row: eight half waves take the parts in turn, four elements a
+// lane. chunk: keys a part, of which those that begin behind the row's end were not written; 0: all parts were.
 template <int PARTS>
 __global__ void __launch_bounds__(kThreads) token_join_kernel(Params p, int chunk, Parts parts) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (at >= static_cast<int64_t>(p.B) * p.Nq * p.H) return;
-  const int b = static_cast<int>(at / (static_cast<int64_t>(p.Nq) * p.H)), lane = threadIdx.x & 63;
-  const int used = chunk > 0 ? (kv_length(p, b) + chunk - 1) / chunk : parts.n;
-  const float* const st = parts.stats + at * parts.n * 2;
-  float m = kNegInf;
-  for (int r = lane; r < used; r += 64) m = fmaxf(m, st[2 * r]);
+  __shared__ __align__(16) float o_lds[8][HZ_TOKEN_MAX_HEAD];
+  __shared__ float l_lds[8];
+  const int64_t rows = static_cast<int64_t>(p.B) * p.Nq * p.H;
+  const int lane = threadIdx.x & 63, half = threadIdx.x >> 5, d = 4 * (threadIdx.x & 31);
+  for (int64_t at = blockIdx.x; at < rows; at += gridDim.x) {
+    const int b = static_cast<int>(at / (static_cast<int64_t>(p.Nq) * p.H));
+    const int used = chunk > 0 ? (kv_length(p, b) + chunk - 1) / chunk : parts.n;
+    const float* const st = parts.stats + at * parts.n * 2;
+    float m = kNegInf;
+    for (int r = lane; r < used; r += 64) m = fmaxf(m, st[2 * r]);
 #pragma unroll
-  for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-  const float base = m == kNegInf ? 0.f : m;
-  // four elements a lane, two half waves on parts of their own
-  const int d = 4 * (lane & 31), half = lane >> 5;
-  float l = 0.f;
-  v4f o = zero4();
+    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+    const float base = m == kNegInf ? 0.f : m;
+    float l = 0.f;
+    v4f o = zero4();
 #pragma unroll 4
-  for (int r = half; r < used; r += 2) {
-    const float a = fast_exp2(st[2 * r] - base);
-    l += a * st[2 * r + 1];
-    if (d < p.D) o += a * *reinterpret_cast<const v4f*>(parts.partial + (at * parts.n + r) * p.D + d);
-  }
-  l = xor32_pair_sum(l);
+    for (int r = half; r < used; r += 8) {
+      const float a = fast_exp2(st[2 * r] - base);
+      l += a * st[2 * r + 1];
+      if (d < p.D) o += a * *reinterpret_cast<const v4f*>(parts.partial + (at * parts.n + r) * p.D + d);
+    }
+    *reinterpret_cast<v4f*>(&o_lds[half][d]) = o;
+    if (d == 0) l_lds[half] = l;
+    __syncthreads();
+    if (half == 0) {
 #pragma unroll
-  for (int x = 0; x < 4; ++x) o[x] = xor32_pair_sum(o[x]);
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  if (half == 0 && d < p.D) store_out<PARTS>(p, at * p.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-  if (p.lse != nullptr && lane == 0) p.lse[at] = l == 0.f ? kNegInf : (m + log2f(l)) * kLn2;
+      for (int x = 1; x < 8; ++x) {
+        l += l_lds[x];
+        o += *reinterpret_cast<const v4f*>(&o_lds[x][d]);
+      }
+      l = __shfl(l, 0, 32);
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      if (d < p.D) store_out<PARTS>(p, at * p.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+      if (p.lse != nullptr && d == 0) p.lse[at] = l == 0.f ? kNegInf : (m + log2f(l)) * kLn2;
+    }
+    __syncthreads();
+  }
 }
 
 // The few-query kernel takes the calls whose rows of query and head fit the 32 columns of one product.
 bool few(const hz_token_attention& a) { return a.Nq * (a.H / a.Hk) <= 32; }
 
-// Keys a run: about 8192 waves in all, at least one block of 32 keys.
+// Keys a run: about 6144 waves in all (two rounds of the card's), at least one block of 32 keys.
 int run_keys(const hz_token_attention& a) {
-  const int64_t keys = (a.B * a.Hk * a.Nk + 8191) / 8192;
+  const int64_t keys = (a.B * a.Hk * a.Nk + 6143) / 6144;
   return static_cast<int>((keys + 31) / 32 * 32);
 }
 
@@ -512,20 +587,23 @@ hipError_t run(const hz_token_attention& a, void* workspace, hipStream_t stream)
   int chunk = 0;
   if (few(a)) {
     chunk = run_keys(a);
-    token_few_kernel<DP, PARTS, CAP><<<static_cast<unsigned>(a.B * a.Hk * ((parts.n + 3) / 4)), kThreads, 0, stream>>>(
-        p, chunk, parts.n, parts);
+    const unsigned grid = static_cast<unsigned>(a.B * a.Hk * ((parts.n + 3) / 4));
+    if (a.Nq * (a.H / a.Hk) <= 16)
+      token_few_kernel<DP, PARTS, CAP, 1><<<grid, kThreads, 0, stream>>>(p, chunk, parts);
+    else
+      token_few_kernel<DP, PARTS, CAP, 2><<<grid, kThreads, 0, stream>>>(p, chunk, parts);
   } else {
     DocTile* const tiles = reinterpret_cast<DocTile*>(static_cast<char*>(workspace) + (parts_bytes(a) + 15) / 16 * 16);
     if (p.documents != nullptr)
       if (hipError_t err = launch_doc_tiles(p, tiles, stream); err != hipSuccess) return err;
     const unsigned grid = static_cast<unsigned>(blocks_of(a) * parts.n);
-    if (CAP && PARTS == 1 && p.slopes == nullptr)
-      token_fwd_kernel<DP, PARTS, CAP, CAP && PARTS == 1><<<grid, kThreads, 0, stream>>>(p, tiles, parts);
+    if (p.slopes != nullptr)
+      token_fwd_kernel<DP, PARTS, CAP, true><<<grid, kThreads, 0, stream>>>(p, tiles, parts);
     else
       token_fwd_kernel<DP, PARTS, CAP, false><<<grid, kThreads, 0, stream>>>(p, tiles, parts);
     if (parts.n == 1) return hipGetLastError();
   }
-  token_join_kernel<PARTS><<<static_cast<unsigned>((rows + 3) / 4), kThreads, 0, stream>>>(p, chunk, parts);
+  token_join_kernel<PARTS><<<static_cast<unsigned>(rows < 65536 ? rows : 65536), kThreads, 0, stream>>>(p, chunk, parts);
   return hipGetLastError();
 }
 

@@ -121,6 +121,15 @@ __device__ __forceinline__ v16f mma(const Frag<3>& a, const Frag<3>& b, v16f c) 
   return c;
 }
 
+__device__ __forceinline__ v4f mma16(const Frag<1>& a, const Frag<1>& b, v4f c) {
+  return mfma16_bf16(as_bf16x8(a.p[0]), as_bf16x8(b.p[0]), c);
+}
+__device__ __forceinline__ v4f mma16(const Frag<3>& a, const Frag<3>& b, v4f c) {
+#pragma unroll
+  for (int t = 0; t < kSplitTerms; ++t) c = mfma16_bf16(as_bf16x8(a.p[kSplitA[t]]), as_bf16x8(b.p[kSplitB[t]]), c);
+  return c;
+}
+
 // Products are waited for here, before any branch: a vector instruction may read a product's result only some
 // wait states after it, and where paths of different lengths lead from one to the other the compiler
 // (ROCm 7.2's) counts them on one path only. Twenty wait states are more than the twelve that the 32 x 32 x 16
@@ -132,6 +141,38 @@ __device__ __forceinline__ void settle(v16f (&x)[N]) {
 #pragma unroll
   for (int n = 0; n < N; ++n) asm volatile("" : "+v"(x[n]));
   __builtin_amdgcn_sched_barrier(0);
+}
+template <int M, int N>
+__device__ __forceinline__ void settle(v4f (&x)[M][N]) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 3");
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int n = 0; n < N; ++n) asm volatile("" : "+v"(x[m][n]));
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// x, which the compiler takes for a new value: addresses formed from it are formed again where they are used
+// and do not hold registers all through a loop.
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// N steps of use(i, load(i)) with the next step's operands read from LDS ahead of each step's products: left alone, the
+// compiler reads an operand right before the product that needs it and waits for LDS every time.
+template <int N, class Load, class Use>
+__device__ __forceinline__ void ahead(Load load, Use use) {
+  auto now = load(0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    auto next = now;
+    if (i + 1 < N) next = load(i + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    use(i, now);
+    now = next;
+  }
 }
 
 // A tile of ROWS rows of DP elements in LDS, PARTS planes.
@@ -179,6 +220,23 @@ struct Tile {
     }
     return f;
   }
+  // The same for the 16 x 16 x 32 product over 32 rows: lane 16 g + c gets column 16 dt + c of the rows
+  // 16 (j / 4) + 4 g + j % 4.
+  __device__ __forceinline__ Frag<PARTS> columns16(int dt, int lane) const {
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    const int g = lane >> 4, m = lane & 15, row = 4 * g + (m >> 2);
+    const int o0 = (at(row, (m & 3) >> 1) ^ (dt << 4)) + 4 * (m & 1);  // chunk 2 dt + ..
+    const int o1 = o0 + 16 * DP;  // the swizzle repeats after sixteen rows
+    Frag<PARTS> f;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(base + i * kPlane + o0));
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(base + i * kPlane + o1));
+      const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
+      f.p[i] = v4u{l.x, l.y, h.x, h.y};
+    }
+    return f;
+  }
 };
 
 // tanh by 1 - 2 / (1 + e^2y). Its error, an absolute 1e-7, is a relative one of small scores, which
@@ -205,6 +263,7 @@ __device__ __forceinline__ int kv_length(const Params& p, int b) {
 constexpr int kNoDocument = -2147483647 - 1;
 struct Sight {
   int pos, last, doc;
+  Sight() = default;
   __device__ __forceinline__ Sight(const Params& p, int b, int i, int n) {
     pos = n - p.Nq + i;
     last = n - 1;
@@ -233,11 +292,19 @@ struct DocTile {
 };
 constexpr int kDocTile = 64;
 
-// The blocks of one kernel in an order that gives each of the 8 XCDs (their L2 caches) a consecutive run.
-__device__ __forceinline__ int64_t xcd_run(int64_t hw, int64_t n) {
-  const int64_t x = hw % 8, each = n / 8, more = n % 8;
-  return x * each + (x < more ? x : more) + hw / 8;
-}
+// Which unit of work a workgroup takes: `inner` workgroups on each of `pairs` pairs of (row of the batch, key head), for
+// one tile after the other, so that every XCD (workgroups go round the 8 by their number) gets its share of the long
+// tiles. (Pairs kept on XCDs of their own, for their L2, were no faster forward and 3 to 10% slower in reverse:
+// attn_train_packed_bf16 761 us so, 787 to 836 with pairs on XCDs.)
+struct Unit {
+  int inner, tile;
+  int64_t pair;
+  __device__ __forceinline__ Unit(int64_t id, int inner_, int64_t pairs) {
+    inner = static_cast<int>(id % inner_);
+    pair = id / inner_ % pairs;
+    tile = static_cast<int>(id / inner_ / pairs);
+  }
+};
 
 // Copies rows of a strided tensor straight into a Tile of bfloat16 (16 bytes a lane, no registers): what a lane
 // reads is chosen so that lane i's 16 bytes land where the tile wants them. Rows behind the last one
@@ -245,7 +312,7 @@ __device__ __forceinline__ int64_t xcd_run(int64_t hw, int64_t n) {
 template <int ROWS, int DP>
 struct Copy {
   static constexpr int CH = DP / 8, LOADS = ROWS * CH / 256;
-  const uint16_t* base;
+  const uint16_t *base, *mine;  // the head's first row at this lane's chunk; this lane's row of the first tile
   int64_t token;
   int row, wave;  // this lane's row in the first of LOADS parts; STEP rows between parts
   static constexpr int STEP = 256 / CH;
@@ -255,14 +322,20 @@ struct Copy {
     const int chunk = (tid % CH) ^ Tile<ROWS, DP, 1>::swizzle(row);
     base = static_cast<const uint16_t*>(t.data) + b * t.batch + h * t.head + (8 * chunk < D ? 8 * chunk : 0);
     token = t.token;
+    mine = base + row * token;
   }
   __device__ __forceinline__ void operator()(uint16_t* lds, int r0, int rows) const {
+    if (r0 + ROWS <= rows) {  // one addition of a scalar an address
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const uint16_t* const src = base + static_cast<int64_t>(min(r0 + row + STEP * j, rows - 1)) * token;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                       (__attribute__((address_space(3))) void*)(lds + (4 * j + wave) * 512), 16, 0, 0);
+      for (int j = 0; j < LOADS; ++j) one(lds, j, mine + (r0 + STEP * j) * token);
+    } else {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) one(lds, j, base + static_cast<int64_t>(min(r0 + row + STEP * j, rows - 1)) * token);
     }
+  }
+  __device__ __forceinline__ void one(uint16_t* lds, int j, const uint16_t* src) const {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)(lds + (4 * j + wave) * 512), 16, 0, 0);
   }
 };
 // The copies issued so far have landed in LDS for every wave that passes the barrier behind this.
