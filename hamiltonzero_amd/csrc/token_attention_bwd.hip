@@ -62,9 +62,18 @@ __device__ __forceinline__ float grad_scale(const Params& p) {
   return CAP && PARTS == 1 ? 4.f * p.scale : p.scale;
 }
 
+// Sums made by several workgroups: `n` shares, partial [n][tensors][elements] in float32 for a last kernel to add up.
+struct Splits {
+  float* partial;
+  int64_t elements;
+  int n;      // 1: not divided, the results go where they belong
+  int heads;  // of dk, dv: shares of the query heads; n / heads parts of the queries
+};
+
 template <int DP, int PARTS, bool CAP, bool SLOPE>
-__global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Params p, hz_token_tensor dout, void* dq,
-                                                                           float* deltas, const DocTile* doc_tiles) {
+__global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_kernel(Params p, hz_token_tensor dout, void* dq,
+                                                                           float* deltas, const DocTile* doc_tiles,
+                                                                                      Splits splits) {
   constexpr int KB = kRows<DP, PARTS>, NB = KB / 32, DT = DP / 32, CH = DP / 8;
   constexpr int LOADS = KB * CH / 256, STEP = 256 / CH;
   constexpr int BUFS = PARTS == 1 ? 2 : 1;
@@ -75,9 +84,10 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
   __shared__ int range_lds[4][2];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, hh = lane >> 5, c = lane & 31;
   const int tiles = (p.Nq + kBlock - 1) / kBlock;
-  const Unit unit(blockIdx.x, p.G, static_cast<int64_t>(p.B) * p.Hk);
+  const Unit unit(blockIdx.x, p.G * splits.n, static_cast<int64_t>(p.B) * p.Hk);
+  const int part = unit.inner % splits.n;
   const int q0 = (tiles - 1 - unit.tile) * kBlock;  // the longest rows of a causal mask first
-  const int hk = static_cast<int>(unit.pair % p.Hk), b = static_cast<int>(unit.pair / p.Hk), h = hk * p.G + unit.inner;
+  const int hk = static_cast<int>(unit.pair % p.Hk), b = static_cast<int>(unit.pair / p.Hk), h = hk * p.G + unit.inner / splits.n;
   const int n = kv_length(p, b);
   const int i = q0 + 32 * wave + c, row = i < p.Nq ? i : p.Nq - 1;
   const Sight me(p, b, row, n);
@@ -85,7 +95,6 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
   const int wave_first = __builtin_amdgcn_readfirstlane(me.last);
   const int wave_last = __builtin_amdgcn_readlane(me.last, 31);
   const int keys = Sight(p, b, min(q0 + kBlock, p.Nq) - 1, n).last + 1;
-  const int end = keys > 0 ? (keys + KB - 1) / KB : 0;
   const bool by_document = p.documents != nullptr;
   int wave_lo = 0, wave_hi = 0, lo = 0, hi = 0;
   bool one_document = false;
@@ -99,7 +108,9 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
   }
   const DocTile* const row_tiles = doc_tiles + static_cast<int64_t>(b) * ((p.Nk + kDocTile - 1) / kDocTile);
   auto range = [row_tiles](int t) { return row_tiles[t * KB / kDocTile]; };
-  Walk<decltype(range)> walk(0, end, by_document, lo, hi, range);
+  Walk<decltype(range)> walk(0, keys > 0 ? (keys + KB - 1) / KB : 0, by_document, lo, hi, range);
+  if (splits.n > 1) walk.take_part(part, splits.n, lane);
+  const int end = walk.end;
   const int64_t at = (static_cast<int64_t>(b) * p.Nq + row) * p.H + h;
 
   Frag<PARTS> q[DP / 16], go[DP / 16];
@@ -126,7 +137,7 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
     go[s] = frag(rg);
   }
   delta = xor32_pair_sum(delta);
-  if (i < p.Nq && hh == 0) deltas[at] = delta;
+  if (i < p.Nq && hh == 0 && part == 0) deltas[at] = delta;
   const float lse = p.lse[at], base = row_base<PARTS, CAP>(p, lse == kNegInf ? 0.f : lse);  // -inf: a row that sees nothing
   const float to_grad = grad_scale<PARTS, CAP>(p);
   v16f acc[DT];
@@ -155,7 +166,7 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
     }
   };
   DocTile here{}, there{};
-  int t = walk.next(0, lane, here);
+  int t = walk.next(walk.begin, lane, here);
   if (t < end) load(t, std::integral_constant<int, 0>{});
   // one tile, in buffer B
   auto step = [&](auto which) __attribute__((always_inline)) {
@@ -189,7 +200,8 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         v16f s = v16f{}, dp = v16f{};
-        ahead<DP / 16>([&](int ds) { return Two<PARTS>{kt.rows(32 * nb, ds, lane), vt.rows(32 * nb, ds, lane)}; },
+        const int l = PARTS == 3 ? anew(lane) : lane;
+        ahead<DP / 16, PARTS>([&](int ds) { return Two<PARTS>{kt.rows(32 * nb, ds, l), vt.rows(32 * nb, ds, l)}; },
                        [&](int ds, const Two<PARTS>& x) {
                          s = mma(x.a, q[ds], s);
                          dp = mma(x.b, go[ds], dp);
@@ -218,7 +230,7 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
           }
         }
         const Frag<PARTS> g[2] = {frag_of<PARTS>(s, 0), frag_of<PARTS>(s, 1)};
-        ahead<2 * DT>([&](int i) { return kt.columns(32 * nb + 16 * (i / DT), i % DT, lane); },
+        ahead<2 * DT, PARTS>([&](int i) { return kt.columns(32 * nb + 16 * (i / DT), i % DT, l); },
                       [&](int i, const Frag<PARTS>& x) { acc[i % DT] = mma(x, g[i / DT], acc[i % DT]); });
       }
     }
@@ -238,23 +250,20 @@ __global__ void __launch_bounds__(256, PARTS == 1 ? 2 : 1) token_dq_kernel(Param
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int d = 32 * dt + 8 * x + 4 * hh;
-      if (d < p.D)
+      if (d >= p.D) continue;
+      if (splits.n > 1)
+        store_four<3>(splits.partial + part * splits.elements, at * p.D + d, acc[dt][4 * x] * to_grad, acc[dt][4 * x + 1] * to_grad,
+                      acc[dt][4 * x + 2] * to_grad, acc[dt][4 * x + 3] * to_grad);
+      else
         store_four<PARTS>(dq, at * p.D + d, acc[dt][4 * x] * to_grad, acc[dt][4 * x + 1] * to_grad,
                           acc[dt][4 * x + 2] * to_grad, acc[dt][4 * x + 3] * to_grad);
     }
 }
 
-// The query heads of a key head in `n` shares, a workgroup each: partial [n][dk, dv][elements] in float32.
-struct Splits {
-  float* partial;
-  int64_t elements;
-  int n;
-};
-
 // WAVES = 8 (bfloat16): waves w and w + 4 own the same 32 keys and take the tile's first and second 32 queries;
 // their sums meet in LDS at the end. So two waves share a SIMD although a workgroup owns 128 keys only.
 template <int DP, int PARTS, bool CAP, bool SLOPE, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params p, hz_token_tensor dout, const float* deltas,
+__global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) token_dkv_kernel(Params p, hz_token_tensor dout, const float* deltas,
                                                                           void* dk, void* dv, const DocTile* doc_tiles, Splits splits) {
   constexpr int THREADS = 64 * WAVES, SETS = WAVES / 4;
   constexpr int QB = kRows<DP, PARTS>, NB = QB / 32 / SETS, DT = DP / 32, CH = DP / 8;
@@ -272,7 +281,8 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
   const Unit unit(blockIdx.x, splits.n, static_cast<int64_t>(p.B) * p.Hk);
   const int key0 = unit.tile * kBlock;  // the first keys are seen by the most queries
   const int hk = static_cast<int>(unit.pair % p.Hk), b = static_cast<int>(unit.pair / p.Hk);
-  const int first_head = unit.inner * p.G / splits.n, last_head = (unit.inner + 1) * p.G / splits.n - 1;
+  const int share = unit.inner / (splits.n / splits.heads), part = unit.inner % (splits.n / splits.heads);
+  const int first_head = share * p.G / splits.heads, last_head = (share + 1) * p.G / splits.heads - 1;
   const int n = kv_length(p, b), shift = n - p.Nq;  // position of query 0
   const int wave0 = key0 + 32 * wave, key = wave0 + c, row = key < n ? key : max(n - 1, 0);
   const int prefix = p.causal && p.prefix != nullptr ? p.prefix[b] : 0;
@@ -312,7 +322,6 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
 
   // the tiles of queries that may see a key of this block
   const int begin = p.causal && key0 >= prefix ? max(0, key0 - shift) / QB : 0;
-  const int end = key0 < n ? (p.Nq + QB - 1) / QB : 0;
   const int doc_row = (p.Nk + kDocTile - 1) / kDocTile;
   const DocTile* const row_tiles = doc_tiles + static_cast<int64_t>(b) * doc_row;
   auto range = [row_tiles, shift, n](int t) {
@@ -323,7 +332,9 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
     const DocTile z = row_tiles[last / kDocTile];
     return DocTile{min(a.lo, z.lo), max(a.hi, z.hi), a.pad | z.pad | (first < 0), 0};
   };
-  Walk<decltype(range)> walk(begin, end, by_document, lo, hi, range);
+  Walk<decltype(range)> walk(begin, key0 < n ? (p.Nq + QB - 1) / QB : 0, by_document, lo, hi, range);
+  if (splits.n > splits.heads) walk.take_part(part, splits.n / splits.heads, lane);
+  const int end = walk.end;
   const int lr = tid / CH, lc = tid % CH;
   Raw8<PARTS> rq[PARTS == 3 ? LOADS : 1], rg[PARTS == 3 ? LOADS : 1];
   float rlse = 0.f, rdelta = 0.f;  // as loaded: waited for where they are used
@@ -358,7 +369,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
     }
   };
   DocTile here{}, there{};
-  int head = first_head, t = walk.next(begin, lane, here);
+  int head = first_head, t = walk.next(walk.begin, lane, here);
   if (t < end) load(head, t, std::integral_constant<int, 0>{});
   // one tile of one head, in buffer B
   auto step = [&](auto which) __attribute__((always_inline)) {
@@ -398,7 +409,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
     int after = walk.next(t + 1, lane, there), next_head = head;
     if (after >= end && head < last_head) {
       next_head = head + 1;
-      after = walk.next(begin, lane, there);
+      after = walk.next(walk.begin, lane, there);
     }
     if (after < end) load(next_head, after, std::integral_constant<int, BUFS == 2 ? 1 - B : 0>{});
     const int p0 = shift + t * QB;  // position of the tile's first query
@@ -413,7 +424,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
         const int r0 = 32 * (nb + (SETS == 2 ? set : 0));
         v16f s = v16f{}, dp = v16f{};
         const int l = anew(lane);
-        ahead<DP / 16>(
+        ahead<DP / 16, PARTS>(
             [&](int ds) { return Three<PARTS>{qt.rows(r0, ds, l), gt.rows(r0, ds, l), vt.rows(32 * wave, ds, l)}; },
             [&](int ds, const Three<PARTS>& x) {
               s = mma(x.a, k[ds], s);
@@ -456,7 +467,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
         }
         const Frag<PARTS> w[2] = {frag_of<PARTS>(s, 0), frag_of<PARTS>(s, 1)};
         const Frag<PARTS> gs[2] = {frag_of<PARTS>(dp, 0), frag_of<PARTS>(dp, 1)};
-        ahead<2 * DT>(
+        ahead<2 * DT, PARTS>(
             [&](int i) { return Two<PARTS>{gt.columns(r0 + 16 * (i / DT), i % DT, l), qt.columns(r0 + 16 * (i / DT), i % DT, l)}; },
             [&](int i, const Two<PARTS>& x) {
               av[i % DT] = mma(x.a, w[i / DT], av[i % DT]);
@@ -536,35 +547,49 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES / 4) token_dkv_kernel(Params
     }
 }
 
-// Sums of the shares, four elements a thread.
+// Sums of the shares of one tensor, or of two of the same size, four elements a thread.
 template <int PARTS>
-__global__ void __launch_bounds__(256) token_dkv_sum_kernel(Splits splits, void* dk, void* dv) {
-  const int64_t quads = splits.elements / 4;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < 2 * quads; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t at = 4 * i;  // [dk, dv][elements]
-    v4f sum = *reinterpret_cast<const v4f*>(splits.partial + at);
-    for (int s = 1; s < splits.n; ++s) sum += *reinterpret_cast<const v4f*>(splits.partial + s * 2 * splits.elements + at);
+__global__ void __launch_bounds__(256) token_sum_kernel(Splits splits, int tensors, void* first, void* second) {
+  const int64_t quads = splits.elements / 4, all = tensors * quads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+    v4f sum = *reinterpret_cast<const v4f*>(splits.partial + 4 * i);
+#pragma unroll 4
+    for (int s = 1; s < splits.n; ++s) sum += *reinterpret_cast<const v4f*>(splits.partial + 4 * (s * all + i));
     if (i < quads)
-      store_four<PARTS>(dk, at, sum[0], sum[1], sum[2], sum[3]);
+      store_four<PARTS>(first, 4 * i, sum[0], sum[1], sum[2], sum[3]);
     else
-      store_four<PARTS>(dv, at - splits.elements, sum[0], sum[1], sum[2], sum[3]);
+      store_four<PARTS>(second, 4 * (i - quads), sum[0], sum[1], sum[2], sum[3]);
   }
 }
 
-int64_t dkv_blocks(const hz_token_attention& a) { return a.B * a.Hk * ((a.Nk + kBlock - 1) / kBlock); }
-
-// Shares of a key head's query heads: until there are two workgroups a CU, as far as the heads divide. (Documents and
-// causal masks make workgroups of very different lengths, which a single round of them cannot even out.)
-int dkv_splits(const hz_token_attention& a) {
-  const int64_t G = a.H / a.Hk, blocks = dkv_blocks(a);
-  int64_t n = 1;
-  while (n < G && (blocks * n < 512 || G % n != 0)) ++n;
-  return static_cast<int>(n);
+template <int PARTS>
+void launch_sum(const Splits& splits, int tensors, void* first, void* second, hipStream_t stream) {
+  if (splits.n == 1) return;
+  const int64_t n = (tensors * splits.elements / 4 + 255) / 256;
+  token_sum_kernel<PARTS><<<static_cast<unsigned>(n < 8192 ? n : 8192), 256, 0, stream>>>(splits, tensors, first, second);
 }
 
+// Workgroups are made more by dividing the keys (dq), the query heads of a key head and then the queries (dk, dv):
+// documents and causal masks make them of very different lengths, which a single round of them cannot even out, and a
+// few long sequences would leave most CUs idle. The sum of the shares costs little beside that
+// (attn_train_packed_bf16: dk and dv in four shares 355 us and 15 for the sum, 661 in one).
+Splits dq_splits(const hz_token_attention& a) {
+  const int64_t blocks = a.B * a.H * ((a.Nq + kBlock - 1) / kBlock);
+  return {nullptr, a.B * a.Nq * a.H * a.D, share_of(blocks, a.Nk, 512), 1};
+}
+
+Splits dkv_splits(const hz_token_attention& a) {
+  const int64_t G = a.H / a.Hk, blocks = a.B * a.Hk * ((a.Nk + kBlock - 1) / kBlock);
+  int64_t heads = 1;
+  while (heads < G && (blocks * heads < 512 || G % heads != 0)) ++heads;
+  return {nullptr, a.B * a.Nk * a.Hk * a.D, static_cast<int>(heads) * share_of(blocks * heads, a.Nq, 512), static_cast<int>(heads)};
+}
+
+// The two sums are made one after the other in the same memory.
 int64_t split_bytes(const hz_token_attention& a) {
-  const int n = dkv_splits(a);
-  return n > 1 ? n * 2 * a.B * a.Nk * a.Hk * a.D * static_cast<int64_t>(sizeof(float)) : 0;
+  auto bytes = [](const Splits& s, int tensors) { return s.n > 1 ? s.n * tensors * s.elements * static_cast<int64_t>(sizeof(float)) : 0; };
+  const int64_t q = bytes(dq_splits(a), 1), kv = bytes(dkv_splits(a), 2);
+  return q > kv ? q : kv;
 }
 
 int64_t delta_bytes(const hz_token_attention& a) {
@@ -577,17 +602,16 @@ hipError_t run(const hz_token_attention& a, const hz_token_tensor& dout, void* d
   constexpr int WAVES = PARTS == 1 ? 8 : 4;
   const Params p = make_params(a);
   float* const deltas = static_cast<float*>(workspace);
-  const Splits splits{reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a)), a.B * a.Nk * a.Hk * a.D, dkv_splits(a)};
+  Splits of_q = dq_splits(a), of_kv = dkv_splits(a);
+  of_q.partial = of_kv.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a));
   DocTile* const tiles = reinterpret_cast<DocTile*>(static_cast<char*>(workspace) + delta_bytes(a) + split_bytes(a));
   if (p.documents != nullptr)
     if (hipError_t err = launch_doc_tiles(p, tiles, stream); err != hipSuccess) return err;
-  const int64_t nq = a.B * a.H * ((a.Nq + kBlock - 1) / kBlock), nk = dkv_blocks(a) * splits.n;
-  token_dq_kernel<DP, PARTS, CAP, SLOPE><<<static_cast<unsigned>(nq), 256, 0, stream>>>(p, dout, dq, deltas, tiles);
-  token_dkv_kernel<DP, PARTS, CAP, SLOPE, WAVES><<<static_cast<unsigned>(nk), 64 * WAVES, 0, stream>>>(p, dout, deltas, dk, dv, tiles, splits);
-  if (splits.n > 1) {
-    const int64_t n = (splits.elements / 2 + 255) / 256;
-    token_dkv_sum_kernel<PARTS><<<static_cast<unsigned>(n < 8192 ? n : 8192), 256, 0, stream>>>(splits, dk, dv);
-  }
+  const int64_t nq = a.B * a.H * ((a.Nq + kBlock - 1) / kBlock) * of_q.n, nk = a.B * a.Hk * ((a.Nk + kBlock - 1) / kBlock) * of_kv.n;
+  token_dq_kernel<DP, PARTS, CAP, SLOPE><<<static_cast<unsigned>(nq), 256, 0, stream>>>(p, dout, dq, deltas, tiles, of_q);
+  launch_sum<PARTS>(of_q, 1, dq, nullptr, stream);
+  token_dkv_kernel<DP, PARTS, CAP, SLOPE, WAVES><<<static_cast<unsigned>(nk), 64 * WAVES, 0, stream>>>(p, dout, deltas, dk, dv, tiles, of_kv);
+  launch_sum<PARTS>(of_kv, 2, dk, dv, stream);
   return hipGetLastError();
 }
 

@@ -172,7 +172,7 @@ struct Parts {
 };
 
 template <int DP, int PARTS, bool CAP, bool SLOPE>
-__global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel(Params p, const DocTile* doc_tiles, Parts parts) {
+__global__ void __launch_bounds__(kThreads, PARTS == 1 || DP <= 64 ? 2 : 1) token_fwd_kernel(Params p, const DocTile* doc_tiles, Parts parts) {
   constexpr int KB = kKeys<DP, PARTS>, NB = KB / 32, DT = DP / 32, CH = DP / 8;
   constexpr int LOADS = KB * CH / kThreads, STEP = kThreads / CH;  // of the copies through registers
   constexpr int BUFS = PARTS == 1 ? 2 : 1;
@@ -198,11 +198,6 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel
   const int wave_last = __builtin_amdgcn_readlane(me.last, 31);
   // keys that any query of the workgroup may see: the last query's
   const int keys = Sight(p, b, min(q0 + kQB, p.Nq) - 1, n).last + 1;
-  int begin = 0, end = keys > 0 ? (keys + KB - 1) / KB : 0;
-  if (parts.n > 1) {
-    begin = static_cast<int>(static_cast<int64_t>(end) * part / parts.n);
-    end = static_cast<int>(static_cast<int64_t>(end) * (part + 1) / parts.n);
-  }
   const bool by_document = p.documents != nullptr;
   int wave_lo = 0, wave_hi = 0, lo = 0, hi = 0;
   bool one_document = false;
@@ -216,7 +211,9 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel
   }
   const DocTile* const row_tiles = doc_tiles + static_cast<int64_t>(b) * ((p.Nk + kDocTile - 1) / kDocTile);
   auto range = [row_tiles](int t) { return row_tiles[t * KB / kDocTile]; };
-  Walk<decltype(range)> walk(begin, end, by_document, lo, hi, range);
+  Walk<decltype(range)> walk(0, keys > 0 ? (keys + KB - 1) / KB : 0, by_document, lo, hi, range);
+  if (parts.n > 1) walk.take_part(part, parts.n, lane);
+  const int end = walk.end;
 
   Frag<PARTS> q[DP / 16];
 #pragma unroll
@@ -253,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel
     }
   };
   DocTile here{}, there{};
-  int t = walk.next(begin, lane, here);
+  int t = walk.next(walk.begin, lane, here);
   if (t < end) load(t, std::integral_constant<int, 0>{});
   // one tile, in buffer B
   auto step = [&](auto which) __attribute__((always_inline)) {
@@ -288,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel
       v16f s[NB];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) s[nb] = v16f{};
-      ahead<DP / 16 * NB>([&](int i) { return kt.rows(32 * (i % NB), i / NB, lane); },
+      ahead<DP / 16 * NB, PARTS>([&](int i) { return kt.rows(32 * (i % NB), i / NB, lane); },
                           [&](int i, const Frag<PARTS>& x) { s[i % NB] = mma(x, q[i / NB], s[i % NB]); });
       settle(s);
       scores<PARTS, CAP, SLOPE, U>(s, p, me, slope2, k0, hh, masked, mixed ? doc_lds[B] : nullptr);
@@ -303,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_fwd_kernel
         w[st] = frag_of<PARTS>(s[st / 2], st % 2);
         add_weights(w[st], s[st / 2], st % 2, run.l);
       }
-      ahead<2 * NB * DT>([&](int i) { return vt.columns(16 * (i / DT), i % DT, lane); },
+      ahead<2 * NB * DT, PARTS>([&](int i) { return vt.columns(16 * (i / DT), i % DT, lane); },
                          [&](int i, const Frag<PARTS>& x) { o[i % DT] = mma(x, w[i / DT], o[i % DT]); });
     }
     t = after;
@@ -509,46 +506,50 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) token_few_kernel
   }
 }
 
-// Joins the parts of one row of (b, i, h), a workgroup a row: eight half waves take the parts in turn, four elements a
-// lane. chunk: keys a part, of which those that begin behind the row's end were not written; 0: all parts were.
-template <int PARTS>
+// Joins the parts of one row of (b, i, h): WAYS half waves take a row's parts in turn, four elements a lane; a workgroup
+// has 8 / WAYS rows at a time. chunk: keys a part, of which those that begin behind the row's end were not written; 0:
+// all parts were.
+template <int PARTS, int WAYS>
 __global__ void __launch_bounds__(kThreads) token_join_kernel(Params p, int chunk, Parts parts) {
   __shared__ __align__(16) float o_lds[8][HZ_TOKEN_MAX_HEAD];
   __shared__ float l_lds[8];
   const int64_t rows = static_cast<int64_t>(p.B) * p.Nq * p.H;
-  const int lane = threadIdx.x & 63, half = threadIdx.x >> 5, d = 4 * (threadIdx.x & 31);
-  for (int64_t at = blockIdx.x; at < rows; at += gridDim.x) {
-    const int b = static_cast<int>(at / (static_cast<int64_t>(p.Nq) * p.H));
-    const int used = chunk > 0 ? (kv_length(p, b) + chunk - 1) / chunk : parts.n;
-    const float* const st = parts.stats + at * parts.n * 2;
-    float m = kNegInf;
-    for (int r = lane; r < used; r += 64) m = fmaxf(m, st[2 * r]);
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-    const float base = m == kNegInf ? 0.f : m;
-    float l = 0.f;
+  const int lane = threadIdx.x & 31, half = threadIdx.x >> 5, way = half % WAYS, d = 4 * lane;
+  for (int64_t at0 = static_cast<int64_t>(blockIdx.x) * (8 / WAYS); at0 < rows; at0 += static_cast<int64_t>(gridDim.x) * (8 / WAYS)) {
+    const int64_t at = at0 + half / WAYS;
+    float m = kNegInf, l = 0.f;
     v4f o = zero4();
-#pragma unroll 4
-    for (int r = half; r < used; r += 8) {
-      const float a = fast_exp2(st[2 * r] - base);
-      l += a * st[2 * r + 1];
-      if (d < p.D) o += a * *reinterpret_cast<const v4f*>(parts.partial + (at * parts.n + r) * p.D + d);
-    }
-    *reinterpret_cast<v4f*>(&o_lds[half][d]) = o;
-    if (d == 0) l_lds[half] = l;
-    __syncthreads();
-    if (half == 0) {
+    if (at < rows) {
+      const int b = static_cast<int>(at / (static_cast<int64_t>(p.Nq) * p.H));
+      const int used = chunk > 0 ? (kv_length(p, b) + chunk - 1) / chunk : parts.n;
+      const float* const st = parts.stats + at * parts.n * 2;
+      for (int r = lane; r < used; r += 32) m = fmaxf(m, st[2 * r]);
 #pragma unroll
-      for (int x = 1; x < 8; ++x) {
-        l += l_lds[x];
-        o += *reinterpret_cast<const v4f*>(&o_lds[x][d]);
+      for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+      const float base = m == kNegInf ? 0.f : m;
+#pragma unroll 4
+      for (int r = way; r < used; r += WAYS) {
+        const float a = fast_exp2(st[2 * r] - base);
+        l += a * st[2 * r + 1];
+        if (d < p.D) o += a * *reinterpret_cast<const v4f*>(parts.partial + (at * parts.n + r) * p.D + d);
       }
-      l = __shfl(l, 0, 32);
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-      if (d < p.D) store_out<PARTS>(p, at * p.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-      if (p.lse != nullptr && d == 0) p.lse[at] = l == 0.f ? kNegInf : (m + log2f(l)) * kLn2;
     }
-    __syncthreads();
+    if constexpr (WAYS > 1) {
+      __syncthreads();
+      *reinterpret_cast<v4f*>(&o_lds[half][d]) = o;
+      if (lane == 0) l_lds[half] = l;
+      __syncthreads();
+      if (way != 0) continue;
+#pragma unroll
+      for (int x = 1; x < WAYS; ++x) {
+        l += l_lds[half + x];
+        o += *reinterpret_cast<const v4f*>(&o_lds[half + x][d]);
+      }
+    }
+    if (at >= rows) continue;
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    if (d < p.D) store_out<PARTS>(p, at * p.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (p.lse != nullptr && lane == 0) p.lse[at] = l == 0.f ? kNegInf : (m + log2f(l)) * kLn2;
   }
 }
 
@@ -563,14 +564,13 @@ int run_keys(const hz_token_attention& a) {
 
 int64_t blocks_of(const hz_token_attention& a) { return a.B * a.H * ((a.Nq + kQB - 1) / kQB); }
 
-// Parts of a row's keys. Many queries: as many as 512 workgroups (two a CU) want, each of at least 512 keys.
+// Parts of a row's keys. Many queries: as many as 1024 workgroups (four a CU) want, each of at least 128 keys.
 int parts_of(const hz_token_attention& a) {
   if (few(a)) {
     const int c = run_keys(a);
     return static_cast<int>((a.Nk + c - 1) / c);
   }
-  const int64_t want = 512 / blocks_of(a), most = a.Nk / 512, n = want < most ? want : most;
-  return static_cast<int>(n > 1 ? n : 1);
+  return share_of(blocks_of(a), a.Nk, 1024);
 }
 
 int64_t parts_bytes(const hz_token_attention& a) {
@@ -603,7 +603,10 @@ hipError_t run(const hz_token_attention& a, void* workspace, hipStream_t stream)
       token_fwd_kernel<DP, PARTS, CAP, false><<<grid, kThreads, 0, stream>>>(p, tiles, parts);
     if (parts.n == 1) return hipGetLastError();
   }
-  token_join_kernel<PARTS><<<static_cast<unsigned>(rows < 65536 ? rows : 65536), kThreads, 0, stream>>>(p, chunk, parts);
+  if (parts.n <= 8)
+    token_join_kernel<PARTS, 1><<<static_cast<unsigned>(rows < 8 * 65536 ? (rows + 7) / 8 : 65536), kThreads, 0, stream>>>(p, chunk, parts);
+  else
+    token_join_kernel<PARTS, 8><<<static_cast<unsigned>(rows < 65536 ? rows : 65536), kThreads, 0, stream>>>(p, chunk, parts);
   return hipGetLastError();
 }
 

@@ -161,9 +161,15 @@ __device__ __forceinline__ int anew(int x) {
 }
 
 // N steps of use(i, load(i)) with the next step's operands read from LDS ahead of each step's products: left alone, the
-// compiler reads an operand right before the product that needs it and waits for LDS every time.
-template <int N, class Load, class Use>
+// compiler reads an operand right before the product that needs it and waits for LDS every time. (Three parts: six
+// products an operand hide that wait, and the registers of a second one cost more: attn_train_sites_f32 3% slower.)
+template <int N, int PARTS, class Load, class Use>
 __device__ __forceinline__ void ahead(Load load, Use use) {
+  if constexpr (PARTS == 3) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) use(i, load(i));
+    return;
+  }
   auto now = load(0);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -240,14 +246,13 @@ struct Tile {
 };
 
 // tanh by 1 - 2 / (1 + e^2y). Its error, an absolute 1e-7, is a relative one of small scores, which
-// float32 tensors get from the series instead (the first term left out is 4e-11 of the result at 1/4).
+// float32 tensors get from the series instead (the first term left out is 1e-9 of the result at 1/8).
 template <int PARTS>
 __device__ __forceinline__ float tanh_of(float y) {
   const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + fast_exp2(2.f * kLog2e * y));
   if constexpr (PARTS == 1) return big;
   const float z = y * y;
-  const float odd = z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835 - z * (1382.f / 155925)))));
-  return fabsf(y) < 0.25f ? y + y * odd : big;
+  return fabsf(y) < 0.125f ? y + y * (z * (-1.f / 3 + z * (2.f / 15 - z * (17.f / 315)))) : big;
 }
 
 // Element i of a lane's sixteen scores of a 32-row block belongs to row 8 (i / 4) + 4 hh + i % 4.
@@ -353,6 +358,28 @@ struct Walk {
   int lo, hi;
   __device__ __forceinline__ Walk(int begin_, int end_, bool by_document_, int lo_, int hi_, Range range_)
       : begin(begin_), end(end_), group(-1), votes(0), mine{}, by_document(by_document_), range(range_), lo(lo_), hi(hi_) {}
+  // Narrows [begin, end) to the first and last tile to visit, and then to one of n equal parts.
+  __device__ __forceinline__ void take_part(int part, int n, int lane) {
+    if (by_document) {
+      DocTile doc;
+      begin = next(begin, lane, doc);
+      int last = begin;
+      for (int g = end > 0 ? (end - 1) & ~63 : -1; g >= begin - 63 && begin < end; g -= 64) {
+        const DocTile x = g + lane < end ? range(g + lane) : DocTile{2147483647, -1, 1, 0};
+        const uint64_t v = __ballot(x.lo <= hi && x.hi >= lo);
+        if (v != 0) {
+          last = g + 64 - __clzll(static_cast<long long>(v));
+          break;
+        }
+      }
+      end = max(begin, last);
+      group = -1;
+    }
+    const int64_t count = end - begin;
+    const int first = begin;
+    begin = first + static_cast<int>(count * part / n);
+    end = first + static_cast<int>(count * (part + 1) / n);
+  }
   // The first tile >= t to visit (end: none), and its documents.
   __device__ __forceinline__ int next(int t, int lane, DocTile& doc) {
     if (!by_document) return t;
@@ -397,6 +424,13 @@ __device__ __forceinline__ void store_four(void* out, int64_t off, float a, floa
     store4<BF16>(out, off, a, b, c, d);
   else
     store4<F32>(out, off, a, b, c, d);
+}
+
+// Into how many parts the n rows that a kernel streams are divided so that its `blocks` workgroups become about `want`;
+// a part has at least 128 rows.
+inline int share_of(int64_t blocks, int64_t n, int64_t want) {
+  const int64_t wanted = want / blocks, most = n / 128, parts = wanted < most ? wanted : most;
+  return static_cast<int>(parts > 1 ? parts : 1);
 }
 
 // Launch of the pass over the documents (token_attention_fwd.hip), where a call has some.
