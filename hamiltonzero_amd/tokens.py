@@ -39,12 +39,15 @@ MAX_BUCKET_RANGE = 4096
 def _on(device: torch.device):
     """The launches need ``device`` as the current one."""
     if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(device)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _ptr(t: Optional[Tensor]) -> int:
@@ -53,15 +56,24 @@ def _ptr(t: Optional[Tensor]) -> int:
 
 def _strided(t: Tensor) -> Tensor:
     """``t`` if the kernels can read it in place (contiguous heads, 16-byte rows), else a copy."""
-    st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 or n == 1 for s, n in zip(st[:-1], t.shape)):
-        return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        st = t.stride()
+        if st[-1] == 1 and all(s % 8 == 0 or n == 1 for s, n in zip(st[:-1], t.shape)):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _fields(t: Tensor) -> tuple:
     """Address and strides of batch, token and head axes; an axis of one element has none."""
-    return (t.data_ptr(), *(0 if n == 1 else s for s, n in zip(t.stride()[:-1], t.shape)))
+    (n0, n1, n2, _), (s0, s1, s2, _) = t.shape, t.stride()
+    return t.data_ptr(), 0 if n0 == 1 else s0, 0 if n1 == 1 else s1, 0 if n2 == 1 else s2
+
+
+def _like(t: Tensor) -> Tensor:
+    """A new contiguous tensor like ``t``, whose own strides may be a view's."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _check(name: str, t: Tensor, device: torch.device, dtype: torch.dtype, shape: tuple) -> None:
@@ -71,7 +83,7 @@ def _check(name: str, t: Tensor, device: torch.device, dtype: torch.dtype, shape
         raise TypeError(f"{name}.dtype must be {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}: every tensor operand must be on {device}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
 
 
@@ -82,7 +94,7 @@ def _check_first(name: str, t: Tensor, layout: str) -> None:
         raise TypeError(f"{name}.dtype must be float32 or bfloat16, got {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{name} is on {t.device}: the token operators need GPU tensors")
-    if t.dim() != 4 or 0 in t.shape:
+    if t.dim() != 4 or t.numel() == 0:
         raise ValueError(f"{name} must be {layout} with every axis at least 1 long, got {tuple(t.shape)}")
 
 
@@ -102,8 +114,7 @@ def _norm_args(q, k, q_out, k_out, w_q, w_k, freqs, positions, interleaved, eps)
 
 def _norm_fwd(q, k, w_q, w_k, freqs, positions, interleaved, eps, out=None):
     q, k = _strided(q), _strided(k)
-    q_out, k_out = out or (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-                           torch.empty(k.shape, dtype=k.dtype, device=k.device))
+    q_out, k_out = out or (_like(q), _like(k))
     args = _norm_args(q, k, q_out, k_out, w_q, w_k, freqs, positions, interleaved, eps)
     with _on(q.device):
         _native.check(_native.lib().hz_qk_norm_rotary_fwd(_stream(q.device), args))
@@ -123,8 +134,7 @@ class _QKNormRotary(torch.autograd.Function):
         q, k, w_q, w_k, freqs, positions = ctx.saved_tensors
         q, k, gq, gk = _strided(q), _strided(k), _strided(gq), _strided(gk)
         dev, D = q.device, q.shape[-1]
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=dev)
+        dq, dk = _like(q), _like(k)
         dw_q = torch.empty(D, dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
         dw_k = torch.empty(D, dtype=torch.float32, device=dev) if ctx.needs_input_grad[3] else None
         args = _norm_args(q, k, gq, gk, w_q, w_k, freqs, positions, *ctx.options)
@@ -210,7 +220,7 @@ def token_attention_fwd(q: Tensor, k: Tensor, v: Tensor, opts: tuple,
     needs besides (``out_low``, what the rounding of ``out`` left out, for bfloat16 only)."""
     q, k, v = _strided(q), _strided(k), _strided(v)
     dev = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out = _like(q)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if for_backward else None
     out_low = torch.empty_like(out) if for_backward and q.dtype == torch.bfloat16 else None
     args = _attention_args(q, k, v, out, out_low, lse, opts)
@@ -236,9 +246,7 @@ class _TokenAttention(torch.autograd.Function):
         q, k, v, out, out_low, lse, *tables = ctx.saved_tensors
         q, k, v, dout = _strided(q), _strided(k), _strided(v), _strided(dout)
         dev = q.device
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk = torch.empty(k.shape, dtype=q.dtype, device=dev)
-        dv = torch.empty(v.shape, dtype=q.dtype, device=dev)
+        dq, dk, dv = _like(q), _like(k), _like(v)
         args = _attention_args(q, k, v, out, out_low, lse, (*tables, *ctx.options))
         lib = _native.lib()
         with _on(dev):
