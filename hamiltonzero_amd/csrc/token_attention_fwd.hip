@@ -558,7 +558,7 @@ bool few(const hz_token_attention& a) { return a.Nq * (a.H / a.Hk) <= 32; }
 
 // Keys a run: about 6144 waves in all (two rounds of the card's), at least one block of 32 keys.
 int run_keys(const hz_token_attention& a) {
-  const int64_t keys = (a.B * a.Hk * a.Nk + 6143) / 6144;
+  const int64_t wanted = (a.B * a.Hk * a.Nk + 6143) / 6144, keys = wanted < a.Nk ? wanted : a.Nk;
   return static_cast<int>((keys + 31) / 32 * 32);
 }
 
