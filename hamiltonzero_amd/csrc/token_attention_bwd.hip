@@ -229,9 +229,12 @@ __global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_
             }
           }
         }
-        const Frag<PARTS> g[2] = {frag_of<PARTS>(s, 0), frag_of<PARTS>(s, 1)};
+        Frag<PARTS == 1 ? 2 : 3> g;
         ahead<2 * DT, PARTS>([&](int i) { return kt.columns(32 * nb + 16 * (i / DT), i % DT, l); },
-                      [&](int i, const Frag<PARTS>& x) { acc[i % DT] = mma(x, g[i / DT], acc[i % DT]); });
+                      [&](int i, const Frag<PARTS>& x) {
+                        if (i % DT == 0) g = grad_frag<PARTS>(s, i / DT);
+                        acc[i % DT] = mma(x, g, acc[i % DT]);
+                      });
       }
     }
     t = after;
@@ -465,13 +468,14 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
             }
           }
         }
-        const Frag<PARTS> w[2] = {frag_of<PARTS>(s, 0), frag_of<PARTS>(s, 1)};
-        const Frag<PARTS> gs[2] = {frag_of<PARTS>(dp, 0), frag_of<PARTS>(dp, 1)};
+        Frag<PARTS> w;
+        Frag<PARTS == 1 ? 2 : 3> gs;
         ahead<2 * DT, PARTS>(
             [&](int i) { return Two<PARTS>{gt.columns(r0 + 16 * (i / DT), i % DT, l), qt.columns(r0 + 16 * (i / DT), i % DT, l)}; },
             [&](int i, const Two<PARTS>& x) {
-              av[i % DT] = mma(x.a, w[i / DT], av[i % DT]);
-              ak[i % DT] = mma(x.b, gs[i / DT], ak[i % DT]);
+              if (i % DT == 0) w = frag_of<PARTS>(s, i / DT), gs = grad_frag<PARTS>(dp, i / DT);
+              av[i % DT] = mma(x.a, w, av[i % DT]);
+              ak[i % DT] = mma(x.b, gs, ak[i % DT]);
             });
       }
     }
@@ -488,7 +492,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
   settle(ak);
   settle(av);
   if constexpr (SETS == 2) {
-    // 16 accumulators a lane and round: 4 waves of 64 lanes fill the 16 DP KiB of one tile buffer's two halves
+    // 16 accumulators a lane and round: what one tile buffer of queries and one of dout hold
     float* const to[2] = {reinterpret_cast<float*>(q_lds0), reinterpret_cast<float*>(g_lds0)};
     constexpr int each = QT::kBytes / (4 * 64 * 16);  // quadruples a lane that one buffer holds
     auto join = [&](v16f(&a)[DT]) {
