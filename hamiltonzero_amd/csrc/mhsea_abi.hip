@@ -293,8 +293,12 @@ int check_token_dims(const hz_token_attention* p) {
 
 int check_token_attention(const hz_token_attention* p) {
   if (int rc = check_token_dims(p)) return rc;
-  if (!std::isfinite(p->scale)) return fail(HZ_EINVAL, "scale must be finite");
+  if (!(std::fabs(p->scale) <= 0x1p100f)) return fail(HZ_EINVAL, "scale must be finite and at most 2^100");
   if (!(p->softcap >= 0.f) || !std::isfinite(p->softcap)) return fail(HZ_EINVAL, "softcap must be finite and >= 0");
+  // an error of 1e-7 in tanh is 1e-3 in the score at the first, a quarter of bfloat16's step at 1
+  const float cap = p->dtype == HZ_DTYPE_BF16 ? 8192.f : 0x1p100f;
+  if (p->softcap > cap || (p->softcap > 0.f && !(std::fabs(p->scale) / p->softcap <= 0x1p100f)))
+    return fail(HZ_EINVAL, "softcap must be at most %g here, and scale / softcap at most 2^100", cap);
   if (p->causal != 0 && p->causal != 1) return fail(HZ_EINVAL, "causal must be 0 or 1, got %d", p->causal);
   if (p->prefix != nullptr && !p->causal) return fail(HZ_EINVAL, "prefix needs causal");
   if (int rc = check_strided("q", p->q)) return rc;

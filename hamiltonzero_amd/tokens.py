@@ -10,8 +10,8 @@ The reference has no counterpart.
   :mod:`hamiltonzero_amd.kernels` and of the rectangular attention; :func:`relative_buckets` makes
   its plan.
 
-All three are differentiable in reverse mode (once) through ``torch.autograd``; a call that needs no
-gradient enqueues the forward alone. Tensors are float32 or bfloat16 GPU tensors on one device; work goes to
+All three are differentiable in reverse mode (once) through ``torch.autograd``, not in forward mode; a call that
+needs no gradient enqueues the forward alone. Tensors are float32 or bfloat16 GPU tensors on one device; work goes to
 the current stream of that device. There is no CPU fallback. Query, key and value tensors (and their
 cotangents) may be strided views whose last axis is contiguous (slices of one projection, a cache's
 rows); others are copied first. Every axis must be at least 1 long.
@@ -23,6 +23,7 @@ import contextlib
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native
@@ -99,6 +100,8 @@ def _check_first(name: str, t: Tensor, layout: str) -> None:
 
 
 def _wants_grad(*tensors: Optional[Tensor]) -> bool:
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("the token operators have no forward mode")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
@@ -200,6 +203,10 @@ def qk_norm_rotary(
             _check(name, t, dev, q.dtype, tuple(like.shape))
             if _strided(t) is not t:
                 raise ValueError(f"{name} must have contiguous heads and 16-byte aligned rows, got strides {t.stride()}")
+            if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+                raise ValueError(f"{name} must not hold one element at several places, got strides {t.stride()}")
+        if out[0].data_ptr() == out[1].data_ptr() or any(o.data_ptr() == t.data_ptr() for o in out for t in (q, k)):
+            raise ValueError("out must not overlap the inputs, nor one result the other")
     return _norm_fwd(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), float(eps), out)
 
 
@@ -282,7 +289,8 @@ def token_attention(
     no gradient) is None. Key j is seen if ``j < kv_len[b]``, and with ``causal`` if ``j <= p_i`` or
     ``j < prefix[b]`` (int32 ``[B]``), and with ``documents`` (int32 ``[B, Nk]``, negative: padding) if it and
     position p_i are of the same document. A query that sees nothing gets zeros and no gradient;
-    keys behind ``kv_len`` and padding are never used, whatever they hold. D is a multiple of 8 up to 128.
+    keys behind ``kv_len`` and padding are never used, whatever they hold. D is a multiple of 8 up to 128,
+    ``softcap`` at most 8192 for bfloat16.
 
     For single tokens ``k`` and ``v`` are the caches (strided views are read in place) and the new token's
     key and value are already in them."""

@@ -83,6 +83,96 @@ def test_divided_attention(case, dtype):
         within(name, x, want[name], want["t_" + name])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+@pytest.mark.parametrize("N,D", [(24, 64), (200, 16), (333, 128)])
+def test_errors_are_those_of_a_float32_computation(N, D, cap, dtype):
+    """Root mean squares of the errors, next to those of the definition in float32 operations rounded to the type. A
+    weight rounded to bfloat16 where it meets v or dout adds as much again as a result's rounding, sqrt(2) in all; the
+    score gradients have two parts; so half again bounds every one. (float32: 1e-6 where there is next to no error.)"""
+    g = gen(16)
+    B, H, dt = 4, 4, DT[dtype]
+    x = [normal(g, B, N, H, D, std=s, dtype=dt).requires_grad_() for s in (3.0, 1.0, 1.0)]
+    cot = normal(g, B, N, H, D, dtype=dt)
+    out = hz.token_attention(*x, causal=True, softcap=cap)
+    got = [out, *torch.autograd.grad(out, x, cot)]
+
+    def definition(float_, device):
+        q, k, v = (t.detach().to(device, float_).transpose(1, 2).contiguous().requires_grad_() for t in x)
+        y = (q @ k.transpose(-1, -2).contiguous()) * D**-0.5
+        if cap:
+            y = cap * torch.tanh(y / cap)
+        y = y.masked_fill(torch.ones(N, N, dtype=torch.bool, device=device).triu(1), -torch.inf)
+        o = y.softmax(-1) @ v
+        res = [o, *torch.autograd.grad(o, (q, k, v), cot.to(device, float_).transpose(1, 2))]
+        return [r.detach().transpose(1, 2) for r in res]
+
+    for name, a, b, c in zip(("out", "dq", "dk", "dv"), got, definition(torch.float32, "cuda"), definition(torch.float64, "cpu")):
+        size = c.norm()
+        own = ((a.detach().double().cpu() - c).norm() / size).item()
+        plain_ = ((b.to(dt).double().cpu() - c).norm() / size).item()
+        print(f"  {name}: {own:.2e}, in float32 operations {plain_:.2e}", flush=True)
+        assert own <= max(1.5 * plain_, 1e-6), name
+
+
+def test_tables_anywhere():
+    """Tables and positions that start in the middle of an allocation, one element past a 16-byte border."""
+    s = inputs(21, torch.float32)
+    for n in ("q", "k", "v", "dq", "dk", "pos", "n", "docs", "de"):
+        s[n] = s[n][:1]
+    want = everything(leaves(s))
+    moved = dict(s)
+    for n in ("w", "freqs", "slopes", "pos", "table", "n", "docs", "plan"):
+        room = torch.empty(s[n].numel() + 1, dtype=s[n].dtype, device="cuda")
+        moved[n] = room[1:].view(s[n].shape).copy_(s[n])
+        assert moved[n].data_ptr() % 16 and moved[n].is_contiguous()
+    for n in ("w", "table"):
+        moved[n].requires_grad_()
+    for n in ("q", "k", "v"):
+        moved[n] = s[n].clone().requires_grad_()
+    for a, b in zip(everything(moved), want):
+        assert torch.equal(a, b)
+
+
+def test_some_leaves_only_and_one_leaf_for_all():
+    g = gen(17)
+    x, k = normal(g, 2, 70, 4, 32), normal(g, 2, 70, 4, 32)
+    three = [x.clone().requires_grad_() for _ in range(3)]
+    out = hz.token_attention(*three, causal=True)
+    want = torch.autograd.grad(out.sum(), three)
+    one = x.clone().requires_grad_()
+    same = hz.token_attention(one, one, one, causal=True)
+    assert torch.equal(same, out)
+    got, = torch.autograd.grad(same.sum(), one)  # the three are added in an order of torch's own
+    assert (got - sum(want)).abs().max() <= 4 * F * sum(w.abs() for w in want).max()
+    full = [x.clone().requires_grad_(), k.clone().requires_grad_(), x.clone().requires_grad_()]
+    want = torch.autograd.grad(hz.token_attention(*full).square().sum(), full)
+    for i in range(3):
+        part = [t.detach().clone().requires_grad_(i == j) for j, t in enumerate(full)]
+        got, = torch.autograd.grad(hz.token_attention(*part).square().sum(), part[i])
+        assert torch.equal(got, want[i])
+
+
+def test_more_refusals():
+    x = torch.zeros(2, 8, 4, 32, device="cuda")
+    y, room = torch.empty_like(x), torch.empty(1, 8, 4, 32, device="cuda").expand(2, 8, 4, 32)
+    for out in ((x, y), (y, x), (y, y), (room, y)):
+        with pytest.raises(ValueError, match="overlap|several places"):
+            hz.qk_norm_rotary(x, x.clone(), out=out)
+    import torch.autograd.forward_ad as fwd
+
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: hz.token_attention(x, d, x), lambda: hz.qk_norm_rotary(d, x)):
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                call()
+        assert hz.token_attention(x, x, x).shape == x.shape
+    with pytest.raises(RuntimeError):  # once differentiable
+        q = x.clone().requires_grad_()
+        a, = torch.autograd.grad(hz.token_attention(q, x, x).sum(), q, create_graph=True)
+        torch.autograd.grad(a.sum(), q)
+
+
 # --- together -------------------------------------------------------------------------------------
 
 

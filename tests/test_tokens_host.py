@@ -158,7 +158,8 @@ def test_norm_backward_refuses(lib):
     (dict(H=6, Hk=4), E.HZ_EINVAL, "multiple of Hk"), (dict(Nq=0), E.HZ_EINVAL, ">= 1"), (dict(Nk=0), E.HZ_EINVAL, ">= 1"),
     (dict(Nk=1 << 30), E.HZ_EINVAL, "2^30"), (dict(B=1 << 21), E.HZ_EINVAL, "grid limit"), (dict(dtype=-1), E.HZ_EINVAL, "dtype"),
     (dict(scale=float("inf")), E.HZ_EINVAL, "scale"), (dict(softcap=-1.0), E.HZ_EINVAL, "softcap"),
-    (dict(softcap=float("nan")), E.HZ_EINVAL, "softcap"), (dict(causal=2), E.HZ_EINVAL, "causal"),
+    (dict(softcap=float("nan")), E.HZ_EINVAL, "softcap"), (dict(softcap=1e-37, scale=1.0), E.HZ_EINVAL, "softcap"),
+    (dict(softcap=8193.0, dtype=1), E.HZ_EINVAL, "softcap"), (dict(scale=1e31), E.HZ_EINVAL, "scale"), (dict(causal=2), E.HZ_EINVAL, "causal"),
     (dict(causal=0, prefix=A), E.HZ_EINVAL, "prefix needs causal"), (dict(prefix=A + 2), E.HZ_EALIGN, "prefix"),
     (dict(documents=A + 1), E.HZ_EALIGN, "documents"), (dict(kv_len=A + 1), E.HZ_EALIGN, "kv_len"),
     (dict(slopes=A + 2), E.HZ_EALIGN, "slopes"), (dict(lse=A + 2), E.HZ_EALIGN, "lse"), (dict(out=0), E.HZ_ENULL, "out"),
