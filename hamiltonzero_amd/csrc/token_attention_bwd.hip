@@ -263,8 +263,11 @@ __global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_
     }
 }
 
-// WAVES = 8 (bfloat16): waves w and w + 4 own the same 32 keys and take the tile's first and second 32 queries;
-// their sums meet in LDS at the end. So two waves share a SIMD although a workgroup owns 128 keys only.
+// WAVES = 8: waves w and w + 4 own the same 32 keys and take the tile's first and second 32 queries; their sums meet in LDS
+// at the end. So two waves share a SIMD although a workgroup owns 128 keys only (float32 heads of 64:
+// attn_train_both_f32 269 us with four waves, 234 with eight). The values' rows are in LDS, and the keys' too where
+// there are not the registers for them: float32, and bfloat16 heads of 128, where it saves the spilling of addresses
+// (attn_train_packed_bf16 814 -> 798 us); heads of 64 and 32 keep them in registers (1% and 2% faster).
 template <int DP, int PARTS, bool CAP, bool SLOPE, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) token_dkv_kernel(Params p, hz_token_tensor dout, const float* deltas,
                                                                           void* dk, void* dv, const DocTile* doc_tiles, Splits splits) {
@@ -272,12 +275,14 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
   constexpr int QB = kRows<DP, PARTS>, NB = QB / 32 / SETS, DT = DP / 32, CH = DP / 8;
   constexpr int LOADS = QB * CH / THREADS, STEP = THREADS / CH;
   constexpr int BUFS = PARTS == 1 ? 2 : 1;
+  constexpr bool KEYS_IN_LDS = WAVES == 8 && (PARTS == 3 || DP == 128);
   typedef Tile<QB, DP, PARTS> QT;
   __shared__ __align__(16) uint16_t q_lds0[QT::kPlane * PARTS], g_lds0[QT::kPlane * PARTS];
   __shared__ __align__(16) uint16_t q_lds1[PARTS == 1 ? QT::kPlane : 8], g_lds1[PARTS == 1 ? QT::kPlane : 8];
   __shared__ __align__(16) float base_lds[BUFS][QB], delta_lds[BUFS][QB];
   __shared__ __align__(16) int doc_lds[BUFS][QB];
   __shared__ __align__(16) uint16_t v_lds[kBlock * DP * PARTS];
+  __shared__ __align__(16) uint16_t k_lds[KEYS_IN_LDS ? kBlock * DP * PARTS : 8];
   __shared__ uint64_t bad_lds[BUFS];
   __shared__ int range_lds[4][2];
   const int tid = threadIdx.x, wave = (tid >> 6) & 3, set = tid >> 8, lane = tid & 63, hh = lane >> 5, c = lane & 31;
@@ -303,21 +308,26 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
     hi = max(max(range_lds[0][1], range_lds[1][1]), max(range_lds[2][1], range_lds[3][1]));
   }
 
-  // the keys' rows stay in registers, the values' in LDS: with both in registers the sums would not fit
-  Frag<PARTS> k[DP / 16];
+  Frag<PARTS> k[KEYS_IN_LDS ? 1 : DP / 16];
+  if constexpr (!KEYS_IN_LDS) {
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    Raw8<PARTS> rk;
-    const int d = 16 * s + 8 * hh;
-    rk.load(p.k.data, b * p.k.batch + row * p.k.token + hk * p.k.head + d, key < n && d < p.D);
-    k[s] = frag(rk);
+    for (int s = 0; s < DP / 16; ++s) {
+      Raw8<PARTS> rk;
+      const int d = 16 * s + 8 * hh;
+      rk.load(p.k.data, b * p.k.batch + row * p.k.token + hk * p.k.head + d, key < n && d < p.D);
+      k[s] = frag(rk);
+    }
   }
-  const Tile<kBlock, DP, PARTS> vt{v_lds};
+  const Tile<kBlock, DP, PARTS> vt{v_lds}, keys{k_lds};
   for (int i = tid; i < kBlock * CH; i += THREADS) {
     const int r = i / CH, ch = i % CH;
     Raw8<PARTS> rv;
     rv.load(p.v.data, b * p.v.batch + (key0 + r) * p.v.token + hk * p.v.head + 8 * ch, key0 + r < n && 8 * ch < p.D);
     vt.put(r, ch, frag(rv));
+    if constexpr (KEYS_IN_LDS) {
+      rv.load(p.k.data, b * p.k.batch + (key0 + r) * p.k.token + hk * p.k.head + 8 * ch, key0 + r < n && 8 * ch < p.D);
+      keys.put(r, ch, frag(rv));
+    }
   }
   v16f ak[DT], av[DT];
 #pragma unroll
@@ -430,7 +440,10 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
         ahead<DP / 16, PARTS>(
             [&](int ds) { return Three<PARTS>{qt.rows(r0, ds, l), gt.rows(r0, ds, l), vt.rows(32 * wave, ds, l)}; },
             [&](int ds, const Three<PARTS>& x) {
-              s = mma(x.a, k[ds], s);
+              if constexpr (KEYS_IN_LDS)
+                s = mma(x.a, keys.rows(32 * wave, ds, l), s);
+              else
+                s = mma(x.a, k[ds], s);
               dp = mma(x.b, x.c, dp);
             });
         const int r1 = r0 + 4 * hh;
@@ -576,7 +589,7 @@ void launch_sum(const Splits& splits, int tensors, void* first, void* second, hi
 // Workgroups are made more by dividing the keys (dq), the query heads of a key head and then the queries (dk, dv):
 // documents and causal masks make them of very different lengths, which a single round of them cannot even out, and a
 // few long sequences would leave most CUs idle. The sum of the shares costs little beside that
-// (attn_train_packed_bf16: dk and dv in four shares 355 us and 15 for the sum, 661 in one).
+// (attn_train_packed_bf16 825 us in all, undivided 1097; attn_train_both_f32 262 and 434).
 Splits dq_splits(const hz_token_attention& a) {
   const int64_t blocks = a.B * a.H * ((a.Nq + kBlock - 1) / kBlock);
   return {nullptr, a.B * a.Nq * a.H * a.D, share_of(blocks, a.Nk, 512), 1};
@@ -603,7 +616,7 @@ int64_t delta_bytes(const hz_token_attention& a) {
 template <int DP, int PARTS, bool CAP, bool SLOPE>
 hipError_t run(const hz_token_attention& a, const hz_token_tensor& dout, void* dq, void* dk, void* dv, void* workspace,
                hipStream_t stream) {
-  constexpr int WAVES = PARTS == 1 ? 8 : 4;
+  constexpr int WAVES = PARTS == 1 || DP == 64 ? 8 : 4;
   const Params p = make_params(a);
   float* const deltas = static_cast<float*>(workspace);
   Splits of_q = dq_splits(a), of_kv = dkv_splits(a);
