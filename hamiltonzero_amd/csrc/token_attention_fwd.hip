@@ -6,10 +6,13 @@
 // are copied straight into one of two LDS buffers while the other is used; float32 ones pass through
 // registers, where they are split. Tiles that no query of the workgroup can see (behind the last visible key,
 // or of other documents) are not visited; a wave forms masks only in tiles where some pair is hidden. Where
-// there are few workgroups and many keys, the keys are divided and the parts joined by a second kernel.
+// there are few workgroups and many keys, the keys are divided and the parts joined by a second kernel. Bound by the
+// exponentials' and the cap's vector work beside the products: attn_prompt_bf16 (2 x 4096 tokens, 16 on 4 heads of 128,
+// causal, capped) 196 us, 700 TFLOP/s; 173 without the cap's tanh, 168 without either of the products.
 //
 // Few queries (at most 32 rows of query and head share a key head): a wave owns a run of keys and
-// all of those rows, so the cache is read once, and the same second kernel joins the runs.
+// all of those rows, so the cache is read once, and the same second kernel joins the runs. Bound by those bytes:
+// attn_token_long_bf16 (16 rows of 32768 keys, 8 key heads of 128) 265 us, 4.9 TB/s.
 #include "token_device.h"
 
 namespace hz {
