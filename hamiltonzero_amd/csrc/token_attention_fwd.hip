@@ -568,14 +568,15 @@ int run_keys(const hz_token_attention& a) {
 
 int64_t blocks_of(const hz_token_attention& a) { return a.B * a.H * ((a.Nq + kQB - 1) / kQB); }
 
-// Parts of a row's keys. Many queries: as many as 1024 workgroups (four a CU) want, each of at least 128 keys
-// (attn_train_both_f32's forward: 66 us, undivided 90).
+// Parts of a row's keys. Many queries: as many as 512 workgroups (two a CU) want, each of at least 128 keys
+// (attn_train_both_f32's forward, 192 workgroups undivided: 90 us, 66 so and for 1024; where 512 need no division, 1024 would
+// cost 13%, 2 x 2048 tokens of 16 bfloat16 heads of 128, causal: 67 us and 75).
 int parts_of(const hz_token_attention& a) {
   if (few(a)) {
     const int c = run_keys(a);
     return static_cast<int>((a.Nk + c - 1) / c);
   }
-  return share_of(blocks_of(a), a.Nk, 1024);
+  return share_of(blocks_of(a), a.Nk, 512);
 }
 
 int64_t parts_bytes(const hz_token_attention& a) {
