@@ -15,7 +15,7 @@ namespace {
 
 using namespace token;
 
-constexpr int kBlock = 128;  // queries (dq) or keys (dk, dv) a workgroup, 32 a wave
+constexpr int kBlock = kOrderBlock;  // queries (dq) or keys (dk, dv) a workgroup, 32 a wave
 
 // Rows of a streamed tile: two tensors, float32 ones in three parts.
 template <int DP, int PARTS>
@@ -86,10 +86,9 @@ __global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_
   __shared__ int range_lds[4][2];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, hh = lane >> 5, c = lane & 31;
   const int tiles = (p.Nq + kBlock - 1) / kBlock;
-  const Unit unit(blockIdx.x, p.G * splits.n, static_cast<int64_t>(p.B) * p.Hk);
+  const Unit unit(p, blockIdx.x, p.G * splits.n, tiles, true, p.q_order);  // the longest rows of a causal mask first
   const int part = unit.inner % splits.n;
-  const int q0 = (tiles - 1 - unit.tile) * kBlock;  // the longest rows of a causal mask first
-  const int hk = static_cast<int>(unit.pair % p.Hk), b = static_cast<int>(unit.pair / p.Hk), h = hk * p.G + unit.inner / splits.n;
+  const int q0 = unit.tile * kBlock, hk = unit.hk, b = unit.b, h = hk * p.G + unit.inner / splits.n;
   const int n = kv_length(p, b);
   const int i = q0 + 32 * wave + c, row = i < p.Nq ? i : p.Nq - 1;
   const Sight me(p, b, row, n);
@@ -288,9 +287,9 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
   __shared__ uint64_t bad_lds[BUFS];
   __shared__ int range_lds[4][2];
   const int tid = threadIdx.x, wave = (tid >> 6) & 3, set = tid >> 8, lane = tid & 63, hh = lane >> 5, c = lane & 31;
-  const Unit unit(blockIdx.x, splits.n, static_cast<int64_t>(p.B) * p.Hk);
-  const int key0 = unit.tile * kBlock;  // the first keys are seen by the most queries
-  const int hk = static_cast<int>(unit.pair % p.Hk), b = static_cast<int>(unit.pair / p.Hk);
+  // the first keys of a causal mask are seen by the most queries
+  const Unit unit(p, blockIdx.x, splits.n, (p.Nk + kBlock - 1) / kBlock, false, p.k_order);
+  const int key0 = unit.tile * kBlock, hk = unit.hk, b = unit.b;
   const int share = unit.inner / (splits.n / splits.heads), part = unit.inner % (splits.n / splits.heads);
   const int first_head = share * p.G / splits.heads, last_head = (share + 1) * p.G / splits.heads - 1;
   const int n = kv_length(p, b), shift = n - p.Nq;  // position of query 0
@@ -620,13 +619,12 @@ template <int DP, int PARTS, bool CAP, bool SLOPE>
 hipError_t run(const hz_token_attention& a, const hz_token_tensor& dout, void* dq, void* dk, void* dv, void* workspace,
                hipStream_t stream) {
   constexpr int WAVES = PARTS == 1 || DP == 64 ? 8 : 4;
-  const Params p = make_params(a);
+  Params p = make_params(a);
   float* const deltas = static_cast<float*>(workspace);
   Splits of_q = dq_splits(a), of_kv = dkv_splits(a);
   of_q.partial = of_kv.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a));
   DocTile* const tiles = reinterpret_cast<DocTile*>(static_cast<char*>(workspace) + delta_bytes(a) + split_bytes(a));
-  if (p.documents != nullptr)
-    if (hipError_t err = launch_doc_tiles(p, tiles, stream); err != hipSuccess) return err;
+  if (hipError_t err = launch_docs(a, p, true, tiles, stream); err != hipSuccess) return err;
   const int64_t nq = a.B * a.H * ((a.Nq + kBlock - 1) / kBlock) * of_q.n, nk = a.B * a.Hk * ((a.Nk + kBlock - 1) / kBlock) * of_kv.n;
   token_dq_kernel<DP, PARTS, CAP, SLOPE><<<static_cast<unsigned>(nq), 256, 0, stream>>>(p, dout, dq, deltas, tiles, of_q);
   launch_sum<PARTS>(of_q, 1, dq, nullptr, stream);
@@ -638,7 +636,7 @@ hipError_t run(const hz_token_attention& a, const hz_token_tensor& dout, void* d
 }  // namespace
 
 int64_t token_attention_bwd_workspace(const hz_token_attention& a) {
-  return delta_bytes(a) + split_bytes(a) + static_cast<int64_t>(doc_tiles_bytes(a));
+  return delta_bytes(a) + split_bytes(a) + doc_bytes(a);
 }
 
 hipError_t launch_token_attention_bwd(const hz_token_attention& a, const hz_token_tensor& dout, void* dq, void* dk,

@@ -31,6 +31,7 @@ struct Params {
   float* lse;
   const float* slopes;
   const int32_t *prefix, *documents, *kv_len;
+  const int *q_order, *k_order;  // the blocks of all rows, the longest first (null: in their own order)
   int B, Nq, Nk, H, Hk, G, D, causal;
   float scale;      // of the dot products
   float cap;        // 0: not capped
@@ -328,17 +329,27 @@ struct DocTile {
 };
 constexpr int kDocTile = 64;
 
-// Which unit of work a workgroup takes: `inner` workgroups on each of `pairs` pairs of (row of the batch, key head), for
-// one tile after the other, so that every XCD (workgroups go round the 8 by their number) gets its share of the long
-// tiles. (Pairs kept on XCDs of their own, for their L2, were no faster forward and 3 to 10% slower in reverse:
+// Which unit of work a workgroup takes: `inner` workgroups on each key head of a block of 128 rows, for one block after
+// the other, so that every XCD (workgroups go round the 8 by their number) gets its share of the long blocks. Blocks
+// are taken in `order` where there is one, else the last or first of every row before the next. (Pairs of row and
+// key head kept on XCDs of their own, for their L2, were no faster forward and 3 to 10% slower in reverse:
 // attn_train_packed_bf16 761 us so, 787 to 836 with pairs on XCDs.)
 struct Unit {
-  int inner, tile;
-  int64_t pair;
-  __device__ __forceinline__ Unit(int64_t id, int inner_, int64_t pairs) {
+  int inner, hk, b, tile;
+  __device__ __forceinline__ Unit(const Params& p, int64_t id, int inner_, int tiles, bool last_first, const int* order) {
     inner = static_cast<int>(id % inner_);
-    pair = id / inner_ % pairs;
-    tile = static_cast<int>(id / inner_ / pairs);
+    id /= inner_;
+    hk = static_cast<int>(id % p.Hk);
+    id /= p.Hk;
+    if (order != nullptr) {
+      const int e = order[id];
+      b = e / tiles;
+      tile = e - b * tiles;
+    } else {
+      b = static_cast<int>(id % p.B);
+      const int t = static_cast<int>(id / p.B);
+      tile = last_first ? tiles - 1 - t : t;
+    }
   }
 };
 
@@ -464,9 +475,11 @@ inline int share_of(int64_t blocks, int64_t n, int64_t want) {
   return static_cast<int>(parts > 1 ? parts : 1);
 }
 
-// Launch of the pass over the documents (token_attention_fwd.hip), where a call has some.
-size_t doc_tiles_bytes(const hz_token_attention& a);
-hipError_t launch_doc_tiles(const Params& p, DocTile* tiles, hipStream_t stream);
+// The passes over the documents (token_attention_fwd.hip), where a call has some: the DocTiles at `memory`, and the
+// order of the blocks of queries, and of keys, behind them.
+constexpr int kOrderBlock = 128;  // rows of a block
+int64_t doc_bytes(const hz_token_attention& a);
+hipError_t launch_docs(const hz_token_attention& a, Params& p, bool keys, void* memory, hipStream_t stream);
 
 }  // namespace token
 }  // namespace hz

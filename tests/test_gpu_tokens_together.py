@@ -84,6 +84,38 @@ def test_divided_attention(case, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,Nq,Nk,H,Hk,D,kw", [  # more than 512 blocks of queries: they begin the longest first
+    (71, 40, 40, 8, 4, 16, dict()), (5, 300, 300, 48, 2, 8, dict(causal=True)), (9, 130, 700, 32, 8, 16, dict(causal=True, prefix=True)),
+    (3, 700, 333, 32, 16, 8, dict(kv_len=True)), (2, 2000, 2100, 17, 1, 8, dict(causal=True, kv_len=True)),
+], ids=lambda v: str(v) if not isinstance(v, dict) else "-".join(v) or "both")
+def test_documents_of_many_blocks(B, Nq, Nk, H, Hk, D, kw, dtype):
+    _say(f"many blocks {B} {Nq} {Nk} {H} {Hk} {D} {kw} {dtype}")
+    g, cpu, dt = gen(18), torch.Generator().manual_seed(3), DT[dtype]
+    q, k, v = (normal(g, *s, dtype=dt).requires_grad_() for s in ((B, Nq, H, D), (B, Nk, Hk, D), (B, Nk, Hk, D)))
+    docs = torch.randint(0, 5, (B, Nk), generator=cpu).sort(1).values.to(torch.int32)
+    docs[:, -3:] = -1
+    docs[1] = torch.randint(-1, 4, (Nk,), generator=cpu).to(torch.int32)  # in no order
+    kw = dict(kw, documents=docs.cuda())
+    if "prefix" in kw:
+        kw["prefix"] = torch.randint(0, Nk, (B,), generator=cpu).to(torch.int32).cuda()
+    if "kv_len" in kw:
+        kw["kv_len"] = torch.randint(0, Nk + 1, (B,), generator=cpu).to(torch.int32).cuda()
+    out = hz.token_attention(q, k, v, **kw)
+    dout = normal(g, *out.shape, dtype=dt)
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    again = hz.token_attention(q, k, v, **kw)
+    assert torch.equal(out, again)
+    for a, b in zip(grads, torch.autograd.grad(again, (q, k, v), dout)):
+        assert torch.equal(a, b)
+    okw = {n: x.cpu().numpy() if isinstance(x, torch.Tensor) else x for n, x in kw.items()}
+    rows = slice(0, 4)
+    okw = {n: x[rows] if isinstance(x, np.ndarray) else x for n, x in okw.items()}
+    want = O.attention(arr(q)[rows], arr(k)[rows], arr(v)[rows], scale=float(np.float32(D**-0.5)), dout=arr(dout)[rows], bf16=dtype == "bf16", **okw)
+    for name, x in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        within(name, x[rows], want[name], want["t_" + name])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("cap", [0.0, 50.0])
 @pytest.mark.parametrize("N,D", [(24, 64), (200, 16), (333, 128)])
 def test_errors_are_those_of_a_float32_computation(N, D, cap, dtype):
