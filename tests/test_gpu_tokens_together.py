@@ -344,6 +344,9 @@ def everything(s):
     for kw in (dict(causal=True, softcap=5.0, documents=s["docs"]), dict(causal=True, slopes=s["slopes"])):
         out = hz.token_attention(s["q"], s["k"], s["v"], **kw)
         res += [out, *torch.autograd.grad(out, (s["q"], s["k"], s["v"]), s["dq"])]
+    wide = s["q"].detach().repeat(1, 1, 70, 1)  # more than 512 blocks: documents put them in order
+    out = hz.token_attention(wide, s["k"], s["v"], documents=s["docs"])
+    res += [out, *torch.autograd.grad(out, (s["k"], s["v"]), wide)]
     res.append(hz.token_attention(s["q"].detach()[:, :2], s["k"].detach(), s["v"].detach(), causal=True, kv_len=s["n"]))
     for layout, de in (("qhk", s["de"]), ("qkh", s["de"].transpose(2, 3))):
         e = hz.bucket_bias(s["table"], s["plan"], s["pos"], s["pos"], e_layout=layout, dtype=s["q"].dtype)
@@ -382,6 +385,35 @@ def test_side_streams(dtype):
         with torch.cuda.stream(st):
             got.append(everything(leaves(s)))
     torch.cuda.synchronize()
+    for r in got:
+        for a, b in zip(r, want):
+            assert torch.equal(a, b)
+
+
+def test_two_threads():
+    """Each thread on a stream of its own, all operators several times: the bits of one thread alone."""
+    import threading
+
+    s = inputs(22, torch.bfloat16)
+    want = everything(leaves(s))
+    torch.cuda.synchronize()
+    got, failed = [], []
+
+    def work():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got.append(everything(leaves(s)))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # shown by the assertion below
+            failed.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and len(got) == 10
     for r in got:
         for a, b in zip(r, want):
             assert torch.equal(a, b)
