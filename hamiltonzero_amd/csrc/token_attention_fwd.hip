@@ -643,10 +643,11 @@ __global__ void __launch_bounds__(32 * kHalves<WAYS>) token_join_kernel(Params p
 bool few(const hz_token_attention& a) { return a.Nq * (a.H / a.Hk) <= 32; }
 
 // Keys a run: about 6144 waves in all, at least one block of 32 keys (attn_token_long_bf16: 265 us, 295 with a third of
-// the waves, 270 with twice as many).
+// the waves, 270 with twice as many); heads up to 32, whose waves hold fewer registers, 8192 (32 rows of 4000 keys, 16 on 8
+// heads of 32: 30 us, 35 with 6144).
 int run_keys(const hz_token_attention& a) {
-  const int64_t wanted = (a.B * a.Hk * a.Nk + 6143) / 6144, keys = wanted < a.Nk ? wanted : a.Nk;
-  return static_cast<int>((keys + 31) / 32 * 32);
+  const int64_t waves = a.D <= 32 ? 8192 : 6144, wanted = (a.B * a.Hk * a.Nk + waves - 1) / waves;
+  return static_cast<int>(((wanted < a.Nk ? wanted : a.Nk) + 31) / 32 * 32);
 }
 
 int64_t blocks_of(const hz_token_attention& a) { return a.B * a.H * ((a.Nq + kQB - 1) / kQB); }
