@@ -3,11 +3,11 @@
 //
 // Two kernels, each with its sums in registers, so that nothing is added atomically: one owns queries and
 // streams keys (dq, and rowsum(dout out) for the other), one owns keys and streams the queries of
-// every head that shares them (dk, dv). Both rebuild P = exp(s - lse) from the forward's lse, so scores and dP
-// are formed twice: nine products a tile pair (two for the score gradients' second bfloat16 part) where one kernel with
-// atomic dq sums would need seven. Bound by the products and, between them, the exponentials' vector work;
-// attn_train_packed_bf16 (8192 tokens in four documents, 16 on 4 heads of 128): 259 us for dq, 423 for dk and dv. Tiles
-// are copied, skipped and masked as in the forward.
+// every head that shares them (dk, dv). Both rebuild P = exp(s - lse) from the forward's lse (far from zero, from the
+// row's largest score and sum, which the first forms again), so scores and dP are formed twice: nine products a tile
+// pair (two for the score gradients' second bfloat16 part) where one kernel with atomic dq sums would need seven. Bound by
+// the products and, between them, the exponentials' vector work; attn_train_packed_bf16 (8192 tokens in four documents, 16
+// on 4 heads of 128): 259 us for dq, 423 for dk and dv. Tiles are copied, skipped and masked as in the forward.
 #include "token_device.h"
 
 namespace hz {
@@ -21,30 +21,67 @@ constexpr int kBlock = kOrderBlock;  // queries (dq) or keys (dk, dv) a workgrou
 template <int DP, int PARTS>
 constexpr int kRows = (DP == 128 && PARTS == 3) ? 32 : 64;
 
-// Weight and score gradient of one pair from its dot product x, its dP and the distance between query and key;
-// `base` is the exponent's part of the query, as row_base gives it. bfloat16, capped: with u = 1 / (1 + e^2y), tanh y =
-// 1 - 2 u and its derivative is 4 u (1 - u), whose 4 is left to the end (grad_scale).
+// What the exponent of a row's weights begins with: a score has its row's largest one, or lse2 (the logarithm of their
+// sum, all in base 2), taken off. bfloat16, capped, no distance bias: with u = 1 / (1 + e^2y), tanh y = 1 - 2 u, and the
+// score cap2 - 2 cap2 u has that taken off in one fused operation.
+template <int PARTS, bool CAP, bool SLOPE>
+constexpr bool kFused = CAP && PARTS == 1 && !SLOPE;
+template <int PARTS, bool CAP, bool SLOPE>
+__device__ __forceinline__ float row_base(const Params& p, float top2) {
+  return (kFused<PARTS, CAP, SLOPE> ? p.to_score2 : 0.f) - top2;
+}
+
+// Exponent (base 2) of one pair's weight from its dot product x and the distance between query and key, and the cap's
+// derivative g. A score is rounded before the row's base is added, never fused with it: the largest score of a row whose
+// base it is then gives 2^0, however large it is, and so it is in every kernel that forms it. (Fused scores are at
+// most 8192 log2 e: off by 2^-10 there.) bfloat16, capped: the derivative 4 u (1 - u) leaves its 4 to the end (grad_scale).
+template <int PARTS, bool CAP, bool SLOPE>
+__device__ __forceinline__ float exponent(const Params& p, float x, float slope2, float distance, float base, float& g) {
+#pragma clang fp contract(off)
+  float s;
+  if constexpr (CAP && PARTS == 1) {
+    const float u = __builtin_amdgcn_rcpf(1.f + fast_exp2(x * p.to_exp2));
+    g = fmaf(-u, u, u);
+    s = fmaf(-2.f * p.to_score2, u, SLOPE ? p.to_score2 : base);
+    if constexpr (!SLOPE) return s;
+  } else if constexpr (CAP) {
+    const float t = tanh_of<PARTS>(x * p.to_tanh);
+    g = fmaf(-t, t, 1.f);
+    s = t * p.to_score2;
+  } else {
+    g = 1.f;
+    s = x * p.to_score2;
+  }
+  if constexpr (SLOPE) s = fmaf(-slope2, fabsf(distance), s);
+  return s + base;
+}
+
+// Weight and score gradient of one pair. The weight is at most 1: rebuilt from a rounded logarithm it comes out above 1 by
+// that rounding.
 template <int PARTS, bool CAP, bool SLOPE>
 __device__ __forceinline__ void pair(const Params& p, float x, float dp, float slope2, float distance, float base,
                                      float delta, float& w, float& ds) {
-  constexpr bool U = CAP && PARTS == 1;
-  float g = 1.f, s;
-  if constexpr (U) {
-    const float u = __builtin_amdgcn_rcpf(1.f + fast_exp2(x * p.to_exp2));
-    s = base - 2.f * p.to_score2 * u;
-    g = u - u * u;
-  } else if constexpr (CAP) {
-    const float t = tanh_of<PARTS>(x * p.to_tanh);
-    s = t * p.to_score2 + base;
-    g = 1.f - t * t;
-  } else {
-    s = x * p.to_score2 + base;
-  }
-  if constexpr (SLOPE) s -= slope2 * fabsf(distance);
-  w = fast_exp2(s);
+  float g;
+  w = lse_weight(exponent<PARTS, CAP, SLOPE>(p, x, slope2, distance, base, g));
   ds = w * (dp - delta);
   if constexpr (CAP) ds *= g;
 }
+
+// lse is a rounded logarithm, and its change of base rounds again: a weight rebuilt from it is off by up to five times
+// 2^-24 |lse| of itself, all of a row's by the same factor. Rows whose lse is above this (or is not finite) get their largest
+// score and their sum formed again, from the scores as the reverse pass forms them: weights 2^(s - m) / l. Below it they are
+// off by 1e-5 (float32) and 8e-5 (bfloat16) at most; without it a lone key's weight was off by 7e-4 at a score of 10^4, 9%
+// at 10^6, and NaN or 0 at 10^10. Where every block has such a row the reverse pass takes a quarter to a third longer (4 x
+// 2048 tokens of 16 on 4 bfloat16 heads of 64: 250 us and 356; float32, 4 x 1024: 213 and 273), and twice as long
+// where the keys are divided, since each part goes over all of them.
+template <int PARTS>
+constexpr float kFar = PARTS == 1 ? 256.f : 32.f;
+
+// What dk, dv need of a query: the base of its weights' exponents (-inf: it sees nothing), rowsum(dout out), and
+// what its weights are multiplied by (1 where the base holds their sum).
+struct RowStats {
+  float base, delta, inv, unused;
+};
 // Operands that are read together.
 template <int PARTS>
 struct Two {
@@ -55,10 +92,6 @@ struct Three {
   Frag<PARTS> a, b, c;
 };
 
-template <int PARTS, bool CAP>
-__device__ __forceinline__ float row_base(const Params& p, float lse) {
-  return (CAP && PARTS == 1 ? p.to_score2 : 0.f) - lse * kLog2e;
-}
 template <int PARTS, bool CAP>
 __device__ __forceinline__ float grad_scale(const Params& p) {
   return CAP && PARTS == 1 ? 4.f * p.scale : p.scale;
@@ -74,7 +107,7 @@ struct Splits {
 
 template <int DP, int PARTS, bool CAP, bool SLOPE>
 __global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_kernel(Params p, hz_token_tensor dout, void* dq,
-                                                                           float* deltas, const DocTile* doc_tiles,
+                                                                           RowStats* stats, const DocTile* doc_tiles,
                                                                                       Splits splits) {
   constexpr int KB = kRows<DP, PARTS>, NB = KB / 32, DT = DP / 32, CH = DP / 8;
   constexpr int LOADS = KB * CH / 256, STEP = 256 / CH;
@@ -84,6 +117,8 @@ __global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_
   __shared__ __align__(16) uint16_t k_lds1[PARTS == 1 ? KV::kPlane : 8], v_lds1[PARTS == 1 ? KV::kPlane : 8];
   __shared__ __align__(16) int doc_lds[BUFS][KB];
   __shared__ int range_lds[4][2];
+  __shared__ int far_lds[4];
+  __shared__ float inv_lds[kBlock];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, hh = lane >> 5, c = lane & 31;
   const int tiles = (p.Nq + kBlock - 1) / kBlock;
   const Unit unit(p, blockIdx.x, p.G * splits.n, tiles, true, p.q_order);  // the longest rows of a causal mask first
@@ -91,6 +126,9 @@ __global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_
   const int q0 = unit.tile * kBlock, hk = unit.hk, b = unit.b, h = hk * p.G + unit.inner / splits.n;
   const int n = kv_length(p, b);
   const int i = q0 + 32 * wave + c, row = i < p.Nq ? i : p.Nq - 1;
+  const int64_t at = (static_cast<int64_t>(b) * p.Nq + row) * p.H + h;
+  const float lse = p.lse[at];
+  const bool far = !(fabsf(lse) <= kFar<PARTS>) && lse != kNegInf;
   const Sight me(p, b, row, n);
   const float slope2 = SLOPE ? p.slopes[h] * kLog2e : 0.f;
   const int wave_first = __builtin_amdgcn_readfirstlane(me.last);
@@ -103,24 +141,105 @@ __global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_
     document_range(me.doc, wave_lo, wave_hi);
     one_document = wave_lo == wave_hi && !__any(me.doc < 0);
     if (lane == 0) range_lds[wave][0] = wave_lo, range_lds[wave][1] = wave_hi;
-    __syncthreads();
+  }
+  const bool wave_far = __any(far);
+  if (lane == 0) far_lds[wave] = wave_far;
+  __syncthreads();
+  if (by_document) {
     lo = min(min(range_lds[0][0], range_lds[1][0]), min(range_lds[2][0], range_lds[3][0]));
     hi = max(max(range_lds[0][1], range_lds[1][1]), max(range_lds[2][1], range_lds[3][1]));
   }
+  const bool any_far = (far_lds[0] | far_lds[1] | far_lds[2] | far_lds[3]) != 0;
   const DocTile* const row_tiles = doc_tiles + static_cast<int64_t>(b) * ((p.Nk + kDocTile - 1) / kDocTile);
   auto range = [row_tiles](int t) { return row_tiles[t * KB / kDocTile]; };
   Walk<decltype(range)> walk(0, keys > 0 ? (keys + KB - 1) / KB : 0, by_document, lo, hi, range);
-  if (splits.n > 1) walk.take_part(part, splits.n, lane);
-  const int end = walk.end;
-  const int64_t at = (static_cast<int64_t>(b) * p.Nq + row) * p.H + h;
 
   Frag<PARTS> q[DP / 16], go[DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    Raw8<PARTS> r;
+    const int d = 16 * s + 8 * hh;
+    r.load(p.q.data, b * p.q.batch + row * p.q.token + h * p.q.head + d, d < p.D);
+    q[s] = frag(r);
+  }
+  const Copy<KB, DP> copy_k(p.k, b, hk, p.D, tid), copy_v(p.v, b, hk, p.D, tid);
+  const int lr = tid / CH, lc = tid % CH;
+  float base = row_base<PARTS, CAP, SLOPE>(p, lse == kNegInf ? 0.f : lse * kLog2e);  // -inf: a row that sees nothing
+  if (hh == 0) inv_lds[32 * wave + c] = 1.f;
+  if (any_far) {
+    // The rows' largest scores m and sums l of 2^(s - m), over all keys that they see (kFar): the scores' part of the loop
+    // below with the softmax's running maximum, one tile at a time.
+    const KV kt{k_lds0};
+    Walk<decltype(range)> all = walk;
+    DocTile here{};
+    float m = kNegInf, l = 0.f;
+    for (int t = all.next(all.begin, lane, here); t < all.end; t = all.next(t + 1, lane, here)) {
+      const int k0 = t * KB;
+      if (by_document && tid < KB) doc_lds[0][tid] = k0 + tid < n ? key_document(p, b, k0 + tid) : -1;
+      if constexpr (PARTS == 1) {
+        copy_k(k_lds0, k0, n);
+        copies_done();
+      } else {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+          const int key = k0 + lr + STEP * j;
+          Raw8<PARTS> r;
+          r.load(p.k.data, b * p.k.batch + key * p.k.token + hk * p.k.head + 8 * lc, key < n && 8 * lc < p.D);
+          kt.put(lr + STEP * j, lc, frag(r));
+        }
+      }
+      __syncthreads();
+      if (k0 <= wave_last) {
+#pragma unroll 1
+        for (int nb = 0; nb < NB; ++nb) {
+          v16f s[1] = {v16f{}};
+#pragma unroll
+          for (int ds = 0; ds < DP / 16; ++ds) s[0] = mma(kt.rows(32 * nb, ds, lane), q[ds], s[0]);
+          settle(s);
+          const int k1 = k0 + 32 * nb + 4 * hh;
+          const float away = static_cast<float>(me.pos - k1);
+          float top = kNegInf;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float g;
+            const float y = exponent<PARTS, CAP, SLOPE>(p, s[0][e], slope2, away - static_cast<float>(row_of(e, 0)),
+                                                        row_base<PARTS, CAP, SLOPE>(p, 0.f), g);
+            const bool seen = row_of(e, 0) <= me.last - k1 &&
+                              (!by_document || doc_lds[0][32 * nb + 4 * hh + row_of(e, 0)] == me.doc);
+            top = seen ? fmaxf(top, y) : top;
+          }
+          const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+          top = fmaxf(m, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+          l *= m == kNegInf ? 0.f : fast_exp2(m - top);
+          m = top;
+          const float from = row_base<PARTS, CAP, SLOPE>(p, m == kNegInf ? 0.f : m);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float g;
+            const float y = exponent<PARTS, CAP, SLOPE>(p, s[0][e], slope2, away - static_cast<float>(row_of(e, 0)), from, g);
+            const bool seen = row_of(e, 0) <= me.last - k1 &&
+                              (!by_document || doc_lds[0][32 * nb + 4 * hh + row_of(e, 0)] == me.doc);
+            // (a NaN, or a score of +inf, makes a NaN of the sum, and so of all of the row's weights)
+            l += seen ? (y > 0.f ? 1.f : fast_exp2(y)) : 0.f;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    l = xor32_pair_sum(l);
+    if (far && l != 0.f) {
+      base = l == l ? row_base<PARTS, CAP, SLOPE>(p, m) : l;
+      if (hh == 0) inv_lds[32 * wave + c] = 1.f / l;
+    }
+  }
+  if (splits.n > 1) walk.take_part(part, splits.n, lane);
+  const int end = walk.end;
+
   float delta = 0.f;
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
-    Raw8<PARTS> rq, rg, ro;
+    Raw8<PARTS> rg, ro;
     const int d = 16 * s + 8 * hh;
-    rq.load(p.q.data, b * p.q.batch + row * p.q.token + h * p.q.head + d, d < p.D);
     rg.load(dout.data, b * dout.batch + row * dout.token + h * dout.head + d, d < p.D);
     ro.load(p.out, at * p.D + d, d < p.D);
     float x[8], y[8];
@@ -134,19 +253,15 @@ __global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta += x[j] * y[j];
     }
-    q[s] = frag(rq);
     go[s] = frag(rg);
   }
   delta = xor32_pair_sum(delta);
-  if (i < p.Nq && hh == 0 && part == 0) deltas[at] = delta;
-  const float lse = p.lse[at], base = row_base<PARTS, CAP>(p, lse == kNegInf ? 0.f : lse);  // -inf: a row that sees nothing
-  const float to_grad = grad_scale<PARTS, CAP>(p);
+  if (i < p.Nq && hh == 0 && part == 0)
+    *reinterpret_cast<float4*>(stats + at) = make_float4(lse == kNegInf ? kNegInf : base, delta, inv_lds[32 * wave + c], 0.f);
   v16f acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = v16f{};
 
-  const Copy<KB, DP> copy_k(p.k, b, hk, p.D, tid), copy_v(p.v, b, hk, p.D, tid);
-  const int lr = tid / CH, lc = tid % CH;
   Raw8<PARTS> rk[PARTS == 3 ? LOADS : 1], rv[PARTS == 3 ? LOADS : 1];
   int rdoc = -1;  // as loaded: waited for where it is used
   auto load = [&](int t, auto to) __attribute__((always_inline)) {
@@ -249,6 +364,7 @@ __global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_
   }
   settle(acc);
   if (i >= p.Nq) return;
+  const float to_grad = grad_scale<PARTS, CAP>(p) * inv_lds[32 * wave + c];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -270,7 +386,7 @@ __global__ void __launch_bounds__(256, PARTS == 1 || DP <= 64 ? 2 : 1) token_dq_
 // there are not the registers for them: float32, and bfloat16 heads of 128, where it saves the spilling of addresses
 // (attn_train_packed_bf16 814 -> 798 us); heads of 64 and 32 keep them in registers (1% and 2% faster).
 template <int DP, int PARTS, bool CAP, bool SLOPE, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) token_dkv_kernel(Params p, hz_token_tensor dout, const float* deltas,
+__global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) token_dkv_kernel(Params p, hz_token_tensor dout, const RowStats* stats,
                                                                           void* dk, void* dv, const DocTile* doc_tiles, Splits splits) {
   constexpr int THREADS = 64 * WAVES, SETS = WAVES / 4;
   constexpr int QB = kRows<DP, PARTS>, NB = QB / 32 / SETS, DT = DP / 32, CH = DP / 8;
@@ -280,11 +396,11 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
   typedef Tile<QB, DP, PARTS> QT;
   __shared__ __align__(16) uint16_t q_lds0[QT::kPlane * PARTS], g_lds0[QT::kPlane * PARTS];
   __shared__ __align__(16) uint16_t q_lds1[PARTS == 1 ? QT::kPlane : 8], g_lds1[PARTS == 1 ? QT::kPlane : 8];
-  __shared__ __align__(16) float base_lds[BUFS][QB], delta_lds[BUFS][QB];
+  __shared__ __align__(16) float base_lds[BUFS][QB], delta_lds[BUFS][QB], inv_lds[BUFS][QB];
   __shared__ __align__(16) int doc_lds[BUFS][QB];
   __shared__ __align__(16) uint16_t v_lds[kBlock * DP * PARTS];
   __shared__ __align__(16) uint16_t k_lds[KEYS_IN_LDS ? kBlock * DP * PARTS : 8];
-  __shared__ uint64_t bad_lds[BUFS];
+  __shared__ uint64_t bad_lds[BUFS], scaled_lds[BUFS];
   __shared__ int range_lds[4][2];
   const int tid = threadIdx.x, wave = (tid >> 6) & 3, set = tid >> 8, lane = tid & 63, hh = lane >> 5, c = lane & 31;
   // the first keys of a causal mask are seen by the most queries
@@ -351,15 +467,14 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
   const int end = walk.end;
   const int lr = tid / CH, lc = tid % CH;
   Raw8<PARTS> rq[PARTS == 3 ? LOADS : 1], rg[PARTS == 3 ? LOADS : 1];
-  float rlse = 0.f, rdelta = 0.f;  // as loaded: waited for where they are used
+  float4 rstat = make_float4(0.f, 0.f, 1.f, 0.f);  // as loaded: waited for where they are used
   int rdoc = 0;
   auto load = [&](int head, int t, auto to) __attribute__((always_inline)) {
     const int h = hk * p.G + head, q0 = t * QB;
     if (tid < QB) {
       const int i = min(q0 + tid, p.Nq - 1);
-      const int64_t at = (static_cast<int64_t>(b) * p.Nq + i) * p.H + h;
-      rlse = q0 + tid < p.Nq ? p.lse[at] : kNegInf;
-      rdelta = deltas[at];
+      rstat = *reinterpret_cast<const float4*>(stats + (static_cast<int64_t>(b) * p.Nq + i) * p.H + h);
+      if (q0 + tid >= p.Nq) rstat.x = kNegInf;
       if (by_document) rdoc = shift + i >= 0 ? p.documents[static_cast<int64_t>(b) * p.Nk + shift + i] : -1;
     }
     if constexpr (PARTS == 1) {
@@ -392,12 +507,13 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
     auto put_rows = [&] {
       if (tid < QB) {
         // a query that sees nothing, or is none: weights of 2^-inf
-        const bool bad = rlse == kNegInf;
-        const uint64_t votes = __ballot(bad);
-        base_lds[B][tid] = bad ? kNegInf : row_base<PARTS, CAP>(p, rlse);
-        delta_lds[B][tid] = bad ? 0.f : rdelta;
+        const bool bad = rstat.x == kNegInf;
+        const uint64_t votes = __ballot(bad), scaled = __ballot(!bad && rstat.z != 1.f);
+        base_lds[B][tid] = rstat.x;
+        delta_lds[B][tid] = bad ? 0.f : rstat.y;
+        inv_lds[B][tid] = rstat.z;
         if (by_document) doc_lds[B][tid] = rdoc >= 0 ? rdoc : kNoDocument;
-        if (tid == 0) bad_lds[B] = votes;
+        if (tid == 0) bad_lds[B] = votes, scaled_lds[B] = scaled;
       }
     };
     if constexpr (PARTS == 1) {
@@ -433,6 +549,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
     if (!unseen) {
       const bool mixed = by_document && !(one_document && here.lo == here.hi && here.lo == wave_lo && !here.pad);
       const bool masked = mixed || wave0 + 31 >= n || (p.causal && wave0 + 31 >= prefix && p0 < wave0 + 31);
+      const bool scaled = scaled_lds[B] != 0;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const int r0 = 32 * (nb + (SETS == 2 ? set : 0));
@@ -442,10 +559,10 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
             [&](int ds) { return Three<PARTS>{qt.rows(r0, ds, l), gt.rows(r0, ds, l), vt.rows(32 * wave, ds, l)}; },
             [&](int ds, const Three<PARTS>& x) {
               if constexpr (KEYS_IN_LDS)
-                s = mma(x.a, keys.rows(32 * wave, ds, l), s);
+                s = mma_turned(x.a, keys.rows(32 * wave, ds, l), s);
               else
-                s = mma(x.a, k[ds], s);
-              dp = mma(x.b, x.c, dp);
+                s = mma_turned(x.a, k[ds], s);
+              dp = mma_turned(x.b, x.c, dp);
             });
         const int r1 = r0 + 4 * hh;
         const float away = static_cast<float>(p0 + r1 - key);
@@ -459,6 +576,14 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 32 ? 2 : 1) to
             pair<PARTS, CAP, SLOPE>(p, s[4 * e + x], dp[4 * e + x], slope2, away + static_cast<float>(8 * e + x), b0[x], d[x], w, gs);
             s[4 * e + x] = w;
             dp[4 * e + x] = gs;
+          }
+        }
+        if (scaled) {  // weights 2^(s - m) get their rows' 1 / l
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const v4f inv = *reinterpret_cast<const v4f*>(&inv_lds[B][r1 + 8 * e]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[4 * e + x] *= inv[x], dp[4 * e + x] *= inv[x];
           }
         }
         if (masked) {
@@ -611,24 +736,22 @@ int64_t split_bytes(const hz_token_attention& a) {
   return q > kv ? q : kv;
 }
 
-int64_t delta_bytes(const hz_token_attention& a) {
-  return (a.B * a.Nq * a.H * static_cast<int64_t>(sizeof(float)) + 15) / 16 * 16;
-}
+int64_t stats_bytes(const hz_token_attention& a) { return a.B * a.Nq * a.H * static_cast<int64_t>(sizeof(RowStats)); }
 
 template <int DP, int PARTS, bool CAP, bool SLOPE>
 hipError_t run(const hz_token_attention& a, const hz_token_tensor& dout, void* dq, void* dk, void* dv, void* workspace,
                hipStream_t stream) {
   constexpr int WAVES = PARTS == 1 || DP == 64 ? 8 : 4;
   Params p = make_params(a);
-  float* const deltas = static_cast<float*>(workspace);
+  RowStats* const stats = static_cast<RowStats*>(workspace);
   Splits of_q = dq_splits(a), of_kv = dkv_splits(a);
-  of_q.partial = of_kv.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a));
-  DocTile* const tiles = reinterpret_cast<DocTile*>(static_cast<char*>(workspace) + delta_bytes(a) + split_bytes(a));
+  of_q.partial = of_kv.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(a));
+  DocTile* const tiles = reinterpret_cast<DocTile*>(static_cast<char*>(workspace) + stats_bytes(a) + split_bytes(a));
   if (hipError_t err = launch_docs(a, p, true, tiles, stream); err != hipSuccess) return err;
   const int64_t nq = a.B * a.H * ((a.Nq + kBlock - 1) / kBlock) * of_q.n, nk = a.B * a.Hk * ((a.Nk + kBlock - 1) / kBlock) * of_kv.n;
-  token_dq_kernel<DP, PARTS, CAP, SLOPE><<<static_cast<unsigned>(nq), 256, 0, stream>>>(p, dout, dq, deltas, tiles, of_q);
+  token_dq_kernel<DP, PARTS, CAP, SLOPE><<<static_cast<unsigned>(nq), 256, 0, stream>>>(p, dout, dq, stats, tiles, of_q);
   launch_sum<PARTS>(of_q, 1, dq, nullptr, stream);
-  token_dkv_kernel<DP, PARTS, CAP, SLOPE, WAVES><<<static_cast<unsigned>(nk), 64 * WAVES, 0, stream>>>(p, dout, deltas, dk, dv, tiles, of_kv);
+  token_dkv_kernel<DP, PARTS, CAP, SLOPE, WAVES><<<static_cast<unsigned>(nk), 64 * WAVES, 0, stream>>>(p, dout, stats, dk, dv, tiles, of_kv);
   launch_sum<PARTS>(of_kv, 2, dk, dv, stream);
   return hipGetLastError();
 }
@@ -636,7 +759,7 @@ hipError_t run(const hz_token_attention& a, const hz_token_tensor& dout, void* d
 }  // namespace
 
 int64_t token_attention_bwd_workspace(const hz_token_attention& a) {
-  return delta_bytes(a) + split_bytes(a) + doc_bytes(a);
+  return stats_bytes(a) + split_bytes(a) + doc_bytes(a);
 }
 
 hipError_t launch_token_attention_bwd(const hz_token_attention& a, const hz_token_tensor& dout, void* dq, void* dk,

@@ -189,9 +189,11 @@ __device__ __forceinline__ void scores(v16f (&s)[N], const Params& p, const Sigh
 // weight is then 1, which bfloat16 rounds exactly (with a base up to 2^8 behind, attn_prompt_bf16 is 3% faster and
 // its output 0.0020 of its size off, not 0.0018).
 // Softmax weights of N score blocks; true (in every lane of the wave) if sums made before have to
-// be multiplied by alpha.
+// be multiplied by alpha. (Scores are rounded before the base is taken off, never fused with it: the largest one's
+// weight is then 2^0 at any size of the scores.)
 template <bool U, int N>
 __device__ __forceinline__ bool weigh(v16f (&s)[N], const Params& p, Running& r, float& alpha) {
+#pragma clang fp contract(off)
   float top = s[0][0];
 #pragma unroll
   for (int n = 0; n < N; ++n)
@@ -200,7 +202,7 @@ __device__ __forceinline__ bool weigh(v16f (&s)[N], const Params& p, Running& r,
   const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
   top = U ? fminf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) : fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
   const float cap2 = p.to_score2;
-  if (U) top = cap2 - 2.f * cap2 * top;
+  if (U) top = fmaf(-2.f * cap2, top, cap2);
   const bool move = top > r.m;
   const bool any = __any(move);
   if (any) {
@@ -214,7 +216,7 @@ __device__ __forceinline__ bool weigh(v16f (&s)[N], const Params& p, Running& r,
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[n][i] = fast_exp2(U ? a - 2.f * cap2 * s[n][i] : s[n][i] + a);
+    for (int i = 0; i < 16; ++i) s[n][i] = fast_exp2(U ? fmaf(-2.f * cap2, s[n][i], a) : s[n][i] + a);
   return any;
 }
 

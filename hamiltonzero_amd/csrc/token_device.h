@@ -146,6 +146,15 @@ __device__ __forceinline__ v16f mma(const Frag<3>& a, const Frag<3>& b, v16f c) 
   return c;
 }
 
+// The product of the transposed operands (a takes b's place): the same terms in the same order, so that the sums of S and of S^T
+// have the same bits.
+__device__ __forceinline__ v16f mma_turned(const Frag<1>& a, const Frag<1>& b, v16f c) { return mma(a, b, c); }
+__device__ __forceinline__ v16f mma_turned(const Frag<3>& a, const Frag<3>& b, v16f c) {
+#pragma unroll
+  for (int t = 0; t < kSplitTerms; ++t) c = mfma32_bf16(as_bf16x8(a.p[kSplitB[t]]), as_bf16x8(b.p[kSplitA[t]]), c);
+  return c;
+}
+
 __device__ __forceinline__ v4f mma16(const Frag<1>& a, const Frag<1>& b, v4f c) {
   return mfma16_bf16(as_bf16x8(a.p[0]), as_bf16x8(b.p[0]), c);
 }

@@ -115,6 +115,8 @@ int hz_token_attention_fwd(hipStream_t stream, const hz_token_attention* p, void
  * Its reverse mode for the cotangent dout (strided) of out; out and lse are the forward's:
  *     P = exp(s - lse),  dP = dout v^T,  dS = P (dP - rowsum(dout out)) (1 - tanh^2(x / softcap))
  *     dq = scale dS k,  dk = scale sum over the key head's query heads of dS^T q,  dv = the same of P^T dout
+ * P is at most 1. Rows whose lse is above 32 in size (256 for bfloat16) have their largest score and sum formed again, so that
+ * their weights keep their precision at any size of the scores.
  * dq [B, Nq, H, D], dk, dv [B, Nk, Hk, D]; what no visible pair reaches is zero.
  */
 int64_t hz_token_attention_bwd_workspace(const hz_token_attention* p);
