@@ -72,6 +72,64 @@ def _fields(t: Tensor) -> tuple:
     return t.data_ptr(), 0 if n0 == 1 else s0, 0 if n1 == 1 else s1, 0 if n2 == 1 else s2
 
 
+def _reaches(d: int, terms: list) -> bool:
+    """Whether ``d`` is a sum of ``c * step`` with ``low <= c <= high`` for each ``(step, low, high)`` of ``terms`` (positive
+    steps in descending order). Steps that enclose each other, as a view's do, leave a choice or two each."""
+    if not terms:
+        return d == 0
+    step, low, high = terms[0]
+    rest = terms[1:]
+    first = max(low, -((sum(s * h for s, _, h in rest) - d) // step))
+    last = min(high, (d - sum(s * l for s, l, _ in rest)) // step)
+    return any(_reaches(d - c * step, rest) for c in range(first, last + 1))
+
+
+def _steps(t: Tensor) -> list:
+    """``(bytes, count)`` of each axis of ``t`` that moves, with its elements' bytes as one more."""
+    size = t.element_size()
+    return [(s * size, n) for s, n in zip(t.stride(), t.shape) if n > 1 and s] + [(1, size)]
+
+
+def _end(t: Tensor) -> int:
+    """The address behind the last element of a strided [B, N, H, D] tensor."""
+    (n0, n1, n2, n3), (s0, s1, s2, s3) = t.shape, t.stride()
+    return t.data_ptr() + ((n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + (n3 - 1) * s3 + 1) * t.element_size()
+
+
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether two strided tensors share a byte. (Views of one buffer may lie between each other's rows and share none.)"""
+    d = b.data_ptr() - a.data_ptr()
+    low, high = {}, {}
+    for s, n in _steps(a):
+        high[s] = high.get(s, 0) + n - 1
+    for s, n in _steps(b):
+        low[s] = low.get(s, 0) + 1 - n
+    return _reaches(d, [(s, low.get(s, 0), high.get(s, 0)) for s in sorted({*low, *high}, reverse=True)])
+
+
+def _holds_twice(t: Tensor) -> bool:
+    """Whether two elements of a strided tensor lie at one place."""
+    if t.is_contiguous():
+        return False
+    far, nested = 0, True
+    for s, n in sorted(zip(t.stride(), t.shape)):
+        if n > 1:
+            nested = nested and s > far
+            far += s * (n - 1)
+    if nested or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        return not nested
+    # the same sum of steps from indices that first differ at some axis
+    steps = sorted(_steps(t), reverse=True)
+    return any(_reaches(0, [(s, 1, n - 1), *((s2, 1 - n2, n2 - 1) for s2, n2 in steps[i + 1:])]) for i, (s, n) in enumerate(steps) if n > 1)
+
+
+def _meet(out: Tuple[Tensor, Tensor], inputs: Tuple[Tensor, Tensor]) -> bool:
+    """Whether the results share memory with each other or with an input; ranges of addresses first, which mostly are apart."""
+    all_ = [(t, t.data_ptr(), _end(t)) for t in (*out, *inputs)]
+    return any(begin < last and first < end and _overlap(t, x)
+               for i, (t, begin, end) in enumerate(all_[:2]) for x, first, last in (all_[1:] if i == 0 else all_[2:]))
+
+
 def _like(t: Tensor) -> Tensor:
     """A new contiguous tensor like ``t``, whose own strides may be a view's."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
@@ -203,9 +261,9 @@ def qk_norm_rotary(
             _check(name, t, dev, q.dtype, tuple(like.shape))
             if _strided(t) is not t:
                 raise ValueError(f"{name} must have contiguous heads and 16-byte aligned rows, got strides {t.stride()}")
-            if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+            if _holds_twice(t):
                 raise ValueError(f"{name} must not hold one element at several places, got strides {t.stride()}")
-        if out[0].data_ptr() == out[1].data_ptr() or any(o.data_ptr() == t.data_ptr() for o in out for t in (q, k)):
+        if _meet(out, (q, k)):
             raise ValueError("out must not overlap the inputs, nor one result the other")
     return _norm_fwd(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), float(eps), out)
 
