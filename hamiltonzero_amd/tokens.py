@@ -24,6 +24,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 from torch.autograd.function import once_differentiable
 
 from . import _native
@@ -230,7 +231,8 @@ def qk_norm_rotary(
     D is a multiple of 8 up to 256.
 
     Returns the two results, new tensors or ``out``: strided views of the same shapes that do not overlap
-    the inputs or each other (a cache's rows, say), for calls that need no gradient."""
+    the inputs or each other (a cache's rows, say), for calls that need no gradient. What is written there counts as
+    changed in place: the backward of an earlier call that saved it raises."""
     _check_first("q", q, "[B, N, H, D]")
     _check_first("k", k, "[B, N, Hk, D]")
     B, N, H, D = q.shape
@@ -261,11 +263,16 @@ def qk_norm_rotary(
             _check(name, t, dev, q.dtype, tuple(like.shape))
             if _strided(t) is not t:
                 raise ValueError(f"{name} must have contiguous heads and 16-byte aligned rows, got strides {t.stride()}")
+            if t.requires_grad and torch.is_grad_enabled():
+                raise ValueError(f"{name} requires a gradient, which a result written into it has not: call under torch.no_grad()")
             if _holds_twice(t):
                 raise ValueError(f"{name} must not hold one element at several places, got strides {t.stride()}")
         if _meet(out, (q, k)):
             raise ValueError("out must not overlap the inputs, nor one result the other")
-    return _norm_fwd(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), float(eps), out)
+    res = _norm_fwd(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), float(eps), out)
+    if out is not None:
+        increment_version(res)  # as after an in-place write: a graph that saved what is overwritten says so
+    return res
 
 
 # --- attention ------------------------------------------------------------------------------------

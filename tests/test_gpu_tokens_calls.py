@@ -65,3 +65,22 @@ def test_out_beside_its_input_is_taken():
     k_cache = torch.empty_like(cache[:, :, :Hk])
     hz.qk_norm_rotary(q, k, out=(cache[:, N:], k_cache[:, N:]))
     assert torch.equal(cache[:, N:], want[0]) and torch.equal(k_cache[:, N:], want[1])
+
+
+def test_out_counts_as_a_change():
+    """A tensor that a differentiable call saved is written by ``out=``: its backward says so, as after an in-place write."""
+    g = gen(61)
+    q, v = normal(g, 1, 4, 2, 32), normal(g, 1, 8, 2, 32)
+    cache = normal(g, 1, 8, 2, 32)
+    leaf = q.clone().requires_grad_()
+    for part, row in ((slice(0, 1), 0), (slice(1, 2), 1)):
+        out = hz.token_attention(leaf, cache, v, causal=True)
+        x, into = torch.zeros(1, 4, 2, 32, device="cuda"), [torch.empty(1, 4, 2, 32, device="cuda"), cache[:, 4:]]
+        versions = [t._version for t in into]
+        with torch.no_grad():
+            hz.qk_norm_rotary(x, x, out=tuple(into[::-1]) if row else tuple(into))
+        assert all(t._version > n for t, n in zip(into, versions))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out.sum(), leaf)
+    with pytest.raises(ValueError, match="gradient"):  # a leaf of a graph is no place for results
+        hz.qk_norm_rotary(x, x, out=(torch.empty_like(x).requires_grad_(), torch.empty_like(x)))
