@@ -254,21 +254,19 @@ def qk_norm_rotary(
         _check("positions", positions, dev, torch.int32, (B, N))
         positions = positions.contiguous()
     cw_q, cw_k = (None if w is None else w.contiguous() for w in (w_q, w_k))
-    if _wants_grad(q, k, w_q, w_k):
-        if out is not None:
-            raise ValueError("out= holds results without gradients: call under torch.no_grad()")
-        return _QKNormRotary.apply(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), float(eps))
     if out is not None:
         for name, t, like in (("out[0]", out[0], q), ("out[1]", out[1], k)):
             _check(name, t, dev, q.dtype, tuple(like.shape))
             if _strided(t) is not t:
                 raise ValueError(f"{name} must have contiguous heads and 16-byte aligned rows, got strides {t.stride()}")
-            if t.requires_grad and torch.is_grad_enabled():
-                raise ValueError(f"{name} requires a gradient, which a result written into it has not: call under torch.no_grad()")
             if _holds_twice(t):
                 raise ValueError(f"{name} must not hold one element at several places, got strides {t.stride()}")
         if _meet(out, (q, k)):
             raise ValueError("out must not overlap the inputs, nor one result the other")
+    if _wants_grad(q, k, w_q, w_k, freqs, *(out or ())):
+        if out is not None:
+            raise ValueError("out= holds results without gradients: call under torch.no_grad()")
+        return _QKNormRotary.apply(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), float(eps))
     res = _norm_fwd(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), float(eps), out)
     if out is not None:
         increment_version(res)  # as after an in-place write: a graph that saved what is overwritten says so
@@ -388,7 +386,7 @@ def token_attention(
         kv_len = kv_len.contiguous()
     opts = (slopes, prefix, documents, kv_len, float(D) ** -0.5 if scale is None else float(scale), float(softcap),
             bool(causal))
-    if _wants_grad(q, k, v):
+    if _wants_grad(q, k, v, slopes):
         return _TokenAttention.apply(q, k, v, opts)
     return token_attention_fwd(q, k, v, opts, False)[0]
 

@@ -4,6 +4,7 @@ form."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import hamiltonzero_amd as hz
 
@@ -84,3 +85,24 @@ def test_out_counts_as_a_change():
             torch.autograd.grad(out.sum(), leaf)
     with pytest.raises(ValueError, match="gradient"):  # a leaf of a graph is no place for results
         hz.qk_norm_rotary(x, x, out=(torch.empty_like(x).requires_grad_(), torch.empty_like(x)))
+
+
+# --- forward mode, leaves that only inference has ----------------------------------------------------
+
+
+def test_tangents_of_tables_are_refused():
+    x = torch.zeros(2, 8, 4, 32, device="cuda")
+    slopes, freqs = torch.ones(4, device="cuda"), torch.ones(16, dtype=torch.float64, device="cuda")
+    with fwd.dual_level():
+        s = fwd.make_dual(slopes, torch.ones_like(slopes))
+        f = fwd.make_dual(freqs, torch.ones_like(freqs))
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            hz.token_attention(x, x, x, slopes=s)
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            hz.qk_norm_rotary(x, x, freqs=f)
+        with pytest.raises(NotImplementedError, match="forward mode"), torch.no_grad():
+            hz.token_attention(x, x, x, slopes=s)
+        assert hz.token_attention(x, x, x, slopes=slopes).shape == x.shape
+        out = torch.empty_like(x)
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            hz.qk_norm_rotary(x, x, out=(fwd.make_dual(out, out), torch.empty_like(x)))
