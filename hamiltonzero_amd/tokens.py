@@ -247,7 +247,7 @@ def qk_norm_rotary(
         if freqs.dim() != 1 or freqs.shape[0] % 4 or not 0 < 2 * freqs.shape[0] <= D:
             raise ValueError(f"freqs must hold a multiple of 4 frequencies, at most D / 2 = {D // 2}, got {tuple(freqs.shape)}")
         _check("freqs", freqs, dev, torch.float64, (freqs.shape[0],))
-        if freqs.requires_grad:
+        if freqs.requires_grad and torch.is_grad_enabled():
             raise ValueError("freqs has no gradient here: detach it")
         freqs = freqs.contiguous()
     if positions is not None:

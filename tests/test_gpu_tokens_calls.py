@@ -106,3 +106,17 @@ def test_tangents_of_tables_are_refused():
         out = torch.empty_like(x)
         with pytest.raises(NotImplementedError, match="forward mode"):
             hz.qk_norm_rotary(x, x, out=(fwd.make_dual(out, out), torch.empty_like(x)))
+
+
+def test_parameters_serve_without_gradients():
+    """Frequencies that are a parameter are refused where a gradient would be dropped, and taken where none is asked."""
+    g = gen(62)
+    q = normal(g, 1, 5, 2, 32)
+    freqs = torch.rand(16, generator=g, dtype=torch.float64, device="cuda")
+    leaf = freqs.clone().requires_grad_()
+    with pytest.raises(ValueError, match="no gradient"):
+        hz.qk_norm_rotary(q, q, freqs=leaf)
+    with torch.no_grad():
+        got = hz.qk_norm_rotary(q, q, freqs=leaf)
+    for a, b in zip(got, hz.qk_norm_rotary(q, q, freqs=freqs)):
+        assert torch.equal(a, b)
