@@ -391,24 +391,29 @@ int bwd_slots(const BucketParams& p) {
   return static_cast<int>(n < 1 ? 1 : n < most ? n : most);
 }
 
+// The most dynamic LDS a kernel is launched with: a limit of the function's, so every call sets the same one, and calls of
+// other sizes in other threads do not lower it between this and the launch.
+constexpr size_t kMostBuckets = (2 * HZ_BUCKET_MAX_RANGE + 1) * sizeof(uint16_t);
+constexpr size_t kMostTable = HZ_BUCKET_MAX_TABLE * sizeof(float);  // (n_buckets + 1) rows of H, or of 64 threads
+static_assert((HZ_BUCKET_MAX + 1) * 64 <= HZ_BUCKET_MAX_TABLE && kMostTable + kMostBuckets <= (160u << 10));
 template <class K>
-hipError_t allow_lds(K kernel, size_t bytes) {
+hipError_t allow_lds(K kernel, size_t most) {
   return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(bytes));
+                             static_cast<int>(most));
 }
 
 template <class S, int V>
 hipError_t run_qhk(const BucketParams& p, const void* de, float* partial, hipStream_t stream) {
   const int T = qhk_threads(p);
   const size_t lds = (static_cast<size_t>(p.nb) + 1) * T * sizeof(float) + bucket_bytes(p);
-  if (hipError_t err = allow_lds(bucket_bias_bwd_qhk_kernel<S, V>, lds); err != hipSuccess) return err;
+  if (hipError_t err = allow_lds(bucket_bias_bwd_qhk_kernel<S, V>, kMostTable + kMostBuckets); err != hipSuccess) return err;
   bucket_bias_bwd_qhk_kernel<S, V><<<dim3(bwd_slots(p), p.H), T, lds, stream>>>(p, Divider::of(static_cast<int>(p.Nq)), de, partial);
   return hipGetLastError();
 }
 
 template <class S, int HB, bool WIDE>
 hipError_t run_qkh(const BucketParams& p, const void* de, float* partial, hipStream_t stream) {
-  if (hipError_t err = allow_lds(bucket_bias_bwd_qkh_kernel<S, HB, WIDE>, bucket_bytes(p)); err != hipSuccess) return err;
+  if (hipError_t err = allow_lds(bucket_bias_bwd_qkh_kernel<S, HB, WIDE>, kMostBuckets); err != hipSuccess) return err;
   const dim3 grid(bwd_slots(p), (p.H + 16 * HB - 1) / (16 * HB), (p.nb + 16 * kBlocks - 1) / (16 * kBlocks));
   const int64_t rows = p.B * p.Nq, most = (int64_t(1) << 30) / p.Nk, each = most < 1 ? 1 : most < rows ? most : rows;
   bucket_bias_bwd_qkh_kernel<S, HB, WIDE><<<grid, kThreads, bucket_bytes(p), stream>>>(
@@ -431,7 +436,7 @@ hipError_t launch_bucket_bias_fwd(const BucketParams& p, const float* table, voi
   const unsigned grid = static_cast<unsigned>(n < 2048 ? n : 2048);
   auto go = [&](auto kernel, size_t table_bytes) {
     const size_t lds = table_bytes + bucket_bytes(p);
-    if (hipError_t err = allow_lds(kernel, lds); err != hipSuccess) return err;
+    if (hipError_t err = allow_lds(kernel, kMostTable + kMostBuckets); err != hipSuccess) return err;
     kernel<<<grid, kThreads, lds, stream>>>(p, table, e);
     return hipGetLastError();
   };
