@@ -2,11 +2,15 @@
 with tangents, gradients of broadcast and shared leaves, tables of different sizes at once; and the cache kernel's widest
 form."""
 
+import threading
+
+import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
 import hamiltonzero_amd as hz
+from oracle import token_oracle as O
 
 pytestmark = pytest.mark.gpu
 F = 2.0**-24
@@ -120,3 +124,138 @@ def test_parameters_serve_without_gradients():
         got = hz.qk_norm_rotary(q, q, freqs=leaf)
     for a, b in zip(got, hz.qk_norm_rotary(q, q, freqs=freqs)):
         assert torch.equal(a, b)
+
+
+# --- gradients of broadcast and shared leaves ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("N", [7, 70, 150])
+def test_gradients_through_broadcasts(N, dtype):
+    """Keys and values expanded over batch and heads, and a cotangent expanded over all but D: the same bits as for
+    copies of them, which torch then adds up over the broadcast axes."""
+    _say(f"broadcast {N} {dtype}")
+    g = gen(63)
+    dt, B, H, D = DT[dtype], 2, 4, 32
+    q = normal(g, B, N, H, D, dtype=dt).requires_grad_()
+    k = normal(g, 1, N, 2, D, dtype=dt).requires_grad_()
+    v = normal(g, B, N, 1, D, dtype=dt).requires_grad_()
+    cot = normal(g, 1, 1, 1, D, dtype=dt)
+    out = hz.token_attention(q, k.expand(B, N, 2, D), v.expand(B, N, 2, D), causal=True)
+    got = torch.autograd.grad(out, (q, k, v), cot.expand_as(out))
+    full = [t.detach().expand(B, N, h, D).contiguous().requires_grad_() for t, h in ((q, H), (k, 2), (v, 2))]
+    same = hz.token_attention(*full, causal=True)
+    assert torch.equal(same, out)
+    dq, dk, dv = torch.autograd.grad(same, full, cot.expand_as(out).contiguous())
+    assert torch.equal(got[0], dq)
+    u = F if dtype == "f32" else 2.0**-8
+    for a, b, axis in ((got[1], dk, 0), (got[2], dv, 2)):  # two terms and one rounding
+        want = b.double().sum(axis, keepdim=True)
+        assert ((a.double() - want).abs() <= u * want.abs() + 2 * F * b.double().abs().sum(axis, keepdim=True)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norm_gradients_through_broadcasts(dtype):
+    g = gen(64)
+    dt, B, N, H, D = DT[dtype], 3, 5, 4, 32
+    q, k = normal(g, 1, N, 1, D, dtype=dt).requires_grad_(), normal(g, B, N, 2, D, dtype=dt).requires_grad_()
+    freqs = torch.rand(16, generator=g, dtype=torch.float64, device="cuda")
+    cot = normal(g, 1, 1, 1, D, dtype=dt)
+    out = hz.qk_norm_rotary(q.expand(B, N, H, D), k, freqs=freqs)
+    got = torch.autograd.grad(out, (q, k), [cot.expand_as(o) for o in out])
+    full = [q.detach().expand(B, N, H, D).contiguous().requires_grad_(), k.detach().clone().requires_grad_()]
+    same = hz.qk_norm_rotary(*full, freqs=freqs)
+    for a, b in zip(same, out):
+        assert torch.equal(a, b)
+    dq, dk = torch.autograd.grad(same, full, [cot.expand_as(o).contiguous() for o in same])
+    assert torch.equal(got[1], dk)
+    want, size = dq.double().sum((0, 2), keepdim=True), dq.double().abs().sum((0, 2), keepdim=True)
+    u = F if dtype == "f32" else 2.0**-8
+    # torch sums the three batches and then the heads (or both at once), each result rounded to the type
+    assert ((got[0].double() - want).abs() <= 2 * (u + 12 * F) * size).all()
+
+
+# --- the cache kernel's widest form -----------------------------------------------------------------------
+
+WIDE = [  # B, Nq, Nk, H, Hk, D, options: 17 to 32 rows of query and head share a key head
+    (2, 5, 700, 8, 2, 128, dict(softcap=20.0, causal=True, kv_len=[700, 233])),
+    (1, 1, 333, 32, 1, 128, dict(causal=True)),
+    (2, 3, 200, 8, 1, 80, dict(causal=True, slopes=True)),
+    (2, 17, 130, 1, 1, 64, dict(causal=True, documents=True)),
+    (1, 3, 900, 7, 1, 64, dict(softcap=5.0, slopes=True, causal=True, documents=True)),
+    (2, 6, 90, 4, 1, 40, dict(softcap=3.0, documents=True)),
+    (1, 8, 41, 12, 3, 128, dict(causal=True, prefix=[30], slopes=True)),
+    (3, 20, 20, 1, 1, 128, dict(causal=True, softcap=8.0, kv_len=[20, 0, 7])),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("case", WIDE, ids=lambda c: "%d-%d-%d-%d-%d-%d-%s" % (*c[:6], "-".join(c[6])))
+def test_two_blocks_of_columns(case, dtype):
+    B, Nq, Nk, H, Hk, D, o = case
+    assert 16 < Nq * (H // Hk) <= 32
+    _say(f"wide {case} {dtype}")
+    g, dt = gen(65), DT[dtype]
+    q, k, v = (normal(g, *s, dtype=dt, std=d).requires_grad_()
+               for s, d in (((B, Nq, H, D), 2.0), ((B, Nk, Hk, D), 1.0), ((B, Nk, Hk, D), 1.0)))
+    kw = {n: o[n] for n in ("softcap", "causal") if n in o}
+    for n in ("kv_len", "prefix"):
+        if n in o:
+            kw[n] = torch.tensor(o[n], dtype=torch.int32, device="cuda")
+    if "slopes" in o:
+        kw["slopes"] = 2.0 ** (-8.0 * torch.arange(1, H + 1, device="cuda") / H).float()
+    if "documents" in o:
+        kw["documents"] = torch.randint(0, 3, (B, Nk), generator=torch.Generator().manual_seed(6)).sort(1).values.to(torch.int32).cuda()
+        kw["documents"][:, -(Nq // 3):] = -1
+    out = hz.token_attention(q, k, v, **kw)
+    dout = normal(g, *out.shape, dtype=dt)
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    with torch.no_grad():
+        assert torch.equal(hz.token_attention(q, k, v, **kw), out)
+    okw = {n: x.cpu().numpy() if isinstance(x, torch.Tensor) else x for n, x in kw.items()}
+    want = O.attention(arr(q), arr(k), arr(v), scale=float(np.float32(D**-0.5)), dout=arr(dout), bf16=dtype == "bf16", **okw)
+    for name, x in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        off = np.abs(arr(x) - want[name])
+        print(f"  {name}: {float(np.max(off / np.maximum(want['t_' + name], 1e-300))):.3f} of its bound", flush=True)
+        assert (off <= want["t_" + name]).all(), name
+
+
+# --- tables of different sizes at once -----------------------------------------------------------------
+
+
+def test_tables_of_different_sizes_in_two_threads():
+    """A thread with the largest table beside one with the smallest: each call's memory is its own."""
+    _say("two tables")
+    pos = torch.arange(20, dtype=torch.int32, device="cuda")[None]
+    sizes = [(512, 60, 4096), (2, 60, 1)]
+    calls = []
+    for nb, H, R in sizes:
+        g = gen(nb)
+        calls.append((normal(g, nb, H), torch.randint(0, nb, (2 * R + 1,), generator=g, device="cuda").to(torch.int32)))
+
+    def one(table, plan, layout):
+        t = table.clone().requires_grad_()
+        e = hz.bucket_bias(t, plan, pos, pos, e_layout=layout)
+        return e.detach(), torch.autograd.grad(e, t, torch.ones_like(e))[0]
+
+    want = [[one(*c, layout) for layout in ("qhk", "qkh")] for c in calls]
+    torch.cuda.synchronize()
+    failed, start = [], threading.Barrier(2)
+
+    def work(i):
+        try:
+            start.wait()
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(100):
+                    for layout, w in zip(("qhk", "qkh"), want[i]):
+                        for a, b in zip(one(*calls[i], layout), w):
+                            assert torch.equal(a, b)
+        except Exception as e:  # shown by the assertion below
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed[0]

@@ -203,3 +203,30 @@ def test_a_row_of_nan_stays_one(Nq, dtype):
         assert torch.equal(got[i][0][rest], want[i][0][rest])
     assert got[3][0, :100 - Nq + 3, 1].isnan().all()
     assert torch.equal(got[3][0, :, 0], want[3][0, :, 0])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("Nq", [3, 120])
+def test_padding_may_hold_anything_beside_large_scores(Nq, dtype):
+    _say(f"far padding {Nq} {dtype}")
+    g = torch.Generator(device="cuda").manual_seed(53)
+    B, Nk, H, Hk, D = 2, 150, 4, 2, 64
+    q, k, v, dout = (normal(g, B, n, h, D, dtype=DT[dtype]) for n, h in ((Nq, H), (Nk, Hk), (Nk, Hk), (Nq, H)))
+    docs = (torch.arange(Nk, device="cuda") > 70).int().repeat(B, 1)
+    docs[:, 20:30], docs[0, 139:] = -1, -1
+    n = torch.tensor([140, 150], dtype=torch.int32, device="cuda")
+
+    def go(q, k, v, dout):
+        x = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = hz.token_attention(*x, causal=True, documents=docs, kv_len=n, scale=1e4)
+        return (out, *torch.autograd.grad(out, x, dout))
+
+    want = go(q, k, v, dout)
+    for bad in (float("nan"), float("-inf")):
+        k2, v2, q2, d2 = (t.clone() for t in (k, v, q, dout))
+        for t in (k2, v2):
+            t[:, 20:30], t[0, 139:] = bad, bad
+        for t in (q2, d2):
+            t[0, -1:] = bad
+        for a, b in zip(go(q2, k2, v2, d2), want):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
