@@ -272,6 +272,7 @@ int check_norm_rotary(const hz_qk_norm_rotary* p) {
   return check_strided("k_out", p->k_out);
 }
 
+// (Only the reverse mode has a grid of the keys' size: a forward without one takes any cache that memory holds.)
 int check_token_dims(const hz_token_attention* p) {
   if (p == nullptr) return fail(HZ_ENULL, "p must not be NULL");
   if (int rc = check_dtype(p->dtype)) return rc;
@@ -286,8 +287,10 @@ int check_token_dims(const hz_token_attention* p) {
   // grids of one-dimensional launches, with room for their thread counts
   const int64_t most = int64_t(1) << 20;
   if (p->B > most || p->H > most || p->B * p->H > most || p->B * p->H * ((p->Nq + 127) / 128) > most ||
-      p->B * p->Hk * ((p->Nk + 127) / 128) > most)
+      (p->lse != nullptr && p->B * p->Hk * ((p->Nk + 127) / 128) > most))
     return fail(HZ_EINVAL, "B * heads * ceil(N / 128) exceeds the grid limit of %lld", (long long)most);
+  if (p->documents != nullptr && p->B > (int64_t(1) << 31) / p->Nk)
+    return fail(HZ_EINVAL, "documents of B * Nk = %lld tokens exceed the supported size", (long long)(p->B * p->Nk));
   return HZ_OK;
 }
 

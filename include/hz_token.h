@@ -88,8 +88,8 @@ int hz_qk_norm_rotary_bwd(hipStream_t stream, const hz_qk_norm_rotary* p, void* 
  * (padding) are never used, whatever they hold; the other tokens' values must be finite.
  * q [B, Nq, H, D], k, v [B, Nk, Hk, D] strided; out [B, Nq, H, D]; lse [B, Nq, H] float32 or NULL (a
  * forward without a reverse pass). slopes [H] float32, prefix [B], documents [B, Nk] and kv_len [B]
- * int32. D a multiple of 8 up to HZ_TOKEN_MAX_HEAD, H a multiple of Hk, Nq, Nk < 2^30; prefix only
- * with causal.
+ * int32. D a multiple of 8 up to HZ_TOKEN_MAX_HEAD, H a multiple of Hk, Nq, Nk < 2^30, B H ceil(Nq / 128) and, with
+ * lse, B Hk ceil(Nk / 128) at most 2^20, B Nk at most 2^31 with documents; prefix only with causal.
  * out_low [B, Nq, H, D] or NULL, for bfloat16: what out's rounding left out, rounded to bfloat16. The
  * reverse pass takes rowsum(dout out) from both where it is given: from out alone the row sum's error is as large
  * as that of all other roundings of dq and dk together.

@@ -259,3 +259,26 @@ def test_tables_of_different_sizes_in_two_threads():
     for t in threads:
         t.join()
     assert not failed, failed[0]
+
+
+# --- caches that fill the card -------------------------------------------------------------------------
+
+
+def test_more_keys_than_a_reverse_pass_takes():
+    """A thousand rows of 131072 keys (here the same ones): a forward alone has no grid of the keys' size."""
+    _say("many long rows")
+    g = gen(66)
+    B, Nk, Hk, D = 1024, 131072, 2, 64
+    k, v = (normal(g, 1, Nk, Hk, D, dtype=torch.bfloat16).expand(B, Nk, Hk, D) for _ in range(2))
+    q = normal(g, B, 1, 4, D, dtype=torch.bfloat16)
+    n = torch.full((B,), Nk, dtype=torch.int32, device="cuda")
+    n[-1] = Nk - 77
+    out = hz.token_attention(q, k, v, causal=True, kv_len=n)
+    for b in (0, 517, B - 1):
+        for h in range(4):
+            keys, values = k[b, :n[b], h // 2].double(), v[b, :n[b], h // 2].double()
+            w = torch.softmax(keys @ q[b, 0, h].double() * D**-0.5, 0)
+            want, size = w @ values, w @ values.abs()
+            assert ((out[b, 0, h].double() - want).abs() <= size * (2.0**-8 + 0.08 * 2**-8) + want.abs() * 2.0**-8).all()
+    with pytest.raises(hz._native.HzError, match="grid limit"):
+        hz.token_attention(q.clone().requires_grad_(), k, v)
