@@ -20,6 +20,7 @@ rows); others are copied first. Every axis must be at least 1 long.
 from __future__ import annotations
 
 import contextlib
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -50,6 +51,12 @@ _HERE = contextlib.nullcontext()
 
 def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _float32(x: float) -> float:
+    """``x`` as the library's structures hold it: infinite beyond float32's range, which it refuses."""
+    x = float(x)
+    return x if not abs(x) > 3.4028234663852886e38 else math.copysign(math.inf, x)
 
 
 def _ptr(t: Optional[Tensor]) -> int:
@@ -266,8 +273,8 @@ def qk_norm_rotary(
     if _wants_grad(q, k, w_q, w_k, freqs, *(out or ())):
         if out is not None:
             raise ValueError("out= holds results without gradients: call under torch.no_grad()")
-        return _QKNormRotary.apply(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), float(eps))
-    res = _norm_fwd(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), float(eps), out)
+        return _QKNormRotary.apply(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), _float32(eps))
+    res = _norm_fwd(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), _float32(eps), out)
     if out is not None:
         increment_version(res)  # as after an in-place write: a graph that saved what is overwritten says so
     return res
@@ -384,7 +391,7 @@ def token_attention(
     if kv_len is not None:
         _check("kv_len", kv_len, dev, torch.int32, (B,))
         kv_len = kv_len.contiguous()
-    opts = (slopes, prefix, documents, kv_len, float(D) ** -0.5 if scale is None else float(scale), float(softcap),
+    opts = (slopes, prefix, documents, kv_len, float(D) ** -0.5 if scale is None else _float32(scale), _float32(softcap),
             bool(causal))
     if _wants_grad(q, k, v, slopes):
         return _TokenAttention.apply(q, k, v, opts)

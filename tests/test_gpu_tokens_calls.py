@@ -282,3 +282,11 @@ def test_more_keys_than_a_reverse_pass_takes():
             assert ((out[b, 0, h].double() - want).abs() <= size * (2.0**-8 + 0.08 * 2**-8) + want.abs() * 2.0**-8).all()
     with pytest.raises(hz._native.HzError, match="grid limit"):
         hz.token_attention(q.clone().requires_grad_(), k, v)
+
+
+def test_options_beyond_float32_are_refused():
+    x = torch.zeros(1, 4, 2, 32, device="cuda")
+    for call in (lambda: hz.token_attention(x, x, x, scale=1e39), lambda: hz.token_attention(x, x, x, softcap=1e300),
+                 lambda: hz.qk_norm_rotary(x, x, eps=1e39)):
+        with pytest.raises(hz._native.HzError):
+            call()

@@ -1,8 +1,11 @@
 """Sizes that the token attention's C entry takes and refuses, by its workspace calls and checks (nothing is enqueued)."""
 
+import math
+import struct
+
 import pytest
 
-from hamiltonzero_amd import _native
+from hamiltonzero_amd import _native, tokens
 
 A = 0x10000  # a fake address: never read
 
@@ -38,3 +41,10 @@ def test_documents_of_too_many_tokens(lib):
     assert "documents" in lib.hz_last_error().decode()
     assert lib.hz_token_attention_fwd(None, attn(256, 1, 1 << 24, 1, 1, 8, documents=A), A, 1 << 60) == _native.HZ_EINVAL
     assert lib.hz_token_attention_fwd_workspace(attn(128, 200, 1 << 24, 1, 1, 8, documents=A)) > 0
+
+
+@pytest.mark.parametrize("x", [0.0, 1.5, -3.4028234663852886e38, 3.402823567e38, 1e39, -1e300, math.inf, -math.inf, math.nan])
+def test_options_beyond_float32(x):
+    """They reach the library, whose checks name them, as infinities: no error of the packing comes first."""
+    got, = struct.unpack("f", struct.pack("f", tokens._float32(x)))
+    assert (math.isnan(got) and math.isnan(x)) or got == x or (math.isinf(got) and got * x > 0 and abs(x) > 3.4028234e38)
