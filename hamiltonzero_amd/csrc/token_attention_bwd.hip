@@ -7,7 +7,7 @@
 // row's largest score and sum, which the first forms again), so scores and dP are formed twice: nine products a tile
 // pair (two for the score gradients' second bfloat16 part) where one kernel with atomic dq sums would need seven. Bound by
 // the products and, between them, the exponentials' vector work; attn_train_packed_bf16 (8192 tokens in four documents, 16
-// on 4 heads of 128): 259 us for dq, 423 for dk and dv. Tiles are copied, skipped and masked as in the forward.
+// on 4 heads of 128): 220 us for dq, 354 for dk and dv, matrix cores busy 34% and 25%. Tiles are copied, skipped and masked as in the forward.
 #include "token_device.h"
 
 namespace hz {

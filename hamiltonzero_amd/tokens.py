@@ -234,7 +234,7 @@ def qk_norm_rotary(
 
     ``freqs`` float64, in radians a position (None: no rotation), its length a multiple of 4;
     ``positions [B, N]`` int32 (None: 0 .. N - 1). A pair is elements ``p`` and ``p + len(freqs)``, or ``2 p``
-    and ``2 p + 1`` with ``interleaved``. Angles are formed in float64, so far positions keep their bits.
+    and ``2 p + 1`` with ``interleaved``. Angles are formed in float64 and reduced to a turn there, so that far positions are as exact as near ones.
     D is a multiple of 8 up to 256.
 
     Returns the two results, new tensors or ``out``: strided views of the same shapes that do not overlap
