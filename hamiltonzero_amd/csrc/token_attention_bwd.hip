@@ -70,8 +70,8 @@ __device__ __forceinline__ void pair(const Params& p, float x, float dp, float s
 // lse is a rounded logarithm, and its change of base rounds again: a weight rebuilt from it is off by up to five times
 // 2^-24 |lse| of itself, all of a row's by the same factor. Rows whose lse is above this (or is not finite) get their largest
 // score and their sum formed again, from the scores as the reverse pass forms them: weights 2^(s - m) / l. Below it they are
-// off by 1e-5 (float32) and 8e-5 (bfloat16) at most; without it a lone key's weight was off by 7e-4 at a score of 10^4, 9%
-// at 10^6, and NaN or 0 at 10^10. Where every block has such a row the reverse pass takes a quarter to a third longer (4 x
+// off by 1e-5 (float32) and 8e-5 (bfloat16) at most; without it a lone key's weight was off by up to 1.4e-3 at a score of
+// 10^4, 16% at 10^6, and NaN at 10^10. Where every block has such a row the reverse pass takes a quarter to a third longer (4 x
 // 2048 tokens of 16 on 4 bfloat16 heads of 64: 250 us and 356; float32, 4 x 1024: 213 and 273), and twice as long
 // where the keys are divided, since each part goes over all of them.
 template <int PARTS>
