@@ -14,7 +14,9 @@ Public surface, named after the reference modules it replaces:
   the large-N caller's head collapse fused into it (``gated_rectangular_edge_attention``,
   ``sequence_attention_output``: ``src/hamiltonzero/evaluation/sequence_trunk.py``).
 * :mod:`hamiltonzero_amd.tokens` — operators of token sequences (no reference counterpart):
-  ``qk_norm_rotary``, ``token_attention`` and ``bucket_bias`` with ``relative_buckets``.
+  ``qk_norm_rotary``, ``qk_rotary``, ``token_attention`` and ``bucket_bias`` with ``relative_buckets``.
+* :mod:`hamiltonzero_amd.paged` — paged caches of token sequences (no reference counterpart): ``paged_append``,
+  ``paged_attention`` and ``paged_evict``.
 * :mod:`hamiltonzero_amd.kernels` — tensor-level calls of the C ABI
   (``include/hz_mhsea.h``): forward, tangent, fused forward+tangent, backward,
   gated forward+tangent, rectangular forward.
@@ -30,6 +32,7 @@ from .mhsea_tuned import (
     mhsea_tuned_jvp,
     mhsea_with_tuned_ad,
 )
+from .paged import paged_append, paged_attention, paged_evict
 from .rect_attention import (
     BlockSizes,
     gated_rectangular_edge_attention,
@@ -37,7 +40,7 @@ from .rect_attention import (
     pallas_rectangular_edge_attention,
     sequence_attention_output,
 )
-from .tokens import bucket_bias, qk_norm_rotary, relative_buckets, token_attention
+from .tokens import bucket_bias, qk_norm_rotary, qk_rotary, relative_buckets, token_attention
 
 __all__ = [
     "BlockSizes",
@@ -52,8 +55,12 @@ __all__ = [
     "mhsea_tuned_jvp",
     "mhsea_with_tuned_ad",
     "noncausal_bias_mha",
+    "paged_append",
+    "paged_attention",
+    "paged_evict",
     "pallas_rectangular_edge_attention",
     "qk_norm_rotary",
+    "qk_rotary",
     "reference_edge_attention",
     "relative_buckets",
     "sequence_attention_output",

@@ -1,5 +1,5 @@
 """ctypes binding of ``libhz_mhsea.so`` (the C ABI declared in ``include/hz_mhsea.h``,
-``include/hz_executor.h``, ``include/hz_pair_bias.h`` and ``include/hz_token.h``).
+``include/hz_executor.h``, ``include/hz_pair_bias.h``, ``include/hz_token.h`` and ``include/hz_paged.h``).
 
 The library is the only compute path of this package: there is no CPU fallback. A
 missing library raises :class:`NativeLibraryMissing` on first use.
@@ -60,6 +60,14 @@ EXPORTED_SYMBOLS = (
     "hz_bucket_bias_fwd",
     "hz_bucket_bias_workspace",
     "hz_bucket_bias_bwd",
+    "hz_qk_rotary_fwd",
+    "hz_qk_rotary_workspace",
+    "hz_qk_rotary_bwd",
+    "hz_paged_append",
+    "hz_paged_attention_workspace",
+    "hz_paged_attention",
+    "hz_paged_evict_workspace",
+    "hz_paged_evict",
 )
 
 
@@ -75,12 +83,20 @@ class HzError(RuntimeError):
         self.code = code
 
 
-# The structures of hz_token.h as the bytes that the calls take (native alignment).
+# The structures of hz_token.h and hz_paged.h as the bytes that the calls take (native alignment).
 TOKEN_TENSOR = struct.Struct("@Pqqq")  # data, strides of batch, token, head
 # q, k, q_out, k_out, w_q, w_k, freqs, positions, B, N, H, Hk, D, n_freqs, eps, interleaved, dtype
 QK_NORM_ROTARY = struct.Struct("@" + 4 * "Pqqq" + "4P6qf2i4x")
 # q, k, v, out, out_low, lse, slopes, prefix, documents, kv_len, B, Nq, Nk, H, Hk, D, scale, softcap, causal, dtype
 TOKEN_ATTENTION = struct.Struct("@" + 3 * "Pqqq" + "7P6q2f2i")
+# an hz_qk_norm_rotary's fields, axes, n_axes, norm
+QK_ROTARY = struct.Struct("@" + 4 * "Pqqq" + "4P6qf2i4x" + "Pqi4x")
+# k, v, page_table, lengths, B, pages, page_size, table_width, Hk, D, dtype
+PAGED_CACHE = struct.Struct("@" + 2 * "Pqqq" + "2P6qi4x")
+# behind a cache's fields: q, out, slopes, scores, scores_out, Nq, H, scale, softcap, decay
+PAGED_ATTENTION_REST = struct.Struct("@" + "Pqqq" + "4P2q3f4x")
+# behind a cache's fields: scores, scores_out, sources, lengths_out, budget, sinks, recent
+PAGED_EVICT_REST = struct.Struct("@4P3q")
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -89,7 +105,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _F = ctypes.c_float
-_S = ctypes.c_char_p  # a structure of hz_token.h as bytes
+_S = ctypes.c_char_p  # a structure of hz_token.h or hz_paged.h as bytes
 
 _SIGNATURES = {
     "hz_version": ([], _INT),
@@ -164,6 +180,20 @@ _SIGNATURES = {
     # stream, de, buckets, q_positions, k_positions, dtable, workspace, workspace_bytes, B, Nq, Nk, H,
     # n_buckets, R, dtype, flags
     "hz_bucket_bias_bwd": ([_P] * 7 + [_I64] * 7 + [_INT, _INT], _INT),
+    # stream, p
+    "hz_qk_rotary_fwd": ([_P, _S], _INT),
+    # B, N, D, norm
+    "hz_qk_rotary_workspace": ([_I64] * 3 + [_INT], _I64),
+    # stream, p, dq, dk, dw_q, dw_k, workspace, workspace_bytes
+    "hz_qk_rotary_bwd": ([_P, _S] + [_P] * 5 + [_I64], _INT),
+    # stream, cache, k, v, N
+    "hz_paged_append": ([_P, _S, _S, _S, _I64], _INT),
+    # p
+    "hz_paged_attention_workspace": ([_S], _I64),
+    # stream, p, workspace, workspace_bytes
+    "hz_paged_attention": ([_P, _S, _P, _I64], _INT),
+    "hz_paged_evict_workspace": ([_S], _I64),
+    "hz_paged_evict": ([_P, _S, _P, _I64], _INT),
 }
 
 

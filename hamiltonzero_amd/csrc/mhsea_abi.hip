@@ -10,6 +10,7 @@
 #include "../../include/hz_pair_bias.h"
 #include "../../include/hz_mhsea.h"
 #include "mhsea_launch.h"
+#include "paged_launch.h"
 #include "token_launch.h"
 
 namespace {
@@ -248,7 +249,8 @@ int check_workspace(const void* workspace, int64_t bytes, int64_t need) {
 
 constexpr int64_t kTokenAxis = int64_t(1) << 30;
 
-int check_norm_rotary(const hz_qk_norm_rotary* p) {
+// inputs: whether q and k are read (the reverse mode of a rotation alone does not).
+int check_norm_rotary(const hz_qk_norm_rotary* p, bool inputs = true) {
   if (p == nullptr) return fail(HZ_ENULL, "p must not be NULL");
   if (int rc = check_dtype(p->dtype)) return rc;
   if (p->B < 1 || p->N < 1 || p->H < 1 || p->Hk < 1)
@@ -266,8 +268,10 @@ int check_norm_rotary(const hz_qk_norm_rotary* p) {
   if (int rc = check_elements("w_k", p->w_k, 4)) return rc;
   if (int rc = check_elements("freqs", p->freqs, 8)) return rc;
   if (int rc = check_elements("positions", p->positions, 4)) return rc;
-  if (int rc = check_strided("q", p->q)) return rc;
-  if (int rc = check_strided("k", p->k)) return rc;
+  if (inputs) {
+    if (int rc = check_strided("q", p->q)) return rc;
+    if (int rc = check_strided("k", p->k)) return rc;
+  }
   if (int rc = check_strided("q_out", p->q_out)) return rc;
   return check_strided("k_out", p->k_out);
 }
@@ -294,14 +298,19 @@ int check_token_dims(const hz_token_attention* p) {
   return HZ_OK;
 }
 
+int check_score_options(float scale, float softcap, int dtype) {
+  if (!(std::fabs(scale) <= 0x1p100f)) return fail(HZ_EINVAL, "scale must be finite and at most 2^100");
+  if (!(softcap >= 0.f) || !std::isfinite(softcap)) return fail(HZ_EINVAL, "softcap must be finite and >= 0");
+  // an error of 1e-7 in tanh is 1e-3 in the score at the first, a quarter of bfloat16's step at 1
+  const float cap = dtype == HZ_DTYPE_BF16 ? 8192.f : 0x1p100f;
+  if (softcap > cap || (softcap > 0.f && !(std::fabs(scale) / softcap <= 0x1p100f)))
+    return fail(HZ_EINVAL, "softcap must be at most %g here, and scale / softcap at most 2^100", cap);
+  return HZ_OK;
+}
+
 int check_token_attention(const hz_token_attention* p) {
   if (int rc = check_token_dims(p)) return rc;
-  if (!(std::fabs(p->scale) <= 0x1p100f)) return fail(HZ_EINVAL, "scale must be finite and at most 2^100");
-  if (!(p->softcap >= 0.f) || !std::isfinite(p->softcap)) return fail(HZ_EINVAL, "softcap must be finite and >= 0");
-  // an error of 1e-7 in tanh is 1e-3 in the score at the first, a quarter of bfloat16's step at 1
-  const float cap = p->dtype == HZ_DTYPE_BF16 ? 8192.f : 0x1p100f;
-  if (p->softcap > cap || (p->softcap > 0.f && !(std::fabs(p->scale) / p->softcap <= 0x1p100f)))
-    return fail(HZ_EINVAL, "softcap must be at most %g here, and scale / softcap at most 2^100", cap);
+  if (int rc = check_score_options(p->scale, p->softcap, p->dtype)) return rc;
   if (p->causal != 0 && p->causal != 1) return fail(HZ_EINVAL, "causal must be 0 or 1, got %d", p->causal);
   if (p->prefix != nullptr && !p->causal) return fail(HZ_EINVAL, "prefix needs causal");
   if (int rc = check_strided("q", p->q)) return rc;
@@ -315,6 +324,82 @@ int check_token_attention(const hz_token_attention* p) {
   if (p->out == nullptr) return fail(HZ_ENULL, "out must not be NULL");
   if (!aligned16(p->out)) return fail(HZ_EALIGN, "out must be 16-byte aligned");
   if (!aligned16(p->out_low)) return fail(HZ_EALIGN, "out_low must be 16-byte aligned");
+  return HZ_OK;
+}
+
+// The paged operators (hz_paged.h).
+int check_qk_rotary(const hz_qk_rotary* p, bool inputs) {
+  if (p == nullptr) return fail(HZ_ENULL, "p must not be NULL");
+  if (p->norm != 0 && p->norm != 1) return fail(HZ_EINVAL, "norm must be 0 or 1, got %d", p->norm);
+  if (p->n_axes < 1 || p->n_axes > HZ_ROTARY_MAX_AXES)
+    return fail(HZ_EINVAL, "n_axes must be in [1, %d], got %lld", HZ_ROTARY_MAX_AXES, (long long)p->n_axes);
+  if (p->n_axes > 1 && p->rotary.positions == nullptr) return fail(HZ_ENULL, "positions must not be NULL with several axes");
+  if (int rc = check_elements("axes", p->axes, 4)) return rc;
+  return check_norm_rotary(&p->rotary, inputs);
+}
+
+int check_paged_cache(const hz_paged_cache& c) {
+  if (int rc = check_dtype(c.dtype)) return rc;
+  if (c.B < 1 || c.pages < 1 || c.page_size < 1 || c.table_width < 1 || c.Hk < 1)
+    return fail(HZ_EINVAL, "B, pages, page_size, table_width and Hk must be >= 1, got %lld, %lld, %lld, %lld and %lld", (long long)c.B,
+                (long long)c.pages, (long long)c.page_size, (long long)c.table_width, (long long)c.Hk);
+  if (c.D < 8 || c.D > HZ_TOKEN_MAX_HEAD || c.D % 8 != 0)
+    return fail(HZ_EINVAL, "head dimension must be a multiple of 8 in [8, %d], got %lld", HZ_TOKEN_MAX_HEAD, (long long)c.D);
+  if (c.pages >= kTokenAxis || c.page_size >= kTokenAxis || c.table_width > (kTokenAxis - 1) / c.page_size)
+    return fail(HZ_EINVAL, "pages and table_width * page_size must be below 2^30");
+  const int64_t most = int64_t(1) << 23;  // workgroups of a launch, with room for their thread counts
+  if (c.B > most || c.Hk > most || c.B * c.Hk > most) return fail(HZ_EINVAL, "B * Hk exceeds the grid limit of %lld", (long long)most);
+  return HZ_OK;
+}
+
+int check_paged_tables(const hz_paged_cache& c) {
+  if (int rc = check_strided("k_cache", c.k)) return rc;
+  if (int rc = check_strided("v_cache", c.v)) return rc;
+  if (c.page_table == nullptr) return fail(HZ_ENULL, "page_table must not be NULL");
+  if (c.lengths == nullptr) return fail(HZ_ENULL, "lengths must not be NULL");
+  if (int rc = check_elements("page_table", c.page_table, 4)) return rc;
+  return check_elements("lengths", c.lengths, 4);
+}
+
+int check_paged_attention_dims(const hz_paged_attention_args* p) {
+  if (p == nullptr) return fail(HZ_ENULL, "p must not be NULL");
+  const hz_paged_cache& c = p->cache;
+  if (int rc = check_paged_cache(c)) return rc;
+  if (p->Nq < 1 || p->H < 1) return fail(HZ_EINVAL, "Nq and H must be >= 1, got %lld and %lld", (long long)p->Nq, (long long)p->H);
+  if (p->H % c.Hk != 0) return fail(HZ_EINVAL, "H must be a multiple of Hk, got %lld and %lld", (long long)p->H, (long long)c.Hk);
+  const int64_t most = int64_t(1) << 23;
+  if (p->H > most || p->Nq > most || p->H * p->Nq > most || c.B * p->H * p->Nq > most)
+    return fail(HZ_EINVAL, "B * Nq * H exceeds the grid limit of %lld", (long long)most);
+  if (p->scores_out != nullptr && c.B * c.Hk * ((c.page_size * c.table_width + 1023) / 1024) > most)
+    return fail(HZ_EINVAL, "scores of B * Hk * table_width * page_size slots exceed the supported size");
+  return HZ_OK;
+}
+
+int check_paged_attention(const hz_paged_attention_args* p) {
+  if (int rc = check_paged_attention_dims(p)) return rc;
+  if (int rc = check_paged_tables(p->cache)) return rc;
+  if (int rc = check_score_options(p->scale, p->softcap, p->cache.dtype)) return rc;
+  if (!std::isfinite(p->decay)) return fail(HZ_EINVAL, "decay must be finite");
+  if (int rc = check_strided("q", p->q)) return rc;
+  if (int rc = check_elements("slopes", p->slopes, 4)) return rc;
+  HZ_REQUIRE(p->out);
+  HZ_OPTIONAL(p->scores);
+  HZ_OPTIONAL(p->scores_out);
+  if (p->scores != nullptr && p->scores_out == nullptr) return fail(HZ_ENULL, "scores needs scores_out");
+  return HZ_OK;
+}
+
+int check_paged_evict_dims(const hz_paged_evict_args* p) {
+  if (p == nullptr) return fail(HZ_ENULL, "p must not be NULL");
+  const hz_paged_cache& c = p->cache;
+  if (int rc = check_paged_cache(c)) return rc;
+  if (p->budget < 1 || p->budget >= kTokenAxis) return fail(HZ_EINVAL, "budget must be in [1, 2^30), got %lld", (long long)p->budget);
+  if (p->sinks < 0 || p->recent < 0 || p->sinks > p->budget || p->recent > p->budget - p->sinks)
+    return fail(HZ_EINVAL, "sinks and recent must be >= 0 and at most the budget together, got %lld and %lld of %lld", (long long)p->sinks,
+                (long long)p->recent, (long long)p->budget);
+  const int64_t slots = c.page_size * c.table_width, moves = slots - p->budget < p->budget ? slots - p->budget : p->budget;
+  if (c.B * c.Hk > (int64_t(1) << 20) || (moves > 0 && c.B * c.Hk * ((moves + 63) / 64) > (int64_t(1) << 23)))
+    return fail(HZ_EINVAL, "B * Hk rows of this budget exceed the grid limit");
   return HZ_OK;
 }
 
@@ -965,6 +1050,71 @@ int hz_bucket_bias_bwd(hipStream_t stream, const void* de, const int32_t* bucket
   const hz::BucketParams p = bucket_params(buckets, q_positions, k_positions, B, Nq, Nk, H, n_buckets, R, dtype, flags);
   if (int rc = check_workspace(workspace, workspace_bytes, hz::bucket_bias_workspace(p))) return rc;
   return launched(hz::launch_bucket_bias_bwd(p, de, dtable, workspace, stream));
+}
+
+int hz_qk_rotary_fwd(hipStream_t stream, const hz_qk_rotary* p) {
+  if (int rc = check_qk_rotary(p, true)) return rc;
+  return launched(hz::launch_qk_rotary_fwd(*p, stream));
+}
+
+int64_t hz_qk_rotary_workspace(int64_t B, int64_t N, int64_t D, int32_t norm) {
+  if (B < 1 || N < 1 || D < 1 || B > kTokenAxis || N > kTokenAxis || D > HZ_ROTARY_MAX_HEAD || (norm != 0 && norm != 1)) return -1;
+  return hz::qk_rotary_workspace(B * N, D, norm != 0);
+}
+
+int hz_qk_rotary_bwd(hipStream_t stream, const hz_qk_rotary* p, void* dq, void* dk, float* dw_q, float* dw_k,
+                     void* workspace, int64_t workspace_bytes) {
+  if (int rc = check_qk_rotary(p, p != nullptr && p->norm != 0)) return rc;
+  HZ_REQUIRE(dq);
+  HZ_REQUIRE(dk);
+  if (!p->norm && (dw_q != nullptr || dw_k != nullptr)) return fail(HZ_EINVAL, "dw_q and dw_k need the norms");
+  if (int rc = check_elements("dw_q", dw_q, 4)) return rc;
+  if (int rc = check_elements("dw_k", dw_k, 4)) return rc;
+  const int64_t need = hz::qk_rotary_workspace(p->rotary.B * p->rotary.N, p->rotary.D, p->norm != 0);
+  if (int rc = check_workspace(workspace, workspace_bytes, need)) return rc;
+  return launched(hz::launch_qk_rotary_bwd(*p, dq, dk, dw_q, dw_k, workspace, stream));
+}
+
+int hz_paged_append(hipStream_t stream, const hz_paged_cache* cache, const hz_token_tensor* k, const hz_token_tensor* v,
+                    int64_t N) {
+  if (cache == nullptr || k == nullptr || v == nullptr) return fail(HZ_ENULL, "cache, k and v must not be NULL");
+  if (int rc = check_paged_cache(*cache)) return rc;
+  if (int rc = check_paged_tables(*cache)) return rc;
+  if (N < 1 || N >= kTokenAxis) return fail(HZ_EINVAL, "N must be in [1, 2^30), got %lld", (long long)N);
+  if (cache->B * cache->Hk > (int64_t(1) << 31) / N) return fail(HZ_EINVAL, "B * N * Hk exceeds the grid limit");
+  if (int rc = check_strided("k", *k)) return rc;
+  if (int rc = check_strided("v", *v)) return rc;
+  return launched(hz::launch_paged_append(*cache, *k, *v, N, stream));
+}
+
+int64_t hz_paged_attention_workspace(const hz_paged_attention_args* p) {
+  if (check_paged_attention_dims(p)) return -1;
+  return hz::paged_attention_workspace(*p);
+}
+
+int hz_paged_attention(hipStream_t stream, const hz_paged_attention_args* p, void* workspace, int64_t workspace_bytes) {
+  if (int rc = check_paged_attention(p)) return rc;
+  if (int rc = check_workspace(workspace, workspace_bytes, hz::paged_attention_workspace(*p))) return rc;
+  return launched(hz::launch_paged_attention(*p, workspace, stream));
+}
+
+int64_t hz_paged_evict_workspace(const hz_paged_evict_args* p) {
+  if (check_paged_evict_dims(p)) return -1;
+  return hz::paged_evict_workspace(*p);
+}
+
+int hz_paged_evict(hipStream_t stream, const hz_paged_evict_args* p, void* workspace, int64_t workspace_bytes) {
+  if (int rc = check_paged_evict_dims(p)) return rc;
+  if (int rc = check_paged_tables(p->cache)) return rc;
+  HZ_REQUIRE(p->scores);
+  HZ_REQUIRE(p->scores_out);
+  if (p->sources == nullptr || p->lengths_out == nullptr) return fail(HZ_ENULL, "sources and lengths_out must not be NULL");
+  if (int rc = check_elements("sources", p->sources, 4)) return rc;
+  if (int rc = check_elements("lengths_out", p->lengths_out, 4)) return rc;
+  if (p->scores == p->scores_out || p->lengths_out == p->cache.lengths)
+    return fail(HZ_EINVAL, "scores_out and lengths_out must not be the inputs");
+  if (int rc = check_workspace(workspace, workspace_bytes, hz::paged_evict_workspace(*p))) return rc;
+  return launched(hz::launch_paged_evict(*p, workspace, stream));
 }
 
 }  // extern "C"

@@ -13,6 +13,7 @@
 // heads of 64: 107 to 116 us, 151 in reverse mode, 4.8 TB/s); bfloat16: by vector instructions beside them, issued 98% of the time (4 x
 // 4096 tokens of 40 heads of 128: 90 us, 3.7 TB/s, and 119 us, 4.2 TB/s).
 #include "mhsea_device.h"
+#include "paged_launch.h"
 #include "token_launch.h"
 
 namespace hz {
@@ -26,9 +27,9 @@ struct NormParams {
   hz_token_tensor q, k, qo, ko;
   const float *wq, *wk;
   const double* freqs;
-  const int32_t* positions;
+  const int32_t *positions, *axes;  // positions of n_axes a token; axes null: the first
   int64_t tokens;
-  int N, H, HT, D, nf, interleaved, each;  // each: tokens a workgroup at a time
+  int N, H, HT, D, nf, n_axes, interleaved, each;  // each: tokens a workgroup at a time
   float eps;
 };
 
@@ -51,7 +52,9 @@ __device__ __forceinline__ void put_angles(const NormParams& p, int64_t token0, 
   for (int a = threadIdx.x; a < count * p.nf; a += kThreads) {
     const int x = a / p.nf, f = a - x * p.nf;
     const int64_t token = token0 + x;
-    const double pos = p.positions != nullptr ? p.positions[token] : static_cast<int>(token % p.N);
+    const int axis = p.axes != nullptr ? p.axes[f] : 0;
+    const bool known = axis >= 0 && axis < p.n_axes;  // a pair of no axis stays as it is
+    const double pos = !known ? 0 : p.positions != nullptr ? p.positions[token * p.n_axes + axis] : static_cast<int>(token % p.N);
     double turn = pos * p.freqs[f] * 0.15915494309189533577;  // radians to turns
     turn -= rint(turn);
     float s, c;
@@ -140,8 +143,8 @@ struct Item {
   }
 };
 
-template <class S, int GS, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p) {
+template <class S, int GS, bool INTERLEAVED, bool NORM>
+__global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p, float dir) {
   __shared__ Angles angles;
   constexpr int SLOTS = kThreads / GS;
   const int t = threadIdx.x % GS, slot = threadIdx.x / GS;
@@ -167,13 +170,15 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p)
       float x[8];
       next.get(x, lane.on);
       load(i + SLOTS);
-      float ss = 0.f;
+      if constexpr (NORM) {
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-      const float r = 1.f / sqrtf(head_sum<GS>(ss) / static_cast<float>(p.D) + p.eps);
+        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+        const float r = 1.f / sqrtf(head_sum<GS>(ss) / static_cast<float>(p.D) + p.eps);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= r * (it.is_q ? wq[e] : wk[e]);
-      if (lane.turns) turn8<INTERLEAVED>(x, &angles[it.token][4 * t], 1.f);
+        for (int e = 0; e < 8; ++e) x[e] *= r * (it.is_q ? wq[e] : wk[e]);
+      }
+      if (lane.turns) turn8<INTERLEAVED>(x, &angles[it.token][4 * t], dir);
       if (lane.on) store8<S>(const_cast<void*>(it.data(p.qo, p.ko)), it.offset(p.qo, p.ko), lane, x);
     }
     __syncthreads();
@@ -287,7 +292,7 @@ NormParams params(const hz_qk_norm_rotary& a) {
   p.wq = a.w_q, p.wk = a.w_k, p.freqs = a.freqs, p.positions = a.positions;
   p.tokens = a.B * a.N;
   p.N = static_cast<int>(a.N), p.H = static_cast<int>(a.H), p.HT = static_cast<int>(a.H + a.Hk);
-  p.D = static_cast<int>(a.D), p.nf = static_cast<int>(a.n_freqs), p.interleaved = a.interleaved;
+  p.D = static_cast<int>(a.D), p.nf = static_cast<int>(a.n_freqs), p.interleaved = a.interleaved, p.n_axes = 1;
   p.each = tokens_each(p.tokens, kMaxBlocks);
   p.eps = a.eps;
   return p;
@@ -308,6 +313,13 @@ void by_group(int64_t D, F f) {
   f(std::integral_constant<int, 32>{});
 }
 
+NormParams params(const hz_qk_rotary& a) {
+  NormParams p = params(a.rotary);
+  p.axes = a.axes, p.n_axes = static_cast<int>(a.n_axes);
+  if (!a.norm) p.wq = p.wk = nullptr;
+  return p;
+}
+
 template <class F>
 void by_variant(const hz_qk_norm_rotary& a, F f) {
   by_group(a.D, [&](auto gs) {
@@ -318,24 +330,18 @@ void by_variant(const hz_qk_norm_rotary& a, F f) {
   });
 }
 
-}  // namespace
-
-int64_t qk_norm_rotary_workspace(int64_t tokens, int64_t D) {
-  return (tokens < kMaxBlocks ? tokens : kMaxBlocks) * 2 * D * static_cast<int64_t>(sizeof(float));
-}
-
-hipError_t launch_qk_norm_rotary_fwd(const hz_qk_norm_rotary& a, hipStream_t stream) {
-  const NormParams p = params(a);
+// dir -1: the rotation back, what the reverse mode of a rotation without norms is.
+template <bool NORM>
+hipError_t run_fwd(const NormParams& p, const hz_qk_norm_rotary& a, float dir, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(blocks(p, 1 << 20)));
   by_variant(a, [&](auto type, auto gs, auto inter) {
-    norm_rotary_fwd_kernel<decltype(type), gs.value, inter.value><<<grid, kThreads, 0, stream>>>(p);
+    norm_rotary_fwd_kernel<decltype(type), gs.value, inter.value, NORM><<<grid, kThreads, 0, stream>>>(p, dir);
   });
   return hipGetLastError();
 }
 
-hipError_t launch_qk_norm_rotary_bwd(const hz_qk_norm_rotary& a, void* dq, void* dk, float* dw_q, float* dw_k,
-                                     void* workspace, hipStream_t stream) {
-  const NormParams p = params(a);
+hipError_t run_bwd(const NormParams& p, const hz_qk_norm_rotary& a, void* dq, void* dk, float* dw_q, float* dw_k,
+                   void* workspace, hipStream_t stream) {
   const int rows = static_cast<int>(blocks(p, kMaxBlocks));
   float* const partial = static_cast<float*>(workspace);
   by_variant(a, [&](auto type, auto gs, auto inter) {
@@ -344,6 +350,38 @@ hipError_t launch_qk_norm_rotary_bwd(const hz_qk_norm_rotary& a, void* dq, void*
   if (dw_q != nullptr || dw_k != nullptr)
     weight_sum_kernel<<<2 * p.D / 4, kThreads, 0, stream>>>(partial, rows, p.D, dw_q, dw_k);
   return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t qk_norm_rotary_workspace(int64_t tokens, int64_t D) {
+  return (tokens < kMaxBlocks ? tokens : kMaxBlocks) * 2 * D * static_cast<int64_t>(sizeof(float));
+}
+
+hipError_t launch_qk_norm_rotary_fwd(const hz_qk_norm_rotary& a, hipStream_t stream) {
+  return run_fwd<true>(params(a), a, 1.f, stream);
+}
+
+hipError_t launch_qk_norm_rotary_bwd(const hz_qk_norm_rotary& a, void* dq, void* dk, float* dw_q, float* dw_k,
+                                     void* workspace, hipStream_t stream) {
+  return run_bwd(params(a), a, dq, dk, dw_q, dw_k, workspace, stream);
+}
+
+int64_t qk_rotary_workspace(int64_t tokens, int64_t D, bool norm) { return norm ? qk_norm_rotary_workspace(tokens, D) : 0; }
+
+hipError_t launch_qk_rotary_fwd(const hz_qk_rotary& a, hipStream_t stream) {
+  const NormParams p = params(a);
+  return a.norm ? run_fwd<true>(p, a.rotary, 1.f, stream) : run_fwd<false>(p, a.rotary, 1.f, stream);
+}
+
+hipError_t launch_qk_rotary_bwd(const hz_qk_rotary& a, void* dq, void* dk, float* dw_q, float* dw_k, void* workspace,
+                                hipStream_t stream) {
+  NormParams p = params(a);
+  if (a.norm) return run_bwd(p, a.rotary, dq, dk, dw_q, dw_k, workspace, stream);
+  p.q = p.qo, p.k = p.ko;
+  p.qo = {dq, static_cast<int64_t>(p.N) * p.H * p.D, static_cast<int64_t>(p.H) * p.D, p.D};
+  p.ko = {dk, static_cast<int64_t>(p.N) * (p.HT - p.H) * p.D, static_cast<int64_t>(p.HT - p.H) * p.D, p.D};
+  return run_fwd<false>(p, a.rotary, -1.f, stream);
 }
 
 }  // namespace hz

@@ -2,15 +2,15 @@
 wavefunction over the same sites, or a model of token sequences, needs next to the MHSEA kernels.
 The reference has no counterpart.
 
-* :func:`qk_norm_rotary` — RMS norms of queries and keys for each head, and the rotation by position in
-  the same pass.
+* :func:`qk_norm_rotary` — RMS norms of queries and keys for each head, and the rotation by position (of one axis or
+  several) in the same pass; :func:`qk_rotary` — the rotation alone.
 * :func:`token_attention` — attention with shared key heads, tanh-capped scores, a distance bias and
   causal, prefix, document and length masks; single tokens over a cache.
 * :func:`bucket_bias` — a learned relative position bias by buckets, in the bias layouts of
   :mod:`hamiltonzero_amd.kernels` and of the rectangular attention; :func:`relative_buckets` makes
   its plan.
 
-All three are differentiable in reverse mode (once) through ``torch.autograd``, not in forward mode; a call that
+All are differentiable in reverse mode (once) through ``torch.autograd``, not in forward mode; a call that
 needs no gradient enqueues the forward alone. Tensors are float32 or bfloat16 GPU tensors on one device; work goes to
 the current stream of that device. There is no CPU fallback. Query, key and value tensors (and their
 cotangents) may be strided views whose last axis is contiguous (slices of one projection, a cache's
@@ -35,6 +35,7 @@ Tensor = torch.Tensor
 _DTYPES = {torch.float32: _native.HZ_DTYPE_F32, torch.bfloat16: _native.HZ_DTYPE_BF16}
 MAX_HEAD_DIM = 128
 MAX_ROTARY_HEAD_DIM = 256
+MAX_AXES = 16
 MAX_BUCKETS = 512
 MAX_BUCKET_RANGE = 4096
 
@@ -174,46 +175,120 @@ def _wants_grad(*tensors: Optional[Tensor]) -> bool:
 # --- norms and rotation ---------------------------------------------------------------------------
 
 
-def _norm_args(q, k, q_out, k_out, w_q, w_k, freqs, positions, interleaved, eps) -> bytes:
-    B, N, H, D = q.shape
-    return _native.QK_NORM_ROTARY.pack(
-        *_fields(q), *_fields(k), *_fields(q_out), *_fields(k_out), _ptr(w_q), _ptr(w_k), _ptr(freqs), _ptr(positions),
-        B, N, H, k.shape[2], D, 0 if freqs is None else freqs.shape[0], eps, interleaved, _DTYPES[q.dtype])
+def _rotary_args(q, k, q_out, k_out, w_q, w_k, rot, eps) -> bytes:
+    """An ``hz_qk_norm_rotary``'s fields, those of an ``hz_qk_rotary`` where there are axes or no norms. ``q`` and ``k`` may be None in the
+    reverse mode of a rotation alone; the shapes are then the cotangents'."""
+    freqs, positions, axes, n_axes, interleaved, norm = rot
+    B, N, H, D = q_out.shape
+    none = (0, 0, 0, 0)
+    one = _native.QK_NORM_ROTARY if norm and n_axes is None else _native.QK_ROTARY
+    args = (*(none if q is None else _fields(q)), *(none if k is None else _fields(k)), *_fields(q_out), *_fields(k_out), _ptr(w_q),
+            _ptr(w_k), _ptr(freqs), _ptr(positions), B, N, H, k_out.shape[2], D, 0 if freqs is None else freqs.shape[0], eps,
+            interleaved, _DTYPES[q_out.dtype])
+    return one.pack(*args) if one is _native.QK_NORM_ROTARY else one.pack(*args, _ptr(axes), n_axes or 1, norm)
 
 
-def _norm_fwd(q, k, w_q, w_k, freqs, positions, interleaved, eps, out=None):
+def _rotary_fwd(q, k, w_q, w_k, rot, eps, out=None):
     q, k = _strided(q), _strided(k)
     q_out, k_out = out or (_like(q), _like(k))
-    args = _norm_args(q, k, q_out, k_out, w_q, w_k, freqs, positions, interleaved, eps)
+    args = _rotary_args(q, k, q_out, k_out, w_q, w_k, rot, eps)
+    lib = _native.lib()
+    call = lib.hz_qk_norm_rotary_fwd if len(args) == _native.QK_NORM_ROTARY.size else lib.hz_qk_rotary_fwd
     with _on(q.device):
-        _native.check(_native.lib().hz_qk_norm_rotary_fwd(_stream(q.device), args))
+        _native.check(call(_stream(q.device), args))
     return q_out, k_out
 
 
 class _QKNormRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, w_q, w_k, freqs, positions, interleaved, eps):
-        ctx.save_for_backward(q, k, w_q, w_k, freqs, positions)
-        ctx.options = (interleaved, eps)
-        return _norm_fwd(q, k, w_q, w_k, freqs, positions, interleaved, eps)
+    def forward(ctx, q, k, w_q, w_k, freqs, positions, axes, options):
+        n_axes, interleaved, eps = options
+        ctx.save_for_backward(q, k, w_q, w_k, freqs, positions, axes)
+        ctx.options = options
+        return _rotary_fwd(q, k, w_q, w_k, (freqs, positions, axes, n_axes, interleaved, True), eps)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        q, k, w_q, w_k, freqs, positions = ctx.saved_tensors
+        q, k, w_q, w_k, freqs, positions, axes = ctx.saved_tensors
+        n_axes, interleaved, eps = ctx.options
         q, k, gq, gk = _strided(q), _strided(k), _strided(gq), _strided(gk)
         dev, D = q.device, q.shape[-1]
         dq, dk = _like(q), _like(k)
         dw_q = torch.empty(D, dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
         dw_k = torch.empty(D, dtype=torch.float32, device=dev) if ctx.needs_input_grad[3] else None
-        args = _norm_args(q, k, gq, gk, w_q, w_k, freqs, positions, *ctx.options)
+        args = _rotary_args(q, k, gq, gk, w_q, w_k, (freqs, positions, axes, n_axes, interleaved, True), eps)
         lib = _native.lib()
+        call = lib.hz_qk_norm_rotary_bwd if len(args) == _native.QK_NORM_ROTARY.size else lib.hz_qk_rotary_bwd
         size = lib.hz_qk_norm_rotary_workspace(q.shape[0], q.shape[1], D)
         work = torch.empty(size, dtype=torch.uint8, device=dev)
         with _on(dev):
-            _native.check(lib.hz_qk_norm_rotary_bwd(_stream(dev), args, _ptr(dq), _ptr(dk), _ptr(dw_q), _ptr(dw_k),
-                                                    _ptr(work), size))
+            _native.check(call(_stream(dev), args, _ptr(dq), _ptr(dk), _ptr(dw_q), _ptr(dw_k), _ptr(work), size))
         return dq, dk, dw_q, dw_k, None, None, None, None
+
+
+class _QKRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, freqs, positions, axes, options):
+        n_axes, interleaved = options
+        ctx.save_for_backward(freqs, positions, axes)
+        ctx.options = options
+        return _rotary_fwd(q, k, None, None, (freqs, positions, axes, n_axes, interleaved, False), 0.0)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        n_axes, interleaved = ctx.options
+        gq, gk = _strided(gq), _strided(gk)
+        dev = gq.device
+        dq, dk = _like(gq), _like(gk)
+        args = _rotary_args(None, None, gq, gk, None, None, (*ctx.saved_tensors, n_axes, interleaved, False), 0.0)
+        with _on(dev):
+            _native.check(_native.lib().hz_qk_rotary_bwd(_stream(dev), args, _ptr(dq), _ptr(dk), 0, 0, 0, 0))
+        return dq, dk, None, None, None, None
+
+
+def _check_rotary(q, k, freqs, positions, axes):
+    """Checks the operands that both rotations have; ``freqs, positions, axes, n_axes`` as the kernels take them (``n_axes`` None: positions
+    of one axis)."""
+    _check_first("q", q, "[B, N, H, D]")
+    _check_first("k", k, "[B, N, Hk, D]")
+    B, N, H, D = q.shape
+    dev = q.device
+    _check("k", k, dev, q.dtype, (B, N, k.shape[2], D))
+    if D % 8 or D > MAX_ROTARY_HEAD_DIM:
+        raise ValueError(f"head dimension must be a multiple of 8 up to {MAX_ROTARY_HEAD_DIM}, got {D}")
+    if freqs is not None:
+        if freqs.dim() != 1 or freqs.shape[0] % 4 or not 0 < 2 * freqs.shape[0] <= D:
+            raise ValueError(f"freqs must hold a multiple of 4 frequencies, at most D / 2 = {D // 2}, got {tuple(freqs.shape)}")
+        _check("freqs", freqs, dev, torch.float64, (freqs.shape[0],))
+        if freqs.requires_grad and torch.is_grad_enabled():
+            raise ValueError("freqs has no gradient here: detach it")
+        freqs = freqs.contiguous()
+    n_axes = None
+    if axes is not None:
+        if freqs is None or positions is None:
+            raise ValueError("axes needs freqs and positions")
+        if not isinstance(positions, Tensor) or positions.dim() != 3 or not 1 <= positions.shape[2] <= MAX_AXES:
+            raise ValueError(f"positions must be [B, N, n_axes] with 1 to {MAX_AXES} axes where axes is given")
+        n_axes = positions.shape[2]
+        _check("axes", axes, dev, torch.int32, (freqs.shape[0],))
+        axes = axes.contiguous()
+    if positions is not None:
+        _check("positions", positions, dev, torch.int32, (B, N) if n_axes is None else (B, N, n_axes))
+        positions = positions.contiguous()
+    return freqs, positions, axes, n_axes
+
+
+def _check_rotary_out(out, q, k):
+    for name, t, like in (("out[0]", out[0], q), ("out[1]", out[1], k)):
+        _check(name, t, q.device, q.dtype, tuple(like.shape))
+        if _strided(t) is not t:
+            raise ValueError(f"{name} must have contiguous heads and 16-byte aligned rows, got strides {t.stride()}")
+        if _holds_twice(t):
+            raise ValueError(f"{name} must not hold one element at several places, got strides {t.stride()}")
+    if _meet(out, (q, k)):
+        raise ValueError("out must not overlap the inputs, nor one result the other")
 
 
 def qk_norm_rotary(
@@ -224,6 +299,7 @@ def qk_norm_rotary(
     *,
     freqs: Optional[Tensor] = None,
     positions: Optional[Tensor] = None,
+    axes: Optional[Tensor] = None,
     interleaved: bool = False,
     eps: float = 1e-6,
     out: Optional[Tuple[Tensor, Tensor]] = None,
@@ -237,46 +313,56 @@ def qk_norm_rotary(
     and ``2 p + 1`` with ``interleaved``. Angles are formed in float64 and reduced to a turn there, so that far positions are as exact as near ones.
     D is a multiple of 8 up to 256.
 
+    With ``axes`` (int32, as long as ``freqs``) positions have several axes, ``positions [B, N, n_axes]`` (row and column of a
+    lattice site, layer, time; up to 16), and pair p turns by ``positions[..., axes[p]] * freqs[p]``; a pair whose number is no axis
+    stays as it is.
+
     Returns the two results, new tensors or ``out``: strided views of the same shapes that do not overlap
     the inputs or each other (a cache's rows, say), for calls that need no gradient. What is written there counts as
     changed in place: the backward of an earlier call that saved it raises."""
-    _check_first("q", q, "[B, N, H, D]")
-    _check_first("k", k, "[B, N, Hk, D]")
-    B, N, H, D = q.shape
-    dev = q.device
-    _check("k", k, dev, q.dtype, (B, N, k.shape[2], D))
-    if D % 8 or D > MAX_ROTARY_HEAD_DIM:
-        raise ValueError(f"head dimension must be a multiple of 8 up to {MAX_ROTARY_HEAD_DIM}, got {D}")
+    freqs, positions, axes, n_axes = _check_rotary(q, k, freqs, positions, axes)
+    D, dev = q.shape[3], q.device
     for name, w in (("w_q", w_q), ("w_k", w_k)):
         if w is not None:
             _check(name, w, dev, torch.float32, (D,))
-    if freqs is not None:
-        if freqs.dim() != 1 or freqs.shape[0] % 4 or not 0 < 2 * freqs.shape[0] <= D:
-            raise ValueError(f"freqs must hold a multiple of 4 frequencies, at most D / 2 = {D // 2}, got {tuple(freqs.shape)}")
-        _check("freqs", freqs, dev, torch.float64, (freqs.shape[0],))
-        if freqs.requires_grad and torch.is_grad_enabled():
-            raise ValueError("freqs has no gradient here: detach it")
-        freqs = freqs.contiguous()
-    if positions is not None:
-        _check("positions", positions, dev, torch.int32, (B, N))
-        positions = positions.contiguous()
     cw_q, cw_k = (None if w is None else w.contiguous() for w in (w_q, w_k))
     if out is not None:
-        for name, t, like in (("out[0]", out[0], q), ("out[1]", out[1], k)):
-            _check(name, t, dev, q.dtype, tuple(like.shape))
-            if _strided(t) is not t:
-                raise ValueError(f"{name} must have contiguous heads and 16-byte aligned rows, got strides {t.stride()}")
-            if _holds_twice(t):
-                raise ValueError(f"{name} must not hold one element at several places, got strides {t.stride()}")
-        if _meet(out, (q, k)):
-            raise ValueError("out must not overlap the inputs, nor one result the other")
+        _check_rotary_out(out, q, k)
     if _wants_grad(q, k, w_q, w_k, freqs, *(out or ())):
         if out is not None:
             raise ValueError("out= holds results without gradients: call under torch.no_grad()")
-        return _QKNormRotary.apply(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), _float32(eps))
-    res = _norm_fwd(q, k, cw_q, cw_k, freqs, positions, bool(interleaved), _float32(eps), out)
+        return _QKNormRotary.apply(q, k, cw_q, cw_k, freqs, positions, axes, (n_axes, bool(interleaved), _float32(eps)))
+    res = _rotary_fwd(q, k, cw_q, cw_k, (freqs, positions, axes, n_axes, bool(interleaved), True), _float32(eps), out)
     if out is not None:
         increment_version(res)  # as after an in-place write: a graph that saved what is overwritten says so
+    return res
+
+
+def qk_rotary(
+    q: Tensor,
+    k: Tensor,
+    *,
+    freqs: Tensor,
+    positions: Optional[Tensor] = None,
+    axes: Optional[Tensor] = None,
+    interleaved: bool = False,
+    out: Optional[Tuple[Tensor, Tensor]] = None,
+) -> Tuple[Tensor, Tensor]:
+    """The rotation of :func:`qk_norm_rotary` without its norms: the first ``2 * len(freqs)`` elements of each head of ``q [B, N,
+    H, D]`` and ``k [B, N, Hk, D]`` by the angles ``positions * freqs``, or with ``axes`` by ``positions[..., axes[p]] *
+    freqs[p]``. Arguments, ``out`` and errors as there. (Its gradient is the rotation back: no input is kept for it.)"""
+    if not isinstance(freqs, Tensor):
+        raise TypeError(f"freqs must be a tensor, got {type(freqs).__name__}")
+    freqs, positions, axes, n_axes = _check_rotary(q, k, freqs, positions, axes)
+    if out is not None:
+        _check_rotary_out(out, q, k)
+    if _wants_grad(q, k, freqs, *(out or ())):
+        if out is not None:
+            raise ValueError("out= holds results without gradients: call under torch.no_grad()")
+        return _QKRotary.apply(q, k, freqs, positions, axes, (n_axes, bool(interleaved)))
+    res = _rotary_fwd(q, k, None, None, (freqs, positions, axes, n_axes, bool(interleaved), False), 0.0, out)
+    if out is not None:
+        increment_version(res)
     return res
 
 
@@ -516,4 +602,4 @@ def bucket_bias(
     return _bias_fwd(*args)
 
 
-__all__ = ["bucket_bias", "qk_norm_rotary", "relative_buckets", "token_attention"]
+__all__ = ["bucket_bias", "qk_norm_rotary", "qk_rotary", "relative_buckets", "token_attention"]
