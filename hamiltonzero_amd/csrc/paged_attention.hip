@@ -1,16 +1,17 @@
 // Attention of new tokens over paged caches (formulas: include/hz_paged.h; operand layouts: token_device.h).
 //
-// All rows of query and head that share a key head, up to 32 of them, are the columns of one wave's products, and a wave
-// owns a run of slots, so that a cache is read once. How long a run is, each wave works out from the rows' real lengths:
-// the sum of them over a number of runs that fills the card, so that one long row among
-// short ones is divided as finely as many of its length would be coarsely. A row that is one run gets its results at once; the
-// others' runs are joined by a second kernel.
+// All rows of query and head that share a key head, up to 32 of them, are the columns of one workgroup's products, and the
+// workgroup owns a run of slots, so that a cache is read once. How long a run is, it works out from the rows' real lengths:
+// the sum of them over a number of runs that fills the card, so that one long row among short ones is divided as
+// finely as many of its length would be coarsely. Its four waves take blocks of 32 slots in turn and
+// join their sums in LDS; a row that is one run gets its results there, the others' runs are joined by a second
+// kernel.
 //
-// 32 slots at a time on v_mfma_f32_16x16x32_bf16: keys go from memory into the products' registers, values through
+// A block is 32 slots on v_mfma_f32_16x16x32_bf16: keys go from memory into the products' registers, values through
 // LDS of the wave's own. Where the slots lie is looked up two blocks ahead, so that no load waits for the page table.
 //
 // Accumulated weights need every row's final maximum and sum: the scores are kept in memory (4 bytes for each row
-// and slot beside the 4 D or 8 D that are read) and a third kernel adds up exp2 of them.
+// and slot beside the 4 D or 8 D that are read) and the second kernel adds up exp2 of them.
 #include "paged_launch.h"
 #include "token_device.h"
 
@@ -29,59 +30,125 @@ struct PagedParams {
   const float *slopes, *scores;
   float* scores_out;
   float *partial, *stats, *kept, *lse;  // workspace: see layout()
-  int B, Nq, H, Hk, G, D, rows, blocks;  // rows: Nq G; blocks of 32 of them
+  int B, Nq, H, Hk, G, D, rows, blocks;  // rows: Nq G; blocks of 16 or 32 of them
   int64_t slots_kept;                    // of a row of kept scores: the slots, rounded up to 32
-  int64_t runs_wanted;                   // for one key head and block of rows, over all batch rows
+  int64_t runs_wanted, runs_fill;        // for one key head and block of rows, over all batch rows: at most, and to fill the card
+  const int* plan;                       // of more than 64 batch rows
+  int waves, step;                       // waves of a run; slots that they take at a time, of which runs are multiples
   float cap, to_tanh, to_score2, decay;
 };
 
-// How the rows are divided: runs of `chunk` slots; those of batch row b are the numbers first .. first + runs - 1.
+// How the rows are divided: runs of `chunk` slots, at least one a row (more steps than the quotient of all by those wanted, so that the
+// further runs are fewer than wanted; longer ones, up to kLong steps, while there are runs enough to fill the card). Run 0 of batch row b has number b; the further runs of all
+// rows follow in order. Up to 64 rows, every wave works it out for itself, a length a lane; more rows have it
+// worked out once by paged_plan_kernel (512 rows in every wave: 8 us more of a workgroup's time than a lookup).
+constexpr int kPlanRows = 64;
+struct Found {
+  int b, run;
+};
+__device__ __forceinline__ int further(int n, int chunk) { return n <= chunk ? 0 : (n - 1) / chunk; }
+__device__ __forceinline__ int steps_of(const PagedParams& p, int n) { return (n + p.step - 1) / p.step; }
+constexpr int kLong = 8;
+template <class T>
+__device__ __forceinline__ int chunk_of(const PagedParams& p, T steps) {
+  T each = steps / static_cast<T>(p.runs_wanted) + 1;
+  if (each < kLong) {
+    const T fill = steps / static_cast<T>(p.runs_fill) + 1;
+    each = fill > kLong ? kLong : fill > each ? fill : each;
+  }
+  const T most = steps_of(p, p.c.slots);
+  return static_cast<int>(each < most ? each : most) * p.step;
+}
+
+// x of this lane and all before it.
+__device__ __forceinline__ int scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from 1, 2, 4 and 8 lanes below in the row of sixteen
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the row's last lane to the next row, of rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
+  return x;
+}
+
 struct Plan {
-  int chunk;
-  __device__ __forceinline__ static int runs(int n, int chunk) { return n <= chunk ? 1 : (n + chunk - 1) / chunk; }
-  __device__ __forceinline__ Plan(const PagedParams& p, int lane) {
-    int64_t sum = 0;
-    for (int b = lane; b < p.B; b += 64) sum += p.c.length(b);
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x, 64);
-    const int64_t each = (sum + p.runs_wanted - 1) / p.runs_wanted;
-    chunk = static_cast<int>(each < 1 ? kBlock : (each + kBlock - 1) / kBlock * kBlock);
+  int chunk, all, mine, upto;  // all: number of further runs; this lane's row's, and those of the rows up to it (without a table)
+  const int* table;            // chunk, all, [B] the further runs before each row, then their Founds
+  __device__ __forceinline__ Plan(const PagedParams& p, int lane) : mine(0), upto(0), table(p.plan) {
+    if (table != nullptr) {
+      chunk = table[0];
+      all = table[1];
+      return;
+    }
+    const int n = lane < p.B ? p.c.length(lane) : 0;
+    // (the steps of 64 rows are below 2^31)
+    chunk = chunk_of(p, static_cast<uint32_t>(__builtin_amdgcn_readlane(scan(steps_of(p, n)), 63)));
+    mine = further(n, chunk);
+    upto = scan(mine);
+    all = __builtin_amdgcn_readlane(upto, 63);
   }
   // The batch row of run `at`, and its number there; false behind the last one.
-  __device__ __forceinline__ bool find(const PagedParams& p, int64_t at, int lane, int& b, int& run) const {
-    int64_t base = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-      const int mine = b0 + lane < p.B ? runs(p.c.length(b0 + lane), chunk) : 0;
-      int x = mine;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-      }
-      const uint64_t behind = __ballot(base + x > at);
-      if (behind != 0) {
-        const int l = __ffsll(static_cast<unsigned long long>(behind)) - 1;
-        b = b0 + l;
-        run = static_cast<int>(at - base) - (__builtin_amdgcn_readlane(x, l) - __builtin_amdgcn_readlane(mine, l));
-        return true;
-      }
-      base += __builtin_amdgcn_readlane(x, 63);
+  __device__ __forceinline__ bool find(const PagedParams& p, int at, Found& f) const {
+    if (at >= p.B + all) return false;
+    if (at < p.B) {
+      f = Found{at, 0};
+    } else if (table != nullptr) {
+      f = reinterpret_cast<const Found*>(table + 2 + (p.B + 1) / 2 * 2)[at - p.B];
+    } else {
+      const int l = __ffsll(static_cast<unsigned long long>(__ballot(upto > at - p.B))) - 1;
+      f = Found{l, 1 + at - p.B - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l))};
     }
-    return false;
+    return true;
   }
-  // The first run of batch row b.
-  __device__ __forceinline__ int64_t first(const PagedParams& p, int b, int lane) const {
-    int64_t sum = 0;
-    for (int x = lane; x < b; x += 64) sum += runs(p.c.length(x), chunk);
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x, 64);
-    return sum;
+  // The number of run 1 of batch row b.
+  __device__ __forceinline__ int second(const PagedParams& p, int b) const {
+    return p.B + (table != nullptr ? table[2 + b] : __builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(mine, b));
   }
 };
 
-// Where a run's results lie: of batch-wide run number `at`, key head hk and row r of its Nq G.
-__device__ __forceinline__ int64_t result_at(const PagedParams& p, int64_t at, int hk, int r) {
-  return (at * p.Hk + hk) * p.rows + r;
+// The table of more than 64 rows. One workgroup.
+__global__ void __launch_bounds__(1024) paged_plan_kernel(PagedParams p, int* table) {
+  __shared__ int64_t sums[16];
+  __shared__ int counts[16];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  int64_t steps = 0;
+  for (int b = tid; b < p.B; b += 1024) steps += steps_of(p, p.c.length(b));
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) steps += __shfl_xor(steps, d, 64);
+  if (lane == 0) sums[wave] = steps;
+  __syncthreads();
+  steps = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) steps += sums[w];
+  const int chunk = chunk_of(p, steps);
+  Found* const found = reinterpret_cast<Found*>(table + 2 + (p.B + 1) / 2 * 2);
+  int base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 1024) {
+    const int b = b0 + tid, more = b < p.B ? further(p.c.length(b), chunk) : 0;
+    int x = more;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(x, d, 64);
+      if (lane >= d) x += y;
+    }
+    if (lane == 63) counts[wave] = x;
+    __syncthreads();
+    int before = base + x - more;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) before += counts[w];
+      base += counts[w];
+    }
+    if (b < p.B) table[2 + b] = before;
+    for (int r = 0; r < more; ++r) found[before + r] = Found{b, 1 + r};
+    __syncthreads();
+  }
+  if (tid == 0) table[0] = chunk, table[1] = base;
+}
+
+// Where a run's results lie: of run number `at`, key head hk and row r of its Nq G.
+__device__ __forceinline__ int64_t result_at(const PagedParams& p, int at, int hk, int r) {
+  return (static_cast<int64_t>(at) * p.Hk + hk) * p.rows + r;
 }
 
 __device__ __forceinline__ void wave_fence() {
@@ -90,25 +157,220 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int DP, int PARTS, bool CAP, int CB>
+// A block's values in LDS. bfloat16: a Tile, whose reads transpose. float32: the floats themselves, split into parts as they are read
+// (three bfloat16 planes would take half as much again, and a workgroup a CU less); chunk i of four of row r lies at chunk
+// i ^ (4 (r / 4 % 2)), so that the rows that a wave reads at once, four apart, lie in both halves of the banks.
+template <int DP, int PARTS>
+struct Values;
+template <int DP>
+struct Values<DP, 1> {
+  typedef uint16_t Element;
+  Element* base;
+  __device__ __forceinline__ void put(int row, int chunk, const Raw8<1>& r) const { Tile<kBlock, DP, 1>{base}.put(row, chunk, frag(r)); }
+  __device__ __forceinline__ Frag<1> columns(int dt, int lane) const { return Tile<kBlock, DP, 1>{base}.columns16(dt, lane); }
+};
+template <int DP>
+struct Values<DP, 3> {
+  typedef float Element;
+  Element* base;
+  __device__ __forceinline__ static int at(int row, int chunk) { return row * DP + ((chunk ^ ((row >> 2 & 1) << 2)) << 2); }
+  __device__ __forceinline__ void put(int row, int chunk, const Raw8<3>& r) const {
+    *reinterpret_cast<v4f*>(base + at(row, 2 * chunk)) = r.a;
+    *reinterpret_cast<v4f*>(base + at(row, 2 * chunk + 1)) = r.b;
+  }
+  // Lane 16 g + c gets column 16 dt + c of the rows 16 (j / 4) + 4 g + j % 4.
+  __device__ __forceinline__ Frag<3> columns(int dt, int lane) const {
+    const int g = lane >> 4, c = lane & 15;
+    const float* const from = base + at(4 * g, 4 * dt + (c >> 2)) + (c & 3);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = from[(16 * (j / 4) + j % 4) * DP];
+    const Split8 s = split8(x);
+    return Frag<3>{{s.h, s.m, s.l}};
+  }
+};
+
+// Where the 32 slots of a block lie, and the loads of their keys and values into a wave's registers: lane 16 g + c gets of the keys what
+// the products' operand wants (rows c and 16 + c, elements 32 s + 8 g .. + 7), and of the values rows lane / CH
+// + STEP j. Slots of no page, and behind the run's end, become zeros and are not read.
+//
+// Keys of bfloat16: a lane's operand is 16 bytes of each 64 of its row, and four lanes reading 64 bytes together make requests of half
+// a cache line. Eight lanes read 128 bytes of a row instead, of rows 0 .. 7 and then 8 .. 15, and lanes eight apart
+// exchange what belongs to the other (paged_token_long_bf16 260 -> 234 us).
+template <int DP, int PARTS>
+struct Lanes {
+  static constexpr int DS = DP / 32, CH = DP / 8, LOADS = kBlock * CH / 64, STEP = 64 / CH, BYTES = PARTS == 1 ? 2 : 4;
+  static constexpr bool TURNED = PARTS == 1 && DS >= 2;
+  __device__ __forceinline__ static int key_row(int lane, int s) { return TURNED ? (lane & 7) + 8 * (s & 1) : lane & 15; }
+  __device__ __forceinline__ static int key_element(int lane, int s) {
+    return TURNED ? 64 * (s / 2) + 8 * (lane >> 4) + (lane & 8 ? 32 : 0) : 32 * s + 8 * (lane >> 4);
+  }
+  __device__ __forceinline__ static void keys(const Raw8<PARTS> (&raw)[DS], Frag<PARTS> (&k)[DS], int lane) {
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) k[ds] = frag(raw[ds]);
+    if constexpr (TURNED) {
+      const bool low = (lane & 8) == 0;
+#pragma unroll
+      for (int ds = 0; ds < DS; ds += 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t a = k[ds].p[0][i], b = k[ds + 1].p[0][i];
+          const uint32_t other = __builtin_amdgcn_mov_dpp(low ? b : a, 0x128, 0xf, 0xf, true);  // of the lane eight on in the sixteen
+          k[ds].p[0][i] = low ? a : other;
+          k[ds + 1].p[0][i] = low ? other : b;
+        }
+    }
+  }
+};
+
+// Pages of a multiple of 16 slots: sixteen slots lie one behind the other. Each half of a block is a buffer whose end the
+// hardware checks: base and end are scalars, a lane's offset never changes, and no address is formed in vector registers.
+// ONCE: past the caches (a long bfloat16 cache 10% faster, paged_token_long_bf16 267 -> 241 us); not for pages that rows share (the same
+// with four fifths of its pages shared 155 us from the caches, 229 past them) and float32 (16 x 8192 slots of 8 heads of 128: 203 us, 214).
+enum Reads { kApart, kCached, kOnce };
+template <int DP, int PARTS, Reads READS>
+struct Slots : Lanes<DP, PARTS> {
+  typedef Lanes<DP, PARTS> L;
+  const PagedParams& p;
+  const int32_t* table;
+  const char *k, *v;  // of the key head
+  int stop, lane;
+  uint32_t at_k[L::DS], at_v[L::LOADS / 2];
+  int page_then[2];  // of the block two on
+  struct Half {
+    int page, in, count;  // count: its slots
+  };
+  Half next[2];
+
+  __device__ __forceinline__ Slots(const PagedParams& p_, const int32_t* table_, int hk, int stop_, int lane_, int64_t (*)[kBlock][2])
+      : p(p_), table(table_), k(static_cast<const char*>(p_.c.k) + hk * p_.c.head_k * L::BYTES),
+        v(static_cast<const char*>(p_.c.v) + hk * p_.c.head_v * L::BYTES), stop(stop_), lane(lane_) {
+    constexpr uint32_t kBehind = 0x7fffffffu;  // behind every buffer's end
+#pragma unroll
+    for (int s = 0; s < L::DS; ++s) {
+      const int d = L::key_element(lane, s);
+      at_k[s] = d < p.D ? (L::key_row(lane, s) * static_cast<uint32_t>(p.c.token_k) + d) * L::BYTES : kBehind;
+    }
+#pragma unroll
+    for (int j = 0; j < L::LOADS / 2; ++j) {
+      const int d = lane % L::CH * 8;
+      at_v[j] = d < p.D ? ((lane / L::CH + L::STEP * j) * static_cast<uint32_t>(p.c.token_v) + d) * L::BYTES : kBehind;
+    }
+  }
+  __device__ __forceinline__ void look(int k0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) page_then[i] = k0 + 16 * i < stop ? table[p.c.page_of(k0 + 16 * i)] : -1;
+  }
+  // Makes the block looked up the next one; its slots that lie in a page.
+  __device__ __forceinline__ uint32_t take(int k0, int) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int slot = k0 + 16 * i, page = __builtin_amdgcn_readfirstlane(page_then[i]);
+      next[i].page = page;
+      next[i].in = slot - p.c.page_of(slot) * p.c.size;
+      next[i].count = page >= 0 && page < p.c.pages ? min(16, stop - slot) : 0;
+    }
+    return ((1u << next[0].count) - 1) | ((1u << next[1].count) - 1) << 16;
+  }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const char* base, const Half& h, int64_t page, int64_t token) const {
+    const int64_t bytes = h.count > 0 ? ((h.count - 1) * token + p.D) * L::BYTES : 0;
+    const char* const from = h.count > 0 ? base + (h.page * page + h.in * token) * L::BYTES : base;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(from), 0, static_cast<int>(bytes), 0x00027000);
+  }
+  __device__ __forceinline__ static void one(Raw8<1>& r, __amdgpu_buffer_rsrc_t from, uint32_t at) {
+    r.u = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, READS == kOnce ? 2 : 0);
+  }
+  __device__ __forceinline__ static void one(Raw8<3>& r, __amdgpu_buffer_rsrc_t from, uint32_t at) {
+    r.a = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, READS == kOnce ? 2 : 0));
+    r.b = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, at + 16, 0, READS == kOnce ? 2 : 0));
+  }
+  __device__ __forceinline__ void load_k(Raw8<PARTS> (&rk)[2][L::DS], int) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __amdgpu_buffer_rsrc_t from = buffer(k, next[i], p.c.page_k, p.c.token_k);
+#pragma unroll
+      for (int s = 0; s < L::DS; ++s) one(rk[i][s], from, at_k[s]);
+    }
+  }
+  __device__ __forceinline__ void load_v(Raw8<PARTS> (&rv)[L::LOADS], int) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __amdgpu_buffer_rsrc_t from = buffer(v, next[i], p.c.page_v, p.c.token_v);
+#pragma unroll
+      for (int j = 0; j < L::LOADS / 2; ++j) one(rv[i * (L::LOADS / 2) + j], from, at_v[j]);
+    }
+  }
+};
+
+// Other pages: every slot is looked up by a lane of its own, and its offsets go to the others through LDS.
+template <int DP, int PARTS>
+struct Slots<DP, PARTS, kApart> : Lanes<DP, PARTS> {
+  typedef Lanes<DP, PARTS> L;
+  const PagedParams& p;
+  const int32_t* table;
+  int hk, stop, lane, page_then;
+  int64_t (*where)[kBlock][2];  // two blocks' offsets of keys and values; -1: no page
+
+  __device__ __forceinline__ Slots(const PagedParams& p_, const int32_t* table_, int hk_, int stop_, int lane_, int64_t (*where_)[kBlock][2])
+      : p(p_), table(table_), hk(hk_), stop(stop_), lane(lane_), where(where_) {}
+  __device__ __forceinline__ void look(int k0) {
+    const int slot = k0 + (lane & 31);
+    page_then = slot < stop ? table[p.c.page_of(slot)] : -1;
+  }
+  __device__ __forceinline__ uint32_t take(int k0, int buffer) {
+    const int slot = k0 + (lane & 31), in = slot - p.c.page_of(slot) * p.c.size;
+    const bool known = page_then >= 0 && page_then < p.c.pages;
+    if (lane < 32) {
+      where[buffer][lane][0] = known ? page_then * p.c.page_k + in * p.c.token_k : -1;
+      where[buffer][lane][1] = known ? page_then * p.c.page_v + in * p.c.token_v : -1;
+    }
+    wave_fence();
+    return static_cast<uint32_t>(__ballot(known));
+  }
+  __device__ __forceinline__ void load_k(Raw8<PARTS> (&rk)[2][L::DS], int buffer) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int s = 0; s < L::DS; ++s) {
+        const int64_t at = where[buffer][16 * i + L::key_row(lane, s)][0];
+        const int d = L::key_element(lane, s);
+        rk[i][s].load(p.c.k, at + hk * p.c.head_k + d, at >= 0 && d < p.D);
+      }
+  }
+  __device__ __forceinline__ void load_v(Raw8<PARTS> (&rv)[L::LOADS], int buffer) const {
+#pragma unroll
+    for (int j = 0; j < L::LOADS; ++j) {
+      const int64_t at = where[buffer][lane / L::CH + L::STEP * j][1];
+      const int d = lane % L::CH * 8;
+      rv[j].load(p.c.v, at + hk * p.c.head_v + d, at >= 0 && d < p.D);
+    }
+  }
+};
+
+template <int DP, int PARTS, bool CAP, int CB, Reads READS>
 __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_kernel(PagedParams p) {
-  constexpr int DS = DP / 32, DT = DP / 16, CH = DP / 8, LOADS = kBlock * CH / 64, STEP = 64 / CH;
-  typedef Tile<kBlock, DP, PARTS> V;
-  __shared__ __align__(16) uint16_t v_lds[4][V::kPlane * PARTS];
-  __shared__ __align__(16) int64_t where_lds[4][2][kBlock][2];  // offsets of a block's keys and values; -1: no page
+  typedef Slots<DP, PARTS, READS> S;
+  constexpr int DS = S::DS, DT = DP / 16, CH = S::CH, LOADS = S::LOADS, STEP = S::STEP;
+  typedef Values<DP, PARTS> V;
+  __shared__ __align__(16) typename V::Element v_lds[4][kBlock * DP];
+  __shared__ __align__(16) int64_t where_lds[READS == kApart ? 4 : 1][2][kBlock][2];
+  __shared__ float sums_lds[4][16 * CB][3];  // each wave's base, sum and sum of unrounded weights
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const V vt{v_lds[wave]};
-  int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  const int hk = static_cast<int>(id % p.Hk);
+  // waves 4: the workgroup's run; waves 1: one of each wave, which then share nothing
+  const bool together = p.waves == 4;
+  int id = together ? static_cast<int>(blockIdx.x) : 4 * static_cast<int>(blockIdx.x) + __builtin_amdgcn_readfirstlane(wave);
+  const int hk = id % p.Hk;
   id /= p.Hk;
-  const int r0 = static_cast<int>(id % p.blocks) * 32;
+  const int r0 = id % p.blocks * (16 * CB);
   id /= p.blocks;
   const Plan plan(p, lane);
-  int b, run_id;
-  if (!plan.find(p, id, lane, b, run_id)) return;  // waves share nothing: no barriers
-  const int n = p.c.length(b);
+  Found found;
+  if (!plan.find(p, id, found)) return;  // all waves of the run
+  const int b = found.b, n = p.c.length(b);
   const bool alone = n <= plan.chunk;
-  const int first = run_id * plan.chunk, stop = alone ? n : min(n, first + plan.chunk);
+  const int begin = found.run * plan.chunk, stop = alone ? n : min(n, begin + plan.chunk);
+  const int first = begin + (together ? kBlock * __builtin_amdgcn_readfirstlane(wave) : 0), step = p.step;
   const int32_t* const table = p.c.table + static_cast<int64_t>(b) * p.c.width;
 
   Frag<PARTS> q[CB][DS];
@@ -137,59 +399,30 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     for (int dt = 0; dt < DT; ++dt) o[cb][dt] = zero4();
   }
 
-  // slots k0 .. k0 + 31: lanes 0 .. 31 look up a slot each
-  auto page_at = [&](int k0) {
-    const int slot = k0 + (lane & 31);
-    return slot < stop ? table[p.c.page_of(slot)] : -1;
-  };
-  auto put_where = [&](int k0, int page) -> uint32_t {
-    const int slot = k0 + (lane & 31), in = slot - p.c.page_of(slot) * p.c.size;
-    const bool known = page >= 0 && page < p.c.pages;
-    if (lane < 32) {
-      where_lds[wave][(k0 >> 5) & 1][lane][0] = known ? page * p.c.page_k + in * p.c.token_k : -1;
-      where_lds[wave][(k0 >> 5) & 1][lane][1] = known ? page * p.c.page_v + in * p.c.token_v : -1;
-    }
-    return static_cast<uint32_t>(__ballot(known));
-  };
+  S slots(p, table, hk, stop, lane, where_lds[READS == kApart ? wave : 0]);
   const int lr = lane / CH, lc = lane % CH;
   Raw8<PARTS> rk[2][DS], rv[LOADS];
-  auto load_k = [&](int k0) {
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const int64_t at = where_lds[wave][(k0 >> 5) & 1][16 * kb + c][0];
-#pragma unroll
-      for (int s = 0; s < DS; ++s) {
-        const int d = 32 * s + 8 * g;
-        rk[kb][s].load(p.c.k, at + hk * p.c.head_k + d, at >= 0 && d < p.D);
-      }
-    }
-  };
-  auto load_v = [&](int k0) {
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int64_t at = where_lds[wave][(k0 >> 5) & 1][lr + STEP * j][1];
-      rv[j].load(p.c.v, at + hk * p.c.head_v + 8 * lc, at >= 0 && 8 * lc < p.D);
-    }
-  };
   uint32_t known = 0, known_next = 0;  // slots of the block at hand, and of the next, that lie in a page
+  int buffer = 0;
   if (first < stop) {
-    known = put_where(first, page_at(first));
-    known_next = put_where(first + 32, page_at(first + 32));
-    wave_fence();
-    load_v(first);
-    load_k(first);
+    slots.look(first);
+    known = slots.take(first, 0);
+    slots.look(first + step);
+    slots.load_v(rv, 0);
+    slots.load_k(rk, 0);
+    known_next = slots.take(first + step, 1);
   }
-  for (int k0 = first; k0 < stop; k0 += 32) {
-    const int page_next = page_at(k0 + 64);
+  for (int k0 = first; k0 < stop; k0 += step, buffer ^= 1) {
+    const bool more = k0 + step < stop;
+    slots.look(k0 + 2 * step);
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) vt.put(lr + STEP * j, lc, frag(rv[j]));
-    if (k0 + 32 < stop) load_v(k0 + 32);
+    for (int j = 0; j < LOADS; ++j) vt.put(lr + STEP * j, lc, rv[j]);
+    if (more) slots.load_v(rv, buffer ^ 1);
     v4f s[CB][2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       Frag<PARTS> k[DS];
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds) k[ds] = frag(rk[kb][ds]);
+      S::keys(rk[kb], k, lane);
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) {
         s[cb][kb] = zero4();
@@ -197,10 +430,10 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
         for (int ds = 0; ds < DS; ++ds) s[cb][kb] = mma16(k[ds], q[cb][ds], s[cb][kb]);
       }
     }
-    if (k0 + 32 < stop) load_k(k0 + 32);
+    if (more) slots.load_k(rk, buffer ^ 1);
     settle(s);
     wave_fence();
-    const uint32_t known_then = put_where(k0 + 64, page_next);  // this block's offsets have all been read
+    const uint32_t known_then = slots.take(k0 + 2 * step, buffer);  // what this block needed of it has been read
     Frag<PARTS> w[CB];
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
@@ -242,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const Frag<PARTS> v = vt.columns16(dt, lane);
+      const Frag<PARTS> v = vt.columns(dt, lane);
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) o[cb][dt] = mma16(v, w[cb], o[cb][dt]);
     }
@@ -251,95 +484,171 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     known_next = known_then;
   }
   settle(o);
+  // the run's sums, sixteen columns at a time, through the values' LDS: chunk ch of four elements of column x lies
+  // at chunk ch ^ (x & 7), so that the columns' writes go to different banks
+  const int ways = p.waves, w0 = together ? 0 : wave, threads = together ? kThreads : 64;
+  float* const mine = reinterpret_cast<float*>(v_lds[wave]);
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
     const float sum = group_sum(l[cb]), exact = group_sum(l_exact[cb]);
-    if (r0 + 16 * cb + c >= p.rows) continue;
-    if (alone) {
-      const int i = row[cb] / p.G, h = hk * p.G + row[cb] % p.G;
-      const int64_t at = (static_cast<int64_t>(b) * p.Nq + i) * p.H + h;
-      const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    if (g == 0) sums_lds[wave][16 * cb + c][0] = m[cb], sums_lds[wave][16 * cb + c][1] = sum, sums_lds[wave][16 * cb + c][2] = exact;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const int d = 16 * dt + 4 * g;
-        if (d < p.D) store_four<PARTS>(p.out, at * p.D + d, o[cb][dt][0] * inv, o[cb][dt][1] * inv, o[cb][dt][2] * inv, o[cb][dt][3] * inv);
+    for (int dt = 0; dt < DT; ++dt)
+      *reinterpret_cast<v4f*>(mine + c * DP + ((4 * dt + g) ^ (c & 7)) * 4) = o[cb][dt];
+    together ? __syncthreads() : wave_fence();
+    const int columns = min(16, p.rows - r0 - 16 * cb);
+    for (int x = together ? threadIdx.x : lane; x < columns * (DP / 4); x += threads) {
+      const int col = x / (DP / 4), ch = x % (DP / 4), r = r0 + 16 * cb + col, d = 4 * ch;
+      if (d >= p.D) continue;
+      float top = kNegInf, all = 0.f, all_exact = 0.f;
+      for (int w = w0; w < w0 + ways; ++w) top = fmaxf(top, sums_lds[w][16 * cb + col][0]);
+      const float base = top == kNegInf ? 0.f : top;
+      v4f y = zero4();
+      for (int w = w0; w < w0 + ways; ++w) {
+        const float a = fast_exp2(sums_lds[w][16 * cb + col][0] - base);
+        all += a * sums_lds[w][16 * cb + col][1];
+        all_exact += a * sums_lds[w][16 * cb + col][2];
+        y += a * *reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(v_lds[w]) + col * DP + (ch ^ (col & 7)) * 4);
       }
-      if (p.kept != nullptr && g == 0) p.lse[at] = exact > 0.f ? m[cb] + log2f(exact) : 0.f;
-      continue;
+      if (alone) {
+        const int64_t at = (static_cast<int64_t>(b) * p.Nq + r / p.G) * p.H + hk * p.G + r % p.G;
+        const float inv = all > 0.f || all != all ? 1.f / all : 0.f;
+        store_four<PARTS>(p.out, at * p.D + d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        if (p.kept != nullptr && ch == 0) p.lse[at] = all_exact > 0.f ? top + log2f(all_exact) : 0.f;
+      } else {
+        const int64_t to = result_at(p, id, hk, r);
+        *reinterpret_cast<v4f*>(p.partial + to * p.D + d) = y;
+        if (ch == 0) *reinterpret_cast<v4f*>(p.stats + to * 4) = v4f{top, all, all_exact, 0.f};
+      }
     }
-    const int64_t to = result_at(p, id, hk, row[cb]);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const int d = 16 * dt + 4 * g;
-      if (d < p.D) *reinterpret_cast<v4f*>(p.partial + to * p.D + d) = o[cb][dt];
-    }
-    if (g == 0) *reinterpret_cast<v4f*>(p.stats + to * 4) = v4f{m[cb], sum, exact, 0.f};
+    if (cb + 1 < CB) together ? __syncthreads() : wave_fence();
   }
 }
 
-// Joins the runs of rows that have several: eight half waves a row of (b, i, h), four elements a lane.
+// The run results of one row of (b, i, h).
+struct Runs {
+  int64_t first, others;  // where the first run's lie, and behind it those of run 1 on, `step` apart
+  int64_t step;
+  int count;
+  __device__ __forceinline__ Runs(const PagedParams& p, const Plan& plan, int b, int n, int hk, int r)
+      : first(result_at(p, b, hk, r)), others(result_at(p, plan.second(p, b) - 1, hk, r)), step(static_cast<int64_t>(p.Hk) * p.rows),
+        count(1 + further(n, plan.chunk)) {}
+  __device__ __forceinline__ int64_t at(int run) const { return run == 0 ? first : others + run * step; }
+};
+
+// Behind the attention, in one launch. Workgroups 0 .. joins - 1 join the runs of rows that have several: 4 * lanes elements of a row of
+// (b, i, h) at a time, 256 / lanes ways taking the runs in turn. lanes 8, four workgroups to a row of 128
+// elements, where there are few rows (122 runs of 96 rows 7 us, 12 with a workgroup a row); else 32 (12 runs of 512 rows 6 us,
+// 9 with four). The others add up the weights that each slot has had, 1024 slots of a row and key head a workgroup,
+// four a thread.
+constexpr int kRowTile = 64;
 template <int PARTS>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(PagedParams p) {
-  constexpr int WAYS = 8;
-  __shared__ __align__(16) float o_lds[WAYS][HZ_TOKEN_MAX_HEAD];
-  __shared__ float l_lds[WAYS][2];
-  const int lane = threadIdx.x & 31, way = threadIdx.x >> 5, d = 4 * lane;
-  const Plan plan(p, threadIdx.x & 63);
-  const int64_t at = blockIdx.x;
-  const int b = static_cast<int>(at / (static_cast<int64_t>(p.Nq) * p.H)), n = p.c.length(b);
-  if (n <= plan.chunk) return;
-  const int64_t first = plan.first(p, b, threadIdx.x & 63);
-  const int runs = Plan::runs(n, plan.chunk);
-  const int within = static_cast<int>(at - static_cast<int64_t>(b) * p.Nq * p.H), i = within / p.H, h = within % p.H, hk = h / p.G;
-  const int64_t from = result_at(p, first, hk, i * p.G + h % p.G), step = static_cast<int64_t>(p.Hk) * p.rows;
-  float m = kNegInf, l = 0.f, exact = 0.f;
-  v4f o = zero4();
+__global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, int joins, int lanes, int per_row) {
+  __shared__ __align__(16) float o_lds[4][32][4];
+  __shared__ float l_lds[4], lse_lds[kRowTile];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const Plan plan(p, lane);
+  if (static_cast<int>(blockIdx.x) < joins) {
+    if (plan.all == 0) return;
+    const int way = tid / lanes, ways = kThreads / lanes, dl = tid % lanes;
+    const int per = p.Nq * p.H, quarters = (p.D + 4 * lanes - 1) / (4 * lanes);
+    for (int64_t unit = blockIdx.x; unit < static_cast<int64_t>(p.B) * per * quarters; unit += joins) {
+      const int64_t at = unit / quarters;
+      const int d = (static_cast<int>(unit % quarters) * lanes + dl) * 4, b = static_cast<int>(at / per), n = p.c.length(b);
+      if (n <= plan.chunk) continue;  // all of the workgroup
+      const int within = static_cast<int>(at - static_cast<int64_t>(b) * per), i = within / p.H, h = within % p.H;
+      const Runs runs(p, plan, b, n, h / p.G, i * p.G + h % p.G);
+      float m = kNegInf, l = 0.f;
+      v4f o = zero4();
 #pragma unroll 4
-  for (int r = lane; r < runs; r += 32) m = fmaxf(m, p.stats[(from + r * step) * 4]);
+      for (int r = lane; r < runs.count; r += 64) m = fmaxf(m, p.stats[runs.at(r) * 4]);
 #pragma unroll
-  for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-  const float base = m == kNegInf ? 0.f : m;
+      for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+      const float base = m == kNegInf ? 0.f : m;
 #pragma unroll 4
-  for (int r = way; r < runs; r += WAYS) {
-    const v4f st = *reinterpret_cast<const v4f*>(p.stats + (from + r * step) * 4);
-    const float a = fast_exp2(st[0] - base);
-    l += a * st[1];
-    exact += a * st[2];
-    if (d < p.D) o += a * *reinterpret_cast<const v4f*>(p.partial + (from + r * step) * p.D + d);
-  }
-  *reinterpret_cast<v4f*>(&o_lds[way][d]) = o;
-  if (lane == 0) l_lds[way][0] = l, l_lds[way][1] = exact;
-  __syncthreads();
-  if (way != 0) return;
+      for (int r = way; r < runs.count; r += ways) {
+        const v4f st = *reinterpret_cast<const v4f*>(p.stats + runs.at(r) * 4);
+        const float a = fast_exp2(st[0] - base);
+        l += a * st[1];
+        if (d < p.D) o += a * *reinterpret_cast<const v4f*>(p.partial + runs.at(r) * p.D + d);
+      }
+      for (int x = lanes; x < 64; x <<= 1) {
+        l += __shfl_xor(l, x, 64);
 #pragma unroll
-  for (int x = 1; x < WAYS; ++x) {
-    l += l_lds[x][0];
-    exact += l_lds[x][1];
-    o += *reinterpret_cast<const v4f*>(&o_lds[x][d]);
+        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x, 64);
+      }
+      if (lane < lanes) *reinterpret_cast<v4f*>(o_lds[wave][dl]) = o;
+      if (lane == 0) l_lds[wave] = l;
+      __syncthreads();
+      if (tid < lanes) {
+        o = zero4(), l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          o += *reinterpret_cast<const v4f*>(o_lds[w][dl]);
+          l += l_lds[w];
+        }
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        if (d < p.D) store_four<PARTS>(p.out, at * p.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+      }
+      __syncthreads();
+    }
+    return;
   }
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  if (d < p.D) store_four<PARTS>(p.out, at * p.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-  if (p.kept != nullptr && lane == 0) p.lse[at] = exact > 0.f ? m + log2f(exact) : 0.f;
-}
-
-// The weights that each slot has had: 1024 slots of a row and key head a workgroup, four a thread.
-__global__ void __launch_bounds__(kThreads) paged_weights_kernel(PagedParams p, int per_row) {
-  const int64_t unit = blockIdx.x / per_row;
-  const int b = static_cast<int>(unit / p.Hk), hk = static_cast<int>(unit % p.Hk);
-  const int slot = (static_cast<int>(blockIdx.x) % per_row * kThreads + static_cast<int>(threadIdx.x)) * 4, n = p.c.length(b);
-  if (slot >= p.c.slots) return;
+  const int id = static_cast<int>(blockIdx.x) - joins, unit = id / per_row;
+  const int b = unit / p.Hk, hk = unit % p.Hk, n = p.c.length(b);
+  const int slot0 = id % per_row * (4 * kThreads), slot = slot0 + 4 * tid;
   v4f sum = zero4();
-  if (slot < n) {
-    const float* const kept = p.kept + unit * p.rows * p.slots_kept + slot;
+  const float* const kept = p.kept + static_cast<int64_t>(unit) * p.rows * p.slots_kept + slot;
+  for (int r0 = 0; r0 < p.rows && slot0 < n; r0 += kRowTile) {
+    const int rows = min(kRowTile, p.rows - r0);
+    if (r0 > 0) __syncthreads();
+    // each row's base and sum, together the base-2 logarithm of its sum: eight lanes a row
+    const int d8 = tid & 7;
+    for (int r = tid >> 3; r < rows; r += kThreads / 8) {
+      const int i = (r0 + r) / p.G, g = (r0 + r) % p.G;
+      float lse;
+      if (n <= plan.chunk) {
+        lse = p.lse[(static_cast<int64_t>(b) * p.Nq + i) * p.H + hk * p.G + g];
+      } else {
+        const Runs runs(p, plan, b, n, hk, r0 + r);
+        float m = kNegInf, exact = 0.f;
 #pragma unroll 4
-    for (int r = 0; r < p.rows; ++r) {
-      const float lse = p.lse[(static_cast<int64_t>(b) * p.Nq + r / p.G) * p.H + hk * p.G + r % p.G];
-      const v4f x = *reinterpret_cast<const v4f*>(kept + r * p.slots_kept);
+        for (int x = d8; x < runs.count; x += 8) m = fmaxf(m, p.stats[runs.at(x) * 4]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += fast_exp2(x[e] - lse);
+        for (int x = 1; x < 8; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+        const float base = m == kNegInf ? 0.f : m;
+#pragma unroll 4
+        for (int x = d8; x < runs.count; x += 8) {
+          const v4f st = *reinterpret_cast<const v4f*>(p.stats + runs.at(x) * 4);
+          exact += fast_exp2(st[0] - base) * st[2];
+        }
+#pragma unroll
+        for (int x = 1; x < 8; x <<= 1) exact += __shfl_xor(exact, x, 64);
+        lse = exact > 0.f ? m + log2f(exact) : 0.f;
+      }
+      if (d8 == 0) lse_lds[r] = lse;
+    }
+    __syncthreads();
+    if (slot < n) {
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r) {
+        const v4f x = *reinterpret_cast<const v4f*>(kept + (r0 + r) * p.slots_kept);
+        const float lse = lse_lds[r];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += fast_exp2(x[e] - lse);
+      }
     }
   }
-  const int64_t at = unit * p.c.slots + slot;
+  if (slot >= p.c.slots) return;
+  const int64_t at = static_cast<int64_t>(unit) * p.c.slots + slot;
+  if (slot + 4 <= p.c.slots && p.c.slots % 4 == 0) {
+    v4f x = zero4();
+    if (slot < n && p.scores != nullptr) x = p.decay * *reinterpret_cast<const v4f*>(p.scores + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = slot + e < n ? x[e] + sum[e] : 0.f;
+    *reinterpret_cast<v4f*>(p.scores_out + at) = x;
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (slot + e >= p.c.slots) break;
@@ -349,23 +658,34 @@ __global__ void __launch_bounds__(kThreads) paged_weights_kernel(PagedParams p, 
   }
 }
 
-// Waves that fill the card: a row of one key head is divided so that there are about as many.
-constexpr int64_t kWaves = 6144;
+// Workgroups that fill the card: the rows are divided so that there are about kFill, three for each place of most kernels (half as many
+// take 16% longer where rows are long, paged_token_long_bf16; twice as many 3%). While a workgroup's run is below kLong steps
+// they are as few as kLeast (16 x 8192 float32 slots of 8 heads of 128: 150 us, 178 by kFill alone).
+// Where there are rows of key heads for all its waves, kAlone, each wave has one to itself and shares nothing
+// (paged_walkers_f32 84 -> 67 us).
+constexpr int64_t kFill = 1536, kLeast = 512, kAlone = 2048;
 
 struct Layout {
-  int64_t rows, blocks, runs_wanted, runs, slots_kept, partial, stats, kept, lse, total;
+  int64_t rows, block, blocks, waves, step, runs_wanted, runs_fill, runs, slots_kept, partial, stats, kept, lse, plan, total;
 };
 
+// Rows of query and head in a workgroup's products: 16, or 32 where there are more; float32 heads of more than 64 elements have
+// no registers for 32, and read their keys and values again for every 16.
 // The workspace, in floats: partial outputs and statistics of every run, kept scores, a base and sum for each row.
 Layout layout(const hz_paged_attention_args& a) {
   const hz_paged_cache& c = a.cache;
   Layout w{};
   const int64_t slots = c.page_size * c.table_width;
   w.rows = a.Nq * (a.H / c.Hk);
-  w.blocks = (w.rows + 31) / 32;
-  const int64_t wanted = kWaves / (c.Hk * w.blocks), longest = (slots + kBlock - 1) / kBlock;
+  w.block = w.rows <= 16 || (c.dtype == HZ_DTYPE_F32 && c.D > 64) ? 16 : 32;
+  w.blocks = (w.rows + w.block - 1) / w.block;
+  w.waves = c.B * c.Hk * w.blocks >= kAlone ? 1 : 4;
+  w.step = w.waves * kBlock;
+  const int64_t wanted = (w.waves == 1 ? kAlone : kFill) / (c.Hk * w.blocks), longest = (slots + w.step - 1) / w.step;
   w.runs_wanted = wanted > 1 ? wanted : 1;
-  // runs are at least (all lengths) / wanted long, and at least one block: each row has one, and all together at most `wanted` more
+  const int64_t fill = (w.waves == 1 ? kAlone : kLeast) / (c.Hk * w.blocks);
+  w.runs_fill = fill > 1 ? fill : 1;
+  // runs are at least (all lengths) / wanted and step long: each row has one, and all together less than `wanted` more
   const int64_t most = c.B * longest;
   w.runs = w.runs_wanted + c.B < most ? w.runs_wanted + c.B : most;
   auto take = [&](int64_t floats) {
@@ -375,7 +695,8 @@ Layout layout(const hz_paged_attention_args& a) {
   };
   w.partial = take(w.runs * c.Hk * w.rows * c.D);
   w.stats = take(w.runs * c.Hk * w.rows * 4);
-  w.slots_kept = longest * kBlock;
+  w.plan = take(c.B > kPlanRows ? 2 + (c.B + 1) / 2 * 2 + 2 * (w.runs - c.B) : 0);
+  w.slots_kept = (slots + kBlock - 1) / kBlock * kBlock;
   if (a.scores_out != nullptr) {
     w.kept = take(c.B * c.Hk * w.rows * w.slots_kept);
     w.lse = take(c.B * a.Nq * a.H);
@@ -393,18 +714,31 @@ hipError_t run(const hz_paged_attention_args& a, void* workspace, hipStream_t st
   PagedParams p{Pages(c), a.q, a.out, a.slopes, a.scores, a.scores_out, ws + w.partial, ws + w.stats,
                 want ? ws + w.kept : nullptr, want ? ws + w.lse : nullptr, static_cast<int>(c.B), static_cast<int>(a.Nq),
                 static_cast<int>(a.H), static_cast<int>(c.Hk), static_cast<int>(a.H / c.Hk), static_cast<int>(c.D),
-                static_cast<int>(w.rows), static_cast<int>(w.blocks), w.slots_kept, w.runs_wanted, a.softcap,
+                static_cast<int>(w.rows), static_cast<int>(w.blocks), w.slots_kept, w.runs_wanted, w.runs_fill,
+                c.B > kPlanRows ? reinterpret_cast<int*>(ws + w.plan) : nullptr, static_cast<int>(w.waves), static_cast<int>(w.step), a.softcap,
                 capped ? a.scale / a.softcap : 0.f, (capped ? a.softcap : a.scale) * kLog2e, a.decay};
-  const unsigned grid = static_cast<unsigned>((w.runs * c.Hk * w.blocks + 3) / 4);
-  if (w.rows <= 16)
-    paged_attention_kernel<DP, PARTS, CAP, 1><<<grid, kThreads, 0, stream>>>(p);
-  else
-    paged_attention_kernel<DP, PARTS, CAP, 2><<<grid, kThreads, 0, stream>>>(p);
-  if (w.slots_kept > kBlock) paged_join_kernel<PARTS><<<static_cast<unsigned>(c.B * a.Nq * a.H), kThreads, 0, stream>>>(p);
-  if (want) {
-    const int per_row = static_cast<int>((p.c.slots + 4 * kThreads - 1) / (4 * kThreads));
-    paged_weights_kernel<<<static_cast<unsigned>(c.B * c.Hk * per_row), kThreads, 0, stream>>>(p, per_row);
-  }
+  const unsigned grid = static_cast<unsigned>((w.runs * c.Hk * w.blocks * w.waves + 3) / 4);
+  if (c.B > kPlanRows) paged_plan_kernel<<<1, 1024, 0, stream>>>(p, reinterpret_cast<int*>(ws + w.plan));
+  auto attend = [&](auto reads) {
+    if (w.block == 16)
+      paged_attention_kernel<DP, PARTS, CAP, 1, reads.value><<<grid, kThreads, 0, stream>>>(p);
+    else if constexpr (PARTS == 1 || DP < 128)
+      paged_attention_kernel<DP, PARTS, CAP, 2, reads.value><<<grid, kThreads, 0, stream>>>(p);
+  };
+  // sixteen slots as a buffer: one behind the other, apart, within 31 bits
+  const int64_t least = c.k.token < c.v.token ? c.k.token : c.v.token, most = c.k.token > c.v.token ? c.k.token : c.v.token;
+  if (c.page_size % 16 != 0 || least < c.D || most >= int64_t(1) << 24)
+    attend(std::integral_constant<Reads, kApart>{});
+  else if (PARTS == 3 || c.B * c.table_width > c.pages || w.blocks > 1)
+    attend(std::integral_constant<Reads, kCached>{});
+  else if constexpr (PARTS == 1)
+    attend(std::integral_constant<Reads, kOnce>{});
+  const int64_t outputs = w.runs > c.B ? c.B * a.Nq * a.H : 0;  // where a row may have several runs
+  const int lanes = outputs * ((c.D + 31) / 32) <= 1024 ? 8 : 32;
+  const int64_t units = lanes == 8 ? outputs * ((c.D + 31) / 32) : outputs;
+  const int joins = static_cast<int>(units < 2048 ? units : 2048), per_row = (p.c.slots + 4 * kThreads - 1) / (4 * kThreads);
+  const int64_t finish = joins + (want ? c.B * c.Hk * per_row : 0);
+  if (finish > 0) paged_finish_kernel<PARTS><<<static_cast<unsigned>(finish), kThreads, 0, stream>>>(p, joins, lanes, per_row);
   return hipGetLastError();
 }
 
