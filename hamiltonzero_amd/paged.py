@@ -27,41 +27,59 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _native
-from .tokens import MAX_HEAD_DIM, _DTYPES, _check, _check_first, _fields, _float32, _holds_twice, _on, _overlap, _ptr, _stream, _strided, _wants_grad
+from .tokens import MAX_HEAD_DIM, _DTYPES, _check, _check_first, _end, _fields, _float32, _holds_twice, _on, _overlap, _ptr, _stream, _strided, _wants_grad
 
 Tensor = torch.Tensor
+
+
+def _in_place(name: str, t: Tensor) -> tuple:
+    """Address and strides of a cache that the kernels read and write where it is."""
+    fields = _fields(t)
+    if not t.is_contiguous() and (t.stride(3) != 1 or fields[1] % 8 or fields[2] % 8 or fields[3] % 8) or fields[0] % 16:
+        raise ValueError(f"{name} must have contiguous heads and 16-byte aligned rows, got strides {t.stride()}")
+    return fields
 
 
 def _cache(k_cache: Tensor, v_cache: Tensor, page_table: Tensor, lengths: Tensor) -> Tuple[bytes, tuple]:
     """The library's structure of a checked cache, and ``(B, slots, Hk, D)``. The tables that it points to are the caller's: they
     stay as long as its arguments do."""
     _check_first("k_cache", k_cache, "[pages, page_size, Hk, D]")
-    P, S, Hk, D = k_cache.shape
-    dev = k_cache.device
+    shape = k_cache.shape
+    P, S, Hk, D = shape
+    dev, dtype = k_cache.device, k_cache.dtype
     if D % 8 or D > MAX_HEAD_DIM:
         raise ValueError(f"head dimension must be a multiple of 8 up to {MAX_HEAD_DIM}, got {D}")
-    _check("v_cache", v_cache, dev, k_cache.dtype, (P, S, Hk, D))
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.data_ptr() % 16 or t.stride(3) != 1 or any(s % 8 and n > 1 for s, n in zip(t.stride()[:3], t.shape)):
-            raise ValueError(f"{name} must have contiguous heads and 16-byte aligned rows, got strides {t.stride()}")
-    if not isinstance(page_table, Tensor) or page_table.dim() != 2 or 0 in page_table.shape:
+    _check("v_cache", v_cache, dev, dtype, shape)
+    if not isinstance(page_table, Tensor) or page_table.dim() != 2 or page_table.numel() == 0:
         raise ValueError("page_table must be [B, width] with both axes at least 1 long")
-    B, width = page_table.shape
-    _check("page_table", page_table, dev, torch.int32, (B, width))
+    table_shape = page_table.shape
+    B, width = table_shape
+    _check("page_table", page_table, dev, torch.int32, table_shape)
     _check("lengths", lengths, dev, torch.int32, (B,))
     if not page_table.is_contiguous() or not lengths.is_contiguous():
         raise ValueError("page_table and lengths must be contiguous")
-    args = _native.PAGED_CACHE.pack(*_fields(k_cache), *_fields(v_cache), page_table.data_ptr(), lengths.data_ptr(), B, P, S, width,
-                                    Hk, D, _DTYPES[k_cache.dtype])
+    args = _native.PAGED_CACHE.pack(*_in_place("k_cache", k_cache), *_in_place("v_cache", v_cache), page_table.data_ptr(),
+                                    lengths.data_ptr(), B, P, S, width, Hk, D, _DTYPES[dtype])
     return args, (B, width * S, Hk, D)
 
 
-def _written(k_cache: Tensor, v_cache: Tensor) -> None:
+def _range(t: Tensor) -> Tuple[int, int]:
+    begin = t.data_ptr()
+    return begin, begin + t.numel() * t.element_size() if t.is_contiguous() else _end(t)
+
+
+def _check_written(k_cache: Tensor, v_cache: Tensor, *others: Tensor) -> None:
+    """The caches of a call that writes them: no element at two places, apart from each other and from ``others``."""
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if _holds_twice(t):
             raise ValueError(f"{name} must not hold one element at several places, got strides {t.stride()}")
-    if _overlap(k_cache, v_cache):
+    (k0, k1), (v0, v1) = _range(k_cache), _range(v_cache)
+    if k0 < v1 and v0 < k1 and _overlap(k_cache, v_cache):
         raise ValueError("k_cache and v_cache must not overlap")
+    for t in others:
+        t0, t1 = _range(t)
+        if (t0 < k1 and k0 < t1 and _overlap(t, k_cache)) or (t0 < v1 and v0 < t1 and _overlap(t, v_cache)):
+            raise ValueError("k and v must not overlap the caches")
 
 
 def _no_grad(*tensors: Optional[Tensor]) -> None:
@@ -79,11 +97,9 @@ def paged_append(k_cache: Tensor, v_cache: Tensor, k: Tensor, v: Tensor, page_ta
     N = k.shape[1]
     for name, t in (("k", k), ("v", v)):
         _check(name, t, k_cache.device, k_cache.dtype, (B, N, Hk, D))
-    _written(k_cache, v_cache)
+    _check_written(k_cache, v_cache, k, v)
     _no_grad(k_cache, v_cache, k, v)
     k, v = _strided(k), _strided(v)
-    if any(_overlap(t, c) for t in (k, v) for c in (k_cache, v_cache)):
-        raise ValueError("k and v must not overlap the caches")
     with _on(k_cache.device):
         _native.check(_native.lib().hz_paged_append(_stream(k_cache.device), args, _native.TOKEN_TENSOR.pack(*_fields(k)),
                                                     _native.TOKEN_TENSOR.pack(*_fields(v)), N))
@@ -195,7 +211,7 @@ def paged_evict(
         raise ValueError(f"budget must be in [1, 2^30), got {budget}")
     if sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"sinks and recent must not be negative and at most the budget together, got {sinks} and {recent} of {budget}")
-    _written(k_cache, v_cache)
+    _check_written(k_cache, v_cache)
     _no_grad(k_cache, v_cache, scores)
     scores = scores.contiguous()
     if scores.data_ptr() % 16:
