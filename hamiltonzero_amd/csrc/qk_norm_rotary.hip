@@ -119,20 +119,23 @@ __device__ __forceinline__ void weights(const float* w, const Lane& l, float (&x
   }
 }
 
+// The first of the tokens at hand: one 64-bit division for all of them.
+struct First {
+  int64_t b;
+  int n;
+  __device__ __forceinline__ First(const NormParams& p, int64_t token0) : b(token0 / p.N), n(static_cast<int>(token0 - b * p.N)) {}
+};
+
 // One (token, head) of the tokens at hand: which tensor, and where its head lies in the strided ones and in
 // a contiguous one.
 struct Item {
   bool is_q;
-  int token, head;
-  int64_t b, n;
-  __device__ __forceinline__ Item(const NormParams& p, int64_t token0, int i) {
-    token = i / p.HT;
-    const int h = i - token * p.HT;
-    is_q = h < p.H;
-    head = is_q ? h : h - p.H;
-    const int64_t at = token0 + token;
-    b = at / p.N;
-    n = at - b * p.N;
+  int token, head, n;
+  int64_t b;
+  __device__ __forceinline__ Item(const NormParams& p, const First& first, int i) : Item(p, first, i / p.HT, i % p.HT) {}
+  __device__ __forceinline__ Item(const NormParams& p, const First& first, int token_, int h)
+      : is_q(h < p.H), token(token_), head(h < p.H ? h : h - p.H), n(first.n + token_), b(first.b) {
+    while (n >= p.N) n -= p.N, ++b;  // (a few tokens)
   }
   // (by value: a reference to one of two kernel arguments would put both into scratch memory)
   __device__ __forceinline__ const void* data(const hz_token_tensor& q, const hz_token_tensor& k) const {
@@ -143,8 +146,8 @@ struct Item {
   }
 };
 
-template <class S, int GS, bool INTERLEAVED, bool NORM>
-__global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p, float dir) {
+template <class S, int GS, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p) {
   __shared__ Angles angles;
   constexpr int SLOTS = kThreads / GS;
   const int t = threadIdx.x % GS, slot = threadIdx.x / GS;
@@ -155,10 +158,11 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p,
   for (int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.each; token0 < p.tokens;
        token0 += static_cast<int64_t>(gridDim.x) * p.each) {
     const int count = static_cast<int>(p.tokens - token0 < p.each ? p.tokens - token0 : p.each), items = count * p.HT;
+    const First first(p, token0);
     Raw<S> next;
     auto load = [&](int i) {
       if (i < items && lane.on) {
-        const Item it(p, token0, i);
+        const Item it(p, first, i);
         next.load(it.data(p.q, p.k), it.offset(p.q, p.k), lane);
       }
     };
@@ -166,19 +170,17 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p,
     put_angles(p, token0, count, angles);
     __syncthreads();
     for (int i = slot; i < items; i += SLOTS) {
-      const Item it(p, token0, i);
+      const Item it(p, first, i);
       float x[8];
       next.get(x, lane.on);
       load(i + SLOTS);
-      if constexpr (NORM) {
-        float ss = 0.f;
+      float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-        const float r = 1.f / sqrtf(head_sum<GS>(ss) / static_cast<float>(p.D) + p.eps);
+      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+      const float r = 1.f / sqrtf(head_sum<GS>(ss) / static_cast<float>(p.D) + p.eps);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= r * (it.is_q ? wq[e] : wk[e]);
-      }
-      if (lane.turns) turn8<INTERLEAVED>(x, &angles[it.token][4 * t], dir);
+      for (int e = 0; e < 8; ++e) x[e] *= r * (it.is_q ? wq[e] : wk[e]);
+      if (lane.turns) turn8<INTERLEAVED>(x, &angles[it.token][4 * t], 1.f);
       if (lane.on) store8<S>(const_cast<void*>(it.data(p.qo, p.ko)), it.offset(p.qo, p.ko), lane, x);
     }
     __syncthreads();
@@ -200,10 +202,11 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_bwd_kernel(NormParams p,
   for (int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.each; token0 < p.tokens;
        token0 += static_cast<int64_t>(gridDim.x) * p.each) {
     const int count = static_cast<int>(p.tokens - token0 < p.each ? p.tokens - token0 : p.each), items = count * p.HT;
+    const First first(p, token0);
     Raw<S> next_x, next_g;
     auto load = [&](int i) {
       if (i < items && lane.on) {
-        const Item it(p, token0, i);
+        const Item it(p, first, i);
         next_x.load(it.data(p.q, p.k), it.offset(p.q, p.k), lane);
         next_g.load(it.data(p.qo, p.ko), it.offset(p.qo, p.ko), lane);
       }
@@ -212,7 +215,7 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_bwd_kernel(NormParams p,
     put_angles(p, token0, count, angles);
     __syncthreads();
     for (int i = slot; i < items; i += SLOTS) {
-      const Item it(p, token0, i);
+      const Item it(p, first, i);
       float x[8], g[8];
       next_x.get(x, lane.on);
       next_g.get(g, lane.on);
@@ -278,6 +281,116 @@ __global__ void __launch_bounds__(kThreads) weight_sum_kernel(const float* parti
   }
 }
 
+// U elements of a head as they lie in memory.
+template <class S, int U>
+struct Chunk;
+template <>
+struct Chunk<F32, 4> {
+  typedef uint32_t V __attribute__((ext_vector_type(4)));
+  V v;
+  __device__ __forceinline__ void get(float (&x)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
+  }
+  __device__ __forceinline__ void set(const float (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(x[i]);
+  }
+};
+template <int U>
+struct Chunk<BF16, U> {
+  typedef uint32_t V __attribute__((ext_vector_type(U / 2)));
+  V v;
+  __device__ __forceinline__ void get(float (&x)[U]) const {
+#pragma unroll
+    for (int i = 0; i < U / 2; ++i) x[2 * i] = __uint_as_float(v[i] << 16), x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+  }
+  __device__ __forceinline__ void set(const float (&x)[U]) {
+#pragma unroll
+    for (int i = 0; i < U / 2; ++i) v[i] = pack2_bf16(x[2 * i], x[2 * i + 1]);
+  }
+};
+
+// The rotation alone, from q and k to qo and ko, and back (dir -1), which is its reverse mode. A thread has two chunks of U elements of one
+// head after the other, two heads in flight: a chunk and the one that it turns with (behind the rotated part: the next), or
+// with interleaved pairs one in each half of the head, so that a wave's 16 bytes lie one behind the other. They are read once,
+// past the caches (2 x 8160 tokens of 40 bfloat16 heads of 128: 60 us, 66 through them; 76 with chunks of 4, as behind the norms).
+// Bound by those bytes: 5.6 TB/s.
+template <class S, int U, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(NormParams p, float dir) {
+  __shared__ Angles angles;
+  typedef typename S::T T;
+  typedef typename Chunk<S, U>::V V;
+  const int units = p.D / (2 * U), slots = kThreads / units, t = static_cast<int>(threadIdx.x) % units, slot = static_cast<int>(threadIdx.x) / units;
+  const bool turns = U * t < p.nf;
+  const int o0 = INTERLEAVED || turns ? U * t : 2 * U * t, o1 = INTERLEAVED ? p.D / 2 + U * t : turns ? p.nf + U * t : o0 + U;
+  const int step_token = slots / p.HT, step_head = slots % p.HT;  // from a slot's item to its next
+  for (int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.each; token0 < p.tokens;
+       token0 += static_cast<int64_t>(gridDim.x) * p.each) {
+    const int count = static_cast<int>(p.tokens - token0 < p.each ? p.tokens - token0 : p.each);
+    const First first(p, token0);
+    struct At {
+      int token, head;
+    };
+    auto after = [&](At a) {
+      a.token += step_token, a.head += step_head;
+      if (a.head >= p.HT) a.head -= p.HT, ++a.token;
+      return a;
+    };
+    Chunk<S, U> x[2], y[2];
+    auto load = [&](At a, int i) __attribute__((always_inline)) {
+      if (a.token >= count) return;
+      const Item it(p, first, a.token, a.head);
+      const T* const from = static_cast<const T*>(it.data(p.q, p.k)) + it.offset(p.q, p.k);
+      x[i].v = __builtin_nontemporal_load(reinterpret_cast<const V*>(from + o0));
+      y[i].v = __builtin_nontemporal_load(reinterpret_cast<const V*>(from + o1));
+    };
+    auto use = [&](At a, int i) __attribute__((always_inline)) {
+      const Item it(p, first, a.token, a.head);
+      float u[U], v[U];
+      x[i].get(u), y[i].get(v);
+      auto turn = [&](float& p0, float& p1, float2 angle) __attribute__((always_inline)) {
+        const float c = angle.x, s = dir * angle.y, m = p0, n = p1;
+        p0 = m * c - n * s;
+        p1 = n * c + m * s;
+      };
+      if constexpr (INTERLEAVED) {
+        auto pairs = [&](Chunk<S, U>& chunk, float (&w)[U], int pair) __attribute__((always_inline)) {
+          if (pair >= p.nf) return;
+#pragma unroll
+          for (int e = 0; e < U / 2; ++e) turn(w[2 * e], w[2 * e + 1], angles[a.token][pair + e]);
+          chunk.set(w);
+        };
+        pairs(x[i], u, o0 / 2);
+        pairs(y[i], v, o1 / 2);
+      } else if (turns) {
+#pragma unroll
+        for (int e = 0; e < U; ++e) turn(u[e], v[e], angles[a.token][U * t + e]);
+        x[i].set(u), y[i].set(v);
+      }
+      T* const to = static_cast<T*>(const_cast<void*>(it.data(p.qo, p.ko))) + it.offset(p.qo, p.ko);
+      *reinterpret_cast<V*>(to + o0) = x[i].v;
+      *reinterpret_cast<V*>(to + o1) = y[i].v;
+    };
+    At a{slot / p.HT, slot % p.HT}, b = after(a);
+    if (slot >= slots) a.token = b.token = count;
+    load(a, 0);
+    load(b, 1);
+    put_angles(p, token0, count, angles);
+    __syncthreads();
+    while (a.token < count) {
+      use(a, 0);
+      a = after(b);
+      load(a, 0);
+      if (b.token >= count) break;
+      use(b, 1);
+      b = after(a);
+      load(b, 1);
+    }
+    __syncthreads();
+  }
+}
+
 // Tokens a workgroup at a time: several where that leaves at least `blocks` workgroups, so that the angles are
 // formed by all lanes and the loads of several heads overlap (the forwards of
 // qk_train_bf16 and qk_train_sites_f32: 90 and 93 us, 115 and 220 with one token).
@@ -330,13 +443,28 @@ void by_variant(const hz_qk_norm_rotary& a, F f) {
   });
 }
 
-// dir -1: the rotation back, what the reverse mode of a rotation without norms is.
-template <bool NORM>
-hipError_t run_fwd(const NormParams& p, const hz_qk_norm_rotary& a, float dir, hipStream_t stream) {
+hipError_t run_fwd(const NormParams& p, const hz_qk_norm_rotary& a, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(blocks(p, 1 << 20)));
   by_variant(a, [&](auto type, auto gs, auto inter) {
-    norm_rotary_fwd_kernel<decltype(type), gs.value, inter.value, NORM><<<grid, kThreads, 0, stream>>>(p, dir);
+    norm_rotary_fwd_kernel<decltype(type), gs.value, inter.value><<<grid, kThreads, 0, stream>>>(p);
   });
+  return hipGetLastError();
+}
+
+hipError_t run_rotary(const NormParams& p, float dir, int32_t dtype, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(blocks(p, 1 << 20)));
+  auto run = [&](auto type, auto u) {
+    if (p.interleaved)
+      rotary_kernel<decltype(type), u.value, true><<<grid, kThreads, 0, stream>>>(p, dir);
+    else
+      rotary_kernel<decltype(type), u.value, false><<<grid, kThreads, 0, stream>>>(p, dir);
+  };
+  if (dtype == HZ_DTYPE_F32)
+    run(F32{}, std::integral_constant<int, 4>{});
+  else if (p.D % 16 == 0 && p.nf % 8 == 0)
+    run(BF16{}, std::integral_constant<int, 8>{});
+  else
+    run(BF16{}, std::integral_constant<int, 4>{});
   return hipGetLastError();
 }
 
@@ -359,7 +487,7 @@ int64_t qk_norm_rotary_workspace(int64_t tokens, int64_t D) {
 }
 
 hipError_t launch_qk_norm_rotary_fwd(const hz_qk_norm_rotary& a, hipStream_t stream) {
-  return run_fwd<true>(params(a), a, 1.f, stream);
+  return run_fwd(params(a), a, stream);
 }
 
 hipError_t launch_qk_norm_rotary_bwd(const hz_qk_norm_rotary& a, void* dq, void* dk, float* dw_q, float* dw_k,
@@ -371,7 +499,7 @@ int64_t qk_rotary_workspace(int64_t tokens, int64_t D, bool norm) { return norm 
 
 hipError_t launch_qk_rotary_fwd(const hz_qk_rotary& a, hipStream_t stream) {
   const NormParams p = params(a);
-  return a.norm ? run_fwd<true>(p, a.rotary, 1.f, stream) : run_fwd<false>(p, a.rotary, 1.f, stream);
+  return a.norm ? run_fwd(p, a.rotary, stream) : run_rotary(p, 1.f, a.rotary.dtype, stream);
 }
 
 hipError_t launch_qk_rotary_bwd(const hz_qk_rotary& a, void* dq, void* dk, float* dw_q, float* dw_k, void* workspace,
@@ -381,7 +509,7 @@ hipError_t launch_qk_rotary_bwd(const hz_qk_rotary& a, void* dq, void* dk, float
   p.q = p.qo, p.k = p.ko;
   p.qo = {dq, static_cast<int64_t>(p.N) * p.H * p.D, static_cast<int64_t>(p.H) * p.D, p.D};
   p.ko = {dk, static_cast<int64_t>(p.N) * (p.HT - p.H) * p.D, static_cast<int64_t>(p.HT - p.H) * p.D, p.D};
-  return run_fwd<false>(p, a.rotary, -1.f, stream);
+  return run_rotary(p, -1.f, a.rotary.dtype, stream);
 }
 
 }  // namespace hz
