@@ -20,7 +20,8 @@ namespace hz {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 4;     // a workgroup at a time
+constexpr int kMaxTokens = 16;     // a workgroup at a time, forward
+constexpr int kMaxTokensBwd = 4;   // and backward
 constexpr int kMaxBlocks = 1024;  // of the backward: rows of partial weight gradients
 
 struct NormParams {
@@ -46,9 +47,9 @@ struct Lane {
   }
 };
 
-typedef float2 Angles[kMaxTokens][HZ_ROTARY_MAX_HEAD / 2];
+typedef float2 Angles[HZ_ROTARY_MAX_HEAD / 2];  // of a token
 
-__device__ __forceinline__ void put_angles(const NormParams& p, int64_t token0, int count, Angles& angles) {
+__device__ __forceinline__ void put_angles(const NormParams& p, int64_t token0, int count, Angles* angles) {
   for (int a = threadIdx.x; a < count * p.nf; a += kThreads) {
     const int x = a / p.nf, f = a - x * p.nf;
     const int64_t token = token0 + x;
@@ -148,7 +149,7 @@ struct Item {
 
 template <class S, int GS, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p) {
-  __shared__ Angles angles;
+  __shared__ Angles angles[kMaxTokens];
   constexpr int SLOTS = kThreads / GS;
   const int t = threadIdx.x % GS, slot = threadIdx.x / GS;
   const Lane lane(p, t);
@@ -159,21 +160,22 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p)
        token0 += static_cast<int64_t>(gridDim.x) * p.each) {
     const int count = static_cast<int>(p.tokens - token0 < p.each ? p.tokens - token0 : p.each), items = count * p.HT;
     const First first(p, token0);
-    Raw<S> next;
-    auto load = [&](int i) {
+    Raw<S> next[2];
+    auto load = [&](int i, int k) __attribute__((always_inline)) {
       if (i < items && lane.on) {
         const Item it(p, first, i);
-        next.load(it.data(p.q, p.k), it.offset(p.q, p.k), lane);
+        next[k].load(it.data(p.q, p.k), it.offset(p.q, p.k), lane);
       }
     };
-    load(slot);
+    load(slot, 0);
+    load(slot + SLOTS, 1);
     put_angles(p, token0, count, angles);
     __syncthreads();
-    for (int i = slot; i < items; i += SLOTS) {
+    auto use = [&](int i, int k) __attribute__((always_inline)) {
       const Item it(p, first, i);
       float x[8];
-      next.get(x, lane.on);
-      load(i + SLOTS);
+      next[k].get(x, lane.on);
+      load(i + 2 * SLOTS, k);
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
@@ -182,6 +184,10 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p)
       for (int e = 0; e < 8; ++e) x[e] *= r * (it.is_q ? wq[e] : wk[e]);
       if (lane.turns) turn8<INTERLEAVED>(x, &angles[it.token][4 * t], 1.f);
       if (lane.on) store8<S>(const_cast<void*>(it.data(p.qo, p.ko)), it.offset(p.qo, p.ko), lane, x);
+    };
+    for (int i = slot; i < items; i += 2 * SLOTS) {
+      use(i, 0);
+      if (i + SLOTS < items) use(i + SLOTS, 1);
     }
     __syncthreads();
   }
@@ -190,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p)
 // q and k: the forward's inputs; qo and ko: the cotangents. partial: [gridDim.x][2][D].
 template <class S, int GS, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) norm_rotary_bwd_kernel(NormParams p, void* dq, void* dk, float* partial) {
-  __shared__ Angles angles;
+  __shared__ Angles angles[kMaxTokensBwd];
   __shared__ float red[kThreads * 8];
   constexpr int SLOTS = kThreads / GS;
   const int t = threadIdx.x % GS, slot = threadIdx.x / GS;
@@ -318,7 +324,7 @@ struct Chunk<BF16, U> {
 // Bound by those bytes: 5.6 TB/s.
 template <class S, int U, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(NormParams p, float dir) {
-  __shared__ Angles angles;
+  __shared__ Angles angles[kMaxTokens];
   typedef typename S::T T;
   typedef typename Chunk<S, U>::V V;
   const int units = p.D / (2 * U), slots = kThreads / units, t = static_cast<int>(threadIdx.x) % units, slot = static_cast<int>(threadIdx.x) / units;
@@ -393,10 +399,16 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(NormParams p, float di
 
 // Tokens a workgroup at a time: several where that leaves at least `blocks` workgroups, so that the angles are
 // formed by all lanes and the loads of several heads overlap (the forwards of
-// qk_train_bf16 and qk_train_sites_f32: 90 and 93 us, 115 and 220 with one token).
-int tokens_each(int64_t tokens, int64_t blocks) {
+// qk_train_bf16 and qk_train_sites_f32: 90 and 93 us, 115 and 220 with one token); a power of two, up to 160 heads in all (2 x 8160
+// tokens of 40 heads, 4 and 16 tokens a time: 61 us, 73; 256 x 225 of 16 heads, 4 and 8: 52 and 50, behind norms 116 and 112).
+int tokens_each(int64_t tokens, int64_t blocks, int most) {
   const int64_t n = tokens / blocks;
-  return static_cast<int>(n < 1 ? 1 : n > kMaxTokens ? kMaxTokens : n);
+  return static_cast<int>(n < 1 ? 1 : n > most ? most : n);
+}
+int forward_each(const NormParams& p) {
+  int n = kMaxTokens;
+  while (n > 1 && n * p.HT > 160) n /= 2;
+  return tokens_each(p.tokens, kMaxBlocks, n);
 }
 
 NormParams params(const hz_qk_norm_rotary& a) {
@@ -406,7 +418,7 @@ NormParams params(const hz_qk_norm_rotary& a) {
   p.tokens = a.B * a.N;
   p.N = static_cast<int>(a.N), p.H = static_cast<int>(a.H), p.HT = static_cast<int>(a.H + a.Hk);
   p.D = static_cast<int>(a.D), p.nf = static_cast<int>(a.n_freqs), p.interleaved = a.interleaved, p.n_axes = 1;
-  p.each = tokens_each(p.tokens, kMaxBlocks);
+  p.each = tokens_each(p.tokens, kMaxBlocks, kMaxTokensBwd);
   p.eps = a.eps;
   return p;
 }
@@ -443,7 +455,8 @@ void by_variant(const hz_qk_norm_rotary& a, F f) {
   });
 }
 
-hipError_t run_fwd(const NormParams& p, const hz_qk_norm_rotary& a, hipStream_t stream) {
+hipError_t run_fwd(NormParams p, const hz_qk_norm_rotary& a, hipStream_t stream) {
+  p.each = forward_each(p);
   const dim3 grid(static_cast<unsigned>(blocks(p, 1 << 20)));
   by_variant(a, [&](auto type, auto gs, auto inter) {
     norm_rotary_fwd_kernel<decltype(type), gs.value, inter.value><<<grid, kThreads, 0, stream>>>(p);
@@ -451,7 +464,8 @@ hipError_t run_fwd(const NormParams& p, const hz_qk_norm_rotary& a, hipStream_t 
   return hipGetLastError();
 }
 
-hipError_t run_rotary(const NormParams& p, float dir, int32_t dtype, hipStream_t stream) {
+hipError_t run_rotary(NormParams p, float dir, int32_t dtype, hipStream_t stream) {
+  p.each = forward_each(p);
   const dim3 grid(static_cast<unsigned>(blocks(p, 1 << 20)));
   auto run = [&](auto type, auto u) {
     if (p.interleaved)
