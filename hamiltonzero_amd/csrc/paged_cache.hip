@@ -80,20 +80,31 @@ struct Row {
     scores_out = p.scores_out + row * p.c.slots;
     sources = p.sources + row * p.keep;
   }
-  // What does not depend on the scores, and the slots below the budget as if all of them stayed, by `threads` threads.
+  // What does not depend on the scores, and the slots below the budget as if all of them stayed, by `threads` threads. (Loads are
+  // unconditional, so that none waits for another; 16 bytes at a time where rows are a multiple of four slots.)
   __device__ __forceinline__ void fill(const EvictParams& p, int tid, int threads) const {
     if (tid == 0 && h == 0) p.lengths_out[b] = min(n, m);
-#pragma unroll 8
-    for (int s = tid; s < p.c.slots; s += threads) {
-      const float x = scores[min(s, m - 1)];  // (unconditional, so that the loads do not wait for each other)
-      scores_out[s] = s < n && s < m ? x : 0.f;
+    const int end = min(n, m);
+    if (p.c.slots % 4 == 0) {
+#pragma unroll 4
+      for (int s = 4 * tid; s < p.c.slots; s += 4 * threads) {
+        float4 x = *reinterpret_cast<const float4*>(scores + min(s, (m - 1) & ~3));
+        x.x = s < end ? x.x : 0.f, x.y = s + 1 < end ? x.y : 0.f, x.z = s + 2 < end ? x.z : 0.f, x.w = s + 3 < end ? x.w : 0.f;
+        *reinterpret_cast<float4*>(scores_out + s) = x;
+      }
+    } else {
+#pragma unroll 4
+      for (int s = tid; s < p.c.slots; s += threads) {
+        const float x = scores[min(s, m - 1)];
+        scores_out[s] = s < end ? x : 0.f;
+      }
     }
-#pragma unroll 8
+#pragma unroll 4
     for (int s = tid; s < p.keep; s += threads) sources[s] = s < n ? s : -1;
   }
   // The key of slot s, whose score is x; 0 behind the row.
   __device__ __forceinline__ uint32_t key(int s, float x) const { return s >= n ? 0u : s >= lo && s < hi ? ordered(x) : kFixed; }
-  // A lane's keys of the slots base + step j. The loads are unconditional, so that none waits for another.
+  // A lane's keys of the slots base + step j.
   template <int KEYS>
   __device__ __forceinline__ void keys(int base, int step, uint32_t (&u)[KEYS]) const {
     float x[KEYS];
@@ -101,6 +112,18 @@ struct Row {
     for (int j = 0; j < KEYS; ++j) x[j] = scores[min(base + step * j, n - 1)];
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) u[j] = key(base + step * j, x[j]);
+  }
+  // Of the slots base + j, where rows are a multiple of four slots and base is one.
+  template <int KEYS>
+  __device__ __forceinline__ void keys_by_four(int base, uint32_t (&u)[KEYS]) const {
+    float4 x[KEYS / 4];
+#pragma unroll
+    for (int j = 0; j < KEYS / 4; ++j) x[j] = *reinterpret_cast<const float4*>(scores + min(base + 4 * j, (n - 1) & ~3));
+#pragma unroll
+    for (int j = 0; j < KEYS / 4; ++j) {
+      const int s = base + 4 * j;
+      u[4 * j] = key(s, x[j].x), u[4 * j + 1] = key(s + 1, x[j].y), u[4 * j + 2] = key(s + 2, x[j].z), u[4 * j + 3] = key(s + 3, x[j].w);
+    }
   }
 };
 
@@ -275,7 +298,13 @@ __global__ void __launch_bounds__(kSelect) paged_select_kernel(EvictParams p) {
     return;
   }
   uint32_t u[KEYS];
-  if (ONE) r.keys(KEYS * tid, 1, u);
+  auto read = [&](int base) {
+    if (p.c.slots % 4 == 0)
+      r.keys_by_four(base, u);
+    else
+      r.keys(base, 1, u);
+  };
+  if (ONE) read(KEYS * tid);
   r.fill(p, tid, kSelect);
   // the threshold: slots above it stay, and the first `equal` of those at it
   uint32_t threshold = 0;
@@ -286,7 +315,7 @@ __global__ void __launch_bounds__(kSelect) paged_select_kernel(EvictParams p) {
     *reinterpret_cast<int4*>(hist[tid + kSelect]) = make_int4(0, 0, 0, 0);
     __syncthreads();
     for (int s0 = KEYS * tid; s0 < r.n; s0 += SPAN) {
-      if (!ONE) r.keys(s0, 1, u);
+      if (!ONE) read(s0);
 #pragma unroll
       for (int j = 0; j < KEYS; ++j)
         if (s0 + j < r.n && (top == 32 || (u[j] ^ threshold) >> top == 0))
@@ -315,7 +344,7 @@ __global__ void __launch_bounds__(kSelect) paged_select_kernel(EvictParams p) {
   int holes = 0, late = 0;  // of the spans before
   for (int base = 0; base < r.n; base += SPAN) {
     const int s0 = base + KEYS * tid;
-    if (!ONE) r.keys(s0, 1, u);
+    if (!ONE) read(s0);
     int mine = 0, rank = 0;
     uint32_t total = 0;
 #pragma unroll
@@ -434,7 +463,7 @@ hipError_t launch_paged_evict(const hz_paged_evict_args& a, void* workspace, hip
   else
     paged_select_kernel<32, false><<<groups, kSelect, 0, stream>>>(p);
   if (most == 0) return hipGetLastError();
-  const int per = kThreads / chunks * 8;
+  const int per = kThreads / chunks * 4;
   const unsigned y = static_cast<unsigned>(rows < 65535 ? rows : 65535);
   const dim3 grid(static_cast<unsigned>((most + per - 1) / per), y, static_cast<unsigned>((rows + y - 1) / y));
   paged_move_kernel<<<grid, kThreads, 0, stream>>>(p, per);
