@@ -347,6 +347,75 @@ struct Slots<DP, PARTS, kApart> : Lanes<DP, PARTS> {
   }
 };
 
+// A run of slots and who has it. waves 4: the workgroup; waves 1: each wave one of its own, and they share nothing.
+struct Run {
+  bool together, alone;  // alone: its row has no other
+  int wave, id, b, hk, r0, n, first, stop;
+  const int32_t* table;
+  // Of blocks of `rows` rows of query and head. False behind the last run.
+  __device__ __forceinline__ bool find(const PagedParams& p, const Plan& plan, int wave_, int rows) {
+    wave = __builtin_amdgcn_readfirstlane(wave_);
+    together = p.waves == 4;
+    id = together ? static_cast<int>(blockIdx.x) : 4 * static_cast<int>(blockIdx.x) + wave;
+    hk = id % p.Hk;
+    id /= p.Hk;
+    r0 = id % p.blocks * rows;
+    id /= p.blocks;
+    Found found;
+    if (!plan.find(p, id, found)) return false;
+    b = found.b;
+    n = p.c.length(b);
+    alone = n <= plan.chunk;
+    const int begin = found.run * plan.chunk;
+    stop = alone ? n : min(n, begin + plan.chunk);
+    first = begin + (together ? kBlock * wave : 0);
+    table = p.c.table + static_cast<int64_t>(b) * p.c.width;
+    return true;
+  }
+};
+
+// Where chunk ch of four outputs of column x lies among sixteen columns: the columns' writes go to different banks.
+template <int DP>
+__device__ __forceinline__ int out_at(int x, int ch) { return x * DP + (ch ^ (x & 7)) * 4; }
+
+// The results of a run: rows r0 .. r0 + columns - 1 from its waves' sums of values (out_at, o_wave floats a wave) and their base, sum and sum of
+// unrounded weights (sums_wave floats a wave).
+template <int DP, int PARTS>
+__device__ __forceinline__ void put_run(const PagedParams& p, const Run& run, const float* o, int o_wave, const float* sums, int sums_wave, int columns, int r0) {
+  const int w0 = run.together ? 0 : run.wave, threads = run.together ? kThreads : 64;
+  for (int x = run.together ? threadIdx.x : threadIdx.x & 63; x < columns * (DP / 4); x += threads) {
+    const int col = x / (DP / 4), ch = x % (DP / 4), r = r0 + col, d = 4 * ch;
+    if (d >= p.D) continue;
+    float top = kNegInf, all = 0.f, all_exact = 0.f;
+    for (int w = w0; w < w0 + p.waves; ++w) top = fmaxf(top, sums[w * sums_wave + 3 * col]);
+    const float base = top == kNegInf ? 0.f : top;
+    v4f y = zero4();
+    for (int w = w0; w < w0 + p.waves; ++w) {
+      const float* const s = sums + w * sums_wave + 3 * col;
+      const float a = fast_exp2(s[0] - base);
+      all += a * s[1];
+      all_exact += a * s[2];
+      y += a * *reinterpret_cast<const v4f*>(o + w * o_wave + out_at<DP>(col, ch));
+    }
+    if (run.alone) {
+      const int64_t at = (static_cast<int64_t>(run.b) * p.Nq + r / p.G) * p.H + run.hk * p.G + r % p.G;
+      const float inv = all > 0.f || all != all ? 1.f / all : 0.f;
+      store_four<PARTS>(p.out, at * p.D + d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+      if (p.kept != nullptr && ch == 0) p.lse[at] = all_exact > 0.f ? top + log2f(all_exact) : 0.f;
+    } else {
+      const int64_t to = result_at(p, run.id, run.hk, r);
+      *reinterpret_cast<v4f*>(p.partial + to * p.D + d) = y;
+      if (ch == 0) *reinterpret_cast<v4f*>(p.stats + to * 4) = v4f{top, all, all_exact, 0.f};
+    }
+  }
+}
+
+// Of the lane some places on in the row of sixteen.
+template <int CONTROL>
+__device__ __forceinline__ float row_turned(float x) {
+  return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CONTROL, 0xf, 0xf, true));
+}
+
 template <int DP, int PARTS, bool CAP, int CB, Reads READS>
 __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_kernel(PagedParams p) {
   typedef Slots<DP, PARTS, READS> S;
@@ -357,22 +426,11 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
   __shared__ float sums_lds[4][16 * CB][3];  // each wave's base, sum and sum of unrounded weights
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const V vt{v_lds[wave]};
-  // waves 4: the workgroup's run; waves 1: one of each wave, which then share nothing
-  const bool together = p.waves == 4;
-  int id = together ? static_cast<int>(blockIdx.x) : 4 * static_cast<int>(blockIdx.x) + __builtin_amdgcn_readfirstlane(wave);
-  const int hk = id % p.Hk;
-  id /= p.Hk;
-  const int r0 = id % p.blocks * (16 * CB);
-  id /= p.blocks;
   const Plan plan(p, lane);
-  Found found;
-  if (!plan.find(p, id, found)) return;  // all waves of the run
-  const int b = found.b, n = p.c.length(b);
-  const bool alone = n <= plan.chunk;
-  const int begin = found.run * plan.chunk, stop = alone ? n : min(n, begin + plan.chunk);
-  const int first = begin + (together ? kBlock * __builtin_amdgcn_readfirstlane(wave) : 0), step = p.step;
-  const int32_t* const table = p.c.table + static_cast<int64_t>(b) * p.c.width;
-
+  Run run;
+  if (!run.find(p, plan, wave, 16 * CB)) return;  // all waves of the run
+  const bool together = run.together;
+  const int b = run.b, n = run.n, hk = run.hk, r0 = run.r0, first = run.first, stop = run.stop, step = p.step;
   Frag<PARTS> q[CB][DS];
   int pos[CB], row[CB];
   float slope2[CB];
@@ -399,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     for (int dt = 0; dt < DT; ++dt) o[cb][dt] = zero4();
   }
 
-  S slots(p, table, hk, stop, lane, where_lds[READS == kApart ? wave : 0]);
+  S slots(p, run.table, hk, stop, lane, where_lds[READS == kApart ? wave : 0]);
   const int lr = lane / CH, lc = lane % CH;
   Raw8<PARTS> rk[2][DS], rv[LOADS];
   uint32_t known = 0, known_next = 0;  // slots of the block at hand, and of the next, that lie in a page
@@ -484,45 +542,162 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     known_next = known_then;
   }
   settle(o);
-  // the run's sums, sixteen columns at a time, through the values' LDS: chunk ch of four elements of column x lies
-  // at chunk ch ^ (x & 7), so that the columns' writes go to different banks
-  const int ways = p.waves, w0 = together ? 0 : wave, threads = together ? kThreads : 64;
+  // the run's sums, sixteen columns at a time, through the values' LDS
   float* const mine = reinterpret_cast<float*>(v_lds[wave]);
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
     const float sum = group_sum(l[cb]), exact = group_sum(l_exact[cb]);
     if (g == 0) sums_lds[wave][16 * cb + c][0] = m[cb], sums_lds[wave][16 * cb + c][1] = sum, sums_lds[wave][16 * cb + c][2] = exact;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      *reinterpret_cast<v4f*>(mine + c * DP + ((4 * dt + g) ^ (c & 7)) * 4) = o[cb][dt];
+    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<v4f*>(mine + out_at<DP>(c, 4 * dt + g)) = o[cb][dt];
     together ? __syncthreads() : wave_fence();
-    const int columns = min(16, p.rows - r0 - 16 * cb);
-    for (int x = together ? threadIdx.x : lane; x < columns * (DP / 4); x += threads) {
-      const int col = x / (DP / 4), ch = x % (DP / 4), r = r0 + 16 * cb + col, d = 4 * ch;
-      if (d >= p.D) continue;
-      float top = kNegInf, all = 0.f, all_exact = 0.f;
-      for (int w = w0; w < w0 + ways; ++w) top = fmaxf(top, sums_lds[w][16 * cb + col][0]);
-      const float base = top == kNegInf ? 0.f : top;
-      v4f y = zero4();
-      for (int w = w0; w < w0 + ways; ++w) {
-        const float a = fast_exp2(sums_lds[w][16 * cb + col][0] - base);
-        all += a * sums_lds[w][16 * cb + col][1];
-        all_exact += a * sums_lds[w][16 * cb + col][2];
-        y += a * *reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(v_lds[w]) + col * DP + (ch ^ (col & 7)) * 4);
-      }
-      if (alone) {
-        const int64_t at = (static_cast<int64_t>(b) * p.Nq + r / p.G) * p.H + hk * p.G + r % p.G;
-        const float inv = all > 0.f || all != all ? 1.f / all : 0.f;
-        store_four<PARTS>(p.out, at * p.D + d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
-        if (p.kept != nullptr && ch == 0) p.lse[at] = all_exact > 0.f ? top + log2f(all_exact) : 0.f;
-      } else {
-        const int64_t to = result_at(p, id, hk, r);
-        *reinterpret_cast<v4f*>(p.partial + to * p.D + d) = y;
-        if (ch == 0) *reinterpret_cast<v4f*>(p.stats + to * 4) = v4f{top, all, all_exact, 0.f};
-      }
-    }
+    put_run<DP, PARTS>(p, run, reinterpret_cast<const float*>(v_lds[0]), kBlock * DP * static_cast<int>(sizeof(typename V::Element)) / 4, &sums_lds[0][16 * cb][0], 16 * CB * 3,
+                       min(16, p.rows - r0 - 16 * cb), r0 + 16 * cb);
     if (cb + 1 < CB) together ? __syncthreads() : wave_fence();
   }
+}
+
+// The same for float32 and one or two rows of query and head, on vector instructions: a lane has a part of each key's dot product, as
+// its loads bring it, and of the values' sums over its slots; the weights go from the one to the other through LDS. The matrix cores
+// would take sixteen rows for one or two and have keys and values split into three parts each: 512 rows of up to 225 slots of 8 heads
+// of 64 took 59 us so with one row, 63 with two and 68 on the matrix cores; 16 of up to 8192 of 8 heads of 128 took 122, 125 and 147.
+// Four rows took 94 (matrix cores 68) and 144 (148). Heads of 32: 28, 30 and 38. bfloat16 gains nothing (31.0 us with one row of 64,
+// 32.6 on the matrix cores; 120 and 120 with heads of 128). Heads of 64 keep two workgroups a CU (three spill: 73 us); heads of 128
+// need the registers of one.
+template <int DP, bool CAP, int R, Reads READS>
+__global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(PagedParams p) {
+  typedef Slots<DP, 3, READS> S;
+  constexpr int DS = S::DS, CH = S::CH, LOADS = S::LOADS, STEP = S::STEP;
+  __shared__ __align__(16) int64_t where_lds[READS == kApart ? 4 : 1][2][kBlock][2];
+  __shared__ __align__(16) float w_lds[4][R][kBlock], o_lds[4][R * DP];
+  __shared__ float sums_lds[4][R][3];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const Plan plan(p, lane);
+  Run run;
+  if (!run.find(p, plan, wave, R)) return;  // all waves of the run
+  const int b = run.b, n = run.n, stop = run.stop, step = p.step, hk = run.hk;
+  float q[R][DS][8], slope2[R];
+  int pos[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = r / p.G, h = hk * p.G + r % p.G;
+    pos[r] = n - p.Nq + i;
+    slope2[r] = p.slopes != nullptr ? p.slopes[h] * kLog2e : 0.f;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      Raw8<3> x;
+      const int d = S::key_element(lane, s);
+      x.load(p.q.data, b * p.q.batch + i * p.q.token + h * p.q.head + d, d < p.D);
+      floats(x, q[r][s]);
+    }
+  }
+  float o[R][8] = {}, m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) m[r] = kNegInf, l[r] = 0.f;
+  S slots(p, run.table, hk, stop, lane, where_lds[READS == kApart ? wave : 0]);
+  const int lr = lane / CH, lc = lane % CH;
+  Raw8<3> rk[2][DS], rv[LOADS];
+  uint32_t known = 0, known_next = 0;
+  int buffer = 0;
+  if (run.first < stop) {
+    slots.look(run.first);
+    known = slots.take(run.first, 0);
+    slots.look(run.first + step);
+    slots.load_k(rk, 0);
+    slots.load_v(rv, 0);
+    known_next = slots.take(run.first + step, 1);
+  }
+  for (int k0 = run.first; k0 < stop; k0 += step, buffer ^= 1) {
+    const bool more = k0 + step < stop;
+    slots.look(k0 + 2 * step);
+    float x[R][2] = {};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int s = 0; s < DS; ++s) {
+        float k[8];
+        floats(rk[kb][s], k);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[r][kb] = fmaf(k[e], q[r][s][e], x[r][kb]);
+      }
+    if (more) slots.load_k(rk, buffer ^ 1);
+    const uint32_t seen = known;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = kNegInf;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const int at = 16 * kb + c, key = k0 + at;
+        float y = xor32_pair_sum(xor16_pair_sum(x[r][kb]));
+        y = CAP ? tanh_of<3>(y * p.to_tanh) * p.to_score2 : y * p.to_score2;
+        if (slope2[r] != 0.f) y -= slope2[r] * static_cast<float>(abs(pos[r] - key));
+        y = key <= pos[r] && (seen >> at & 1) ? y : kNegInf;
+        x[r][kb] = y;
+        top = fmaxf(top, y);
+        if (p.kept != nullptr && g == 0)
+          p.kept[(static_cast<int64_t>(b * p.Hk + hk) * p.rows + r) * p.slots_kept + key] = y;
+      }
+      if (__any(top > m[r])) {
+        top = fmaxf(top, row_turned<0x121>(top));
+        top = fmaxf(top, row_turned<0x122>(top));
+        top = fmaxf(top, row_turned<0x124>(top));
+        top = fmaxf(top, row_turned<0x128>(top));
+        const float now = fmaxf(m[r], top), alpha = m[r] == kNegInf ? 0.f : fast_exp2(m[r] - now);
+        m[r] = now;
+        l[r] *= alpha;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[r][e] *= alpha;
+      }
+      const float base = m[r] == kNegInf ? 0.f : m[r];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const float w = fast_exp2(x[r][kb] - base);
+        l[r] += w;
+        if (g == 0) w_lds[wave][r][16 * kb + c] = w;
+      }
+    }
+    wave_fence();
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      float v[8];
+      floats(rv[j], v);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float w = w_lds[wave][r][lr + STEP * j];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[r][e] = fmaf(w, v[e], o[r][e]);
+      }
+    }
+    if (more) slots.load_v(rv, buffer ^ 1);
+    wave_fence();
+    known = known_next;
+    known_next = slots.take(k0 + 2 * step, buffer);  // (the next block's loads are under way)
+  }
+  // a row's sum over the sixteen lanes that have different slots; the values' over the lanes that have the same elements
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float sum = l[r];
+    sum += row_turned<0x128>(sum);
+    sum += row_turned<0x124>(sum);
+    sum += row_turned<0x122>(sum);
+    sum += row_turned<0x121>(sum);
+    if (lane == 0) sums_lds[wave][r][0] = m[r], sums_lds[wave][r][1] = sums_lds[wave][r][2] = sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float y = o[r][e];
+      if constexpr (CH <= 8) y += row_turned<0x128>(y);
+      if constexpr (CH <= 4) y += row_turned<0x124>(y);
+      o[r][e] = xor32_pair_sum(xor16_pair_sum(y));
+    }
+    if (lane < CH) {
+      *reinterpret_cast<v4f*>(o_lds[wave] + out_at<DP>(r, 2 * lc)) = v4f{o[r][0], o[r][1], o[r][2], o[r][3]};
+      *reinterpret_cast<v4f*>(o_lds[wave] + out_at<DP>(r, 2 * lc + 1)) = v4f{o[r][4], o[r][5], o[r][6], o[r][7]};
+    }
+  }
+  run.together ? __syncthreads() : wave_fence();
+  put_run<DP, 3>(p, run, o_lds[0], R * DP, &sums_lds[0][0][0], R * 3, p.rows, 0);
 }
 
 // The run results of one row of (b, i, h).
@@ -720,6 +895,14 @@ hipError_t run(const hz_paged_attention_args& a, void* workspace, hipStream_t st
   const unsigned grid = static_cast<unsigned>((w.runs * c.Hk * w.blocks * w.waves + 3) / 4);
   if (c.B > kPlanRows) paged_plan_kernel<<<1, 1024, 0, stream>>>(p, reinterpret_cast<int*>(ws + w.plan));
   auto attend = [&](auto reads) {
+    if constexpr (PARTS == 3)
+      if (w.rows <= 2) {
+        if (w.rows == 1)
+          paged_rows_kernel<DP, CAP, 1, reads.value><<<grid, kThreads, 0, stream>>>(p);
+        else
+          paged_rows_kernel<DP, CAP, 2, reads.value><<<grid, kThreads, 0, stream>>>(p);
+        return;
+      }
     if (w.block == 16)
       paged_attention_kernel<DP, PARTS, CAP, 1, reads.value><<<grid, kThreads, 0, stream>>>(p);
     else if constexpr (PARTS == 1 || DP < 128)
