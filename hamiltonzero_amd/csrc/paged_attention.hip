@@ -5,13 +5,13 @@
 // the sum of them over a number of runs that fills the card, so that one long row among short ones is divided as
 // finely as many of its length would be coarsely. Its four waves take blocks of 32 slots in turn and
 // join their sums in LDS; a row that is one run gets its results there, the others' runs are joined by a second
-// kernel.
+// kernel. Where the page table leaves no room for long rows, each row is one run and there is no second kernel.
 //
 // A block is 32 slots on v_mfma_f32_16x16x32_bf16: keys go from memory into the products' registers, values through
 // LDS of the wave's own. Where the slots lie is looked up two blocks ahead, so that no load waits for the page table.
 //
 // Accumulated weights need every row's final maximum and sum: the scores are kept in memory (4 bytes for each row
-// and slot beside the 4 D or 8 D that are read) and the second kernel adds up exp2 of them.
+// and slot beside the 4 D or 8 D that are read) and the second kernel, or the run itself where it is its row, adds up exp2 of them.
 #include "paged_launch.h"
 #include "token_device.h"
 
@@ -35,6 +35,7 @@ struct PagedParams {
   int64_t runs_wanted, runs_fill;        // for one key head and block of rows, over all batch rows: at most, and to fill the card
   const int* plan;                       // of more than 64 batch rows
   int waves, step;                       // waves of a run; slots that they take at a time, of which runs are multiples
+  bool whole;                            // each row is one run
   float cap, to_tanh, to_score2, decay;
 };
 
@@ -75,6 +76,11 @@ struct Plan {
   int chunk, all, mine, upto;  // all: number of further runs; this lane's row's, and those of the rows up to it (without a table)
   const int* table;            // chunk, all, [B] the further runs before each row, then their Founds
   __device__ __forceinline__ Plan(const PagedParams& p, int lane) : mine(0), upto(0), table(p.plan) {
+    if (p.whole) {
+      chunk = p.c.slots;
+      all = 0;
+      return;
+    }
     if (table != nullptr) {
       chunk = table[0];
       all = table[1];
@@ -355,7 +361,7 @@ struct Run {
   // Of blocks of `rows` rows of query and head. False behind the last run.
   __device__ __forceinline__ bool find(const PagedParams& p, const Plan& plan, int wave_, int rows) {
     wave = __builtin_amdgcn_readfirstlane(wave_);
-    together = p.waves == 4;
+    together = p.waves > 1;
     id = together ? static_cast<int>(blockIdx.x) : 4 * static_cast<int>(blockIdx.x) + wave;
     hk = id % p.Hk;
     id /= p.Hk;
@@ -379,10 +385,12 @@ template <int DP>
 __device__ __forceinline__ int out_at(int x, int ch) { return x * DP + (ch ^ (x & 7)) * 4; }
 
 // The results of a run: rows r0 .. r0 + columns - 1 from its waves' sums of values (out_at, o_wave floats a wave) and their base, sum and sum of
-// unrounded weights (sums_wave floats a wave).
+// unrounded weights (sums_wave floats a wave). Where the run is its row and weights are added up, the columns' logarithms of their sums go to
+// lse and to memory.
 template <int DP, int PARTS>
-__device__ __forceinline__ void put_run(const PagedParams& p, const Run& run, const float* o, int o_wave, const float* sums, int sums_wave, int columns, int r0) {
-  const int w0 = run.together ? 0 : run.wave, threads = run.together ? kThreads : 64;
+__device__ __forceinline__ void put_run(const PagedParams& p, const Run& run, const float* o, int o_wave, const float* sums, int sums_wave, int columns, int r0,
+                                        float* lse) {
+  const int w0 = run.together ? 0 : run.wave, threads = 64 * p.waves;
   for (int x = run.together ? threadIdx.x : threadIdx.x & 63; x < columns * (DP / 4); x += threads) {
     const int col = x / (DP / 4), ch = x % (DP / 4), r = r0 + col, d = 4 * ch;
     if (d >= p.D) continue;
@@ -401,12 +409,56 @@ __device__ __forceinline__ void put_run(const PagedParams& p, const Run& run, co
       const int64_t at = (static_cast<int64_t>(run.b) * p.Nq + r / p.G) * p.H + run.hk * p.G + r % p.G;
       const float inv = all > 0.f || all != all ? 1.f / all : 0.f;
       store_four<PARTS>(p.out, at * p.D + d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
-      if (p.kept != nullptr && ch == 0) p.lse[at] = all_exact > 0.f ? top + log2f(all_exact) : 0.f;
+      if (p.kept != nullptr && ch == 0) {
+        lse[col] = all_exact > 0.f ? top + log2f(all_exact) : 0.f;
+        if (p.lse != nullptr) p.lse[at] = lse[col];
+      }
     } else {
       const int64_t to = result_at(p, run.id, run.hk, r);
       *reinterpret_cast<v4f*>(p.partial + to * p.D + d) = y;
       if (ch == 0) *reinterpret_cast<v4f*>(p.stats + to * 4) = v4f{top, all, all_exact, 0.f};
     }
+  }
+}
+
+// The weights of four slots of a row of n, from what rows r0 .. r0 + rows - 1 of query and head kept.
+__device__ __forceinline__ void add_kept(const PagedParams& p, int unit, int slot, const float* lse, int r0, int rows, v4f& sum) {
+  const float* const kept = p.kept + (static_cast<int64_t>(unit) * p.rows + r0) * p.slots_kept + slot;
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    const v4f x = *reinterpret_cast<const v4f*>(kept + r * p.slots_kept);
+    const float base = lse[r];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += fast_exp2(x[e] - base);
+  }
+}
+__device__ __forceinline__ void put_weights(const PagedParams& p, int unit, int n, int slot, const v4f& sum) {
+  const int64_t at = static_cast<int64_t>(unit) * p.c.slots + slot;
+  if (slot + 4 <= p.c.slots && p.c.slots % 4 == 0) {
+    v4f x = zero4();
+    if (slot < n && p.scores != nullptr) x = p.decay * *reinterpret_cast<const v4f*>(p.scores + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = slot + e < n ? x[e] + sum[e] : 0.f;
+    *reinterpret_cast<v4f*>(p.scores_out + at) = x;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (slot + e >= p.c.slots) break;
+    float x = 0.f;
+    if (slot + e < n) x = sum[e] + (p.scores != nullptr ? p.decay * p.scores[at + e] : 0.f);
+    p.scores_out[at + e] = x;
+  }
+}
+
+// The weights of a run that is its row, and all rows of query and head, by its threads.
+__device__ __forceinline__ void put_own_weights(const PagedParams& p, const Run& run, const float* lse) {
+  run.together ? __syncthreads() : wave_fence();
+  const int threads = 64 * p.waves, unit = run.b * p.Hk + run.hk;
+  for (int slot = 4 * (run.together ? threadIdx.x : threadIdx.x & 63); slot < p.c.slots; slot += 4 * threads) {
+    v4f sum = zero4();
+    if (slot < run.n) add_kept(p, unit, slot, lse, 0, p.rows, sum);
+    put_weights(p, unit, run.n, slot, sum);
   }
 }
 
@@ -423,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
   typedef Values<DP, PARTS> V;
   __shared__ __align__(16) typename V::Element v_lds[4][kBlock * DP];
   __shared__ __align__(16) int64_t where_lds[READS == kApart ? 4 : 1][2][kBlock][2];
-  __shared__ float sums_lds[4][16 * CB][3];  // each wave's base, sum and sum of unrounded weights
+  __shared__ float sums_lds[4][16 * CB][3], lse_lds[4][16 * CB];  // each wave's base, sum and sum of unrounded weights
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const V vt{v_lds[wave]};
   const Plan plan(p, lane);
@@ -552,9 +604,10 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<v4f*>(mine + out_at<DP>(c, 4 * dt + g)) = o[cb][dt];
     together ? __syncthreads() : wave_fence();
     put_run<DP, PARTS>(p, run, reinterpret_cast<const float*>(v_lds[0]), kBlock * DP * static_cast<int>(sizeof(typename V::Element)) / 4, &sums_lds[0][16 * cb][0], 16 * CB * 3,
-                       min(16, p.rows - r0 - 16 * cb), r0 + 16 * cb);
+                       min(16, p.rows - r0 - 16 * cb), r0 + 16 * cb, lse_lds[together ? 0 : wave] + 16 * cb);
     if (cb + 1 < CB) together ? __syncthreads() : wave_fence();
   }
+  if (p.kept != nullptr && p.lse == nullptr) put_own_weights(p, run, lse_lds[together ? 0 : wave]);
 }
 
 // The same for float32 and one or two rows of query and head, on vector instructions: a lane has a part of each key's dot product, as
@@ -570,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
   constexpr int DS = S::DS, CH = S::CH, LOADS = S::LOADS, STEP = S::STEP;
   __shared__ __align__(16) int64_t where_lds[READS == kApart ? 4 : 1][2][kBlock][2];
   __shared__ __align__(16) float w_lds[4][R][kBlock], o_lds[4][R * DP];
-  __shared__ float sums_lds[4][R][3];
+  __shared__ float sums_lds[4][R][3], lse_lds[4][R];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const Plan plan(p, lane);
   Run run;
@@ -697,7 +750,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
     }
   }
   run.together ? __syncthreads() : wave_fence();
-  put_run<DP, 3>(p, run, o_lds[0], R * DP, &sums_lds[0][0][0], R * 3, p.rows, 0);
+  put_run<DP, 3>(p, run, o_lds[0], R * DP, &sums_lds[0][0][0], R * 3, p.rows, 0, lse_lds[run.together ? 0 : wave]);
+  if (p.kept != nullptr && p.lse == nullptr) put_own_weights(p, run, lse_lds[run.together ? 0 : wave]);
 }
 
 // The run results of one row of (b, i, h).
@@ -773,7 +827,6 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
   const int b = unit / p.Hk, hk = unit % p.Hk, n = p.c.length(b);
   const int slot0 = id % per_row * (4 * kThreads), slot = slot0 + 4 * tid;
   v4f sum = zero4();
-  const float* const kept = p.kept + static_cast<int64_t>(unit) * p.rows * p.slots_kept + slot;
   for (int r0 = 0; r0 < p.rows && slot0 < n; r0 += kRowTile) {
     const int rows = min(kRowTile, p.rows - r0);
     if (r0 > 0) __syncthreads();
@@ -804,33 +857,9 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
       if (d8 == 0) lse_lds[r] = lse;
     }
     __syncthreads();
-    if (slot < n) {
-#pragma unroll 4
-      for (int r = 0; r < rows; ++r) {
-        const v4f x = *reinterpret_cast<const v4f*>(kept + (r0 + r) * p.slots_kept);
-        const float lse = lse_lds[r];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += fast_exp2(x[e] - lse);
-      }
-    }
+    if (slot < n) add_kept(p, unit, slot, lse_lds, r0, rows, sum);
   }
-  if (slot >= p.c.slots) return;
-  const int64_t at = static_cast<int64_t>(unit) * p.c.slots + slot;
-  if (slot + 4 <= p.c.slots && p.c.slots % 4 == 0) {
-    v4f x = zero4();
-    if (slot < n && p.scores != nullptr) x = p.decay * *reinterpret_cast<const v4f*>(p.scores + at);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = slot + e < n ? x[e] + sum[e] : 0.f;
-    *reinterpret_cast<v4f*>(p.scores_out + at) = x;
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (slot + e >= p.c.slots) break;
-    float x = 0.f;
-    if (slot + e < n) x = sum[e] + (p.scores != nullptr ? p.decay * p.scores[at + e] : 0.f);
-    p.scores_out[at + e] = x;
-  }
+  if (slot < p.c.slots) put_weights(p, unit, n, slot, sum);
 }
 
 // Workgroups that fill the card: the rows are divided so that there are about kFill, three for each place of most kernels (half as many
@@ -838,10 +867,16 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
 // they are as few as kLeast (16 x 8192 float32 slots of 8 heads of 128: 150 us, 178 by kFill alone).
 // Where there are rows of key heads for all its waves, kAlone, each wave has one to itself and shares nothing
 // (paged_walkers_f32 84 -> 67 us).
-constexpr int64_t kFill = 1536, kLeast = 512, kAlone = 2048;
+// Rows of at most kWhole slots, by the width of their page table, or twice as many where there is a workgroup for each of the card's
+// units, are not divided: no table of runs, and no second kernel, as a run adds up its own weights (512 rows of up to 225 slots of 8
+// float32 heads of 64: 48 us, 60 with three kernels; 64 of 900 of bfloat16: 20, 25; 32 of 1000: 20, 27). Below a workgroup a unit, 4
+// rows of 450 take 8.9 us, or 9.9 in two kernels, and a launch less; of 777 11.7, or 10.0; 20 of 1000 of bfloat16 16.9, or 14.0. float32 on
+// the matrix cores takes twice the time a slot (4 rows of 500 of heads of 128: 22, or 15), so half as many.
+constexpr int64_t kFill = 1536, kLeast = 512, kAlone = 2048, kWhole = 512, kUnits = 256;
 
 struct Layout {
   int64_t rows, block, blocks, waves, step, runs_wanted, runs_fill, runs, slots_kept, partial, stats, kept, lse, plan, total;
+  bool whole, table, finish_weights;  // each row is one run; a table of the runs; weights by the second kernel
 };
 
 // Rows of query and head in a workgroup's products: 16, or 32 where there are more; float32 heads of more than 64 elements have
@@ -854,7 +889,8 @@ Layout layout(const hz_paged_attention_args& a) {
   w.rows = a.Nq * (a.H / c.Hk);
   w.block = w.rows <= 16 || (c.dtype == HZ_DTYPE_F32 && c.D > 64) ? 16 : 32;
   w.blocks = (w.rows + w.block - 1) / w.block;
-  w.waves = c.B * c.Hk * w.blocks >= kAlone ? 1 : 4;
+  const int64_t units = c.B * c.Hk * w.blocks;
+  w.waves = units >= kAlone ? 1 : 4;
   w.step = w.waves * kBlock;
   const int64_t wanted = (w.waves == 1 ? kAlone : kFill) / (c.Hk * w.blocks), longest = (slots + w.step - 1) / w.step;
   w.runs_wanted = wanted > 1 ? wanted : 1;
@@ -862,19 +898,23 @@ Layout layout(const hz_paged_attention_args& a) {
   w.runs_fill = fill > 1 ? fill : 1;
   // runs are at least (all lengths) / wanted and step long: each row has one, and all together less than `wanted` more
   const int64_t most = c.B * longest;
-  w.runs = w.runs_wanted + c.B < most ? w.runs_wanted + c.B : most;
+  const bool in_parts = c.dtype == HZ_DTYPE_F32 && w.rows > 2;  // float32 on the matrix cores
+  w.whole = slots <= (units >= kUnits ? 2 * kWhole : in_parts ? kWhole / 2 : kWhole);
+  w.runs = w.whole ? c.B : w.runs_wanted + c.B < most ? w.runs_wanted + c.B : most;
   auto take = [&](int64_t floats) {
     const int64_t at = w.total;
     w.total += (floats + 3) / 4 * 4;
     return at;
   };
-  w.partial = take(w.runs * c.Hk * w.rows * c.D);
-  w.stats = take(w.runs * c.Hk * w.rows * 4);
-  w.plan = take(c.B > kPlanRows ? 2 + (c.B + 1) / 2 * 2 + 2 * (w.runs - c.B) : 0);
+  w.partial = take(w.whole ? 0 : w.runs * c.Hk * w.rows * c.D);
+  w.stats = take(w.whole ? 0 : w.runs * c.Hk * w.rows * 4);
+  w.table = !w.whole && c.B > kPlanRows;
+  w.plan = take(w.table ? 2 + (c.B + 1) / 2 * 2 + 2 * (w.runs - c.B) : 0);
   w.slots_kept = (slots + kBlock - 1) / kBlock * kBlock;
   if (a.scores_out != nullptr) {
     w.kept = take(c.B * c.Hk * w.rows * w.slots_kept);
-    w.lse = take(c.B * a.Nq * a.H);
+    w.finish_weights = !w.whole || w.blocks > 1;
+    w.lse = take(w.finish_weights ? c.B * a.Nq * a.H : 0);
   }
   return w;
 }
@@ -887,26 +927,27 @@ hipError_t run(const hz_paged_attention_args& a, void* workspace, hipStream_t st
   const bool want = a.scores_out != nullptr;
   const bool capped = a.softcap > 0.f;
   PagedParams p{Pages(c), a.q, a.out, a.slopes, a.scores, a.scores_out, ws + w.partial, ws + w.stats,
-                want ? ws + w.kept : nullptr, want ? ws + w.lse : nullptr, static_cast<int>(c.B), static_cast<int>(a.Nq),
+                want ? ws + w.kept : nullptr, w.finish_weights ? ws + w.lse : nullptr, static_cast<int>(c.B), static_cast<int>(a.Nq),
                 static_cast<int>(a.H), static_cast<int>(c.Hk), static_cast<int>(a.H / c.Hk), static_cast<int>(c.D),
                 static_cast<int>(w.rows), static_cast<int>(w.blocks), w.slots_kept, w.runs_wanted, w.runs_fill,
-                c.B > kPlanRows ? reinterpret_cast<int*>(ws + w.plan) : nullptr, static_cast<int>(w.waves), static_cast<int>(w.step), a.softcap,
+                w.table ? reinterpret_cast<int*>(ws + w.plan) : nullptr, static_cast<int>(w.waves), static_cast<int>(w.step), w.whole, a.softcap,
                 capped ? a.scale / a.softcap : 0.f, (capped ? a.softcap : a.scale) * kLog2e, a.decay};
-  const unsigned grid = static_cast<unsigned>((w.runs * c.Hk * w.blocks * w.waves + 3) / 4);
-  if (c.B > kPlanRows) paged_plan_kernel<<<1, 1024, 0, stream>>>(p, reinterpret_cast<int*>(ws + w.plan));
+  const unsigned grid = static_cast<unsigned>(w.waves > 1 ? w.runs * c.Hk * w.blocks : (w.runs * c.Hk * w.blocks + 3) / 4);
+  if (w.table) paged_plan_kernel<<<1, 1024, 0, stream>>>(p, reinterpret_cast<int*>(ws + w.plan));
   auto attend = [&](auto reads) {
+    constexpr Reads READS = reads.value;
     if constexpr (PARTS == 3)
       if (w.rows <= 2) {
         if (w.rows == 1)
-          paged_rows_kernel<DP, CAP, 1, reads.value><<<grid, kThreads, 0, stream>>>(p);
+          paged_rows_kernel<DP, CAP, 1, READS><<<grid, kThreads, 0, stream>>>(p);
         else
-          paged_rows_kernel<DP, CAP, 2, reads.value><<<grid, kThreads, 0, stream>>>(p);
+          paged_rows_kernel<DP, CAP, 2, READS><<<grid, kThreads, 0, stream>>>(p);
         return;
       }
     if (w.block == 16)
-      paged_attention_kernel<DP, PARTS, CAP, 1, reads.value><<<grid, kThreads, 0, stream>>>(p);
+      paged_attention_kernel<DP, PARTS, CAP, 1, READS><<<grid, kThreads, 0, stream>>>(p);
     else if constexpr (PARTS == 1 || DP < 128)
-      paged_attention_kernel<DP, PARTS, CAP, 2, reads.value><<<grid, kThreads, 0, stream>>>(p);
+      paged_attention_kernel<DP, PARTS, CAP, 2, READS><<<grid, kThreads, 0, stream>>>(p);
   };
   // sixteen slots as a buffer: one behind the other, apart, within 31 bits
   const int64_t least = c.k.token < c.v.token ? c.k.token : c.v.token, most = c.k.token > c.v.token ? c.k.token : c.v.token;
@@ -916,11 +957,11 @@ hipError_t run(const hz_paged_attention_args& a, void* workspace, hipStream_t st
     attend(std::integral_constant<Reads, kCached>{});
   else if constexpr (PARTS == 1)
     attend(std::integral_constant<Reads, kOnce>{});
-  const int64_t outputs = w.runs > c.B ? c.B * a.Nq * a.H : 0;  // where a row may have several runs
+  const int64_t outputs = !w.whole && w.runs > c.B ? c.B * a.Nq * a.H : 0;  // where a row may have several runs
   const int lanes = outputs * ((c.D + 31) / 32) <= 1024 ? 8 : 32;
   const int64_t units = lanes == 8 ? outputs * ((c.D + 31) / 32) : outputs;
   const int joins = static_cast<int>(units < 2048 ? units : 2048), per_row = (p.c.slots + 4 * kThreads - 1) / (4 * kThreads);
-  const int64_t finish = joins + (want ? c.B * c.Hk * per_row : 0);
+  const int64_t finish = joins + (w.finish_weights ? c.B * c.Hk * per_row : 0);
   if (finish > 0) paged_finish_kernel<PARTS><<<static_cast<unsigned>(finish), kThreads, 0, stream>>>(p, joins, lanes, per_row);
   return hipGetLastError();
 }
