@@ -210,6 +210,13 @@ ATTENTION = [  # B, Nq, H, Hk, D, S, lengths, options
     (4, 1, 4, 2, 128, 5, [200, 100, 37, 5], dict(bad=True, scores=True, softcap=9.0)),
     (2, 1, 128, 1, 16, 16, [77, 20], dict(scores=True)),
     (2, 1, 70, 1, 128, 16, [77, 20], dict(scores=True)),
+    (70, 1, 2, 2, 32, 16, "ragged90", dict(scores=True, wide=1200)),
+    (300, 2, 8, 8, 16, 32, "ragged70", dict(scores=True, wide=1100)),
+    (260, 1, 8, 8, 32, 7, "one long", dict(scores=True)),
+    (2, 1, 4, 4, 64, 16, [700, 1], dict(scores=True, wide=800)),
+    (3, 2, 2, 2, 128, 16, [600, 90, 0], dict(scores=True, slopes=True, wide=800)),
+    (2, 1, 4, 4, 40, 7, [700, 530], dict(scores=True, softcap=4.0)),
+    (3, 2, 3, 3, 64, 9, [512, 511, 2], dict(scores=True, bad=True)),
 ]
 
 
@@ -232,7 +239,7 @@ def test_attention(case, dtype):
     g = gen(11)
     dt = DT[dtype]
     lengths = lengths_of(lengths, B)
-    slots = max(max(lengths), 1) + 5
+    slots = max(max(lengths), 1, o.get("wide", 0)) + 5
     k, v, table, n = rows(g, B, slots, S, Hk, D, dt, lengths, o.get("layout", "plain"), o.get("shared", 0), o.get("bad", False))
     q = normal(g, B, Nq, H, D, dtype=dt, std=2.0)
     kw = dict(softcap=o.get("softcap", 0.0))
