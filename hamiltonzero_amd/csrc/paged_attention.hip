@@ -840,16 +840,24 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
       } else {
         const Runs runs(p, plan, b, n, hk, r0 + r);
         float m = kNegInf, exact = 0.f;
-#pragma unroll 4
-        for (int x = d8; x < runs.count; x += 8) m = fmaxf(m, p.stats[runs.at(x) * 4]);
+        for (int x0 = d8; x0 < runs.count; x0 += 64) {  // eight loads under way
+          v4f st[8];
 #pragma unroll
-        for (int x = 1; x < 8; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-        const float base = m == kNegInf ? 0.f : m;
-#pragma unroll 4
-        for (int x = d8; x < runs.count; x += 8) {
-          const v4f st = *reinterpret_cast<const v4f*>(p.stats + runs.at(x) * 4);
-          exact += fast_exp2(st[0] - base) * st[2];
+          for (int x = 0; x < 8; ++x) st[x] = *reinterpret_cast<const v4f*>(p.stats + runs.at(min(x0 + 8 * x, runs.count - 1)) * 4);
+          float now = m;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) now = fmaxf(now, st[x][0]);
+          const float base = now == kNegInf ? 0.f : now;
+          exact *= fast_exp2(m - base);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) exact += x0 + 8 * x < runs.count ? fast_exp2(st[x][0] - base) * st[x][2] : 0.f;
+          m = now;
         }
+        float now = m;
+#pragma unroll
+        for (int x = 1; x < 8; x <<= 1) now = fmaxf(now, __shfl_xor(now, x, 64));
+        exact *= fast_exp2(m - (now == kNegInf ? 0.f : now));
+        m = now;
 #pragma unroll
         for (int x = 1; x < 8; x <<= 1) exact += __shfl_xor(exact, x, 64);
         lse = exact > 0.f ? m + log2f(exact) : 0.f;
