@@ -299,6 +299,34 @@ def test_attention_weights_at_large_scores():
         within("scores", new, want["scores"], want["t_scores"])
 
 
+@pytest.mark.parametrize("heads", [2, 8], ids=["row", "rows"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("length", [90, 7000])
+def test_attention_passes_nan_on(length, dtype, heads):
+    """A NaN that a query attends to reaches its outputs and weights, wherever in a long row it lies, and nothing else."""
+    _say(f"nan {length} {dtype} {heads}")
+    g = gen(15)
+    k, v, table, n = rows(g, 2, length, 16, 2, 64, DT[dtype], [length, length - 1])
+    q = normal(g, 2, 1, heads, 64, dtype=DT[dtype])
+    scores = torch.zeros(2, 2, table.shape[1] * 16, device="cuda")
+    clean, weights = hz.paged_attention(q, k, v, table, n, scores=scores)
+    G = heads // 2
+    for first, last in ((0, 64), (length - 20, length - 4), (0, length)):
+        bad = k.clone()
+        for s in range(first, last):
+            bad[int(table[0, s // 16]), s % 16, 1, 7] = float("nan")
+        out, new = hz.paged_attention(q, bad, v, table, n, scores=scores)
+        assert out[0, :, G:].isnan().all() and torch.equal(out[0, :, :G], clean[0, :, :G]) and torch.equal(out[1], clean[1])
+        assert new[0, 1, :length].isnan().all() and torch.equal(new[0, 0], weights[0, 0]) and torch.equal(new[1], weights[1])
+        bad = v.clone()
+        for s in range(first, last):
+            bad[int(table[0, s // 16]), s % 16, 1, 7] = float("nan")
+        out, new = hz.paged_attention(q, k, bad, table, n, scores=scores)
+        gone = torch.zeros_like(out, dtype=torch.bool)
+        gone[0, :, G:, 7] = True
+        assert torch.equal(out.isnan(), gone) and torch.equal(out[~gone], clean[~gone]) and torch.equal(new, weights)
+
+
 def test_attention_behind_two_to_the_31():
     """Offsets of slots beyond 32 bits of elements: pages 2^31 elements apart."""
     g = gen(14)
