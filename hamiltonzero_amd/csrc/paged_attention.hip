@@ -773,7 +773,7 @@ struct Runs {
 
 // Behind the attention, in one launch. Workgroups 0 .. joins - 1 join the runs of rows that have several: 4 * lanes elements of a row of
 // (b, i, h) at a time, 256 / lanes ways taking the runs in turn. lanes 8, four workgroups to a row of 128
-// elements, where there are few rows (122 runs of 96 rows 7 us, 12 with a workgroup a row); else 32 (12 runs of 512 rows 6 us,
+// elements, where there are few rows (115 runs of 96 rows 6.6 us, 12 with a workgroup a row); else 32 (12 runs of 512 rows 5.7 us,
 // 9 with four). The others add up the weights that each slot has had, 1024 slots of a row and key head a workgroup,
 // four a thread.
 constexpr int kRowTile = 64;
