@@ -5,13 +5,13 @@
 // chosen so that both elements of each rotated pair are in one lane and no lane exchanges data but
 // for the sum of squares: with half-split pairs lane t holds elements 4 t .. 4 t + 3 and
 // n_freqs + 4 t .. + 3, with interleaved ones (and behind the rotated part) 8 t .. 8 t + 7. Either
-// way it turns pairs 4 t .. 4 t + 3. A workgroup takes up to four tokens at a time: it forms their angles
+// way it turns pairs 4 t .. 4 t + 3. A workgroup takes a few tokens at a time: it forms their angles
 // once, in float64 turns (an angle at position 10^5 has no bits to lose in float32's 24), puts the sines
-// and cosines into LDS, and then runs over the tokens' query and key heads, the next one's data in flight
-// while one is normalised.
+// and cosines into LDS, and then runs over the tokens' query and key heads, the next ones' data in flight
+// while one is normalised. With several axes each pair has its axis' position; the rest is the same.
 // x is read and y written once; the backward reads x and dy and writes dx. float32: bound by those bytes (256 x 225 tokens of 16
-// heads of 64: 107 to 116 us, 151 in reverse mode, 4.8 TB/s); bfloat16: by vector instructions beside them, issued 98% of the time (4 x
-// 4096 tokens of 40 heads of 128: 90 us, 3.7 TB/s, and 119 us, 4.2 TB/s).
+// heads of 64: 112 us, 5.0 TB/s, and 140 in reverse mode, 5.2 TB/s); bfloat16: by vector instructions beside them (4 x
+// 4096 tokens of 40 heads of 128: 84 us, 4.0 TB/s, and 117 us, 4.3 TB/s).
 #include "mhsea_device.h"
 #include "paged_launch.h"
 #include "token_launch.h"
@@ -20,7 +20,7 @@ namespace hz {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 16;     // a workgroup at a time, forward
+constexpr int kMaxTokens = 16;    // a workgroup at a time, forward
 constexpr int kMaxTokensBwd = 4;   // and backward
 constexpr int kMaxBlocks = 1024;  // of the backward: rows of partial weight gradients
 
@@ -193,9 +193,10 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p)
   }
 }
 
-// q and k: the forward's inputs; qo and ko: the cotangents. partial: [gridDim.x][2][D].
+// q and k: the forward's inputs; qo and ko: the cotangents. partial: [gridDim.x][2][D]. Four workgroups a CU, so that all of the grid are
+// there at once (float32 had registers for three: 157 us for 256 x 225 tokens of 16 heads of 64, 140 with four).
 template <class S, int GS, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) norm_rotary_bwd_kernel(NormParams p, void* dq, void* dk, float* partial) {
+__global__ void __launch_bounds__(kThreads, 4) norm_rotary_bwd_kernel(NormParams p, void* dq, void* dk, float* partial) {
   __shared__ Angles angles[kMaxTokensBwd];
   __shared__ float red[kThreads * 8];
   constexpr int SLOTS = kThreads / GS;
