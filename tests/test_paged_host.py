@@ -150,7 +150,8 @@ def test_abi_refuses_attention(lib, over, code, text):
 def test_abi_refuses_caps_of_bfloat16_and_short_workspaces(lib):
     a = cache(dict(dtype=1)) + _native.PAGED_ATTENTION_REST.pack(*flat(changed(ATTN, dict(softcap=8193.0))))
     refused(lib.hz_paged_attention(None, a, A, 1 << 40), E, "softcap", lib)
-    a = cache() + _native.PAGED_ATTENTION_REST.pack(*flat(ATTN))
+    assert lib.hz_paged_attention_workspace(cache() + _native.PAGED_ATTENTION_REST.pack(*flat(ATTN))) == 0  # short rows need none
+    a = cache(dict(page_size=512)) + _native.PAGED_ATTENTION_REST.pack(*flat(ATTN))
     size = lib.hz_paged_attention_workspace(a)
     assert size > 0
     refused(lib.hz_paged_attention(None, a, A, size - 1), E, "workspace", lib)
