@@ -223,11 +223,11 @@ def feed(s, g, i, side=5):
     s["pos"][:, :, 0], s["pos"][:, :, 1] = i // side, i % side
 
 
-@pytest.mark.parametrize("B", [3, 70])
-def test_captured_steps_follow_rows_that_grow(B):
+@pytest.mark.parametrize("B,T", [(3, 7), (70, 7), (3, 30), (70, 30)])
+def test_captured_steps_follow_rows_that_grow(B, T):
     """Two graphs of the same step with a pool of their own, replayed in turn with eager steps between; rows grow through the replays, so the
     division of the rows changes under the captured launches. Every step against an eager twin."""
-    dims = dict(B=B, T=7, S=48, H=4, Hk=2, D=64)
+    dims = dict(B=B, T=T, S=48, H=4, Hk=2, D=64)
     eager, graphed = (new_state(gen(4), torch.bfloat16, **dims) for _ in range(2))
     warm = torch.cuda.Stream()
     with torch.cuda.stream(warm), torch.no_grad():
@@ -246,9 +246,9 @@ def test_captured_steps_follow_rows_that_grow(B):
     a, b = gen(5), gen(5)
     for i in range(40):
         feed(eager, a, i), feed(graphed, b, i)
-        jump = 1 if i % 5 else 37  # many slots at once: what they hold is the pool's numbers
+        jump = 1 if i % 5 else 37 if T == 7 else 200  # many slots at once: what they hold is the pool's numbers
         for s in (eager, graphed):
-            s["n"].add_(jump).clamp_(max=7 * 48)
+            s["n"].add_(jump).clamp_(max=T * 48)
         with torch.no_grad():
             want = decode_step(eager)
         if i % 7 == 3:
