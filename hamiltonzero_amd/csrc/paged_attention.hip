@@ -22,6 +22,7 @@ using namespace token;
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 32;  // slots of a wave's step
+constexpr int kKept = 16;   // slots whose scores are kept row by row
 
 struct PagedParams {
   Pages c;
@@ -31,7 +32,7 @@ struct PagedParams {
   float* scores_out;
   float *partial, *stats, *kept, *lse;  // workspace: see layout()
   int B, Nq, H, Hk, G, D, rows, blocks;  // rows: Nq G; blocks of 16 or 32 of them
-  int64_t blocks_kept;                   // of a row's kept scores: blocks of 32 slots
+  int64_t blocks_kept;                   // of a row's kept scores: blocks of kKept slots
   int64_t runs_wanted, runs_fill;        // for one key head and block of rows, over all batch rows: at most, and to fill the card
   const int* plan;                       // of more than 64 batch rows
   int waves, step;                       // waves of a run; slots that they take at a time, of which runs are multiples
@@ -157,10 +158,11 @@ __device__ __forceinline__ int64_t result_at(const PagedParams& p, int at, int h
   return (static_cast<int64_t>(at) * p.Hk + hk) * p.rows + r;
 }
 
-// Where row r's score of a slot is kept: a block's rows one behind the other, as a wave writes them at once and they are read (a row's
-// slots one behind the other: 512 rows of up to 1800 slots 23.3 us to read, 21.0 so; 131072 slots of 16 rows 53.0 us to write and attend, 51.5).
+// Where row r's score of a slot is kept: sixteen slots' rows one behind the other, which is what a wave's store writes (a row's
+// slots one behind the other: 512 rows of up to 1800 slots 23.3 us to read, 21.0 so; 131072 slots of 24 rows 60.9 us to attend and
+// write, 59.5, by 32 slots 60.1).
 __device__ __forceinline__ int64_t kept_at(const PagedParams& p, int unit, int r, int slot) {
-  return ((unit * p.blocks_kept + slot / kBlock) * p.rows + r) * kBlock + slot % kBlock;
+  return ((unit * p.blocks_kept + slot / kKept) * p.rows + r) * kKept + slot % kKept;
 }
 
 __device__ __forceinline__ void wave_fence() {
@@ -432,7 +434,7 @@ __device__ __forceinline__ void add_kept(const PagedParams& p, int unit, int slo
   const float* const kept = p.kept + kept_at(p, unit, r0, slot);
 #pragma unroll 4
   for (int r = 0; r < rows; ++r) {
-    const v4f x = *reinterpret_cast<const v4f*>(kept + r * kBlock);
+    const v4f x = *reinterpret_cast<const v4f*>(kept + r * kKept);
     const float base = lse[r];
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] += fast_exp2(x[e] - base);
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
       if (p.kept != nullptr && r0 + 16 * cb + c < p.rows) {
         float* const to = p.kept + kept_at(p, b * p.Hk + hk, row[cb], k1);
         *reinterpret_cast<v4f*>(to) = v4f{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<v4f*>(to + 16) = v4f{x[4], x[5], x[6], x[7]};
+        *reinterpret_cast<v4f*>(to + kKept * p.rows) = v4f{x[4], x[5], x[6], x[7]};
       }
       top = group_max(top);
       if (__any(top > m[cb])) {
@@ -895,7 +897,7 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
 // take 16% longer where rows are long, paged_token_long_bf16; twice as many 3%). While a workgroup's run is below kLong steps
 // they are as few as kLeast (16 x 8192 float32 slots of 8 heads of 128: 150 us, 178 by kFill alone).
 // Where there are rows of key heads for all its waves, kAlone, each wave has one to itself and shares nothing
-// (paged_walkers_f32 84 -> 67 us).
+// (512 rows of up to 225 float32 slots of 8 heads of 64: 75 -> 62 us).
 // Rows of at most kWhole slots, by the width of their page table, or twice as many where there is a workgroup for each of the card's
 // units, are not divided: no table of runs, and no second kernel, as a run adds up its own weights (512 rows of up to 225 slots of 8
 // float32 heads of 64: 48 us, 60 with three kernels; 64 of 900 of bfloat16: 20, 25; 32 of 1000: 20, 27). Below a workgroup a unit, 4
@@ -939,9 +941,9 @@ Layout layout(const hz_paged_attention_args& a) {
   w.stats = take(w.whole ? 0 : w.runs * c.Hk * w.rows * 4);
   w.table = !w.whole && c.B > kPlanRows;
   w.plan = take(w.table ? 2 + (c.B + 1) / 2 * 2 + 2 * (w.runs - c.B) : 0);
-  w.blocks_kept = (slots + kBlock - 1) / kBlock;
+  w.blocks_kept = (slots + kBlock - 1) / kBlock * (kBlock / kKept);
   if (a.scores_out != nullptr) {
-    w.kept = take(c.B * c.Hk * w.rows * w.blocks_kept * kBlock);
+    w.kept = take(c.B * c.Hk * w.rows * w.blocks_kept * kKept);
     w.finish_weights = !w.whole || w.blocks > 1;
     w.lse = take(w.finish_weights ? c.B * a.Nq * a.H : 0);
   }
