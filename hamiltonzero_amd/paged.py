@@ -90,8 +90,9 @@ def _no_grad(*tensors: Optional[Tensor]) -> None:
 def paged_append(k_cache: Tensor, v_cache: Tensor, k: Tensor, v: Tensor, page_table: Tensor, lengths: Tensor) -> None:
     """Writes the N new tokens ``k, v [B, N, Hk, D]`` of each row into its last slots: token i of row b into slot
     ``lengths[b] - N + i`` (``lengths`` count the new tokens already). Tokens of negative slots (the padded front of a prompt that is
-    shorter than N) are left out; where a length is more than the table's slots, the row's last slots take the new tokens. ``k`` and ``v`` may be strided views; they must not overlap the caches, and no page
-    may take two rows' new tokens at one slot."""
+    shorter than N) are left out; where a length is more than the table's slots, the row's last slots take the new
+    tokens. ``k`` and ``v`` may be strided views; they must not overlap the caches, and no page may take two rows' new
+    tokens at one slot."""
     args, (B, _, Hk, D) = _cache(k_cache, v_cache, page_table, lengths)
     _check_first("k", k, "[B, N, Hk, D]")
     N = k.shape[1]
