@@ -239,9 +239,11 @@ struct Lanes {
 
 // Pages of a multiple of 16 slots: sixteen slots lie one behind the other. Each half of a block is a buffer whose end the
 // hardware checks: base and end are scalars, a lane's offset never changes, and no address is formed in vector registers.
-// ONCE: past the caches (a long bfloat16 cache 10% faster, paged_token_long_bf16 267 -> 241 us); not for pages that rows share (the same
+// kOnce, kApartOnce: past the caches (a long bfloat16 cache 10% faster, paged_token_long_bf16 267 -> 241 us, in pages of 100 slots 268 -> 241,
+// of one slot 279 -> 253); not for pages that rows share (the same
 // with four fifths of its pages shared 155 us from the caches, 229 past them) and float32 (16 x 8192 slots of 8 heads of 128: 203 us, 214).
-enum Reads { kApart, kCached, kOnce };
+enum Reads { kApart, kCached, kOnce, kApartOnce };
+constexpr bool apart(Reads reads) { return reads == kApart || reads == kApartOnce; }
 template <int DP, int PARTS, Reads READS>
 struct Slots : Lanes<DP, PARTS> {
   typedef Lanes<DP, PARTS> L;
@@ -317,15 +319,15 @@ struct Slots : Lanes<DP, PARTS> {
 };
 
 // Other pages: every slot is looked up by a lane of its own, and its offsets go to the others through LDS.
-template <int DP, int PARTS>
-struct Slots<DP, PARTS, kApart> : Lanes<DP, PARTS> {
+template <int DP, int PARTS, bool ONCE>
+struct SlotsApart : Lanes<DP, PARTS> {
   typedef Lanes<DP, PARTS> L;
   const PagedParams& p;
   const int32_t* table;
   int hk, stop, lane, page_then;
   int64_t (*where)[kBlock][2];  // two blocks' offsets of keys and values; -1: no page
 
-  __device__ __forceinline__ Slots(const PagedParams& p_, const int32_t* table_, int hk_, int stop_, int lane_, int64_t (*where_)[kBlock][2])
+  __device__ __forceinline__ SlotsApart(const PagedParams& p_, const int32_t* table_, int hk_, int stop_, int lane_, int64_t (*where_)[kBlock][2])
       : p(p_), table(table_), hk(hk_), stop(stop_), lane(lane_), where(where_) {}
   __device__ __forceinline__ void look(int k0) {
     const int slot = k0 + (lane & 31);
@@ -341,6 +343,12 @@ struct Slots<DP, PARTS, kApart> : Lanes<DP, PARTS> {
     wave_fence();
     return static_cast<uint32_t>(__ballot(known));
   }
+  __device__ __forceinline__ static void one(Raw8<PARTS>& r, const void* base, int64_t at, bool on) {
+    if constexpr (ONCE)
+      r.u = on ? __builtin_nontemporal_load(reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(base) + at)) : v4u{0u, 0u, 0u, 0u};
+    else
+      r.load(base, at, on);
+  }
   __device__ __forceinline__ void load_k(Raw8<PARTS> (&rk)[2][L::DS], int buffer) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -348,7 +356,7 @@ struct Slots<DP, PARTS, kApart> : Lanes<DP, PARTS> {
       for (int s = 0; s < L::DS; ++s) {
         const int64_t at = where[buffer][16 * i + L::key_row(lane, s)][0];
         const int d = L::key_element(lane, s);
-        rk[i][s].load(p.c.k, at + hk * p.c.head_k + d, at >= 0 && d < p.D);
+        one(rk[i][s], p.c.k, at + hk * p.c.head_k + d, at >= 0 && d < p.D);
       }
   }
   __device__ __forceinline__ void load_v(Raw8<PARTS> (&rv)[L::LOADS], int buffer) const {
@@ -356,9 +364,17 @@ struct Slots<DP, PARTS, kApart> : Lanes<DP, PARTS> {
     for (int j = 0; j < L::LOADS; ++j) {
       const int64_t at = where[buffer][lane / L::CH + L::STEP * j][1];
       const int d = lane % L::CH * 8;
-      rv[j].load(p.c.v, at + hk * p.c.head_v + d, at >= 0 && d < p.D);
+      one(rv[j], p.c.v, at + hk * p.c.head_v + d, at >= 0 && d < p.D);
     }
   }
+};
+template <int DP, int PARTS>
+struct Slots<DP, PARTS, kApart> : SlotsApart<DP, PARTS, false> {
+  using SlotsApart<DP, PARTS, false>::SlotsApart;
+};
+template <int DP>
+struct Slots<DP, 1, kApartOnce> : SlotsApart<DP, 1, true> {
+  using SlotsApart<DP, 1, true>::SlotsApart;
 };
 
 // A run of slots and who has it. waves 4: the workgroup; waves 1: each wave one of its own, and they share nothing.
@@ -482,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
   constexpr int DS = S::DS, DT = DP / 16, CH = S::CH, LOADS = S::LOADS, STEP = S::STEP;
   typedef Values<DP, PARTS> V;
   __shared__ __align__(16) typename V::Element v_lds[4][kBlock * DP];
-  __shared__ __align__(16) int64_t where_lds[READS == kApart ? 4 : 1][2][kBlock][2];
+  __shared__ __align__(16) int64_t where_lds[apart(READS) ? 4 : 1][2][kBlock][2];
   __shared__ float sums_lds[4][16 * CB][3], lse_lds[4][16 * CB];  // each wave's base, sum and sum of unrounded weights
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const V vt{v_lds[wave]};
@@ -517,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     for (int dt = 0; dt < DT; ++dt) o[cb][dt] = zero4();
   }
 
-  S slots(p, run.table, hk, stop, lane, where_lds[READS == kApart ? wave : 0]);
+  S slots(p, run.table, hk, stop, lane, where_lds[apart(READS) ? wave : 0]);
   const int lr = lane / CH, lc = lane % CH;
   Raw8<PARTS> rk[2][DS], rv[LOADS];
   uint32_t known = 0, known_next = 0;  // slots of the block at hand, and of the next, that lie in a page
@@ -629,7 +645,7 @@ template <int DP, bool CAP, int R, Reads READS>
 __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(PagedParams p) {
   typedef Slots<DP, 3, READS> S;
   constexpr int DS = S::DS, CH = S::CH, LOADS = S::LOADS, STEP = S::STEP;
-  __shared__ __align__(16) int64_t where_lds[READS == kApart ? 4 : 1][2][kBlock][2];
+  __shared__ __align__(16) int64_t where_lds[apart(READS) ? 4 : 1][2][kBlock][2];
   __shared__ __align__(16) float w_lds[4][R][kBlock], o_lds[4][R * DP];
   __shared__ float sums_lds[4][R][3], lse_lds[4][R];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -655,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
   float o[R][8] = {}, m[R], l[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) m[r] = kNegInf, l[r] = 0.f;
-  S slots(p, run.table, hk, stop, lane, where_lds[READS == kApart ? wave : 0]);
+  S slots(p, run.table, hk, stop, lane, where_lds[apart(READS) ? wave : 0]);
   const int lr = lane / CH, lc = lane % CH;
   Raw8<3> rk[2][DS], rv[LOADS];
   uint32_t known = 0, known_next = 0;
@@ -982,12 +998,12 @@ hipError_t run(const hz_paged_attention_args& a, void* workspace, hipStream_t st
   };
   // sixteen slots as a buffer: one behind the other, apart, within 31 bits
   const int64_t least = c.k.token < c.v.token ? c.k.token : c.v.token, most = c.k.token > c.v.token ? c.k.token : c.v.token;
-  if (c.page_size % 16 != 0 || least < c.D || most >= int64_t(1) << 24)
-    attend(std::integral_constant<Reads, kApart>{});
-  else if (PARTS == 3 || c.B * c.table_width > c.pages || w.blocks > 1)
-    attend(std::integral_constant<Reads, kCached>{});
+  const bool buffers = c.page_size % 16 == 0 && least >= c.D && most < int64_t(1) << 24;
+  const bool once = PARTS == 1 && c.B * c.table_width <= c.pages && w.blocks == 1;
+  if (!once)
+    buffers ? attend(std::integral_constant<Reads, kCached>{}) : attend(std::integral_constant<Reads, kApart>{});
   else if constexpr (PARTS == 1)
-    attend(std::integral_constant<Reads, kOnce>{});
+    buffers ? attend(std::integral_constant<Reads, kOnce>{}) : attend(std::integral_constant<Reads, kApartOnce>{});
   const int64_t outputs = !w.whole && w.runs > c.B ? c.B * a.Nq * a.H : 0;  // where a row may have several runs
   const int lanes = outputs * ((c.D + 31) / 32) <= 1024 ? 8 : 32;
   const int64_t units = lanes == 8 ? outputs * ((c.D + 31) / 32) : outputs;
