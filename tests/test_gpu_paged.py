@@ -217,6 +217,8 @@ ATTENTION = [  # B, Nq, H, Hk, D, S, lengths, options
     (3, 2, 2, 2, 128, 16, [600, 90, 0], dict(scores=True, slopes=True, wide=800)),
     (2, 1, 4, 4, 40, 7, [700, 530], dict(scores=True, softcap=4.0)),
     (3, 2, 3, 3, 64, 9, [512, 511, 2], dict(scores=True, bad=True)),
+    (2, 1, 128, 1, 48, 9, [77, 20], dict(scores=True, softcap=6.0)),
+    (2, 20, 4, 2, 128, 9, [700, 20], dict(slopes=True, bad=True)),
 ]
 
 
