@@ -233,9 +233,14 @@ __global__ void __launch_bounds__(THREADS) paged_cut_kernel(EvictParams p) {
     uint32_t threshold = 0;
     for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1) {
       int reach = 0;
+      if constexpr (KEYS <= 4) {  // a scalar count a key: 20.2 -> 19.6 us for 2048 rows of four keys a lane, 10.0 -> 11.1 for 32 of sixteen
 #pragma unroll
-      for (int j = 0; j < KEYS; ++j) reach += u[j] >= (threshold | bit) ? 1 : 0;
-      reach = wave_sum(reach);
+        for (int j = 0; j < KEYS; ++j) reach += bits(__ballot(u[j] >= (threshold | bit)));
+      } else {
+#pragma unroll
+        for (int j = 0; j < KEYS; ++j) reach += u[j] >= (threshold | bit) ? 1 : 0;
+        reach = wave_sum(reach);
+      }
       if (reach >= r.m) threshold |= bit;
       if (reach == r.m) {
         --threshold;
