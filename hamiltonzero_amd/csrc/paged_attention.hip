@@ -41,8 +41,8 @@ struct PagedParams {
 };
 
 // How the rows are divided: runs of `chunk` slots, at least one a row (more steps than the quotient of all by those wanted, so that the
-// further runs are fewer than wanted; longer ones, up to kLong steps, while there are runs enough to fill the card). Run 0 of batch row b has number b; the further runs of all
-// rows follow in order. Up to 64 rows, every wave works it out for itself, a length a lane; more rows have it
+// further runs are fewer than wanted; longer ones, up to kLong steps, while there are runs enough to fill the card). Run 0 of
+// batch row b has number b; the further runs of all rows follow in order. Up to 64 rows, every wave works it out for itself, a length a lane; more rows have it
 // worked out once by paged_plan_kernel (512 rows in every wave: 8 us more of a workgroup's time than a lookup).
 constexpr int kPlanRows = 64;
 struct Found {
@@ -627,8 +627,8 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<v4f*>(mine + out_at<DP>(c, 4 * dt + g)) = o[cb][dt];
     together ? __syncthreads() : wave_fence();
-    put_run<DP, PARTS>(p, run, reinterpret_cast<const float*>(v_lds[0]), kBlock * DP * static_cast<int>(sizeof(typename V::Element)) / 4, &sums_lds[0][16 * cb][0], 16 * CB * 3,
-                       min(16, p.rows - r0 - 16 * cb), r0 + 16 * cb, lse_lds[together ? 0 : wave] + 16 * cb);
+    put_run<DP, PARTS>(p, run, reinterpret_cast<const float*>(v_lds[0]), kBlock * DP * static_cast<int>(sizeof(typename V::Element)) / 4,
+                       &sums_lds[0][16 * cb][0], 16 * CB * 3, min(16, p.rows - r0 - 16 * cb), r0 + 16 * cb, lse_lds[together ? 0 : wave] + 16 * cb);
     if (cb + 1 < CB) together ? __syncthreads() : wave_fence();
   }
   if (p.kept != nullptr && p.lse == nullptr) put_own_weights(p, run, lse_lds[together ? 0 : wave]);
