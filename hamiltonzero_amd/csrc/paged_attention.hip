@@ -107,7 +107,7 @@ struct Plan {
     }
     return true;
   }
-  // The number of run 1 of batch row b.
+  // The number of run 1 of batch row b. (Reads other lanes' numbers: all of the wave must be there, also in what encloses the call.)
   __device__ __forceinline__ int second(const PagedParams& p, int b) const {
     return p.B + (table != nullptr ? table[2 + b] : __builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(mine, b));
   }
@@ -783,9 +783,8 @@ struct Runs {
   int64_t first, others;  // where the first run's lie, and behind it those of run 1 on, `step` apart
   int64_t step;
   int count;
-  __device__ __forceinline__ Runs(const PagedParams& p, const Plan& plan, int b, int n, int hk, int r)
-      : first(result_at(p, b, hk, r)), others(result_at(p, plan.second(p, b) - 1, hk, r)), step(static_cast<int64_t>(p.Hk) * p.rows),
-        count(1 + further(n, plan.chunk)) {}
+  __device__ __forceinline__ Runs(const PagedParams& p, int count_, int second, int b, int hk, int r)
+      : first(result_at(p, b, hk, r)), others(result_at(p, second - 1, hk, r)), step(static_cast<int64_t>(p.Hk) * p.rows), count(count_) {}
   __device__ __forceinline__ int64_t at(int run) const { return run == 0 ? first : others + run * step; }
 };
 
@@ -810,7 +809,7 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
       const int d = (static_cast<int>(unit % quarters) * lanes + dl) * 4, b = static_cast<int>(at / per), n = p.c.length(b);
       if (n <= plan.chunk) continue;  // all of the workgroup
       const int within = static_cast<int>(at - static_cast<int64_t>(b) * per), i = within / p.H, h = within % p.H;
-      const Runs runs(p, plan, b, n, h / p.G, i * p.G + h % p.G);
+      const Runs runs(p, 1 + further(n, plan.chunk), plan.second(p, b), b, h / p.G, i * p.G + h % p.G);
       float m = kNegInf, l = 0.f;
       v4f o = zero4();
       for (int r = way; r < runs.count; r += 4 * ways) {  // four loads under way
@@ -865,6 +864,7 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
   const int id = static_cast<int>(blockIdx.x) - joins, unit = id / per_row;
   const int b = unit / p.Hk, hk = unit % p.Hk, n = p.c.length(b);
   const int slot0 = id % per_row * (4 * kThreads), slot = slot0 + 4 * tid;
+  const int count = 1 + further(n, plan.chunk), second = count > 1 ? plan.second(p, b) : 0;  // (before lanes go different ways)
   v4f sum = zero4();
   for (int r0 = 0; r0 < p.rows && slot0 < n; r0 += kRowTile) {
     const int rows = min(kRowTile, p.rows - r0);
@@ -874,10 +874,10 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
     for (int r = tid >> 3; r < rows; r += kThreads / 8) {
       const int i = (r0 + r) / p.G, g = (r0 + r) % p.G;
       float lse;
-      if (n <= plan.chunk) {
+      if (count == 1) {
         lse = p.lse[(static_cast<int64_t>(b) * p.Nq + i) * p.H + hk * p.G + g];
       } else {
-        const Runs runs(p, plan, b, n, hk, r0 + r);
+        const Runs runs(p, count, second, b, hk, r0 + r);
         float m = kNegInf, exact = 0.f;
         for (int x0 = d8; x0 < runs.count; x0 += 64) {  // eight loads under way
           v4f st[8];
