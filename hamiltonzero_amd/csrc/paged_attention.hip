@@ -30,7 +30,8 @@ struct PagedParams {
   void* out;
   const float *slopes, *scores;
   float* scores_out;
-  float *partial, *stats, *kept, *lse;  // workspace: see layout()
+  float *partial, *stats, *kept;  // workspace: see layout()
+  float2* norms;
   int B, Nq, H, Hk, G, D, rows, blocks;  // rows: Nq G; blocks of 16 or 32 of them
   int64_t blocks_kept;                   // of a row's kept scores: blocks of kKept slots
   int64_t runs_wanted, runs_fill;        // for one key head and block of rows, over all batch rows: at most, and to fill the card
@@ -408,12 +409,17 @@ struct Run {
 template <int DP>
 __device__ __forceinline__ int out_at(int x, int ch) { return x * DP + (ch ^ (x & 7)) * 4; }
 
+// What a row's weights are formed by: its largest score and one over its sum of exp2(score - largest). Apart: one number for both, the largest plus
+// the sum's logarithm, would be rounded at the size of the score, an error of 2^-24 of it in all weights of the row. (A row that sees no
+// slot has weights 0, one with a NaN has NaN.)
+__device__ __forceinline__ float2 norm_of(float top, float sum) { return make_float2(top == kNegInf ? 0.f : top, sum == 0.f ? 0.f : 1.f / sum); }
+
 // The results of a run: rows r0 .. r0 + columns - 1 from its waves' sums of values (out_at, o_wave floats a wave) and their base, sum and sum of
-// unrounded weights (sums_wave floats a wave). Where the run is its row and weights are added up, the columns' logarithms of their sums go to
-// lse and to memory.
+// unrounded weights (sums_wave floats a wave). Where the run is its row and weights are added up, what they are formed by goes to norms and to
+// memory.
 template <int DP, int PARTS>
 __device__ __forceinline__ void put_run(const PagedParams& p, const Run& run, const float* o, int o_wave, const float* sums, int sums_wave, int columns, int r0,
-                                        float* lse) {
+                                        float2* norms) {
   const int w0 = run.together ? 0 : run.wave, threads = 64 * p.waves;
   for (int x = run.together ? threadIdx.x : threadIdx.x & 63; x < columns * (DP / 4); x += threads) {
     const int col = x / (DP / 4), ch = x % (DP / 4), r = r0 + col, d = 4 * ch;
@@ -434,8 +440,8 @@ __device__ __forceinline__ void put_run(const PagedParams& p, const Run& run, co
       const float inv = all > 0.f || all != all ? 1.f / all : 0.f;
       store_four<PARTS>(p.out, at * p.D + d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
       if (p.kept != nullptr && ch == 0) {
-        lse[col] = all_exact == 0.f ? 0.f : top + log2f(all_exact);
-        if (p.lse != nullptr) p.lse[at] = lse[col];
+        norms[col] = norm_of(top, all_exact);
+        if (p.norms != nullptr) p.norms[at] = norms[col];
       }
     } else {
       const int64_t to = result_at(p, run.id, run.hk, r);
@@ -446,14 +452,14 @@ __device__ __forceinline__ void put_run(const PagedParams& p, const Run& run, co
 }
 
 // The weights of four slots of a row of n, from what rows r0 .. r0 + rows - 1 of query and head kept.
-__device__ __forceinline__ void add_kept(const PagedParams& p, int unit, int slot, const float* lse, int r0, int rows, v4f& sum) {
+__device__ __forceinline__ void add_kept(const PagedParams& p, int unit, int slot, const float2* norms, int r0, int rows, v4f& sum) {
   const float* const kept = p.kept + kept_at(p, unit, r0, slot);
 #pragma unroll 4
   for (int r = 0; r < rows; ++r) {
     const v4f x = *reinterpret_cast<const v4f*>(kept + r * kKept);
-    const float base = lse[r];
+    const float2 norm = norms[r];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] += fast_exp2(x[e] - base);
+    for (int e = 0; e < 4; ++e) sum[e] = fmaf(fast_exp2(x[e] - norm.x), norm.y, sum[e]);
   }
 }
 __device__ __forceinline__ void put_weights(const PagedParams& p, int unit, int n, int slot, const v4f& sum) {
@@ -476,12 +482,12 @@ __device__ __forceinline__ void put_weights(const PagedParams& p, int unit, int 
 }
 
 // The weights of a run that is its row, and all rows of query and head, by its threads.
-__device__ __forceinline__ void put_own_weights(const PagedParams& p, const Run& run, const float* lse) {
+__device__ __forceinline__ void put_own_weights(const PagedParams& p, const Run& run, const float2* norms) {
   run.together ? __syncthreads() : wave_fence();
   const int threads = 64 * p.waves, unit = run.b * p.Hk + run.hk;
   for (int slot = 4 * (run.together ? threadIdx.x : threadIdx.x & 63); slot < p.c.slots; slot += 4 * threads) {
     v4f sum = zero4();
-    if (slot < run.n) add_kept(p, unit, slot, lse, 0, p.rows, sum);
+    if (slot < run.n) add_kept(p, unit, slot, norms, 0, p.rows, sum);
     put_weights(p, unit, run.n, slot, sum);
   }
 }
@@ -499,7 +505,8 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
   typedef Values<DP, PARTS> V;
   __shared__ __align__(16) typename V::Element v_lds[4][kBlock * DP];
   __shared__ __align__(16) int64_t where_lds[apart(READS) ? 4 : 1][2][kBlock][2];
-  __shared__ float sums_lds[4][16 * CB][3], lse_lds[4][16 * CB];  // each wave's base, sum and sum of unrounded weights
+  __shared__ float sums_lds[4][16 * CB][3];  // each wave's base, sum and sum of unrounded weights
+  __shared__ float2 norms_lds[4][16 * CB];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const V vt{v_lds[wave]};
   const Plan plan(p, lane);
@@ -628,10 +635,10 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<v4f*>(mine + out_at<DP>(c, 4 * dt + g)) = o[cb][dt];
     together ? __syncthreads() : wave_fence();
     put_run<DP, PARTS>(p, run, reinterpret_cast<const float*>(v_lds[0]), kBlock * DP * static_cast<int>(sizeof(typename V::Element)) / 4,
-                       &sums_lds[0][16 * cb][0], 16 * CB * 3, min(16, p.rows - r0 - 16 * cb), r0 + 16 * cb, lse_lds[together ? 0 : wave] + 16 * cb);
+                       &sums_lds[0][16 * cb][0], 16 * CB * 3, min(16, p.rows - r0 - 16 * cb), r0 + 16 * cb, norms_lds[together ? 0 : wave] + 16 * cb);
     if (cb + 1 < CB) together ? __syncthreads() : wave_fence();
   }
-  if (p.kept != nullptr && p.lse == nullptr) put_own_weights(p, run, lse_lds[together ? 0 : wave]);
+  if (p.kept != nullptr && p.norms == nullptr) put_own_weights(p, run, norms_lds[together ? 0 : wave]);
 }
 
 // The same for float32 and one or two rows of query and head, on vector instructions: a lane has a part of each key's dot product, as
@@ -647,7 +654,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
   constexpr int DS = S::DS, CH = S::CH, LOADS = S::LOADS, STEP = S::STEP;
   __shared__ __align__(16) int64_t where_lds[apart(READS) ? 4 : 1][2][kBlock][2];
   __shared__ __align__(16) float w_lds[4][R][kBlock], o_lds[4][R * DP];
-  __shared__ float sums_lds[4][R][3], lse_lds[4][R];
+  __shared__ float sums_lds[4][R][3];
+  __shared__ float2 norms_lds[4][R];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const Plan plan(p, lane);
   Run run;
@@ -774,8 +782,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
     }
   }
   run.together ? __syncthreads() : wave_fence();
-  put_run<DP, 3>(p, run, o_lds[0], R * DP, &sums_lds[0][0][0], R * 3, p.rows, 0, lse_lds[run.together ? 0 : wave]);
-  if (p.kept != nullptr && p.lse == nullptr) put_own_weights(p, run, lse_lds[run.together ? 0 : wave]);
+  put_run<DP, 3>(p, run, o_lds[0], R * DP, &sums_lds[0][0][0], R * 3, p.rows, 0, norms_lds[run.together ? 0 : wave]);
+  if (p.kept != nullptr && p.norms == nullptr) put_own_weights(p, run, norms_lds[run.together ? 0 : wave]);
 }
 
 // The run results of one row of (b, i, h).
@@ -797,7 +805,8 @@ constexpr int kRowTile = 64;
 template <int PARTS>
 __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, int joins, int lanes, int per_row) {
   __shared__ __align__(16) float o_lds[4][32][4];
-  __shared__ float m_lds[4], l_lds[4], lse_lds[kRowTile];
+  __shared__ float m_lds[4], l_lds[4];
+  __shared__ float2 norms_lds[kRowTile];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const Plan plan(p, lane);
   if (static_cast<int>(blockIdx.x) < joins) {
@@ -869,13 +878,13 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
   for (int r0 = 0; r0 < p.rows && slot0 < n; r0 += kRowTile) {
     const int rows = min(kRowTile, p.rows - r0);
     if (r0 > 0) __syncthreads();
-    // each row's base and sum, together the base-2 logarithm of its sum: eight lanes a row
+    // what each row's weights are formed by: eight lanes a row
     const int d8 = tid & 7;
     for (int r = tid >> 3; r < rows; r += kThreads / 8) {
       const int i = (r0 + r) / p.G, g = (r0 + r) % p.G;
-      float lse;
+      float2 norm;
       if (count == 1) {
-        lse = p.lse[(static_cast<int64_t>(b) * p.Nq + i) * p.H + hk * p.G + g];
+        norm = p.norms[(static_cast<int64_t>(b) * p.Nq + i) * p.H + hk * p.G + g];
       } else {
         const Runs runs(p, count, second, b, hk, r0 + r);
         float m = kNegInf, exact = 0.f;
@@ -899,12 +908,12 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
         m = now;
 #pragma unroll
         for (int x = 1; x < 8; x <<= 1) exact += __shfl_xor(exact, x, 64);
-        lse = exact == 0.f ? 0.f : m + log2f(exact);
+        norm = norm_of(m, exact);
       }
-      if (d8 == 0) lse_lds[r] = lse;
+      if (d8 == 0) norms_lds[r] = norm;
     }
     __syncthreads();
-    if (slot < n) add_kept(p, unit, slot, lse_lds, r0, rows, sum);
+    if (slot < n) add_kept(p, unit, slot, norms_lds, r0, rows, sum);
   }
   if (slot < p.c.slots) put_weights(p, unit, n, slot, sum);
 }
@@ -922,13 +931,13 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
 constexpr int64_t kFill = 1536, kLeast = 512, kAlone = 2048, kWhole = 512, kUnits = 256;
 
 struct Layout {
-  int64_t rows, block, blocks, waves, step, runs_wanted, runs_fill, runs, blocks_kept, partial, stats, kept, lse, plan, total;
+  int64_t rows, block, blocks, waves, step, runs_wanted, runs_fill, runs, blocks_kept, partial, stats, kept, norms, plan, total;
   bool whole, table, finish_weights;  // each row is one run; a table of the runs; weights by the second kernel
 };
 
 // Rows of query and head in a workgroup's products: 16, or 32 where there are more; float32 heads of more than 64 elements have
 // no registers for 32, and read their keys and values again for every 16.
-// The workspace, in floats: partial outputs and statistics of every run, kept scores, a base and sum for each row.
+// The workspace, in floats: partial outputs and statistics of every run, kept scores, what each row's weights are formed by.
 Layout layout(const hz_paged_attention_args& a) {
   const hz_paged_cache& c = a.cache;
   Layout w{};
@@ -961,7 +970,7 @@ Layout layout(const hz_paged_attention_args& a) {
   if (a.scores_out != nullptr) {
     w.kept = take(c.B * c.Hk * w.rows * w.blocks_kept * kKept);
     w.finish_weights = !w.whole || w.blocks > 1;
-    w.lse = take(w.finish_weights ? c.B * a.Nq * a.H : 0);
+    w.norms = take(w.finish_weights ? 2 * c.B * a.Nq * a.H : 0);
   }
   return w;
 }
@@ -974,7 +983,7 @@ hipError_t run(const hz_paged_attention_args& a, void* workspace, hipStream_t st
   const bool want = a.scores_out != nullptr;
   const bool capped = a.softcap > 0.f;
   PagedParams p{Pages(c), a.q, a.out, a.slopes, a.scores, a.scores_out, ws + w.partial, ws + w.stats,
-                want ? ws + w.kept : nullptr, w.finish_weights ? ws + w.lse : nullptr, static_cast<int>(c.B), static_cast<int>(a.Nq),
+                want ? ws + w.kept : nullptr, w.finish_weights ? reinterpret_cast<float2*>(ws + w.norms) : nullptr, static_cast<int>(c.B), static_cast<int>(a.Nq),
                 static_cast<int>(a.H), static_cast<int>(c.Hk), static_cast<int>(a.H / c.Hk), static_cast<int>(c.D),
                 static_cast<int>(w.rows), static_cast<int>(w.blocks), w.blocks_kept, w.runs_wanted, w.runs_fill,
                 w.table ? reinterpret_cast<int*>(ws + w.plan) : nullptr, static_cast<int>(w.waves), static_cast<int>(w.step), w.whole, a.softcap,

@@ -3,8 +3,8 @@ be off by.
 
 The rounding model is :mod:`oracle.token_oracle`'s. Joins of runs and of a run's waves multiply each sum by a power of two
 whose exponent is a rounded difference (``2^-24`` of it, and of its value) and add it: 16 F covers them beside the sums
-themselves. The weights that are added up are not rounded: P = 2^(s - lse) is off by the score's and the sum's errors and by the
-roundings of lse and of the difference; one below 2^-126, the least normal float32, is 0, which is off by less than that.
+themselves. The weights that are added up are not rounded: P = 2^(s - largest) / sum is off by the score's and the sum's errors and by the
+rounding of the difference; one below 2^-126, the least normal float32, is 0, which is off by less than that.
 """
 
 from __future__ import annotations
@@ -91,14 +91,13 @@ def attention(q, k_cache, v_cache, page_table, lengths, *, scale, softcap=0.0, s
                 w = np.exp(s - m)
                 z = w.sum(1, keepdims=True)
                 w = w / np.where(z == 0, 1, z)
-                lse = m + np.log(np.where(z == 0, 1, z))
                 worst = 2 * np.where(seen, es, 0).max(1, initial=0)[:, None]
                 rho = worst + _sum_error(n) + (8 + 16) * F
                 r["out"][b, :, h] = w @ vh
                 r["t_out"][b, :, h] = (rho + up) * (w @ np.abs(vh)) + (up + u) * np.abs(w @ vh)
                 had[b, g, :n] += w.sum(0)
-                apart = np.where(seen, np.abs(np.where(seen, s, 0) - lse), 0)
-                t_had[b, g, :n] += (w * (worst + _sum_error(n) + 24 * F + 8 * F * (np.abs(lse) + apart + 2))).sum(0)
+                apart = np.where(seen, m - np.where(seen, s, m), 0)
+                t_had[b, g, :n] += (w * (worst + _sum_error(n) + 24 * F + 8 * F * (apart + 2))).sum(0)
             t_had[b, g, :n] += (Nq * G + 2) * F * had[b, g, :n] + Nq * G * 2.0**-126
     if scores is not None:
         for b in range(B):
