@@ -30,8 +30,8 @@ struct PagedParams {
   void* out;
   const float *slopes, *scores;
   float* scores_out;
-  float *partial, *stats, *kept;  // workspace: see layout()
-  float2* norms;
+  float *partial, *kept;  // workspace: see layout()
+  float2 *stats, *norms;  // each run's base and sum; norm_of() of each row
   int B, Nq, H, Hk, G, D, rows, blocks;  // rows: Nq G; blocks of 16 or 32 of them
   int64_t blocks_kept;                   // of a row's kept scores: blocks of kKept slots
   int64_t runs_wanted, runs_fill;        // for one key head and block of rows, over all batch rows: at most, and to fill the card
@@ -170,6 +170,16 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// A step's weights as the products with the values take them. bfloat16: in two parts, 2^-16 off together, so that an output is rounded once. (In one
+// part outputs were off by 0.0008 of their size beside that rounding's 0.0017.)
+template <int PARTS>
+__device__ __forceinline__ auto weight_frag(const v16f& y) {
+  if constexpr (PARTS == 1)
+    return grad_frag<1>(y, 0);
+  else
+    return frag_of<3>(y, 0);
 }
 
 // A block's values in LDS. bfloat16: a Tile, whose reads transpose. float32: the floats themselves, split into parts as they are read
@@ -414,25 +424,24 @@ __device__ __forceinline__ int out_at(int x, int ch) { return x * DP + (ch ^ (x 
 // slot has weights 0, one with a NaN has NaN.)
 __device__ __forceinline__ float2 norm_of(float top, float sum) { return make_float2(top == kNegInf ? 0.f : top, sum == 0.f ? 0.f : 1.f / sum); }
 
-// The results of a run: rows r0 .. r0 + columns - 1 from its waves' sums of values (out_at, o_wave floats a wave) and their base, sum and sum of
-// unrounded weights (sums_wave floats a wave). Where the run is its row and weights are added up, what they are formed by goes to norms and to
+// The results of a run: rows r0 .. r0 + columns - 1 from its waves' sums of values (out_at, o_wave floats a wave) and their base and sum
+// (sums_wave pairs a wave). Where the run is its row and weights are added up, what they are formed by goes to norms and to
 // memory.
 template <int DP, int PARTS>
-__device__ __forceinline__ void put_run(const PagedParams& p, const Run& run, const float* o, int o_wave, const float* sums, int sums_wave, int columns, int r0,
+__device__ __forceinline__ void put_run(const PagedParams& p, const Run& run, const float* o, int o_wave, const float2* sums, int sums_wave, int columns, int r0,
                                         float2* norms) {
   const int w0 = run.together ? 0 : run.wave, threads = 64 * p.waves;
   for (int x = run.together ? threadIdx.x : threadIdx.x & 63; x < columns * (DP / 4); x += threads) {
     const int col = x / (DP / 4), ch = x % (DP / 4), r = r0 + col, d = 4 * ch;
     if (d >= p.D) continue;
-    float top = kNegInf, all = 0.f, all_exact = 0.f;
-    for (int w = w0; w < w0 + p.waves; ++w) top = fmaxf(top, sums[w * sums_wave + 3 * col]);
+    float top = kNegInf, all = 0.f;
+    for (int w = w0; w < w0 + p.waves; ++w) top = fmaxf(top, sums[w * sums_wave + col].x);
     const float base = top == kNegInf ? 0.f : top;
     v4f y = zero4();
     for (int w = w0; w < w0 + p.waves; ++w) {
-      const float* const s = sums + w * sums_wave + 3 * col;
-      const float a = fast_exp2(s[0] - base);
-      all += a * s[1];
-      all_exact += a * s[2];
+      const float2 s = sums[w * sums_wave + col];
+      const float a = fast_exp2(s.x - base);
+      all += a * s.y;
       y += a * *reinterpret_cast<const v4f*>(o + w * o_wave + out_at<DP>(col, ch));
     }
     if (run.alone) {
@@ -440,13 +449,13 @@ __device__ __forceinline__ void put_run(const PagedParams& p, const Run& run, co
       const float inv = all > 0.f || all != all ? 1.f / all : 0.f;
       store_four<PARTS>(p.out, at * p.D + d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
       if (p.kept != nullptr && ch == 0) {
-        norms[col] = norm_of(top, all_exact);
+        norms[col] = norm_of(top, all);
         if (p.norms != nullptr) p.norms[at] = norms[col];
       }
     } else {
       const int64_t to = result_at(p, run.id, run.hk, r);
       *reinterpret_cast<v4f*>(p.partial + to * p.D + d) = y;
-      if (ch == 0) *reinterpret_cast<v4f*>(p.stats + to * 4) = v4f{top, all, all_exact, 0.f};
+      if (ch == 0) p.stats[to] = make_float2(top, all);
     }
   }
 }
@@ -505,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
   typedef Values<DP, PARTS> V;
   __shared__ __align__(16) typename V::Element v_lds[4][kBlock * DP];
   __shared__ __align__(16) int64_t where_lds[apart(READS) ? 4 : 1][2][kBlock][2];
-  __shared__ float sums_lds[4][16 * CB][3];  // each wave's base, sum and sum of unrounded weights
+  __shared__ float2 sums_lds[4][16 * CB];  // each wave's base and sum
   __shared__ float2 norms_lds[4][16 * CB];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const V vt{v_lds[wave]};
@@ -532,10 +541,10 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     }
   }
   v4f o[CB][DT];
-  float m[CB], l[CB], l_exact[CB];
+  float m[CB], l[CB];
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
-    m[cb] = kNegInf, l[cb] = l_exact[cb] = 0.f;
+    m[cb] = kNegInf, l[cb] = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[cb][dt] = zero4();
   }
@@ -575,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     settle(s);
     wave_fence();
     const uint32_t known_then = slots.take(k0 + 2 * step, buffer);  // what this block needed of it has been read
-    Frag<PARTS> w[CB];
+    Frag<PARTS == 1 ? 2 : 3> w[CB];
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
       const int k1 = k0 + 4 * g;
@@ -600,7 +609,6 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
         const float now = fmaxf(m[cb], top), alpha = m[cb] == kNegInf ? 0.f : fast_exp2(m[cb] - now);
         m[cb] = now;
         l[cb] *= alpha;
-        l_exact[cb] *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[cb][dt] *= alpha;
       }
@@ -609,10 +617,9 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         y[i] = fast_exp2(x[i] - base);
-        l_exact[cb] += y[i];
+        l[cb] += y[i];
       }
-      w[cb] = frag_of<PARTS>(y, 0);
-      add_weights(w[cb], y, 0, l[cb]);
+      w[cb] = weight_frag<PARTS>(y);
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
@@ -629,13 +636,13 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
   float* const mine = reinterpret_cast<float*>(v_lds[wave]);
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
-    const float sum = group_sum(l[cb]), exact = group_sum(l_exact[cb]);
-    if (g == 0) sums_lds[wave][16 * cb + c][0] = m[cb], sums_lds[wave][16 * cb + c][1] = sum, sums_lds[wave][16 * cb + c][2] = exact;
+    const float sum = group_sum(l[cb]);
+    if (g == 0) sums_lds[wave][16 * cb + c] = make_float2(m[cb], sum);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<v4f*>(mine + out_at<DP>(c, 4 * dt + g)) = o[cb][dt];
     together ? __syncthreads() : wave_fence();
     put_run<DP, PARTS>(p, run, reinterpret_cast<const float*>(v_lds[0]), kBlock * DP * static_cast<int>(sizeof(typename V::Element)) / 4,
-                       &sums_lds[0][16 * cb][0], 16 * CB * 3, min(16, p.rows - r0 - 16 * cb), r0 + 16 * cb, norms_lds[together ? 0 : wave] + 16 * cb);
+                       sums_lds[0] + 16 * cb, 16 * CB, min(16, p.rows - r0 - 16 * cb), r0 + 16 * cb, norms_lds[together ? 0 : wave] + 16 * cb);
     if (cb + 1 < CB) together ? __syncthreads() : wave_fence();
   }
   if (p.kept != nullptr && p.norms == nullptr) put_own_weights(p, run, norms_lds[together ? 0 : wave]);
@@ -654,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
   constexpr int DS = S::DS, CH = S::CH, LOADS = S::LOADS, STEP = S::STEP;
   __shared__ __align__(16) int64_t where_lds[apart(READS) ? 4 : 1][2][kBlock][2];
   __shared__ __align__(16) float w_lds[4][R][kBlock], o_lds[4][R * DP];
-  __shared__ float sums_lds[4][R][3];
+  __shared__ float2 sums_lds[4][R];
   __shared__ float2 norms_lds[4][R];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const Plan plan(p, lane);
@@ -768,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
     sum += row_turned<0x124>(sum);
     sum += row_turned<0x122>(sum);
     sum += row_turned<0x121>(sum);
-    if (lane == 0) sums_lds[wave][r][0] = m[r], sums_lds[wave][r][1] = sums_lds[wave][r][2] = sum;
+    if (lane == 0) sums_lds[wave][r] = make_float2(m[r], sum);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float y = o[r][e];
@@ -782,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
     }
   }
   run.together ? __syncthreads() : wave_fence();
-  put_run<DP, 3>(p, run, o_lds[0], R * DP, &sums_lds[0][0][0], R * 3, p.rows, 0, norms_lds[run.together ? 0 : wave]);
+  put_run<DP, 3>(p, run, o_lds[0], R * DP, sums_lds[0], R, p.rows, 0, norms_lds[run.together ? 0 : wave]);
   if (p.kept != nullptr && p.norms == nullptr) put_own_weights(p, run, norms_lds[run.together ? 0 : wave]);
 }
 
@@ -822,23 +829,24 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
       float m = kNegInf, l = 0.f;
       v4f o = zero4();
       for (int r = way; r < runs.count; r += 4 * ways) {  // four loads under way
-        v4f st[4], y[4];
+        float2 st[4];
+        v4f y[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int64_t from = runs.at(min(r + x * ways, runs.count - 1));
-          st[x] = *reinterpret_cast<const v4f*>(p.stats + from * 4);
+          st[x] = p.stats[from];
           y[x] = *reinterpret_cast<const v4f*>(p.partial + from * p.D + (d < p.D ? d : 0));
         }
         float now = m;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) now = fmaxf(now, st[x][0]);
+        for (int x = 0; x < 4; ++x) now = fmaxf(now, st[x].x);
         const float base = now == kNegInf ? 0.f : now, alpha = fast_exp2(m - base);
         m = now, l *= alpha, o *= alpha;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           if (r + x * ways >= runs.count) break;
-          const float a = fast_exp2(st[x][0] - base);  // (a weight of zero passes a NaN on too)
-          l += a * st[x][1];
+          const float a = fast_exp2(st[x].x - base);  // (a weight of zero passes a NaN on too)
+          l += a * st[x].y;
           o += a * y[x];
         }
       }
@@ -887,28 +895,28 @@ __global__ void __launch_bounds__(kThreads) paged_finish_kernel(PagedParams p, i
         norm = p.norms[(static_cast<int64_t>(b) * p.Nq + i) * p.H + hk * p.G + g];
       } else {
         const Runs runs(p, count, second, b, hk, r0 + r);
-        float m = kNegInf, exact = 0.f;
+        float m = kNegInf, l = 0.f;
         for (int x0 = d8; x0 < runs.count; x0 += 64) {  // eight loads under way
-          v4f st[8];
+          float2 st[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) st[x] = *reinterpret_cast<const v4f*>(p.stats + runs.at(min(x0 + 8 * x, runs.count - 1)) * 4);
+          for (int x = 0; x < 8; ++x) st[x] = p.stats[runs.at(min(x0 + 8 * x, runs.count - 1))];
           float now = m;
 #pragma unroll
-          for (int x = 0; x < 8; ++x) now = fmaxf(now, st[x][0]);
+          for (int x = 0; x < 8; ++x) now = fmaxf(now, st[x].x);
           const float base = now == kNegInf ? 0.f : now;
-          exact *= fast_exp2(m - base);
+          l *= fast_exp2(m - base);
 #pragma unroll
-          for (int x = 0; x < 8; ++x) exact += x0 + 8 * x < runs.count ? fast_exp2(st[x][0] - base) * st[x][2] : 0.f;
+          for (int x = 0; x < 8; ++x) l += x0 + 8 * x < runs.count ? fast_exp2(st[x].x - base) * st[x].y : 0.f;
           m = now;
         }
         float now = m;
 #pragma unroll
         for (int x = 1; x < 8; x <<= 1) now = fmaxf(now, __shfl_xor(now, x, 64));
-        exact *= fast_exp2(m - (now == kNegInf ? 0.f : now));
+        l *= fast_exp2(m - (now == kNegInf ? 0.f : now));
         m = now;
 #pragma unroll
-        for (int x = 1; x < 8; x <<= 1) exact += __shfl_xor(exact, x, 64);
-        norm = norm_of(m, exact);
+        for (int x = 1; x < 8; x <<= 1) l += __shfl_xor(l, x, 64);
+        norm = norm_of(m, l);
       }
       if (d8 == 0) norms_lds[r] = norm;
     }
@@ -963,7 +971,7 @@ Layout layout(const hz_paged_attention_args& a) {
     return at;
   };
   w.partial = take(w.whole ? 0 : w.runs * c.Hk * w.rows * c.D);
-  w.stats = take(w.whole ? 0 : w.runs * c.Hk * w.rows * 4);
+  w.stats = take(w.whole ? 0 : w.runs * c.Hk * w.rows * 2);
   w.table = !w.whole && c.B > kPlanRows;
   w.plan = take(w.table ? 2 + (c.B + 1) / 2 * 2 + 2 * (w.runs - c.B) : 0);
   w.blocks_kept = (slots + kBlock - 1) / kBlock * (kBlock / kKept);
@@ -982,8 +990,8 @@ hipError_t run(const hz_paged_attention_args& a, void* workspace, hipStream_t st
   float* const ws = static_cast<float*>(workspace);
   const bool want = a.scores_out != nullptr;
   const bool capped = a.softcap > 0.f;
-  PagedParams p{Pages(c), a.q, a.out, a.slopes, a.scores, a.scores_out, ws + w.partial, ws + w.stats,
-                want ? ws + w.kept : nullptr, w.finish_weights ? reinterpret_cast<float2*>(ws + w.norms) : nullptr, static_cast<int>(c.B), static_cast<int>(a.Nq),
+  PagedParams p{Pages(c), a.q, a.out, a.slopes, a.scores, a.scores_out, ws + w.partial, want ? ws + w.kept : nullptr,
+                reinterpret_cast<float2*>(ws + w.stats), w.finish_weights ? reinterpret_cast<float2*>(ws + w.norms) : nullptr, static_cast<int>(c.B), static_cast<int>(a.Nq),
                 static_cast<int>(a.H), static_cast<int>(c.Hk), static_cast<int>(a.H / c.Hk), static_cast<int>(c.D),
                 static_cast<int>(w.rows), static_cast<int>(w.blocks), w.blocks_kept, w.runs_wanted, w.runs_fill,
                 w.table ? reinterpret_cast<int*>(ws + w.plan) : nullptr, static_cast<int>(w.waves), static_cast<int>(w.step), w.whole, a.softcap,

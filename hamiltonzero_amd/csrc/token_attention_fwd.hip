@@ -220,6 +220,22 @@ __device__ __forceinline__ bool weigh(v16f (&s)[N], const Params& p, Running& r,
   return any;
 }
 
+// The weights' sum, of the rounded ones where the products take rounded ones: numerator and denominator
+// of the mean then err together.
+__device__ __forceinline__ void add_weights(const Frag<1>& w, const v16f&, int, float& l) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 one = __builtin_bit_cast(bf16x2, 0x3f803f80u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t two = w.p[0][i];  // a copy: a bit cast of the vector's element reads its first one
+    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), one, l, false);
+  }
+}
+__device__ __forceinline__ void add_weights(const Frag<3>&, const v16f& s, int half, float& l) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) l += s[8 * half + i];
+}
+
 // Four consecutive outputs, and what their rounding left out where that is wanted.
 template <int PARTS>
 __device__ __forceinline__ void store_out(const Params& p, int64_t off, float a, float b, float c, float d) {

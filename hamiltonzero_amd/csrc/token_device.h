@@ -158,6 +158,10 @@ __device__ __forceinline__ v16f mma_turned(const Frag<3>& a, const Frag<3>& b, v
 __device__ __forceinline__ v4f mma16(const Frag<1>& a, const Frag<1>& b, v4f c) {
   return mfma16_bf16(as_bf16x8(a.p[0]), as_bf16x8(b.p[0]), c);
 }
+__device__ __forceinline__ v4f mma16(const Frag<1>& a, const Frag<2>& b, v4f c) {
+  c = mfma16_bf16(as_bf16x8(a.p[0]), as_bf16x8(b.p[1]), c);
+  return mfma16_bf16(as_bf16x8(a.p[0]), as_bf16x8(b.p[0]), c);
+}
 __device__ __forceinline__ v4f mma16(const Frag<3>& a, const Frag<3>& b, v4f c) {
 #pragma unroll
   for (int t = 0; t < kSplitTerms; ++t) c = mfma16_bf16(as_bf16x8(a.p[kSplitA[t]]), as_bf16x8(b.p[kSplitB[t]]), c);
@@ -466,22 +470,6 @@ __device__ __forceinline__ void document_range(int doc, int& lo, int& hi) {
     lo = min(lo, __shfl_xor(lo, x, 64));
     hi = max(hi, __shfl_xor(hi, x, 64));
   }
-}
-
-// The weights' sum, of the rounded ones where the products take rounded ones: numerator and denominator
-// of the mean then err together.
-__device__ __forceinline__ void add_weights(const Frag<1>& w, const v16f&, int, float& l) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  const bf16x2 one = __builtin_bit_cast(bf16x2, 0x3f803f80u);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t two = w.p[0][i];  // a copy: a bit cast of the vector's element reads its first one
-    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), one, l, false);
-  }
-}
-__device__ __forceinline__ void add_weights(const Frag<3>&, const v16f& s, int half, float& l) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) l += s[8 * half + i];
 }
 
 // Four consecutive elements in the tensor's type.

@@ -54,13 +54,14 @@ def append(k_cache, v_cache, k, v, page_table, lengths):
                 v_cache[page[j], at[j]] = v[b, i]
 
 
-def attention(q, k_cache, v_cache, page_table, lengths, *, scale, softcap=0.0, slopes=None, scores=None, decay=1.0, bf16=False):
-    """``{"out", "t_out"[, "scores", "t_scores"]}``."""
+def attention(q, k_cache, v_cache, page_table, lengths, *, scale, softcap=0.0, slopes=None, scores=None, decay=1.0, bf16=False, up=None):
+    """``{"out", "t_out"[, "scores", "t_scores"]}``. ``up``: what a weight's rounding to the products' type may be off by."""
     q = q.astype(np.float64)
     B, Nq, H, D = q.shape
     P, S, Hk = k_cache.shape[:3]
     G = H // Hk
-    u, up = (2.0**-8, 2.0**-8) if bf16 else (F, 2 * F)
+    u, rounded = (2.0**-8, 2.0**-8) if bf16 else (F, 2 * F)
+    up = rounded if up is None else up
     slots = page_table.shape[1] * S
     r = {"out": np.zeros(q.shape), "t_out": np.zeros(q.shape)}
     had, t_had = np.zeros((B, Hk, slots)), np.zeros((B, Hk, slots))

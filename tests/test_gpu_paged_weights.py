@@ -1,5 +1,6 @@
-"""The weights that paged attention adds up are a softmax's at any size of the scores: those of a query sum to one, to float32's roundings, and one
-number that all of them share (a logarithm of the sum, rounded at the size of the scores) would show."""
+"""The weights of paged attention. Those that it adds up are a softmax's at any size of the scores: those of a query sum to one, to float32's
+roundings, and one number that all of them share (a logarithm of the sum, rounded at the size of the scores) would show. Those that meet the values
+are rounded to 2^-16 and less: an output is rounded once. The same call gives the same bits."""
 
 import numpy as np
 import pytest
@@ -78,3 +79,48 @@ def test_weights_against_the_oracle_at_large_scores():
         _, new = hz.paged_attention(q, k, v, table.cuda(), torch.tensor(n, dtype=torch.int32, device="cuda"), scores=scores)
         want = P.attention(arr(q), arr(k), arr(v), table.numpy(), n, scale=64**-0.5, scores=arr(scores))
         assert (np.abs(arr(new) - want["scores"]) <= want["t_scores"]).all()
+
+
+@pytest.mark.parametrize("o", [dict(), dict(softcap=20.0), dict(slopes=True)], ids=["plain", "cap", "slopes"])
+@pytest.mark.parametrize("B,Nq,H,Hk,D,S,n", [(2, 1, 8, 2, 64, 16, 300), (3, 3, 16, 2, 128, 48, 4000), (1, 5, 8, 1, 32, 10, 2000), (2, 1, 4, 4, 80, 100, 90), (1, 50, 2, 2, 16, 16, 700)],
+                         ids=lambda x: str(x))
+def test_bfloat16_outputs_are_rounded_once(B, Nq, H, Hk, D, S, n, o):
+    """bfloat16's own half step of the result, and 2^-16 (one for a weight's upper part and the rest of it, rounded) of the weights."""
+    print(f"[case] once {B} {Nq} {H} {Hk} {D} {S} {n} {o}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(53)
+    T = -(-n // S)
+    k, v = (torch.randn(B * T, S, Hk, D, generator=g, device="cuda").bfloat16() for _ in range(2))
+    q = (torch.randn(B, Nq, H, D, generator=g, device="cuda") * 2).bfloat16()
+    table = torch.randperm(B * T, generator=torch.Generator().manual_seed(6)).reshape(B, T).to(torch.int32)
+    lengths = [n - 3 * b for b in range(B)]
+    kw = dict(o)
+    if o.get("slopes"):
+        kw["slopes"] = torch.rand(H, generator=g, device="cuda") * 0.1
+    out = hz.paged_attention(q, k, v, table.cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda"), **kw)
+    if o.get("slopes"):
+        kw["slopes"] = arr(kw["slopes"])
+    want = P.attention(arr(q), arr(k), arr(v), table.numpy(), lengths, scale=D**-0.5, bf16=True, up=2.0**-16, **kw)
+    off = np.abs(arr(out) - want["out"])
+    print(f"  out: {(off / np.maximum(want['t_out'], 1e-300)).max():.3f} of its bound", flush=True)
+    assert (off <= want["t_out"]).all(), ((off > want["t_out"]).mean(), (off / np.maximum(want["t_out"], 1e-300)).max())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,Nq,H,Hk,D,S,n", [(4, 1, 32, 8, 128, 64, 9000), (1, 3, 32, 4, 128, 48, 30000), (70, 2, 8, 8, 64, 10, 1500), (300, 1, 8, 8, 64, 16, 200)],
+                         ids=lambda x: str(x))
+def test_the_same_call_gives_the_same_bits(B, Nq, H, Hk, D, S, n, dtype):
+    """Again, and again with other calls between them that use the same memory for their workspaces."""
+    print(f"[case] again {B} {Nq} {H} {Hk} {D} {S} {n} {dtype}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(54)
+    T = -(-n // S)
+    k, v = (torch.randn(B * T, S, Hk, D, generator=g, device="cuda").to(DT[dtype]) for _ in range(2))
+    q = torch.randn(B, Nq, H, D, generator=g, device="cuda").to(DT[dtype])
+    table = torch.randperm(B * T, generator=g, device="cuda").reshape(B, T).to(torch.int32)
+    lengths = torch.randint(n // 3, n + 1, (B,), generator=g, device="cuda").to(torch.int32)
+    scores = torch.rand(B, Hk, T * S, generator=g, device="cuda")
+    first = hz.paged_attention(q, k, v, table, lengths, scores=scores)
+    for turn in range(4):
+        if turn % 2:
+            hz.paged_attention(-q, v, k, table, lengths // 2, scores=scores)
+        again = hz.paged_attention(q, k, v, table, lengths, scores=scores)
+        assert all(torch.equal(a, b) for a, b in zip(first, again)), turn
