@@ -250,12 +250,8 @@ struct Lanes {
 
 // Pages of a multiple of 16 slots: sixteen slots lie one behind the other. Each half of a block is a buffer whose end the
 // hardware checks: base and end are scalars, a lane's offset never changes, and no address is formed in vector registers.
-// kOnce, kApartOnce: past the caches (a long bfloat16 cache 10% faster, paged_token_long_bf16 267 -> 241 us, in pages of 100 slots 268 -> 241,
-// of one slot 279 -> 253); not for pages that rows share (the same
-// with four fifths of its pages shared 155 us from the caches, 229 past them) and float32 (16 x 8192 slots of 8 heads of 128: 203 us, 214).
-enum Reads { kApart, kCached, kOnce, kApartOnce };
-constexpr bool apart(Reads reads) { return reads == kApart || reads == kApartOnce; }
-template <int DP, int PARTS, Reads READS>
+// ONCE: past the caches.
+template <int DP, int PARTS, bool APART>
 struct Slots : Lanes<DP, PARTS> {
   typedef Lanes<DP, PARTS> L;
   const PagedParams& p;
@@ -304,41 +300,45 @@ struct Slots : Lanes<DP, PARTS> {
     const char* const from = h.count > 0 ? base + (h.page * page + h.in * token) * L::BYTES : base;
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(from), 0, static_cast<int>(bytes), 0x00027000);
   }
+  template <bool ONCE>
   __device__ __forceinline__ static void one(Raw8<1>& r, __amdgpu_buffer_rsrc_t from, uint32_t at) {
-    r.u = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, READS == kOnce ? 2 : 0);
+    r.u = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, ONCE ? 2 : 0);
   }
+  template <bool ONCE>
   __device__ __forceinline__ static void one(Raw8<3>& r, __amdgpu_buffer_rsrc_t from, uint32_t at) {
-    r.a = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, READS == kOnce ? 2 : 0));
-    r.b = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, at + 16, 0, READS == kOnce ? 2 : 0));
+    r.a = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, ONCE ? 2 : 0));
+    r.b = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(from, at + 16, 0, ONCE ? 2 : 0));
   }
+  template <bool ONCE>
   __device__ __forceinline__ void load_k(Raw8<PARTS> (&rk)[2][L::DS], int) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const __amdgpu_buffer_rsrc_t from = buffer(k, next[i], p.c.page_k, p.c.token_k);
 #pragma unroll
-      for (int s = 0; s < L::DS; ++s) one(rk[i][s], from, at_k[s]);
+      for (int s = 0; s < L::DS; ++s) one<ONCE>(rk[i][s], from, at_k[s]);
     }
   }
+  template <bool ONCE>
   __device__ __forceinline__ void load_v(Raw8<PARTS> (&rv)[L::LOADS], int) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const __amdgpu_buffer_rsrc_t from = buffer(v, next[i], p.c.page_v, p.c.token_v);
 #pragma unroll
-      for (int j = 0; j < L::LOADS / 2; ++j) one(rv[i * (L::LOADS / 2) + j], from, at_v[j]);
+      for (int j = 0; j < L::LOADS / 2; ++j) one<ONCE>(rv[i * (L::LOADS / 2) + j], from, at_v[j]);
     }
   }
 };
 
 // Other pages: every slot is looked up by a lane of its own, and its offsets go to the others through LDS.
-template <int DP, int PARTS, bool ONCE>
-struct SlotsApart : Lanes<DP, PARTS> {
+template <int DP, int PARTS>
+struct Slots<DP, PARTS, true> : Lanes<DP, PARTS> {
   typedef Lanes<DP, PARTS> L;
   const PagedParams& p;
   const int32_t* table;
   int hk, stop, lane, page_then;
   int64_t (*where)[kBlock][2];  // two blocks' offsets of keys and values; -1: no page
 
-  __device__ __forceinline__ SlotsApart(const PagedParams& p_, const int32_t* table_, int hk_, int stop_, int lane_, int64_t (*where_)[kBlock][2])
+  __device__ __forceinline__ Slots(const PagedParams& p_, const int32_t* table_, int hk_, int stop_, int lane_, int64_t (*where_)[kBlock][2])
       : p(p_), table(table_), hk(hk_), stop(stop_), lane(lane_), where(where_) {}
   __device__ __forceinline__ void look(int k0) {
     const int slot = k0 + (lane & 31);
@@ -354,12 +354,14 @@ struct SlotsApart : Lanes<DP, PARTS> {
     wave_fence();
     return static_cast<uint32_t>(__ballot(known));
   }
+  template <bool ONCE>
   __device__ __forceinline__ static void one(Raw8<PARTS>& r, const void* base, int64_t at, bool on) {
     if constexpr (ONCE)
       r.u = on ? __builtin_nontemporal_load(reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(base) + at)) : v4u{0u, 0u, 0u, 0u};
     else
       r.load(base, at, on);
   }
+  template <bool ONCE>
   __device__ __forceinline__ void load_k(Raw8<PARTS> (&rk)[2][L::DS], int buffer) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -367,31 +369,23 @@ struct SlotsApart : Lanes<DP, PARTS> {
       for (int s = 0; s < L::DS; ++s) {
         const int64_t at = where[buffer][16 * i + L::key_row(lane, s)][0];
         const int d = L::key_element(lane, s);
-        one(rk[i][s], p.c.k, at + hk * p.c.head_k + d, at >= 0 && d < p.D);
+        one<ONCE>(rk[i][s], p.c.k, at + hk * p.c.head_k + d, at >= 0 && d < p.D);
       }
   }
+  template <bool ONCE>
   __device__ __forceinline__ void load_v(Raw8<PARTS> (&rv)[L::LOADS], int buffer) const {
 #pragma unroll
     for (int j = 0; j < L::LOADS; ++j) {
       const int64_t at = where[buffer][lane / L::CH + L::STEP * j][1];
       const int d = lane % L::CH * 8;
-      one(rv[j], p.c.v, at + hk * p.c.head_v + d, at >= 0 && d < p.D);
+      one<ONCE>(rv[j], p.c.v, at + hk * p.c.head_v + d, at >= 0 && d < p.D);
     }
   }
 };
-template <int DP, int PARTS>
-struct Slots<DP, PARTS, kApart> : SlotsApart<DP, PARTS, false> {
-  using SlotsApart<DP, PARTS, false>::SlotsApart;
-};
-template <int DP>
-struct Slots<DP, 1, kApartOnce> : SlotsApart<DP, 1, true> {
-  using SlotsApart<DP, 1, true>::SlotsApart;
-};
-
 // A run of slots and who has it. waves 4: the workgroup; waves 1: each wave one of its own, and they share nothing.
 struct Run {
   bool together, alone;  // alone: its row has no other
-  int wave, id, b, hk, r0, n, first, stop;
+  int wave, id, b, hk, r0, n, begin, first, stop;
   const int32_t* table;
   // Of blocks of `rows` rows of query and head. False behind the last run.
   __device__ __forceinline__ bool find(const PagedParams& p, const Plan& plan, int wave_, int rows) {
@@ -407,11 +401,21 @@ struct Run {
     b = found.b;
     n = p.c.length(b);
     alone = n <= plan.chunk;
-    const int begin = found.run * plan.chunk;
+    begin = found.run * plan.chunk;
     stop = alone ? n : min(n, begin + plan.chunk);
     first = begin + (together ? kBlock * wave : 0);
     table = p.c.table + static_cast<int64_t>(b) * p.c.width;
     return true;
+  }
+  // Whether most of its pages (64 of them, evenly spread, where there are more) lie at the same place of the row before or behind, whose workgroups
+  // then read them too. Rows that share pages without being neighbours are not seen.
+  __device__ __forceinline__ bool shares(const PagedParams& p, int lane) const {
+    if (begin >= stop) return false;
+    const int page0 = p.c.page_of(begin), count = p.c.page_of(stop - 1) - page0 + 1, some = min(count, 64);
+    const int32_t* const at = table + page0 + static_cast<int64_t>(min(lane, some - 1)) * count / some;
+    const int own = *at, before = b > 0 ? *(at - p.c.width) : -1, behind = b + 1 < p.B ? *(at + p.c.width) : -1;
+    const uint64_t votes = __ballot(lane < some && own >= 0 && own < p.c.pages && (own == before || own == behind));
+    return 2 * static_cast<int>(__popcll(votes)) > some;
   }
 };
 
@@ -507,13 +511,20 @@ __device__ __forceinline__ float row_turned(float x) {
   return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CONTROL, 0xf, 0xf, true));
 }
 
-template <int DP, int PARTS, bool CAP, int CB, Reads READS>
+// Which reads go past the caches. float32 none (16 x 8192 slots of 8 heads of 128: 203 us, 214 past them), nor bfloat16 where several workgroups read
+// a run, for more than 32 rows of query and head each. Else bfloat16 does (16 rows of up to 32768 slots of 8 heads of 128: 241 us, 267 through
+// them; in pages of 100 slots 241 and 268, of one slot 253 and 279), but for runs whose pages the rows beside read too (16 x 32768 slots: 346 us;
+// four fifths of the pages shared 283 past the caches, 230 as asked of each run; all of them 268, 181). Rows that are one run each are not asked, which
+// takes 1 us (64 x 900 slots 46.7, 47.7; all of them shared 27.1 past the caches, 27.3 through them; 1024 x 1000 apart 635, 704).
+enum Past { kNone, kUnshared, kAll };
+
+template <int DP, int PARTS, bool CAP, int CB, bool APART, Past PAST>
 __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_kernel(PagedParams p) {
-  typedef Slots<DP, PARTS, READS> S;
+  typedef Slots<DP, PARTS, APART> S;
   constexpr int DS = S::DS, DT = DP / 16, CH = S::CH, LOADS = S::LOADS, STEP = S::STEP;
   typedef Values<DP, PARTS> V;
   __shared__ __align__(16) typename V::Element v_lds[4][kBlock * DP];
-  __shared__ __align__(16) int64_t where_lds[apart(READS) ? 4 : 1][2][kBlock][2];
+  __shared__ __align__(16) int64_t where_lds[APART ? 4 : 1][2][kBlock][2];
   __shared__ float2 sums_lds[4][16 * CB];  // each wave's base and sum
   __shared__ float2 norms_lds[4][16 * CB];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -549,88 +560,94 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
     for (int dt = 0; dt < DT; ++dt) o[cb][dt] = zero4();
   }
 
-  S slots(p, run.table, hk, stop, lane, where_lds[apart(READS) ? wave : 0]);
-  const int lr = lane / CH, lc = lane % CH;
-  Raw8<PARTS> rk[2][DS], rv[LOADS];
-  uint32_t known = 0, known_next = 0;  // slots of the block at hand, and of the next, that lie in a page
-  int buffer = 0;
-  if (first < stop) {
-    slots.look(first);
-    known = slots.take(first, 0);
-    slots.look(first + step);
-    slots.load_v(rv, 0);
-    slots.load_k(rk, 0);
-    known_next = slots.take(first + step, 1);
-  }
-  for (int k0 = first; k0 < stop; k0 += step, buffer ^= 1) {
-    const bool more = k0 + step < stop;
-    slots.look(k0 + 2 * step);
+  S slots(p, run.table, hk, stop, lane, where_lds[APART ? wave : 0]);
+  if (first < stop) slots.look(first);
+  auto attend = [&](auto once) __attribute__((always_inline)) {
+    const int lr = lane / CH, lc = lane % CH;
+    Raw8<PARTS> rk[2][DS], rv[LOADS];
+    uint32_t known = 0, known_next = 0;  // slots of the block at hand, and of the next, that lie in a page
+    int buffer = 0;
+    if (first < stop) {
+      known = slots.take(first, 0);
+      slots.look(first + step);
+      slots.template load_v<once.value>(rv, 0);
+      slots.template load_k<once.value>(rk, 0);
+      known_next = slots.take(first + step, 1);
+    }
+    for (int k0 = first; k0 < stop; k0 += step, buffer ^= 1) {
+      const bool more = k0 + step < stop;
+      slots.look(k0 + 2 * step);
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) vt.put(lr + STEP * j, lc, rv[j]);
-    if (more) slots.load_v(rv, buffer ^ 1);
-    v4f s[CB][2];
+      for (int j = 0; j < LOADS; ++j) vt.put(lr + STEP * j, lc, rv[j]);
+      if (more) slots.template load_v<once.value>(rv, buffer ^ 1);
+      v4f s[CB][2];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      Frag<PARTS> k[DS];
-      S::keys(rk[kb], k, lane);
+      for (int kb = 0; kb < 2; ++kb) {
+        Frag<PARTS> k[DS];
+        S::keys(rk[kb], k, lane);
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {
+          s[cb][kb] = zero4();
+#pragma unroll
+          for (int ds = 0; ds < DS; ++ds) s[cb][kb] = mma16(k[ds], q[cb][ds], s[cb][kb]);
+        }
+      }
+      if (more) slots.template load_k<once.value>(rk, buffer ^ 1);
+      settle(s);
+      wave_fence();
+      const uint32_t known_then = slots.take(k0 + 2 * step, buffer);  // what this block needed of it has been read
+      Frag<PARTS == 1 ? 2 : 3> w[CB];
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) {
-        s[cb][kb] = zero4();
+        const int k1 = k0 + 4 * g;
+        float x[8], top = kNegInf;
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) s[cb][kb] = mma16(k[ds], q[cb][ds], s[cb][kb]);
+        for (int i = 0; i < 8; ++i) {
+          const int at = 16 * (i / 4) + i % 4, key = k1 + at;
+          x[i] = s[cb][i / 4][i % 4];
+          x[i] = CAP ? tanh_of<PARTS>(x[i] * p.to_tanh) * p.to_score2 : x[i] * p.to_score2;
+          if (slope2[cb] != 0.f) x[i] -= slope2[cb] * static_cast<float>(abs(pos[cb] - key));
+          x[i] = key <= pos[cb] && (known >> (at + 4 * g) & 1) ? x[i] : kNegInf;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
+        if (p.kept != nullptr && r0 + 16 * cb + c < p.rows) {
+          float* const to = p.kept + kept_at(p, b * p.Hk + hk, row[cb], k1);
+          *reinterpret_cast<v4f*>(to) = v4f{x[0], x[1], x[2], x[3]};
+          *reinterpret_cast<v4f*>(to + kKept * p.rows) = v4f{x[4], x[5], x[6], x[7]};
+        }
+        top = group_max(top);
+        if (__any(top > m[cb])) {
+          const float now = fmaxf(m[cb], top), alpha = m[cb] == kNegInf ? 0.f : fast_exp2(m[cb] - now);
+          m[cb] = now;
+          l[cb] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[cb][dt] *= alpha;
+        }
+        const float base = m[cb] == kNegInf ? 0.f : m[cb];
+        v16f y = v16f{};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[i] = fast_exp2(x[i] - base);
+          l[cb] += y[i];
+        }
+        w[cb] = weight_frag<PARTS>(y);
       }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const Frag<PARTS> v = vt.columns(dt, lane);
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) o[cb][dt] = mma16(v, w[cb], o[cb][dt]);
+      }
+      wave_fence();
+      known = known_next;
+      known_next = known_then;
     }
-    if (more) slots.load_k(rk, buffer ^ 1);
-    settle(s);
-    wave_fence();
-    const uint32_t known_then = slots.take(k0 + 2 * step, buffer);  // what this block needed of it has been read
-    Frag<PARTS == 1 ? 2 : 3> w[CB];
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-      const int k1 = k0 + 4 * g;
-      float x[8], top = kNegInf;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int at = 16 * (i / 4) + i % 4, key = k1 + at;
-        x[i] = s[cb][i / 4][i % 4];
-        x[i] = CAP ? tanh_of<PARTS>(x[i] * p.to_tanh) * p.to_score2 : x[i] * p.to_score2;
-        if (slope2[cb] != 0.f) x[i] -= slope2[cb] * static_cast<float>(abs(pos[cb] - key));
-        x[i] = key <= pos[cb] && (known >> (at + 4 * g) & 1) ? x[i] : kNegInf;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
-      if (p.kept != nullptr && r0 + 16 * cb + c < p.rows) {
-        float* const to = p.kept + kept_at(p, b * p.Hk + hk, row[cb], k1);
-        *reinterpret_cast<v4f*>(to) = v4f{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<v4f*>(to + kKept * p.rows) = v4f{x[4], x[5], x[6], x[7]};
-      }
-      top = group_max(top);
-      if (__any(top > m[cb])) {
-        const float now = fmaxf(m[cb], top), alpha = m[cb] == kNegInf ? 0.f : fast_exp2(m[cb] - now);
-        m[cb] = now;
-        l[cb] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[cb][dt] *= alpha;
-      }
-      const float base = m[cb] == kNegInf ? 0.f : m[cb];
-      v16f y = v16f{};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        y[i] = fast_exp2(x[i] - base);
-        l[cb] += y[i];
-      }
-      w[cb] = weight_frag<PARTS>(y);
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const Frag<PARTS> v = vt.columns(dt, lane);
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) o[cb][dt] = mma16(v, w[cb], o[cb][dt]);
-    }
-    wave_fence();
-    known = known_next;
-    known_next = known_then;
-  }
+  };
+  if constexpr (PAST == kUnshared)
+    run.shares(p, lane) ? attend(std::false_type{}) : attend(std::true_type{});
+  else
+    attend(std::bool_constant<PAST == kAll>{});
   settle(o);
   // the run's sums, sixteen columns at a time, through the values' LDS
   float* const mine = reinterpret_cast<float*>(v_lds[wave]);
@@ -655,11 +672,11 @@ __global__ void __launch_bounds__(kThreads, PARTS == 1 ? 2 : 1) paged_attention_
 // Four rows took 94 (matrix cores 68) and 144 (148). Heads of 32: 28, 30 and 38. bfloat16 gains nothing (31.0 us with one row of 64,
 // 32.6 on the matrix cores; 120 and 120 with heads of 128). Heads of 64 keep two workgroups a CU (three spill: 73 us); heads of 128
 // need the registers of one.
-template <int DP, bool CAP, int R, Reads READS>
+template <int DP, bool CAP, int R, bool APART>
 __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(PagedParams p) {
-  typedef Slots<DP, 3, READS> S;
+  typedef Slots<DP, 3, APART> S;
   constexpr int DS = S::DS, CH = S::CH, LOADS = S::LOADS, STEP = S::STEP;
-  __shared__ __align__(16) int64_t where_lds[apart(READS) ? 4 : 1][2][kBlock][2];
+  __shared__ __align__(16) int64_t where_lds[APART ? 4 : 1][2][kBlock][2];
   __shared__ __align__(16) float w_lds[4][R][kBlock], o_lds[4][R * DP];
   __shared__ float2 sums_lds[4][R];
   __shared__ float2 norms_lds[4][R];
@@ -686,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
   float o[R][8] = {}, m[R], l[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) m[r] = kNegInf, l[r] = 0.f;
-  S slots(p, run.table, hk, stop, lane, where_lds[apart(READS) ? wave : 0]);
+  S slots(p, run.table, hk, stop, lane, where_lds[APART ? wave : 0]);
   const int lr = lane / CH, lc = lane % CH;
   Raw8<3> rk[2][DS], rv[LOADS];
   uint32_t known = 0, known_next = 0;
@@ -695,8 +712,8 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
     slots.look(run.first);
     known = slots.take(run.first, 0);
     slots.look(run.first + step);
-    slots.load_k(rk, 0);
-    slots.load_v(rv, 0);
+    slots.template load_k<false>(rk, 0);
+    slots.template load_v<false>(rv, 0);
     known_next = slots.take(run.first + step, 1);
   }
   for (int k0 = run.first; k0 < stop; k0 += step, buffer ^= 1) {
@@ -714,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[r][kb] = fmaf(k[e], q[r][s][e], x[r][kb]);
       }
-    if (more) slots.load_k(rk, buffer ^ 1);
+    if (more) slots.template load_k<false>(rk, buffer ^ 1);
     const uint32_t seen = known;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -762,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) paged_rows_kernel(
         for (int e = 0; e < 8; ++e) o[r][e] = fmaf(w, v[e], o[r][e]);
       }
     }
-    if (more) slots.load_v(rv, buffer ^ 1);
+    if (more) slots.template load_v<false>(rv, buffer ^ 1);
     wave_fence();
     known = known_next;
     known_next = slots.take(k0 + 2 * step, buffer);  // (the next block's loads are under way)
@@ -998,29 +1015,38 @@ hipError_t run(const hz_paged_attention_args& a, void* workspace, hipStream_t st
                 capped ? a.scale / a.softcap : 0.f, (capped ? a.softcap : a.scale) * kLog2e, a.decay};
   const unsigned grid = static_cast<unsigned>(w.waves > 1 ? w.runs * c.Hk * w.blocks : (w.runs * c.Hk * w.blocks + 3) / 4);
   if (w.table) paged_plan_kernel<<<1, 1024, 0, stream>>>(p, reinterpret_cast<int*>(ws + w.plan));
-  auto attend = [&](auto reads) {
-    constexpr Reads READS = reads.value;
-    if constexpr (PARTS == 3)
-      if (w.rows <= 2) {
-        if (w.rows == 1)
-          paged_rows_kernel<DP, CAP, 1, READS><<<grid, kThreads, 0, stream>>>(p);
-        else
-          paged_rows_kernel<DP, CAP, 2, READS><<<grid, kThreads, 0, stream>>>(p);
-        return;
-      }
-    if (w.block == 16)
-      paged_attention_kernel<DP, PARTS, CAP, 1, READS><<<grid, kThreads, 0, stream>>>(p);
-    else if constexpr (PARTS == 1 || DP < 128)
-      paged_attention_kernel<DP, PARTS, CAP, 2, READS><<<grid, kThreads, 0, stream>>>(p);
-  };
   // sixteen slots as a buffer: one behind the other, apart, within 31 bits
   const int64_t least = c.k.token < c.v.token ? c.k.token : c.v.token, most = c.k.token > c.v.token ? c.k.token : c.v.token;
   const bool buffers = c.page_size % 16 == 0 && least >= c.D && most < int64_t(1) << 24;
-  const bool once = PARTS == 1 && c.B * c.table_width <= c.pages && w.blocks == 1;
-  if (!once)
-    buffers ? attend(std::integral_constant<Reads, kCached>{}) : attend(std::integral_constant<Reads, kApart>{});
-  else if constexpr (PARTS == 1)
-    buffers ? attend(std::integral_constant<Reads, kOnce>{}) : attend(std::integral_constant<Reads, kApartOnce>{});
+  auto attend = [&](auto apart) {
+    constexpr bool APART = apart.value;
+    if constexpr (PARTS == 3)
+      if (w.rows <= 2) {
+        if (w.rows == 1)
+          paged_rows_kernel<DP, CAP, 1, APART><<<grid, kThreads, 0, stream>>>(p);
+        else
+          paged_rows_kernel<DP, CAP, 2, APART><<<grid, kThreads, 0, stream>>>(p);
+        return;
+      }
+    auto attend16 = [&](auto past) { paged_attention_kernel<DP, PARTS, CAP, 1, APART, past.value><<<grid, kThreads, 0, stream>>>(p); };
+    auto attend32 = [&](auto past) { paged_attention_kernel<DP, PARTS, CAP, 2, APART, past.value><<<grid, kThreads, 0, stream>>>(p); };
+    typedef std::integral_constant<Past, kNone> None;
+    typedef std::integral_constant<Past, kUnshared> Unshared;
+    typedef std::integral_constant<Past, kAll> All;
+    if constexpr (PARTS == 3) {
+      if (w.block == 16)
+        attend16(None{});
+      else if constexpr (DP < 128)
+        attend32(None{});
+    } else if (w.block == 16) {  // (up to 16 rows are one block)
+      w.whole ? attend16(All{}) : attend16(Unshared{});
+    } else if (w.blocks == 1) {
+      w.whole ? attend32(All{}) : attend32(Unshared{});
+    } else {
+      attend32(None{});
+    }
+  };
+  buffers ? attend(std::false_type{}) : attend(std::true_type{});
   const int64_t outputs = !w.whole && w.runs > c.B ? c.B * a.Nq * a.H : 0;  // where a row may have several runs
   const int lanes = outputs * ((c.D + 31) / 32) <= 1024 ? 8 : 32;
   const int64_t units = lanes == 8 ? outputs * ((c.D + 31) / 32) : outputs;

@@ -52,3 +52,33 @@ def test_rows_divided_by_every_wave(B, Nq, H, Hk, dtype):
     within("out", out, want["out"], want["t_out"])
     within("scores", new, want["scores"], want["t_scores"])
     assert torch.equal(hz.paged_attention(q, k, v, table, n), out)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("how", ["groups", "every second", "all", "last rows", "padding"])
+@pytest.mark.parametrize("S", [64, 48, 10, 1])
+def test_shared_pages_in_pools_of_any_size(S, how, dtype):
+    """Whichever pages rows share, and however large the pool: the bits that rows with pages of their own give."""
+    print(f"[case] shared {S} {how} {dtype}", flush=True)
+    B, H, Hk, D, slots = 9, 4, 2, 64, 2000
+    T = -(-slots // S)
+    g = torch.Generator(device="cuda").manual_seed(42)
+    normal = lambda *shape: torch.randn(*shape, generator=g, device="cuda").to(DT[dtype])  # noqa: E731
+    pages = 3 * T + 5  # fewer than all tables have
+    k, v = normal(pages, S, Hk, D), normal(pages, S, Hk, D)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(S)).to(torch.int32)
+    own = [order[i * T:(i + 1) * T] for i in range(3)]
+    first = {"groups": [0, 0, 0, 1, 1, 1, 2, 2, 2], "every second": [0, 1, 2] * 3, "all": [0] * 9, "last rows": [0, 1, 2, 0, 1, 2, 0, 0, 0], "padding": [0, 1, 2] * 3}[how]
+    table = torch.stack([own[i] for i in first])
+    lengths = [2000, 1999, 1000, 1700, 1, 1500, 0, 1300, 1800]
+    if how == "padding":  # behind the lengths: no page, the same one for all, numbers out of range
+        for b, n in enumerate(lengths):
+            table[b, -(-n // S):] = [-1, 0, 2**31 - 1][b % 3]
+    q, n = normal(B, 1, H, D), torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    scores = torch.rand(B, Hk, T * S, generator=g, device="cuda")
+    got = hz.paged_attention(q, k, v, table.cuda(), n, scores=scores)
+    at = table.long().clamp(0, pages - 1).flatten().cuda()
+    apart = torch.arange(B * T, dtype=torch.int32, device="cuda").reshape(B, T)
+    want = hz.paged_attention(q, k[at].contiguous(), v[at].contiguous(), apart, n, scores=scores)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(hz.paged_attention(q, k, v, table.cuda(), n), got[0])
