@@ -1081,7 +1081,9 @@ int hz_paged_append(hipStream_t stream, const hz_paged_cache* cache, const hz_to
   if (int rc = check_paged_cache(*cache)) return rc;
   if (int rc = check_paged_tables(*cache)) return rc;
   if (N < 1 || N >= kTokenAxis) return fail(HZ_EINVAL, "N must be in [1, 2^30), got %lld", (long long)N);
-  if (cache->B * cache->Hk > (int64_t(1) << 31) / N) return fail(HZ_EINVAL, "B * N * Hk exceeds the grid limit");
+  // a thread for each 16 bytes of a head, fewer than 2^32 of them in a launch (B * Hk is at most 2^23, 16 bytes of a head at most 32)
+  const int64_t chunks = cache->D * (cache->dtype == HZ_DTYPE_BF16 ? 2 : 4) / 16;
+  if (cache->B * cache->Hk * N * chunks > (int64_t(1) << 32) - 256) return fail(HZ_EINVAL, "B * N * Hk exceeds the grid limit");
   if (int rc = check_strided("k", *k)) return rc;
   if (int rc = check_strided("v", *v)) return rc;
   return launched(hz::launch_paged_append(*cache, *k, *v, N, stream));

@@ -64,7 +64,7 @@ typedef struct {
 /*
  * Token i of the N new ones of row b (k, v [B, N, Hk, D], strided) goes into slot lengths[b] - N + i: lengths count
  * the new tokens already. Tokens of negative slots (the front of a row shorter than N) are left out. (lengths[b] clamped as
- * everywhere: beyond the table's slots, the row's last ones take the new tokens.)
+ * everywhere: beyond the table's slots, the row's last ones take the new tokens.) B N Hk heads, in pieces of 16 bytes, are at most 2^32 - 256.
  */
 int hz_paged_append(hipStream_t stream, const hz_paged_cache* cache, const hz_token_tensor* k, const hz_token_tensor* v,
                     int64_t N);

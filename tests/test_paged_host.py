@@ -192,6 +192,14 @@ def test_abi_refuses_appends(lib):
     assert lib.hz_paged_append(None, cache(), None, t, 1) == N
 
 
+@pytest.mark.parametrize("over,n", [(dict(D=128, B=1 << 20, Hk=16), 1 << 4), (dict(D=128, B=1, Hk=1), 1 << 28), (dict(D=128, B=1, Hk=1), 1 << 27),
+                                    (dict(D=128, dtype=1, B=4, Hk=4), 1 << 24), (dict(D=8, dtype=1, B=4, Hk=2), 1 << 29)], ids=str)
+def test_abi_refuses_appends_of_more_threads_than_a_launch_has(lib, over, n):
+    """A thread for each 16 bytes of a head: 2^32 and more."""
+    t = _native.TOKEN_TENSOR.pack(*flat(dict(t=dict(TENSOR, batch=0, token=0, head=0))))
+    refused(lib.hz_paged_append(None, cache(over), t, t, n), E, "grid", lib)
+
+
 ROTARY = dict(q=TENSOR, k=TENSOR, q_out=TENSOR, k_out=TENSOR, w_q=None, w_k=None, freqs=A, positions=A, B=2, N=3, H=4, Hk=2, D=32,
               n_freqs=16, eps=1e-6, interleaved=0, dtype=0, axes=A, n_axes=2, norm=0)
 
