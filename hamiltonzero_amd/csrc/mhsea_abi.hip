@@ -400,6 +400,8 @@ int check_paged_evict_dims(const hz_paged_evict_args* p) {
   const int64_t slots = c.page_size * c.table_width, moves = slots - p->budget < p->budget ? slots - p->budget : p->budget;
   if (c.B * c.Hk > (int64_t(1) << 20) || (moves > 0 && c.B * c.Hk * ((moves + 63) / 64) > (int64_t(1) << 23)))
     return fail(HZ_EINVAL, "B * Hk rows of this budget exceed the grid limit");
+  // (workgroups of 256 threads move 32 slots at least; fewer than 2^32 threads in a launch)
+  if ((moves + 31) / 32 >= int64_t(1) << 24) return fail(HZ_EINVAL, "a row of this budget exceeds the grid limit");
   return HZ_OK;
 }
 

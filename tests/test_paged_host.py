@@ -182,6 +182,19 @@ def test_abi_refuses_eviction(lib, over, code, text):
     refused(lib.hz_paged_evict(None, e, A, 1 << 40), code, text, lib)
 
 
+def test_abi_refuses_evictions_of_more_threads_than_a_launch_has(lib):
+    """The moves of one row, 32 of 256 threads: 2^32 threads at 2^29 - 31 of them."""
+    long = dict(D=128, B=1, Hk=1, page_size=1, table_width=(1 << 30) - 1)
+    for budget, most in (((1 << 29) - 1, False), ((1 << 29) - 31, False), ((1 << 29) - 32, True), ((1 << 29) + 40, True)):
+        e = cache(long) + _native.PAGED_EVICT_REST.pack(*flat(changed(EVICT, dict(budget=budget))))
+        if most:  # taken: only the workspace is too small
+            assert lib.hz_paged_evict_workspace(e) > 1 << 31
+            refused(lib.hz_paged_evict(None, e, A, 1), E, "workspace", lib)
+        else:
+            assert lib.hz_paged_evict_workspace(e) == -1
+            refused(lib.hz_paged_evict(None, e, A, 1 << 40), E, "grid", lib)
+
+
 def test_abi_refuses_appends(lib):
     t = _native.TOKEN_TENSOR.pack(*flat(dict(t=TENSOR)))
     for n, text in ((0, "N must"), (1 << 30, "N must"), (1 << 29, "grid")):
