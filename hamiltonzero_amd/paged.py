@@ -68,8 +68,18 @@ def _range(t: Tensor) -> Tuple[int, int]:
     return begin, begin + t.numel() * t.element_size() if t.is_contiguous() else _end(t)
 
 
-def _check_written(k_cache: Tensor, v_cache: Tensor, *others: Tensor) -> None:
-    """The caches of a call that writes them: no element at two places, apart from each other and from ``others``."""
+def _touches(t: Tensor, others: Tuple[Tensor, ...]) -> bool:
+    """Whether ``t`` shares memory with any of ``others``; ranges of addresses first, which mostly are apart."""
+    t0, t1 = _range(t)
+    for x in others:
+        begin, end = _range(x)
+        if t0 < end and begin < t1 and _overlap(t, x):
+            return True
+    return False
+
+
+def _check_written(k_cache: Tensor, v_cache: Tensor, names: str, *others: Tensor) -> None:
+    """The caches of a call that writes them: no element at two places, apart from each other and from ``others``, called ``names``."""
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if _holds_twice(t):
             raise ValueError(f"{name} must not hold one element at several places, got strides {t.stride()}")
@@ -79,7 +89,7 @@ def _check_written(k_cache: Tensor, v_cache: Tensor, *others: Tensor) -> None:
     for t in others:
         t0, t1 = _range(t)
         if (t0 < k1 and k0 < t1 and _overlap(t, k_cache)) or (t0 < v1 and v0 < t1 and _overlap(t, v_cache)):
-            raise ValueError("k and v must not overlap the caches")
+            raise ValueError(f"{names} must not overlap the caches")
 
 
 def _no_grad(*tensors: Optional[Tensor]) -> None:
@@ -98,7 +108,7 @@ def paged_append(k_cache: Tensor, v_cache: Tensor, k: Tensor, v: Tensor, page_ta
     N = k.shape[1]
     for name, t in (("k", k), ("v", v)):
         _check(name, t, k_cache.device, k_cache.dtype, (B, N, Hk, D))
-    _check_written(k_cache, v_cache, k, v)
+    _check_written(k_cache, v_cache, "k and v", k, v)
     _no_grad(k_cache, v_cache, k, v)
     k, v = _strided(k), _strided(v)
     with _on(k_cache.device):
@@ -129,8 +139,8 @@ def paged_attention(
 
     With ``scores`` (float32 ``[B, Hk, width * page_size]``, the weights that each slot has had) returns ``(out,
     new_scores)``: ``decay * scores`` plus the sum of the weights that the queries and heads of the key head
-    give the slot now, and 0 from ``lengths[b]`` on; in a new tensor or in ``scores_out``, which may be ``scores``. Its
-    sums are float32, of weights that are not rounded."""
+    give the slot now, and 0 from ``lengths[b]`` on; in a new tensor or in ``scores_out``, which may be ``scores`` and must not overlap
+    ``q`` or the caches. Its sums are float32, of weights that are not rounded."""
     args, (B, slots, Hk, D) = _cache(k_cache, v_cache, page_table, lengths)
     dev = k_cache.device
     _check_first("q", q, "[B, Nq, H, D]")
@@ -154,7 +164,6 @@ def paged_attention(
                 raise ValueError("scores_out must be scores or not overlap it")
     _no_grad(q, k_cache, v_cache, slopes, scores, scores_out)
     q = _strided(q)
-    out = torch.empty((B, Nq, H, D), dtype=q.dtype, device=dev)
     into = scores_out
     if scores is not None:
         if into is scores and (not scores.is_contiguous() or scores.data_ptr() % 16):
@@ -164,6 +173,9 @@ def paged_attention(
             scores = scores.clone()
         if into is None:
             into = torch.empty_like(scores)
+        elif _touches(into, (q, k_cache, v_cache)):
+            raise ValueError("scores_out must not overlap q or the caches")
+    out = torch.empty((B, Nq, H, D), dtype=q.dtype, device=dev)
     args = args + _native.PAGED_ATTENTION_REST.pack(
         *_fields(q), out.data_ptr(), _ptr(slopes), _ptr(scores), _ptr(into), Nq, H,
         float(D) ** -0.5 if scale is None else _float32(scale), _float32(softcap), _float32(decay))
@@ -191,7 +203,7 @@ def paged_evict(
     recent: int = 0,
 ) -> Tuple[Tensor, Tensor, Tensor]:
     """Cuts the rows longer than ``budget`` slots to it, for each key head by its own weights ``scores [B, Hk, width * page_size]``
-    (float32, as :func:`paged_attention` adds them up). Kept are the first ``sinks`` slots, the last ``recent`` ones, and
+    (float32, as :func:`paged_attention` adds them up; apart from the caches). Kept are the first ``sinks`` slots, the last ``recent`` ones, and
     of the others those of the largest scores (equal ones: the lowest slot first; a NaN is less than any number).
 
     The k-th kept slot at or behind the budget (ascending) moves to the k-th slot below it that was given up; what lies below the
@@ -212,11 +224,11 @@ def paged_evict(
         raise ValueError(f"budget must be in [1, 2^30), got {budget}")
     if sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"sinks and recent must not be negative and at most the budget together, got {sinks} and {recent} of {budget}")
-    _check_written(k_cache, v_cache)
     _no_grad(k_cache, v_cache, scores)
     scores = scores.contiguous()
     if scores.data_ptr() % 16:
         scores = scores.clone()
+    _check_written(k_cache, v_cache, "scores", scores)
     new = torch.empty_like(scores)
     sources = torch.empty((B, Hk, min(budget, slots)), dtype=torch.int32, device=dev)
     new_lengths = torch.empty_like(lengths)

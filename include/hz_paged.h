@@ -75,7 +75,8 @@ int hz_paged_append(hipStream_t stream, const hz_paged_cache* cache, const hz_to
  * q [B, Nq, H, D] strided, out [B, Nq, H, D]. A query that sees no slot gets zeros.
  * scores_out [B, Hk, table_width * page_size] float32 or NULL: with P the softmax,
  *     scores_out[b, g, j] = decay scores[b, g, j] + sum over i and the query heads h of key head g of P_hij
- * for j < n_b, and 0 from n_b on. scores (NULL: zeros) may be scores_out itself; 16-byte aligned both.
+ * for j < n_b, and 0 from n_b on. scores (NULL: zeros) may be scores_out itself; 16-byte aligned both. scores_out may not
+ * overlap anything else that is read.
  */
 typedef struct {
   hz_paged_cache cache;
@@ -99,7 +100,7 @@ int hz_paged_attention(hipStream_t stream, const hz_paged_attention_args* p, voi
  *   sources [B, Hk, m] with m = min(budget, table_width * page_size): the slot whose token lies at s now; -1 from
  *                                  lengths_out[b] on
  *   scores_out (as scores; may not overlap it): the kept ones at their new slots, 0 from lengths_out[b] on
- * The outputs may not be lengths or page_table. budget >= 1, sinks + recent <= budget. Rows that are cut
+ * scores may not lie in the caches. The outputs may not be lengths or page_table. budget >= 1, sinks + recent <= budget. Rows that are cut
  * must not share pages with other rows, and no row may have a page twice.
  */
 typedef struct {
