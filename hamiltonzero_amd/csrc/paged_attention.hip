@@ -38,7 +38,7 @@ struct PagedParams {
   const int* plan;                       // of more than 64 batch rows
   int waves, step;                       // waves of a run; slots that they take at a time, of which runs are multiples
   bool whole;                            // each row is one run
-  float cap, to_tanh, to_score2, decay;
+  float to_tanh, to_score2, decay;
 };
 
 // How the rows are divided: runs of `chunk` slots, at least one a row (more steps than the quotient of all by those wanted, so that the
@@ -63,17 +63,6 @@ __device__ __forceinline__ int chunk_of(const PagedParams& p, T steps) {
   return static_cast<int>(each < most ? each : most) * p.step;
 }
 
-// x of this lane and all before it.
-__device__ __forceinline__ int scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from 1, 2, 4 and 8 lanes below in the row of sixteen
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the row's last lane to the next row, of rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
-  return x;
-}
-
 struct Plan {
   int chunk, all, mine, upto;  // all: number of further runs; this lane's row's, and those of the rows up to it (without a table)
   const int* table;            // chunk, all, [B] the further runs before each row, then their Founds
@@ -90,9 +79,9 @@ struct Plan {
     }
     const int n = lane < p.B ? p.c.length(lane) : 0;
     // (the steps of 64 rows are below 2^31)
-    chunk = chunk_of(p, static_cast<uint32_t>(__builtin_amdgcn_readlane(scan(steps_of(p, n)), 63)));
+    chunk = chunk_of(p, static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan(steps_of(p, n))), 63)));
     mine = further(n, chunk);
-    upto = scan(mine);
+    upto = static_cast<int>(wave_scan(mine));
     all = __builtin_amdgcn_readlane(upto, 63);
   }
   // The batch row of run `at`, and its number there; false behind the last one.
@@ -1011,7 +1000,7 @@ hipError_t run(const hz_paged_attention_args& a, void* workspace, hipStream_t st
                 reinterpret_cast<float2*>(ws + w.stats), w.finish_weights ? reinterpret_cast<float2*>(ws + w.norms) : nullptr, static_cast<int>(c.B), static_cast<int>(a.Nq),
                 static_cast<int>(a.H), static_cast<int>(c.Hk), static_cast<int>(a.H / c.Hk), static_cast<int>(c.D),
                 static_cast<int>(w.rows), static_cast<int>(w.blocks), w.blocks_kept, w.runs_wanted, w.runs_fill,
-                w.table ? reinterpret_cast<int*>(ws + w.plan) : nullptr, static_cast<int>(w.waves), static_cast<int>(w.step), w.whole, a.softcap,
+                w.table ? reinterpret_cast<int*>(ws + w.plan) : nullptr, static_cast<int>(w.waves), static_cast<int>(w.step), w.whole,
                 capped ? a.scale / a.softcap : 0.f, (capped ? a.softcap : a.scale) * kLog2e, a.decay};
   const unsigned grid = static_cast<unsigned>(w.waves > 1 ? w.runs * c.Hk * w.blocks : (w.runs * c.Hk * w.blocks + 3) / 4);
   if (w.table) paged_plan_kernel<<<1, 1024, 0, stream>>>(p, reinterpret_cast<int*>(ws + w.plan));

@@ -161,20 +161,6 @@ __device__ __forceinline__ int put_moves(const Row& r, uint32_t threshold, int e
   return holes;
 }
 
-// x of this lane and all before it. (Unsigned: two numbers of sixteen bits are summed as one.)
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-  auto from = [&](auto control, auto rows) {
-    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), control.value, rows.value, 0xf, false));
-  };
-  typedef std::integral_constant<int, 0xf> All;
-  x += from(std::integral_constant<int, 0x111>{}, All{});  // from 1, 2, 4 and 8 lanes below in the row of sixteen
-  x += from(std::integral_constant<int, 0x112>{}, All{});
-  x += from(std::integral_constant<int, 0x114>{}, All{});
-  x += from(std::integral_constant<int, 0x118>{}, All{});
-  x += from(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // the row's last lane to the next row, of rows 1 and 3
-  x += from(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // lane 31 to rows 2 and 3
-  return x;
-}
 __device__ __forceinline__ int wave_sum(int x) { return __builtin_amdgcn_readlane(static_cast<int>(wave_scan(x)), 63); }
 
 // Moves `count` tokens of one row and key head from the slots from[i] to the slots to[i], by `threads` threads: four in flight

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/hz_paged.h"
 
 namespace hz {
@@ -50,5 +52,20 @@ struct Pages {
     return q * size > slot ? q - 1 : q;
   }
 };
+
+// x of this lane and all before it. (Unsigned: two numbers of sixteen bits are summed as one.)
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  auto from = [&](auto control, auto rows) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), control.value, rows.value, 0xf, false));
+  };
+  typedef std::integral_constant<int, 0xf> All;
+  x += from(std::integral_constant<int, 0x111>{}, All{});  // from 1, 2, 4 and 8 lanes below in the row of sixteen
+  x += from(std::integral_constant<int, 0x112>{}, All{});
+  x += from(std::integral_constant<int, 0x114>{}, All{});
+  x += from(std::integral_constant<int, 0x118>{}, All{});
+  x += from(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // the row's last lane to the next row, of rows 1 and 3
+  x += from(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // lane 31 to rows 2 and 3
+  return x;
+}
 
 }  // namespace hz
