@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p)
 }
 
 // q and k: the forward's inputs; qo and ko: the cotangents. partial: [gridDim.x][2][D]. Four workgroups a CU, so that all of the grid are
-// there at once (float32 had registers for three: 157 us for 256 x 225 tokens of 16 heads of 64, 140 with four).
+// there at once (float32 had registers for three: 157 us for 256 x 225 tokens of 16 heads of 64; with four, heads of more than 16 elements spill two to four registers
+// and take 140).
 template <class S, int GS, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads, 4) norm_rotary_bwd_kernel(NormParams p, void* dq, void* dk, float* partial) {
   __shared__ Angles angles[kMaxTokensBwd];
@@ -400,8 +401,9 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(NormParams p, float di
 
 // Tokens a workgroup at a time: several where that leaves at least `blocks` workgroups, so that the angles are
 // formed by all lanes and the loads of several heads overlap (the forwards of
-// qk_train_bf16 and qk_train_sites_f32: 90 and 93 us, 115 and 220 with one token); a power of two, up to 160 heads in all (2 x 8160
-// tokens of 40 heads, 4 and 16 tokens a time: 61 us, 73; 256 x 225 of 16 heads, 4 and 8: 52 and 50, behind norms 116 and 112).
+// qk_train_bf16 and qk_train_sites_f32: 90 and 93 us, 115 and 220 with one token), at most `most`. Forward that is the largest power of two up to 16
+// whose tokens have 160 heads or fewer in all, or one token (2 x 8160 tokens of 40 heads, 4 and 16 tokens a time: 61 us, 73; 256 x 225 of 16
+// heads, 4 and 8: 52 and 50, behind norms 116 and 112).
 int tokens_each(int64_t tokens, int64_t blocks, int most) {
   const int64_t n = tokens / blocks;
   return static_cast<int>(n < 1 ? 1 : n > most ? most : n);
