@@ -12,7 +12,7 @@ contiguous elements, 16-byte aligned; a pool ``[pages, Hk, page_size, D]`` goes 
 ``page_table [B, width]`` and ``lengths [B]``, int32 on the GPU and read there. Row b has the slots ``0 .. lengths[b] - 1``
 (clamped to ``width * page_size``, its most), slot j in page ``page_table[b, j // page_size]`` at ``j % page_size``. Rows may
 share pages that no call writes. An entry that is no page (negative, or not below ``pages``) hides its slots: the attention
-does not see them, the append does not write them, the eviction does not move them. Slots from ``lengths[b]`` on are neither
+does not see them, the append does not write them, the eviction does not move them (its results count them as slots like others, by their scores). Slots from ``lengths[b]`` on are neither
 read nor written; those below must hold finite values.
 
 Calls for inference: none has a gradient. Work goes to the current stream of the tensors' device; there is no CPU
@@ -140,7 +140,10 @@ def paged_attention(
     With ``scores`` (float32 ``[B, Hk, width * page_size]``, the weights that each slot has had) returns ``(out,
     new_scores)``: ``decay * scores`` plus the sum of the weights that the queries and heads of the key head
     give the slot now, and 0 from ``lengths[b]`` on; in a new tensor or in ``scores_out``, which may be ``scores`` and must not overlap
-    ``q`` or the caches. Its sums are float32, of weights that are not rounded."""
+    ``q`` or the caches. Its sums are float32, of weights that are not rounded. Such a call takes workspace for a score of every query, head and slot
+    of the table, 4 bytes each, whatever the lengths: keep ``width`` near what the rows need.
+
+    For a few queries: the slots are read once for up to 32 queries and heads of a key head (float32 heads above 64: 16), and again for every 32 more."""
     args, (B, slots, Hk, D) = _cache(k_cache, v_cache, page_table, lengths)
     dev = k_cache.device
     _check_first("q", q, "[B, Nq, H, D]")
@@ -209,6 +212,8 @@ def paged_evict(
     The k-th kept slot at or behind the budget (ascending) moves to the k-th slot below it that was given up; what lies below the
     budget and is kept stays where it is. So a slot's number is no longer its token's position: call without ``slopes``
     afterwards, and let ``recent`` count tokens appended since the last eviction (rows cut at ``budget + recent`` slots or more).
+
+    What is given up is not attended to again: results after it approximate those of the whole cache.
 
     Keys and values move in place. Returns ``(lengths, sources, scores)``, new tensors: ``min(lengths[b], budget)``; ``[B, Hk,
     min(budget, width * page_size)]`` int32, the slot whose token lies at s now, -1 from the new length on; and the scores

@@ -16,7 +16,7 @@
  * 0 .. n_b - 1 with n_b = lengths[b], clamped to [0, table_width page_size]; slot j lies in page
  * page_table[b, j / page_size] at j % page_size. Rows may share pages that no call writes. A number outside
  * [0, pages) is no page: its slots are not seen by the attention, not written by the append and not moved by the
- * eviction. Slots from n_b on are neither read nor written; those below must hold finite values.
+ * eviction (whose results count them as slots like others, by their scores). Slots from n_b on are neither read nor written; those below must hold finite values.
  */
 #ifndef HZ_PAGED_H
 #define HZ_PAGED_H
@@ -76,7 +76,8 @@ int hz_paged_append(hipStream_t stream, const hz_paged_cache* cache, const hz_to
  * scores_out [B, Hk, table_width * page_size] float32 or NULL: with P the softmax,
  *     scores_out[b, g, j] = decay scores[b, g, j] + sum over i and the query heads h of key head g of P_hij
  * for j < n_b, and 0 from n_b on. scores (NULL: zeros) may be scores_out itself; 16-byte aligned both. scores_out may not
- * overlap anything else that is read.
+ * overlap anything else that is read. With scores_out the workspace holds B Nq H table_width page_size floats and more, whatever the lengths.
+ * The slots are read once for up to 32 of the Nq H / Hk queries and heads of a key head (float32 with D above 64: 16), and again for every 32 more.
  */
 typedef struct {
   hz_paged_cache cache;
