@@ -503,8 +503,8 @@ __device__ __forceinline__ float row_turned(float x) {
 // Which reads go past the caches. float32 none (16 x 8192 slots of 8 heads of 128: 203 us, 214 past them), nor bfloat16 where several workgroups read
 // a run, for more than 32 rows of query and head each. Else bfloat16 does (16 rows of up to 32768 slots of 8 heads of 128: 241 us, 267 through
 // them; in pages of 100 slots 241 and 268, of one slot 253 and 279), but for runs whose pages the rows beside read too (16 x 32768 slots: 346 us;
-// four fifths of the pages shared 283 past the caches, 230 as asked of each run; all of them 268, 181). Rows that are one run each are not asked, which
-// takes 1 us (64 x 900 slots 46.7, 47.7; all of them shared 27.1 past the caches, 27.3 through them; 1024 x 1000 apart 635, 704).
+// four fifths of the pages shared 283 past the caches, 230 as asked of each run; all of them 268, 181). Rows that are one run each are not asked,
+// which takes 1 us (64 x 900 slots 46.7, 47.7; all of them shared 27.1 past the caches, 27.3 through them; 1024 x 1000 apart 635, 704).
 enum Past { kNone, kUnshared, kAll };
 
 template <int DP, int PARTS, bool CAP, int CB, bool APART, Past PAST>
@@ -997,7 +997,8 @@ hipError_t run(const hz_paged_attention_args& a, void* workspace, hipStream_t st
   const bool want = a.scores_out != nullptr;
   const bool capped = a.softcap > 0.f;
   PagedParams p{Pages(c), a.q, a.out, a.slopes, a.scores, a.scores_out, ws + w.partial, want ? ws + w.kept : nullptr,
-                reinterpret_cast<float2*>(ws + w.stats), w.finish_weights ? reinterpret_cast<float2*>(ws + w.norms) : nullptr, static_cast<int>(c.B), static_cast<int>(a.Nq),
+                reinterpret_cast<float2*>(ws + w.stats), w.finish_weights ? reinterpret_cast<float2*>(ws + w.norms) : nullptr,
+                static_cast<int>(c.B), static_cast<int>(a.Nq),
                 static_cast<int>(a.H), static_cast<int>(c.Hk), static_cast<int>(a.H / c.Hk), static_cast<int>(c.D),
                 static_cast<int>(w.rows), static_cast<int>(w.blocks), w.blocks_kept, w.runs_wanted, w.runs_fill,
                 w.table ? reinterpret_cast<int*>(ws + w.plan) : nullptr, static_cast<int>(w.waves), static_cast<int>(w.step), w.whole,

@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(kThreads) norm_rotary_fwd_kernel(NormParams p)
 }
 
 // q and k: the forward's inputs; qo and ko: the cotangents. partial: [gridDim.x][2][D]. Four workgroups a CU, so that all of the grid are
-// there at once (float32 had registers for three: 157 us for 256 x 225 tokens of 16 heads of 64; with four, heads of more than 16 elements spill two to four registers
-// and take 140).
+// there at once (float32 had registers for three: 157 us for 256 x 225 tokens of 16 heads of 64; with four, heads of more than 16
+// elements spill two to four registers and take 140).
 template <class S, int GS, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads, 4) norm_rotary_bwd_kernel(NormParams p, void* dq, void* dk, float* partial) {
   __shared__ Angles angles[kMaxTokensBwd];
