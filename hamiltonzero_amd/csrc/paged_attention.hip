@@ -501,7 +501,7 @@ __device__ __forceinline__ float row_turned(float x) {
 }
 
 // Which reads go past the caches. float32 none (16 x 8192 slots of 8 heads of 128: 203 us, 214 past them), nor bfloat16 where several workgroups read
-// a run, for more than 32 rows of query and head each. Else bfloat16 does (16 rows of up to 32768 slots of 8 heads of 128: 241 us, 267 through
+// a run (more than 32 rows of query and head). Else bfloat16 does (16 rows of up to 32768 slots of 8 heads of 128: 241 us, 267 through
 // them; in pages of 100 slots 241 and 268, of one slot 253 and 279), but for runs whose pages the rows beside read too (16 x 32768 slots: 346 us;
 // four fifths of the pages shared 283 past the caches, 230 as asked of each run; all of them 268, 181). Rows that are one run each are not asked,
 // which takes 1 us (64 x 900 slots 46.7, 47.7; all of them shared 27.1 past the caches, 27.3 through them; 1024 x 1000 apart 635, 704).

@@ -13,8 +13,7 @@ contiguous elements, 16-byte aligned; a pool ``[pages, Hk, page_size, D]`` goes 
 (clamped to ``width * page_size``, its most), slot j in page ``page_table[b, j // page_size]`` at ``j % page_size``. Rows may
 share pages that no call writes. An entry that is no page (negative, or not below ``pages``) hides its slots: the attention
 does not see them, the append does not write them, the eviction does not move them (its results count them as slots like others, by
-their scores). Slots from ``lengths[b]`` on are neither
-read nor written; those below must hold finite values.
+their scores). Slots from ``lengths[b]`` on are neither read nor written; those below must hold finite values.
 
 Calls for inference: none has a gradient. Work goes to the current stream of the tensors' device; there is no CPU
 fallback. What a call writes counts as changed in place.
